@@ -558,6 +558,110 @@ int pmg_unet_step(pmg_unet* u, const float* points, float* points_out, const flo
 /* Synchronises `stream`; reports (PMG_E_DEVICE) and clears a device-wide wait of a step's metric fit that expired. */
 int pmg_unet_check(pmg_unet* u, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------ *
+ * Dense operators around the sparse convolutions (no counterpart in the reference's flex_gemm; its modules leave them
+ * to torch: nn.Linear of PoolDown / NearestUp / encoder_fuse, flex_sparse_blocks.py:78-105, sparse_unet.py:100-173).
+ * Forward only. None of them allocates or synchronises; all can be captured into a HIP graph.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum { PMG_TYPE_F32 = 0, PMG_TYPE_F16 = 1, PMG_TYPE_BF16 = 2, PMG_TYPE_I8 = 3 };
+enum { PMG_ACT_NONE = 0, PMG_ACT_RELU = 1, PMG_ACT_SILU = 2, PMG_ACT_GELU = 3 /* erf */, PMG_ACT_GELU_TANH = 4 };
+
+/* pmg_linear -- out[m][n] = act((a_scale * sum_k x[m][k] w[n][k]) * w_scale[n] + bias[n]) + residual[m][n]
+ *   type: of x and w. fp32, fp16, bf16: fp32 sums, the scales are not read. int8: exact int32 sums, the int8 arithmetic of
+ *   pmg_spconv_i8. One rounding, to out_type, at the end. x: rows of ldx >= K elements; w [N][K]; residual and out: rows
+ *   of ldr, ldo >= N elements. out may be residual (same type and ldr = ldo); it must not overlap x or w.
+ *   K 1 .. 131072, N 1 .. 2^24, M 0 .. 2^31 - 1, ldx at most 4 MiB; any alignment of whole elements (rows of x and w on
+ *   16 bytes with K a whole number of 16 bytes are read 16 bytes at a time, others element by element). */
+typedef struct {
+    int type;
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t M;
+    int K, N;
+    float a_scale;        /* int8 */
+    const float* w_scale; /* int8: [N], or NULL: ones */
+    const float* bias;    /* [N] or NULL */
+    int act;
+    const void* residual; /* or NULL */
+    int residual_type;    /* f32, f16 or bf16 */
+    int64_t ldr;
+    void* out;
+    int out_type; /* f32, f16 or bf16 */
+    int64_t ldo;
+} pmg_linear_args;
+int pmg_linear(const pmg_linear_args* args, void* stream);
+
+/* pmg_qk_norm_rope -- for each row m and head of q (Hq heads) and k (Hk, may be 0), D values:
+ *   u = x * rsqrt(mean(x^2) + eps) * weight + bias; layer: of x - mean(x)
+ *   then the first `pairs` (<= D / 2) pairs are turned by t = sum over axes of coords[m][1 + axis] * freqs[p][axis]
+ *   (in 64 bits): (a, b) -> (a cos t - b sin t, a sin t + b cos t); pair p is (p, p + D/2), interleaved: (2p, 2p + 1).
+ * D a multiple of 8 up to 128; strides in elements, buffers and strides in whole groups of 4 elements; weights and
+ * biases [D] fp32 or NULL (1, 0). q_out / k_out may be q / k. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    int64_t M;
+    int Hq, Hk, D, pairs;
+    const void* q;
+    int64_t q_row, q_head;
+    const void* k;
+    int64_t k_row, k_head;
+    void* q_out;
+    int64_t q_out_row, q_out_head;
+    void* k_out;
+    int64_t k_out_row, k_out_head;
+    const int32_t* coords; /* [M][4] (b, x, y, z) */
+    const float* freqs;    /* [pairs][3] radians per voxel */
+    const float* q_weight;
+    const float* k_weight;
+    const float* q_bias;
+    const float* k_bias;
+    int layer, interleaved;
+    float eps;
+} pmg_rope_args;
+int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
+
+/* pmg_attention -- attention inside segments of rows (frames, or the cells of a pool cache). Segment s holds the query
+ * positions [q_offsets[s], q_offsets[s + 1]) and the key positions [k_offsets[s], k_offsets[s + 1]) (device, int64
+ * [segments + 1], rising); position p is row index[p], or row p without an index (a pool cache's seg_offsets and
+ * seg_indices). For query row i and head h, over the keys j of i's segment with k_mask[j] != 0 (row-indexed, or NULL):
+ *   x_j = scale q_i . k_j;  cap > 0: x_j = cap tanh(x_j / cap);  x_j -= sum over axes of slopes[h][axis] |c_i - c_j|[axis]
+ *   out_i = sum_j softmax(x)_j v_j, 0 where no key is left. Key head of h: h / (Hq / Hk).
+ * Sums and statistics in fp32; the softmax's weights enter the second product rounded to `type`.
+ * Offsets are held to [0, positions]; a position whose index lies outside the rows is absent. Query rows outside every
+ * segment are left as they were, or zeroed with zero_rest (those that a position names). A row named by two query
+ * positions gets either's result. Differences of coordinates are exact up to 2^23.
+ * D a multiple of 8 up to 128; q, k, v: buffers and strides (elements) in whole 16 bytes, out in groups of 4 elements;
+ * out must not overlap the inputs. Workspace (any contents; may be NULL if 0 bytes): must not be shared by calls that
+ * overlap. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    int Hq, Hk, D;
+    const void* q;
+    int64_t q_row, q_head;
+    const void* k;
+    int64_t k_row, k_head;
+    const void* v;
+    int64_t v_row, v_head;
+    void* out;
+    int64_t out_row, out_head;
+    int64_t q_rows, k_rows;
+    int64_t q_positions, k_positions; /* the index's length, or the rows */
+    int64_t segments;
+    const int64_t* q_offsets;
+    const int64_t* k_offsets;
+    const int32_t* q_index;
+    const int32_t* k_index;
+    const int32_t* q_coords; /* [q_rows][4] (b, x, y, z); with slopes */
+    const int32_t* k_coords;
+    const float* slopes; /* [Hq][3] or NULL */
+    const uint8_t* k_mask;
+    float scale, cap; /* cap 0: none */
+    int zero_rest;
+} pmg_attention_args;
+size_t pmg_attention_workspace_bytes(const pmg_attention_args* args);
+int pmg_attention(const pmg_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

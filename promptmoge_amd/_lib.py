@@ -13,6 +13,8 @@ LIB_PATH = Path(__file__).resolve().with_name("libpmg.so")
 PMG_OK, PMG_E_INVALID, PMG_E_HIP, PMG_E_OVERFLOW, PMG_E_DEVICE = 0, 1, 2, 3, 4
 EPI_ACC, EPI_Q, EPI_R, EPI_BIAS, EPI_SILU, EPI_RLN, EPI_ROUT, EPI_QLIN = 0, 1, 2, 3, 4, 5, 6, 7
 PREC_INT8, PREC_FP16 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 
@@ -84,6 +86,34 @@ class UNetWeights(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("x", vp), ("ldx", i64), ("w", vp), ("M", i64), ("K", i32), ("N", i32), ("a_scale", f32),
+        ("w_scale", vp), ("bias", vp), ("act", i32), ("residual", vp), ("residual_type", i32), ("ldr", i64),
+        ("out", vp), ("out_type", i32), ("ldo", i64),
+    ]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("M", i64), ("Hq", i32), ("Hk", i32), ("D", i32), ("pairs", i32), ("q", vp), ("q_row", i64),
+        ("q_head", i64), ("k", vp), ("k_row", i64), ("k_head", i64), ("q_out", vp), ("q_out_row", i64),
+        ("q_out_head", i64), ("k_out", vp), ("k_out_row", i64), ("k_out_head", i64), ("coords", vp), ("freqs", vp),
+        ("q_weight", vp), ("k_weight", vp), ("q_bias", vp), ("k_bias", vp), ("layer", i32), ("interleaved", i32),
+        ("eps", f32),
+    ]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("Hq", i32), ("Hk", i32), ("D", i32), ("q", vp), ("q_row", i64), ("q_head", i64), ("k", vp),
+        ("k_row", i64), ("k_head", i64), ("v", vp), ("v_row", i64), ("v_head", i64), ("out", vp), ("out_row", i64),
+        ("out_head", i64), ("q_rows", i64), ("k_rows", i64), ("q_positions", i64), ("k_positions", i64),
+        ("segments", i64), ("q_offsets", vp), ("k_offsets", vp), ("q_index", vp), ("k_index", vp), ("q_coords", vp),
+        ("k_coords", vp), ("slopes", vp), ("k_mask", vp), ("scale", f32), ("cap", f32), ("zero_rest", i32),
+    ]
+
+
 UNET_COUNTS, UNET_COORDS, UNET_PARENT, UNET_NMAP, UNET_TILE_MASK, UNET_DOWN, UNET_UP, UNET_ENC_TOKENS, \
     UNET_COL_OFFSETS, UNET_STEP_ST = range(10)
 
@@ -151,6 +181,10 @@ SIGNATURES = {
     "pmg_unet_step_prepare": (i32, [vp, C.POINTER(UNetStepConfig)]),
     "pmg_unet_step": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "pmg_unet_check": (i32, [vp, vp]),
+    "pmg_linear": (i32, [C.POINTER(LinearArgs), vp]),
+    "pmg_qk_norm_rope": (i32, [C.POINTER(RopeArgs), vp]),
+    "pmg_attention_workspace_bytes": (sz, [C.POINTER(AttentionArgs)]),
+    "pmg_attention": (i32, [C.POINTER(AttentionArgs), vp, sz, vp]),
 }
 
 _lib: C.CDLL | None = None

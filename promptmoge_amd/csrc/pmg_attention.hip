@@ -1,0 +1,118 @@
+// Entry points of the attention inside segments: argument checks, and the choice of the kernel's form.
+#include "pmg_attention.h"
+
+using namespace pmg;
+
+namespace {
+
+struct Plan {
+    int seg, waves, splits;
+};
+
+// The forms, by the mean lengths (the offsets are on the device).
+Plan plan_of(const pmg_attention_args& r) {
+    Plan p{0, 4, 1};
+    if (r.segments < 1) return p;
+    const int64_t G = r.Hq / r.Hk;
+    const double nq = (double)r.q_positions / (double)r.segments, nk = (double)r.k_positions / (double)r.segments;
+    p.seg = nq * (double)G <= 16.0 && nk >= 128.0;
+    p.waves = p.seg || nk < 512.0 ? 1 : 4;
+    const int64_t units = p.seg ? r.segments : (r.q_positions * G + 32 * p.waves - 1) / (32 * p.waves);
+    const int64_t waves = units * r.Hk * p.waves;
+    int64_t s = waves > 0 ? 2048 / waves : 1;
+    const int64_t most = (int64_t)(nk / 256.0);
+    s = s < most ? s : most;
+    p.splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    return p;
+}
+
+int attention_args(const pmg_attention_args& r) {
+    PMG_REQUIRE(r.type >= PMG_TYPE_F32 && r.type <= PMG_TYPE_BF16, "type must be f32, f16 or bf16");
+    PMG_REQUIRE(r.Hq >= 1 && r.Hk >= 1 && r.Hq <= 4096 && r.Hq % r.Hk == 0, "query heads must be a multiple of key heads (up to 4096)");
+    PMG_REQUIRE(r.D >= 8 && r.D <= 128 && r.D % 8 == 0, "head width must be a multiple of 8 up to 128");
+    PMG_REQUIRE(r.q_rows >= 0 && r.k_rows >= 0 && r.q_positions >= 0 && r.k_positions >= 0 && r.segments >= 0, "negative size");
+    const int64_t big = (int64_t)1 << 31;
+    PMG_REQUIRE(r.q_rows < big && r.k_rows < big && r.q_positions < big && r.k_positions < big && r.segments < big - 1, "2^31 rows, positions or segments");
+    PMG_REQUIRE(r.q_index || r.q_positions <= r.q_rows, "more query positions than rows");
+    PMG_REQUIRE(r.k_index || r.k_positions <= r.k_rows, "more key positions than rows");
+    PMG_REQUIRE(r.scale > 0.0f && r.scale < 3.0e38f, "scale must be positive");
+    PMG_REQUIRE(r.cap >= 0.0f && r.cap < 3.0e38f, "cap must not be negative");
+    return PMG_OK;
+}
+
+}  // namespace
+
+extern "C" size_t pmg_attention_workspace_bytes(const pmg_attention_args* p) {
+    if (!p || attention_args(*p) != PMG_OK) return 0;
+    const Plan pl = plan_of(*p);
+    if (pl.splits <= 1) return 0;
+    return (size_t)pl.splits * (size_t)p->q_positions * (size_t)p->Hq * ((size_t)p->D * 4 + 8);
+}
+
+extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
+    PMG_REQUIRE(p, "null args");
+    const pmg_attention_args& r = *p;
+    if (int e = attention_args(r)) return e;
+    if (r.q_rows == 0 || r.q_positions == 0) return PMG_OK;
+    PMG_REQUIRE(r.q && r.out && r.q_offsets && r.k_offsets, "null buffer");
+    PMG_REQUIRE(r.k_rows == 0 || r.k_positions == 0 || (r.k && r.v), "null buffer");
+    PMG_REQUIRE(!r.slopes || (r.q_coords && (r.k_coords || r.k_rows == 0)), "slopes need coordinates");
+    const int es = r.type == PMG_TYPE_F32 ? 4 : 2;
+    auto ok = [&](const void* b, int64_t row, int64_t head, int n) {
+        return (reinterpret_cast<uintptr_t>(b) & (uintptr_t)(n * es - 1)) == 0 && row % n == 0 && head % n == 0;
+    };
+    const int per = 16 / es;
+    PMG_REQUIRE(ok(r.q, r.q_row, r.q_head, per) && ok(r.k, r.k_row, r.k_head, per) && ok(r.v, r.v_row, r.v_head, per), "q, k, v: buffers and strides in whole 16 bytes");
+    PMG_REQUIRE(ok(r.out, r.out_row, r.out_head, 4), "out: buffer and strides in whole groups of 4 elements");
+    PMG_REQUIRE(!r.slopes || (aligned16(r.q_coords) && aligned16(r.k_coords)), "coordinates must be 16-byte aligned");
+    const Plan pl = plan_of(r);
+    const size_t need = pmg_attention_workspace_bytes(p);
+    PMG_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), "workspace too small, null or not 16-byte aligned");
+    AttnArgs a{};
+    a.q = r.q;
+    a.k = r.k;
+    a.v = r.v;
+    a.out = r.out;
+    a.q_row = r.q_row;
+    a.q_head = r.q_head;
+    a.k_row = r.k_row;
+    a.k_head = r.k_head;
+    a.v_row = r.v_row;
+    a.v_head = r.v_head;
+    a.o_row = r.out_row;
+    a.o_head = r.out_head;
+    a.Mq = r.q_rows;
+    a.Mk = r.k_rows;
+    a.Pq = r.q_positions;
+    a.Pk = r.k_rows > 0 ? r.k_positions : 0;
+    a.S = r.segments;
+    a.q_off = r.q_offsets;
+    a.k_off = r.k_offsets;
+    a.q_index = r.q_index;
+    a.k_index = r.k_index;
+    a.q_coords = r.q_coords;
+    a.k_coords = r.k_coords;
+    a.slopes = r.slopes;
+    a.k_mask = r.k_mask;
+    a.Hq = r.Hq;
+    a.Hk = r.Hk;
+    a.G = r.Hq / r.Hk;
+    a.D = r.D;
+    const double log2e = 1.4426950408889634;
+    a.scale2 = (float)((double)r.scale * log2e);
+    if (r.cap > 0.0f) {
+        a.cap2 = (float)((double)r.cap * log2e);
+        a.cap_arg = (float)((double)r.scale / (double)r.cap * (r.type == PMG_TYPE_F32 ? 1.0 : 2.0 * log2e));
+    }
+    a.seg = pl.seg;
+    a.splits = pl.splits;
+    a.zero_rest = r.zero_rest;
+    if (pl.splits > 1) {
+        a.part_o = (float*)workspace;
+        a.part_ml = (float2*)((char*)workspace + (size_t)pl.splits * (size_t)r.q_positions * (size_t)r.Hq * (size_t)r.D * 4);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    if (r.type == PMG_TYPE_F32) return launch_attention_f32(a, pl.waves, s);
+    if (r.type == PMG_TYPE_F16) return launch_attention_f16(a, pl.waves, s);
+    return launch_attention_bf16(a, pl.waves, s);
+}

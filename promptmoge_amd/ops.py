@@ -20,6 +20,7 @@ __all__ = [
     "post_depth",
     "math_device", "gauge_poly",
     "nearest_fill",
+    "linear", "linear_i8", "qk_norm_rope", "sparse_attention",
     "EPI_ACC", "EPI_Q", "EPI_R", "EPI_BIAS", "EPI_SILU", "EPI_RLN", "EPI_ROUT", "EPI_QLIN",
 ]
 
@@ -575,3 +576,282 @@ def gauge_poly(depth: torch.Tensor, lidar: torch.Tensor, conf: Optional[torch.Te
     call("pmg_gauge_poly", _p(depth), B, H, W, _p(lidar), _p(conf), h, w, int(degree), int(iters), _p(corr),
          _p(coef), _p(ws), ws_bytes, _stream())
     return (corr, coef) if return_coef else corr
+
+
+# ---------------------------------------------------------------------------------- (5) dense operators around the maps
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16,
+          torch.int8: _lib.TYPE_I8}
+
+
+def _inputs(*named: Tuple[str, Optional[torch.Tensor]]) -> torch.device:
+    """The one device of the given tensors (None: absent); refuses host tensors and tensors that need gradients."""
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{name} must be a GPU tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {dev}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the libpmg operators are inference-only; run under torch.no_grad()")
+    return dev
+
+
+def _on(dev: torch.device, name: str, *args) -> None:
+    """call() on the tensors' own device (the current one or not), on that device's current stream."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, _stream())
+
+
+def _floating(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return _TYPES[t.dtype]
+
+
+def _rows(t: torch.Tensor, name: str) -> int:
+    """The row stride of an (M, C) tensor whose rows are contiguous and do not overlap."""
+    if t.ndim != 2:
+        raise ValueError(f"{name} must be 2-D, got {tuple(t.shape)}")
+    if t.shape[0] <= 1 and (t.shape[1] <= 1 or t.stride(1) == 1):
+        return max(t.shape[1], 1)
+    if (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    return t.stride(0)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
+    dev = _inputs(("x", x), ("w", w), ("bias", bias), ("w_scale", w_scale), ("residual", residual), ("out", out))
+    if w.ndim != 2 or not w.is_contiguous():
+        raise ValueError("w must be a contiguous (N, K) matrix")
+    if w.dtype != x.dtype:
+        raise ValueError(f"w must be {x.dtype}, got {w.dtype}")
+    ldx = _rows(x, "x")
+    M, K = x.shape
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"w expects {w.shape[1]} input channels, x has {K}")
+    for name, t in (("bias", bias), ("w_scale", w_scale)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (N,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 ({N},) vector")
+    if act not in _lib.ACTS:
+        raise ValueError(f"act must be one of {sorted(_lib.ACTS)}, got {act!r}")
+    rt, ldr = 0, 0
+    if residual is not None:
+        rt, ldr = _floating(residual, "residual"), _rows(residual, "residual")
+        if residual.shape != (M, N):
+            raise ValueError(f"residual must be ({M}, {N}), got {tuple(residual.shape)}")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    else:
+        if out.shape != (M, N):
+            raise ValueError(f"out must be ({M}, {N}), got {tuple(out.shape)}")
+        if _overlap(out, x) or _overlap(out, w):
+            raise ValueError("out must not overlap x or w")
+        if residual is not None and _overlap(out, residual) and not (
+                out.data_ptr() == residual.data_ptr() and out.dtype == residual.dtype
+                and out.stride() == residual.stride()):
+            raise ValueError("out may be residual itself, but not overlap it otherwise")
+    args = _lib.LinearArgs(_TYPES[x.dtype], _p(x), ldx, _p(w), M, K, N, a_scale, _p(w_scale), _p(bias),
+                           _lib.ACTS[act], _p(residual), rt, ldr, _p(out), _floating(out, "out"), _rows(out, "out"))
+    _on(dev, "pmg_linear", C.byref(args))
+    return out
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: str = "none",
+           residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x w^T + bias) + residual in one kernel: nn.Linear of the U-Net's PoolDown, NearestUp and projections with what
+    follows it. x: (M, K) fp32 / fp16 / bf16 (rows may be strided); w: (N, K) of x's type; bias: (N,) fp32; act: "none",
+    "relu", "silu", "gelu" (erf) or "gelu_tanh"; residual: (M, N) of any of the three types. Sums in fp32, rounded
+    once to out_dtype (default: x's). `out` may be the residual itself. Forward only."""
+    _inputs(("x", x), ("w", w))
+    _floating(x, "x")
+    return _linear(x, w, bias, 1.0, None, act, residual, out_dtype or (x.dtype if out is None else out.dtype), out)
+
+
+def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, a_scale: float = 1.0,
+              w_scale: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
+              out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear on int8 codes: act((acc * a_scale) * w_scale[n] + bias) + residual with the exact int32 sums acc, the
+    arithmetic of spconv_i8. x: (M, K) int8; w: (N, K) int8; w_scale, bias: (N,) fp32; result fp32, fp16 or bf16."""
+    _inputs(("x", x), ("w", w))
+    if x.dtype != torch.int8:
+        raise ValueError(f"x must be torch.int8, got {x.dtype}")
+    return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype, out)
+
+
+def _heads(t: torch.Tensor, name: str, unit: int) -> torch.Tensor:
+    """An (M, H, D) tensor whose heads are contiguous, on `unit` bytes; copied where its strides or address are not."""
+    if t.ndim != 3:
+        raise ValueError(f"{name} must be (rows, heads, width), got {tuple(t.shape)}")
+    e = t.element_size()
+    if t.stride(2) != 1 or t.data_ptr() % unit or t.stride(0) * e % unit or t.stride(1) * e % unit:
+        t = t.contiguous()
+    return t
+
+
+def _coords(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.shape != (rows, 4):
+        raise ValueError(f"{name} must be ({rows}, 4) int32, got {tuple(t.shape)} {t.dtype}")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous float32 ({n},) vector")
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tensor, freqs: torch.Tensor, *,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, norm: str = "rms",
+                 eps: float = 1e-6, interleaved: bool = False,
+                 out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
+    """The norms of queries and keys per head, then the rotation by voxel coordinates, in one pass over both.
+
+    q: (M, Hq, D), k: (M, Hk, D) or None, fp32 / fp16 / bf16, slices of one product allowed; D a multiple of 8 up to 128.
+    norm: "rms" (x * rsqrt(mean(x^2) + eps) * weight + bias) or "layer" (of x - mean). coords: (M, 4) int32
+    (b, x, y, z); freqs: (P, 3) fp32, P <= D / 2: pair p is turned by the angle x f[p, 0] + y f[p, 1] + z f[p, 2], formed in 64
+    bits. Pair p is (p, p + D/2), or with interleaved (2p, 2p + 1). Returns (q, k) in new tensors, or in `out` (which
+    may be the inputs). Forward only."""
+    dev = _inputs(("q", q), ("k", k), ("coords", coords), ("freqs", freqs), ("q_weight", q_weight),
+                  ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias),
+                  ("out[0]", out[0] if out else None), ("out[1]", out[1] if out else None))
+    ty = _floating(q, "q")
+    unit = 4 * q.element_size()
+    if norm not in ("rms", "layer"):
+        raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+    if q.ndim != 3:
+        raise ValueError(f"q must be (rows, heads, width), got {tuple(q.shape)}")
+    M, Hq, D = q.shape
+    if k is not None and (k.ndim != 3 or k.shape[0] != M or k.shape[2] != D or k.dtype != q.dtype):
+        raise ValueError(f"k must be ({M}, heads, {D}) of q's type")
+    coords = _coords(coords, "coords", M)
+    if freqs.dtype != torch.float32 or freqs.ndim != 2 or freqs.shape[1] != 3 or not freqs.is_contiguous():
+        raise ValueError("freqs must be a contiguous (pairs, 3) float32 tensor")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
+        _vector(t, name, D)
+    if out is None:
+        qo = torch.empty((M, Hq, D), dtype=q.dtype, device=dev)
+        ko = torch.empty((M, k.shape[1], D), dtype=q.dtype, device=dev) if k is not None else None
+    else:
+        qo, ko = out
+        for name, t, o in (("out[0]", q, qo), ("out[1]", k, ko)):
+            if (t is None) != (o is None) or (t is not None and (o.shape != t.shape or o.dtype != q.dtype)):
+                raise ValueError(f"{name} must match its input")
+            if o is not None and _heads(o, name, unit) is not o:
+                raise ValueError(f"{name}: strides and address must be whole groups of 4 elements")
+            for other in (q, k):  # (the inputs themselves are fine: each head is read whole before it is written)
+                if o is not None and other is not None and _overlap(o, other) and not (
+                        o.data_ptr() == t.data_ptr() and o.stride() == t.stride()):
+                    raise ValueError(f"{name} may be its input itself, but not overlap the inputs otherwise")
+        if ko is not None and _overlap(qo, ko) and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
+            raise ValueError("out[0] and out[1] must not overlap")
+    q = _heads(q, "q", unit)
+    k = _heads(k, "k", unit) if k is not None else None
+    args = _lib.RopeArgs(ty, M, Hq, k.shape[1] if k is not None else 0, D, freqs.shape[0], _p(q), q.stride(0),
+                         q.stride(1), _p(k), k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0,
+                         _p(qo), qo.stride(0), qo.stride(1), _p(ko), ko.stride(0) if ko is not None else 0,
+                         ko.stride(1) if ko is not None else 0, _p(coords), _p(freqs), _p(q_weight), _p(k_weight),
+                         _p(q_bias), _p(k_bias), norm == "layer", bool(interleaved), float(eps))
+    _on(dev, "pmg_qk_norm_rope", C.byref(args))
+    return qo, ko
+
+
+def _index(t: Optional[torch.Tensor], name: str) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+
+
+def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                     kv_offsets: Optional[torch.Tensor] = None, *, index: Optional[torch.Tensor] = None,
+                     kv_index: Optional[torch.Tensor] = None, coords: Optional[torch.Tensor] = None,
+                     kv_coords: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None,
+                     kv_mask: Optional[torch.Tensor] = None, cap: float = 0.0, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention inside segments of rows: the frames of a batch, or the cells of a pool cache (its seg_offsets as
+    `offsets` and seg_indices as `index`).
+
+    q: (Mq, Hq, D); k, v: (Mk, Hk, D), Hq a multiple of Hk; fp32 / fp16 / bf16, D a multiple of 8 up to 128. offsets: (S + 1,)
+    int64, rising: segment s holds the positions offsets[s] .. offsets[s + 1] - 1; position p is row index[p] (int32), or
+    row p. Without kv_offsets the keys' segments (and index, and coordinates) are the queries'; with them, segment s of
+    the queries attends to segment s of the keys. Scores: scale q.k (scale: default D^-1/2); cap > 0: cap tanh(x / cap);
+    slopes (Hq, 3) fp32: minus sum over the axes of slopes[h, axis] |difference of coords (M, 4) int32 (b, x, y, z)|;
+    kv_mask (Mk,) bool / uint8: rows with 0 are not attended to. A query with no key left gets 0.
+
+    Rows outside every segment are 0 in a new result and left as they were in a given `out`. Every row should be named
+    by at most one query position. Forward only."""
+    dev = _inputs(("q", q), ("k", k), ("v", v), ("offsets", offsets), ("kv_offsets", kv_offsets), ("index", index),
+                  ("kv_index", kv_index), ("coords", coords), ("kv_coords", kv_coords), ("slopes", slopes),
+                  ("kv_mask", kv_mask), ("out", out))
+    ty = _floating(q, "q")
+    if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"q must be (Mq, Hq, D), k and v (Mk, Hk, D); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("k and v must have q's type")
+    Mq, Hq, D = q.shape
+    Mk, Hk = k.shape[:2]
+    if Hk < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads are not a multiple of {Hk} key heads")
+    own = kv_offsets is None
+    if own:
+        if kv_index is not None or kv_coords is not None:
+            raise ValueError("kv_index and kv_coords go with kv_offsets")
+        if Mk != Mq:
+            raise ValueError(f"without kv_offsets the keys are the queries' rows: {Mq} and {Mk}")
+        kv_offsets, kv_index, kv_coords = offsets, index, coords
+    for name, t in (("offsets", offsets), ("kv_offsets", kv_offsets)):
+        if t.dtype != torch.int64 or t.ndim != 1 or t.numel() < 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous (segments + 1,) int64 tensor")
+    if kv_offsets.numel() != offsets.numel():
+        raise ValueError("offsets and kv_offsets must have the same length")
+    _index(index, "index")
+    _index(kv_index, "kv_index")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or slopes.shape != (Hq, 3) or not slopes.is_contiguous():
+            raise ValueError(f"slopes must be a contiguous ({Hq}, 3) float32 tensor")
+        if coords is None or kv_coords is None:
+            raise ValueError("slopes need coords (and kv_coords with kv_offsets)")
+        same = kv_coords is coords
+        coords = _coords(coords, "coords", Mq)
+        kv_coords = coords if same and Mk == Mq else _coords(kv_coords, "kv_coords", Mk)
+    if kv_mask is not None:
+        if kv_mask.dtype not in (torch.bool, torch.uint8) or kv_mask.shape != (Mk,) or not kv_mask.is_contiguous():
+            raise ValueError(f"kv_mask must be a contiguous ({Mk},) bool or uint8 tensor")
+    fresh = out is None
+    if fresh:
+        whole = index is None or index.numel() == Mq
+        out = (torch.empty if whole else torch.zeros)((Mq, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
+        if _heads(out, "out", 4 * q.element_size()) is not out:
+            raise ValueError("out: strides and address must be whole groups of 4 elements")
+        if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
+            raise ValueError("out must not overlap q, k or v")
+    q, k, v = _heads(q, "q", 16), _heads(k, "k", 16), _heads(v, "v", 16)
+    args = _lib.AttentionArgs(
+        ty, Hq, Hk, D, _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
+        v.stride(1), _p(out), out.stride(0), out.stride(1), Mq, Mk, Mq if index is None else index.numel(),
+        Mk if kv_index is None else kv_index.numel(), offsets.numel() - 1, _p(offsets), _p(kv_offsets), _p(index),
+        _p(kv_index), _p(coords) if slopes is not None else None, _p(kv_coords) if slopes is not None else None,
+        _p(slopes), _p(kv_mask), D ** -0.5 if scale is None else float(scale), float(cap), fresh)
+    ws_bytes = lib().pmg_attention_workspace_bytes(C.byref(args))
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
+    _on(dev, "pmg_attention", C.byref(args), _p(ws), ws_bytes)
+    return out
