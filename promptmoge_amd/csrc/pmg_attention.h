@@ -8,8 +8,10 @@
 // formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds 16 scores of ONE slot: maximum and sum are
 // taken in the lane and once across the two halves of the wave, and the scores, rounded to the inputs' type (the
 // weights of the second product; l sums the unrounded ones), are that product's operand as they lie. V^T comes from
-// row-major V by the transposing LDS read (fp32: by plain reads). K and V tiles are staged through registers (rows are
-// gathered by index, absent ones become zeros) one tile ahead into the other of two LDS buffers.
+// row-major V by the transposing LDS read (fp32: by plain reads). K and V tiles go from memory straight to LDS, one tile
+// ahead into the other of two buffers: each lane names the 16 bytes it fetches, so rows are gathered by index, the
+// banks' swizzle is made by the choice of chunk, and an absent row (masked, behind its segment, a bad index) is fetched
+// from a line of zeros. The rows' numbers, mask and coordinates run two and three tiles ahead.
 //
 // Queries are taken in order of position, 32 NW QT / G positions a block, whatever segments they fall in: the block
 // walks over the keys of all its segments, and each lane counts the keys of its own. No work list is needed, and small
@@ -47,6 +49,8 @@ struct AttnArgs {
     float2* part_ml;
 };
 
+__device__ inline int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
 // The segment of position p: the last s with off[s] <= p, if p < off[s + 1]; -1 otherwise.
 __device__ inline int32_t segment_of(const int64_t* off, int64_t S, int64_t p) {
     int64_t lo = 0, hi = S;  // off[lo] <= p is unknown until checked; invariant: answer in [lo - 1, hi - 1]
@@ -59,7 +63,31 @@ __device__ inline int32_t segment_of(const int64_t* off, int64_t S, int64_t p) {
     return p < off[lo] ? (int32_t)(lo - 1) : -1;
 }
 
-__device__ inline int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+// The segment (as above) of position p of each lane, all lanes of a wave taking part; first: a lower bound of the p. A
+// search with 64 probes a round for `first`, then among the 64 offsets that follow.
+__device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t first, int32_t p) {
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, n = S + 1;  // entries before lo are <= first, those from lo + n on are not
+    while (n > 0) {
+        const int64_t step = (n + 63) >> 6, j = (lane + 1) * step - 1;
+        const bool le = j < n && off[lo + j] <= first;
+        const int t = __popcll(__ballot(le));
+        lo += t * step;
+        n -= t * step;
+        n = n < step - 1 ? n : step - 1;
+    }
+    const int32_t e = lo + lane <= S ? (int32_t)clamp64(off[lo + lane], -1, 0x7fffffff) : 0x7fffffff;
+    int c = 0;
+#pragma unroll
+    for (int b = 32; b > 0; b >>= 1) c += __shfl(e, c + b - 1, 64) <= p ? b : 0;
+    c += __shfl(e, 63, 64) <= p ? 1 : 0;  // (only where all before are)
+    if (c == 64) return segment_of(off, S, p);
+    const int64_t s = lo + c - 1;
+    return s < S ? (int32_t)s : -1;
+}
+
+// What absent keys and values are fetched from.
+__device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};
 
 // The other half's value (lane l <-> l ^ 32).
 __device__ inline float other_half(float v) {
@@ -68,8 +96,19 @@ __device__ inline float other_half(float v) {
     return u2f((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// The kernel's arguments, read anew from here on (kept in scalar registers through the loop over the keys they would be
+// spilled to vector registers, lane by lane).
+__device__ inline const AttnArgs& args_again() {
+    auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttnArgs*)p;
+}
+
+// Registers: with at most 256 the matrix instructions' results stay in ordinary vector registers, where the softmax
+// works on them; only the widest fp32 form of one wave needs more.
 template <class T, int DP, int NW, int QT, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1 : 2) void attention_k(AttnArgs a0) {
+    const AttnArgs& a = a0;
     constexpr int ES = sizeof(T), PER = 16 / ES, CPR = DP / PER, NT = 64 * NW;
     constexpr int BK = (NW == 1 || ES == 4) ? 32 : 64, KB = BK / 32;
     constexpr int NCH = BK * CPR / NT;         // 16-byte chunks of K (and of V) a thread stages
@@ -79,9 +118,10 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
     static_assert(NCH * NT == BK * CPR, "whole chunks");
     __shared__ __attribute__((aligned(16))) char s_k[2][BK * DP * ES];
     __shared__ __attribute__((aligned(16))) char s_v[2][BK * DP * ES];
-    __shared__ uint32_t s_ok[2][KB];
-    __shared__ __attribute__((aligned(16))) uint2 s_c[2][BIAS ? 3 : 1][BIAS ? BK : 1];
-    __shared__ int64_t s_r[4][NW];
+    __shared__ uint32_t s_ok[3][KB];  // which keys there are
+    __shared__ int32_t s_row[3][BK];
+    __shared__ __attribute__((aligned(16))) uint2 s_c[3][BIAS ? 3 : 1][BIAS ? BK : 1];
+    __shared__ int32_t s_r[3][NW];
     __shared__ int s_flag[NW];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -96,20 +136,20 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
         else return c ^ (((row >> 1) ^ (row >> 3)) & 3);
     };
     // V: 32-byte units of a row, so that the four rows of a transposing read lie in different banks
-    const auto vadr = [](int row, int c) {
-        if constexpr (ES == 4) return row * DP * 4 + c * 16;
-        const int f = DP == 64 ? 2 * ((row >> 1) & 1) : DP == 128 ? 2 * (row & 3) : 0;
-        return row * DP * 2 + (((c >> 1) ^ f) * 32) + (c & 1) * 16;
+    const auto vswz = [](int row, int c) {
+        if constexpr (ES == 4) return c;
+        return c ^ (DP == 64 ? 4 * ((row >> 1) & 1) : DP == 128 ? 4 * (row & 3) : 0);
     };
 
     // slots of the block: [slot0, slot1) of all positions' G slots (SEG: of the segment's)
-    int64_t slot0, slot1, seg_lo = 0, seg_hi = 0;
+    int64_t slot0, slot1;
+    int32_t seg_lo = 0, seg_hi = 0;  // (positions and rows fit 32 bits)
     if (a.seg) {
         const int64_t p0 = clamp64(a.q_off[unit], 0, a.Pq), p1 = clamp64(a.q_off[unit + 1], 0, a.Pq);
         slot0 = p0 * a.G;
         slot1 = p1 * a.G;
-        seg_lo = clamp64(a.k_off[unit], 0, a.Pk);
-        seg_hi = clamp64(a.k_off[unit + 1], seg_lo, a.Pk);
+        seg_lo = (int32_t)clamp64(a.k_off[unit], 0, a.Pk);
+        seg_hi = (int32_t)clamp64(a.k_off[unit + 1], seg_lo, a.Pk);
     } else {
         slot0 = (int64_t)unit * (32 * NW * QT);
         slot1 = slot0 + 32 * NW * QT;
@@ -118,26 +158,27 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
 
     for (int64_t base = slot0; base < slot1; base += 32 * NW * QT) {
         // ---- the lane's slots
-        int64_t pos[QT], lo[QT], hi[QT], row[QT];
-        int32_t seg[QT];
-        int head[QT];
-        int64_t blo = a.Pk, bhi = 0;
+        int32_t pos[QT], lo[QT], hi[QT], row[QT], seg[QT], head[QT];
+        int32_t blo = (int32_t)a.Pk, bhi = 0;
+        const int64_t wfirst = base + wave * QT * 32;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int64_t slot = base + (wave * QT + t) * 32 + (lane & 31);
             const bool in = slot < slot1;
-            pos[t] = in ? slot / a.G : -1;
-            head[t] = hk * a.G + (in ? (int)(slot - pos[t] * a.G) : 0);
+            pos[t] = in ? (int32_t)(slot / a.G) : -1;
+            head[t] = hk * a.G + (in ? (int)(slot - (int64_t)pos[t] * a.G) : 0);
             row[t] = -1;
             seg[t] = -1;
             lo[t] = hi[t] = 0;
+            int32_t sg = (int32_t)unit;
+            if (!a.seg && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos[t] : 0x7ffffffe);
             if (in) {
-                int64_t r = a.q_index ? a.q_index[pos[t]] : pos[t];
+                const int32_t r = a.q_index ? a.q_index[pos[t]] : pos[t];
                 row[t] = r >= 0 && r < a.Mq ? r : -1;
-                seg[t] = a.seg ? (int32_t)unit : segment_of(a.q_off, a.S, pos[t]);
+                seg[t] = sg;
                 if (seg[t] >= 0) {
-                    lo[t] = a.seg ? seg_lo : clamp64(a.k_off[seg[t]], 0, a.Pk);
-                    hi[t] = a.seg ? seg_hi : clamp64(a.k_off[seg[t] + 1], lo[t], a.Pk);
+                    lo[t] = a.seg ? seg_lo : (int32_t)clamp64(a.k_off[seg[t]], 0, a.Pk);
+                    hi[t] = a.seg ? seg_hi : (int32_t)clamp64(a.k_off[seg[t] + 1], lo[t], a.Pk);
                     if (hi[t] > lo[t]) {
                         blo = lo[t] < blo ? lo[t] : blo;
                         bhi = hi[t] > bhi ? hi[t] : bhi;
@@ -147,11 +188,13 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
         }
         // the block's keys, and whether some lane sees only a part of them
         for (int o = 32; o > 0; o >>= 1) {
-            const int64_t x = __shfl_xor(blo, o, 64), y = __shfl_xor(bhi, o, 64);
+            const int32_t x = __shfl_xor(blo, o, 64), y = __shfl_xor(bhi, o, 64);
             blo = x < blo ? x : blo;
             bhi = y > bhi ? y : bhi;
         }
-        int64_t wlo = blo, whi = bhi;  // the wave's
+        blo = __builtin_amdgcn_readfirstlane(blo);
+        bhi = __builtin_amdgcn_readfirstlane(bhi);
+        const int32_t wlo = blo, whi = bhi;  // the wave's
         if constexpr (NW > 1) {
             __syncthreads();
             if (lane == 0) {
@@ -164,14 +207,31 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                 blo = s_r[0][w] < blo ? s_r[0][w] : blo;
                 bhi = s_r[1][w] > bhi ? s_r[1][w] : bhi;
             }
+            blo = __builtin_amdgcn_readfirstlane(blo);
+            bhi = __builtin_amdgcn_readfirstlane(bhi);
         }
+        // keys that every slot of the wave sees (slots of no segment take whatever comes)
+        int32_t ilo = 0, ihi = 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+            if (seg[t] >= 0) {
+                ilo = lo[t] > ilo ? lo[t] : ilo;
+                ihi = hi[t] < ihi ? hi[t] : ihi;
+            }
+        for (int o = 32; o > 0; o >>= 1) {
+            const int32_t x = __shfl_xor(ilo, o, 64), y = __shfl_xor(ihi, o, 64);
+            ilo = x > ilo ? x : ilo;
+            ihi = y < ihi ? y : ihi;
+        }
+        ilo = __builtin_amdgcn_readfirstlane(ilo);
+        ihi = __builtin_amdgcn_readfirstlane(ihi);
         bool part_seen = false;
 #pragma unroll
         for (int t = 0; t < QT; ++t) part_seen = part_seen || (seg[t] >= 0 && hi[t] > lo[t] && (lo[t] != blo || hi[t] != bhi));
         if (a.splits > 1 && bhi > blo) {
-            const int64_t each = ((bhi - blo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
-            blo = blo + split * each < bhi ? blo + split * each : bhi;
-            bhi = blo + each < bhi ? blo + each : bhi;
+            const int64_t each = (((int64_t)bhi - blo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+            blo = (int32_t)(blo + split * each < bhi ? blo + split * each : bhi);
+            bhi = (int32_t)(blo + each < bhi ? blo + each : bhi);
         }
 
         // ---- the queries, and their coordinates' operands
@@ -180,7 +240,7 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
         float sl[QT][3];
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const T* qp = (const T*)a.q + (row[t] >= 0 ? row[t] : 0) * a.q_row + head[t] * a.q_head;
+            const T* qp = (const T*)a.q + (int64_t)(row[t] >= 0 ? row[t] : 0) * a.q_row + head[t] * a.q_head;
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
                 const int cc = 2 * c + half;
@@ -192,7 +252,7 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                 // their weights, minus the weights times the query's parts; exact up to 2^24
 #pragma unroll
                 for (int x = 0; x < 3; ++x) {
-                    const int32_t c = row[t] >= 0 ? a.q_coords[row[t] * 4 + 1 + x] : 0;
+                    const int32_t c = row[t] >= 0 ? a.q_coords[(int64_t)row[t] * 4 + 1 + x] : 0;
                     sl[t][x] = -a.slopes[head[t] * 3 + x] * PMG_LOG2E;
                     const float p[4] = {(float)(c & 255), (float)((c >> 8) & 255), (float)((c >> 16) & 255), (float)(c >> 24)};
                     const float w[4] = {1.0f, 256.0f, 65536.0f, 16777216.0f};
@@ -207,69 +267,49 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
 
         int32_t only = -1;  // >= 0: the one segment this turn is for
         for (;;) {
-            int64_t klo = blo, khi = bhi;
+            int32_t klo = blo, khi = bhi;
             if (only >= 0) {
-                const int64_t l0 = clamp64(a.k_off[only], 0, a.Pk), h0 = clamp64(a.k_off[only + 1], l0, a.Pk);
+                const int32_t l0 = (int32_t)clamp64(a.k_off[only], 0, a.Pk), h0 = (int32_t)clamp64(a.k_off[only + 1], l0, a.Pk);
                 klo = l0 > blo ? l0 : blo;
                 khi = h0 < bhi ? h0 : bhi;
             }
-            const int64_t nt = khi > klo ? (khi - klo + BK - 1) / BK : 0;
+            const int32_t nt = khi > klo ? (khi - klo + (BK - 1)) / BK : 0;
 
             v16f O[QT][NB];
-            float m[QT], l[QT];
+            float m[QT], l[QT], grow[QT];
+            const float k2 = a.cap2 != 0.0f ? 1.0f : a.scale2;
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                m[t] = -__builtin_inff();
+                m[t] = 0.0f;
+                grow[t] = -__builtin_inff();
                 l[t] = 0.0f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) O[t][b] = v16f{};
             }
 
-            // ---- staging: row numbers two tiles ahead, data one tile ahead
-            int32_t idx[NCH], midx = -1;
-            chunk kr[NCH], vr[NCH];
-            bool okr[NCH];
+            // ---- the keys: row numbers three tiles ahead, mask and coordinates two, data one
+            const bool mt = tid < BK;  // a thread that looks after a key of each tile
+            int32_t mi = -1;           // its row in the tile whose mask and coordinates come next
+            const auto number = [&](int32_t t) -> int32_t {
+                if (!mt || t >= nt || tid >= khi - klo - t * BK) return -1;
+                const int32_t p = klo + t * BK + tid, r = a.k_index ? a.k_index[p] : p;
+                return r >= 0 && r < (int32_t)a.Mk ? r : -1;
+            };
             int4 mc = make_int4(0, 0, 0, 0);
-            bool mok = false;
-            const auto row_at = [&](int64_t p) -> int32_t {
-                if (p >= khi) return -1;
-                const int64_t r = a.k_index ? (int64_t)a.k_index[p] : p;
-                return r >= 0 && r < a.Mk ? (int32_t)r : -1;
+            uint8_t mm = 1;
+            const auto about = [&]() {  // of row mi
+                const int64_t r = mi >= 0 ? mi : 0;
+                if (a.k_mask) mm = a.k_mask[r];
+                if constexpr (BIAS) mc = *(const int4*)(a.k_coords + r * 4);
             };
-            const auto rows = [&](int64_t t) {
-#pragma unroll
-                for (int i = 0; i < NCH; ++i) idx[i] = row_at(klo + t * BK + (i * NT + tid) / CPR);
-                if (tid < BK) midx = row_at(klo + t * BK + tid);
-            };
-            const auto load = [&]() {
-#pragma unroll
-                for (int i = 0; i < NCH; ++i) {
-                    const int c = (i * NT + tid) % CPR;
-                    const int64_t r = idx[i] >= 0 ? idx[i] : 0;
-                    const int cc = c * PER < a.D ? c * PER : 0;
-                    okr[i] = idx[i] >= 0 && c * PER < a.D;
-                    kr[i] = *(const chunk*)((const T*)a.k + r * a.k_row + hk * a.k_head + cc);
-                    vr[i] = *(const chunk*)((const T*)a.v + r * a.v_row + hk * a.v_head + cc);
-                    if (a.k_mask) okr[i] = okr[i] && a.k_mask[r] != 0;
-                }
-                if (tid < BK) {
-                    const int64_t r = midx >= 0 ? midx : 0;
-                    mok = midx >= 0 && (!a.k_mask || a.k_mask[r] != 0);
-                    if constexpr (BIAS) mc = *(const int4*)(a.k_coords + r * 4);
-                }
-            };
-            const auto put = [&](int b) {
-#pragma unroll
-                for (int i = 0; i < NCH; ++i) {
-                    const int e = i * NT + tid, r = e / CPR, c = e % CPR;
-                    *(chunk*)(s_k[b] + r * DP * ES + 16 * kswz(r, c)) = okr[i] ? kr[i] : chunk{};
-                    *(chunk*)(s_v[b] + vadr(r, c)) = okr[i] ? vr[i] : chunk{};
-                }
+            const auto note = [&](int b, int32_t r) {
                 if (wave == 0) {
-                    const uint64_t w = __ballot(tid < BK && mok);
+                    const bool on = r >= 0 && mm != 0;
+                    const uint64_t w = __ballot(mt && on);
                     if (tid < KB) s_ok[b][tid] = (uint32_t)(w >> (32 * tid));
+                    if (mt) s_row[b][tid] = on ? r : -1;
                     if constexpr (BIAS) {
-                        if (tid < BK) {
+                        if (mt) {
                             const int32_t c[3] = {mc.y, mc.z, mc.w};
 #pragma unroll
                             for (int x = 0; x < 3; ++x) {
@@ -281,38 +321,81 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                     }
                 }
             };
+            // (rows are less than 2^31 bytes apart; a chunk behind the head's width is the line of zeros of every row)
+            const char *kb[NCH], *vb[NCH];
+            uint32_t ks[NCH], vs[NCH];
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int e = (i * NW + wave) * 64 + lane, r = e / CPR, p = e % CPR;
+                const int ck = kswz(r, p) * PER, cv = vswz(r, p) * PER;
+                kb[i] = ck < a.D ? (const char*)((const T*)a.k + hk * a.k_head + ck) : (const char*)&g_zeros;
+                vb[i] = cv < a.D ? (const char*)((const T*)a.v + hk * a.v_head + cv) : (const char*)&g_zeros;
+                ks[i] = ck < a.D ? (uint32_t)a.k_row * ES : 0u;
+                vs[i] = cv < a.D ? (uint32_t)a.v_row * ES : 0u;
+            }
+            const auto fetch = [&](int b, int nb) {  // the tile noted in slot nb, into buffer b
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const int32_t row = s_row[nb][((i * NW + wave) * 64 + lane) / CPR];
+                    const char* kp = row >= 0 ? kb[i] + (uint64_t)(uint32_t)row * ks[i] : (const char*)&g_zeros;
+                    const char* vp = row >= 0 ? vb[i] + (uint64_t)(uint32_t)row * vs[i] : (const char*)&g_zeros;
+                    typedef __attribute__((address_space(1))) const void* gp;
+                    typedef __attribute__((address_space(3))) void* lp;
+                    __builtin_amdgcn_global_load_lds((gp)kp, (lp)(s_k[b] + (i * NW + wave) * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((gp)vp, (lp)(s_v[b] + (i * NW + wave) * 1024), 16, 0, 0);
+                }
+            };
             if (nt > 0) {
-                rows(0);
-                load();
-                rows(1);
-                put(0);
+                mi = number(0);
+                about();
+                const int32_t m1 = number(1);
+                note(0, mi);
+                mi = m1;
+                about();
+                const int32_t m2 = number(2);
+                note(1, mi);
+                mi = m2;
+                __syncthreads();
+                fetch(0, 0);
             }
             __syncthreads();
 
-            for (int64_t it = 0; it < nt; ++it) {
-                const int cur = (int)(it & 1);
+            for (int32_t it = 0; it < nt; ++it) {
+                const int cur = it & 1;
                 const bool more = it + 1 < nt;
+                const int slot = it % 3, next_slot = (it + 1) % 3;
+                int32_t mn = -1;
                 if (more) {
-                    load();
-                    rows(it + 2);
+                    fetch(cur ^ 1, next_slot);
+                    about();
+                    mn = number(it + 3);
                 }
-                const int64_t p0 = klo + it * BK;
-                if (p0 < whi && p0 + BK > wlo) {
+                const int32_t p0 = klo + it * BK;
+                if (p0 < whi && wlo - p0 < BK) {
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
                         v16f s[KB];
-                        // ---- scores, in powers of two
+                        // ---- scores
 #pragma unroll
-                        for (int b = 0; b < KB; ++b) {
-                            s[b] = v16f{};
-                            const int kr_ = 32 * b + (lane & 31);
+                        for (int b = 0; b < KB; ++b) s[b] = v16f{};
+                        constexpr int QG = QC < 4 ? QC : 4;  // operand chunks at a time
 #pragma unroll
-                            for (int c = 0; c < QC; ++c) {
-                                const chunk kf = *(const chunk*)(s_k[cur] + kr_ * DP * ES + 16 * kswz(kr_, 2 * c + half));
-                                s[b] = Mat<T>::mma32(kf, qf[t][c], s[b]);
-                            }
+                        for (int c0 = 0; c0 < QC; c0 += QG) {
+                            chunk kf[KB][QG];
+#pragma unroll
+                            for (int c = 0; c < QG; ++c)
+#pragma unroll
+                                for (int b = 0; b < KB; ++b) {
+                                    const int kr_ = 32 * b + (lane & 31);
+                                    kf[b][c] = *(const chunk*)(s_k[cur] + kr_ * DP * ES + 16 * kswz(kr_, 2 * (c0 + c) + half));
+                                }
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int c = 0; c < QG; ++c)
+#pragma unroll
+                                for (int b = 0; b < KB; ++b) s[b] = Mat<T>::mma32(kf[b][c], qf[t][c0 + c], s[b]);
                         }
-                        float k2 = a.scale2;  // what s is still to be multiplied by
+                        // less the maximum so far, in powers of two
                         if (a.cap2 != 0.0f) {
 #pragma unroll
                             for (int b = 0; b < KB; ++b)
@@ -321,36 +404,41 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                                     if constexpr (ES == 4) s[b][e] = a.cap2 * tanhf(s[b][e] * a.cap_arg);
                                     else s[b][e] = __builtin_fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[b][e] * a.cap_arg)), a.cap2);
                                 }
-                            k2 = 1.0f;
                         }
                         if constexpr (BIAS) {
 #pragma unroll
                             for (int b = 0; b < KB; ++b) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) s[b][e] = s[b][e] * k2;
+                                v16f u;
 #pragma unroll
                                 for (int x = 0; x < 3; ++x) {
-                                    const uint2 kp = s_c[cur][x][32 * b + (lane & 31)];
+                                    const uint2 kp = s_c[slot][x][32 * b + (lane & 31)];
                                     // parts, then the weights 1, 2^8, 2^16, 2^24 in bf16
-                                    const v4i kc = half ? v4i{0, 0, 0, 0} : v4i{(int)kp.x, (int)kp.y, (int)0x43803f80u, (int)0x4b804780u};
+                                    // (both halves of the wave hold them: the query's are 0 in the upper one)
+                                    const v4i kc = v4i{(int)kp.x, (int)kp.y, (int)0x43803f80u, (int)0x4b804780u};
                                     const v16f d = Mat<__bf16>::mma32(__builtin_bit_cast(v8bf, kc), qc[t][x], v16f{});
 #pragma unroll
-                                    for (int e = 0; e < 16; ++e) s[b][e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[t][x], s[b][e]);
+                                    for (int e = 0; e < 16; ++e) u[e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[t][x], x == 0 ? -m[t] : u[e]);
                                 }
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) s[b][e] = __builtin_fmaf(s[b][e], k2, u[e]);
                             }
-                            k2 = 1.0f;
+                        } else {
+#pragma unroll
+                            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) s[b][e] = __builtin_fmaf(s[b][e], k2, -m[t]);
                         }
                         // ---- the keys that count for the lane's slot
-                        const int64_t rl = lo[t] - p0, rh = hi[t] - p0;
-                        const int jl = (int)(rl < 0 ? 0 : rl > BK ? BK : rl), jh = (int)(rh < 0 ? 0 : rh > BK ? BK : rh);
+                        const int jl = lo[t] - p0, jh = hi[t] - p0;
+                        const bool inside = p0 >= ilo && ihi - p0 >= BK;
 #pragma unroll
                         for (int b = 0; b < KB; ++b) {
-                            const int x = jl - 32 * b, y = jh - 32 * b;
-                            uint32_t w = y >= 32 ? 0xffffffffu : y <= 0 ? 0u : (1u << y) - 1u;
-                            w &= x <= 0 ? 0xffffffffu : x >= 32 ? 0u : ~((1u << x) - 1u);
-                            w &= s_ok[cur][b];
-                            if (!__all(w == 0xffffffffu)) {
-                                w >>= 4 * half;
+                            const uint32_t ok = __builtin_amdgcn_readfirstlane(s_ok[slot][b]);
+                            if (!inside || ok != 0xffffffffu) {
+                                const int x = jl - 32 * b, y = jh - 32 * b;
+                                uint32_t w = y >= 32 ? 0xffffffffu : y <= 0 ? 0u : (1u << y) - 1u;
+                                w &= x <= 0 ? 0xffffffffu : x >= 32 ? 0u : ~((1u << x) - 1u);
+                                w = (w & ok) >> (4 * half);
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) {
                                     const uint32_t on = (uint32_t)((int32_t)(w << (31 - ((e & 3) + 8 * (e >> 2)))) >> 31);
@@ -358,30 +446,57 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                                 }
                             }
                         }
-                        // ---- running maximum: moved only when it grows by more than 2^8 somewhere in the wave
+                        // ---- running maximum: set by the first keys, then moved only when it grows by more than
+                        // 2^8 for some slot of the wave (weights of up to 2^8 lose nothing)
                         float mx = s[0][0];
 #pragma unroll
                         for (int b = 0; b < KB; ++b)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[b][e]);
-                        mx = __builtin_fmaxf(mx, other_half(mx)) * k2;
-                        if (__any(mx > m[t] + 8.0f)) {
-                            const float mn = __builtin_fmaxf(m[t], mx);
-                            const float al = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
-                            m[t] = mn;
+                        mx = __builtin_fmaxf(mx, other_half(mx));
+                        if (__any(mx > grow[t])) {
+                            const bool any = mx > -__builtin_inff();  // (a slot without a key so far keeps m = 0)
+                            const float up = any && (mx > 0.0f || grow[t] < 0.0f) ? mx : 0.0f;
+                            const float al = __builtin_amdgcn_exp2f(-up);
+                            grow[t] = any ? 8.0f : grow[t];
+                            m[t] = m[t] + up;
                             l[t] = l[t] * al;
+#pragma unroll
+                            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) s[b][e] = s[b][e] - up;
 #pragma unroll
                             for (int b = 0; b < NB; ++b)
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) O[t][b][e] = O[t][b][e] * al;
                         }
-                        const float ms = m[t] == -__builtin_inff() ? 0.0f : m[t];
+                        // (the first operands of V are on their way while the exponentials are formed)
+                        chunk vf[2][NB];
+                        const auto values = [&](int b, int f) {
+                            typedef short v4s __attribute__((ext_vector_type(4)));
+                            typedef short v8s __attribute__((ext_vector_type(8)));
+                            typedef __attribute__((address_space(3))) v4s* lds4;
+#pragma unroll
+                            for (int n = 0; n < NB; ++n) {
+                                const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                                const int r0 = 32 * b + 16 * f + 4 * half + (i >> 2);
+                                const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + r0 * DP * 2 + 16 * vswz(r0, c) + (i & 1) * 8));
+                                const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + (r0 + 8) * DP * 2 + 16 * vswz(r0 + 8, c) + (i & 1) * 8));
+                                const v8s vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                                vf[f][n] = __builtin_bit_cast(chunk, vv);
+                            }
+                        };
+                        if constexpr (ES == 2) {
+                            values(0, 0);
+                            values(0, 1);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                         float sum = 0.0f;
 #pragma unroll
                         for (int b = 0; b < KB; ++b)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                s[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], k2, -ms));
+                                s[b][e] = __builtin_amdgcn_exp2f(s[b][e]);
                                 sum = sum + s[b][e];
                             }
                         l[t] = l[t] + sum;
@@ -405,26 +520,21 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
 #pragma unroll
                                     for (int i = 0; i < 8; ++i) pf[i] = (T)s[b][8 * f + i];
 #pragma unroll
-                                    for (int n = 0; n < NB; ++n) {
-                                        typedef short v4s __attribute__((ext_vector_type(4)));
-                                        typedef __attribute__((address_space(3))) v4s* lds4;
-                                        const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                                        const int r0 = 32 * b + 16 * f + 4 * half + (i >> 2);
-                                        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + vadr(r0, c) + (i & 1) * 8));
-                                        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + vadr(r0 + 8, c) + (i & 1) * 8));
-                                        typedef short v8s __attribute__((ext_vector_type(8)));
-                                        const v8s vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                                        O[t][n] = Mat<T>::mma32(__builtin_bit_cast(chunk, vv), pf, O[t][n]);
-                                    }
+                                    for (int n = 0; n < NB; ++n) O[t][n] = Mat<T>::mma32(vf[f][n], pf, O[t][n]);
+                                    if (b + 1 < KB) values(b + 1, f);
                                 }
                             }
                         }
                     }
                 }
-                if (more) put(cur ^ 1);
+                if (more) {
+                    note((it + 2) % 3, mi);
+                    mi = mn;
+                }
                 __syncthreads();
             }
 
+            const AttnArgs& a = args_again();
             // ---- values of other segments that are not finite: once more, segment by segment
             if (only < 0) {
                 float bad = 0.0f;
@@ -455,7 +565,7 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                 if (a.splits > 1) {
                     if (mine && seg[t] >= 0) {
                         const int64_t o = ((int64_t)split * a.Pq + pos[t]) * a.Hq + head[t];
-                        if (half == 0) a.part_ml[o] = make_float2(m[t], lt);
+                        if (half == 0) a.part_ml[o] = make_float2(grow[t] > 0.0f ? m[t] : -__builtin_inff(), lt);
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -467,7 +577,7 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
                 } else if (mine && row[t] >= 0 && (seg[t] >= 0 || a.zero_rest)) {
                     const bool none = lt == 0.0f || seg[t] < 0;  // no key left
                     const float inv = 1.0f / lt;
-                    T* op = (T*)a.out + row[t] * a.o_row + head[t] * a.o_head;
+                    T* op = (T*)a.out + (int64_t)row[t] * a.o_row + head[t] * a.o_head;
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -483,12 +593,12 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
             }
             if (only == -1) break;
             // the next segment of the block
-            int64_t next = (int64_t)1 << 40;
+            int32_t next = 0x7fffffff;
 #pragma unroll
             for (int t = 0; t < QT; ++t)
                 if (seg[t] >= 0 && seg[t] > only && seg[t] < next) next = seg[t];
             for (int o = 32; o > 0; o >>= 1) {
-                const int64_t x = __shfl_xor(next, o, 64);
+                const int32_t x = __shfl_xor(next, o, 64);
                 next = x < next ? x : next;
             }
             if constexpr (NW > 1) {
@@ -498,49 +608,62 @@ __global__ __launch_bounds__(64 * NW) void attention_k(AttnArgs a) {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) next = s_r[2][w] < next ? s_r[2][w] : next;
             }
-            if (next == (int64_t)1 << 40) break;
-            only = (int32_t)next;
+            if (next == 0x7fffffff) break;
+            only = __builtin_amdgcn_readfirstlane(next);
         }
     }
 }
 
-// Joins the splits: a wave a (position, head).
-template <class T>
+// Joins the splits: a wave a (position, head). Its lanes are G groups of 16 or 32, each on every G-th split and 4 columns a
+// lane; the groups' sums are added in order at the end.
+template <class T, int CL>
 __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
+    constexpr int G = 64 / CL;
+    const int lane = threadIdx.x & 63, g = lane / CL, d = 4 * (lane % CL);
     const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (item >= a.Pq * a.Hq) return;
     const int64_t pos = item / a.Hq;
     const int head = (int)(item - pos * a.Hq);
-    const int64_t r = a.q_index ? a.q_index[pos] : pos;
-    if (r < 0 || r >= a.Mq) return;
-    T* op = (T*)a.out + r * a.o_row + head * a.o_head;
-    if (segment_of(a.q_off, a.S, pos) < 0) {
-        if (a.zero_rest)
-            for (int d = lane; d < a.D; d += 64) op[d] = (T)0.0f;
+    const int32_t r = a.q_index ? a.q_index[pos] : (int32_t)pos;
+    const bool in = segment_of(a.q_off, a.S, pos) >= 0;
+    if (r < 0 || r >= a.Mq || (!in && !a.zero_rest)) return;
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    v4t* op = (v4t*)((T*)a.out + (int64_t)r * a.o_row + head * a.o_head + d);
+    const bool mine = g == 0 && d < a.D;
+    if (!in) {
+        if (mine) *op = v4t{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
         return;
     }
     const int64_t step = a.Pq * a.Hq;
     float m = -__builtin_inff();
-    for (int s = lane; s < a.splits; s += 64) {
-        const float2 ml = a.part_ml[item + s * step];
-        m = __builtin_fmaxf(m, ml.x);
-    }
+    for (int s = lane; s < a.splits; s += 64) m = __builtin_fmaxf(m, a.part_ml[item + s * step].x);
     for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
     const float ms = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {  // in the splits' order
+    float l = 0.0f;
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = g; s < a.splits; s += G) {
         const float2 ml = a.part_ml[item + s * step];
+        const v4f po = d < a.D ? *(const v4f*)(a.part_o + (item + s * step) * a.D + d) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
         const float w = __builtin_amdgcn_exp2f(ml.x - ms);
-        if (ml.y == 0.0f) continue;  // a part without keys
-        l = __builtin_fmaf(ml.y, w, l);
-        const float* po = a.part_o + (item + s * step) * a.D;
-        if (lane < a.D) o0 = __builtin_fmaf(po[lane], w, o0);
-        if (lane + 64 < a.D) o1 = __builtin_fmaf(po[lane + 64], w, o1);
+        if (ml.y != 0.0f) {  // (a part without keys counts for nothing)
+            l = __builtin_fmaf(ml.y, w, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(po[i], w, acc[i]);
+        }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (lane < a.D) op[lane] = (T)(l == 0.0f ? 0.0f : o0 * inv);
-    if (lane + 64 < a.D) op[lane + 64] = (T)(l == 0.0f ? 0.0f : o1 * inv);
+#pragma unroll
+    for (int o = CL; o < 64; o <<= 1) {
+        l = l + __shfl_xor(l, o, 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = acc[i] + __shfl_xor(acc[i], o, 64);
+    }
+    if (!mine) return;
+    const float inv = 1.0f / l;
+    v4t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (T)(l == 0.0f ? 0.0f : acc[i] * inv);
+    *op = v;
 }
 
 // The rows outside every segment, where blocks go by segment.
@@ -576,7 +699,9 @@ int launch_attention_t(AttnArgs& a, int waves, hipStream_t s) {
     int e = a.D <= 32 ? launch_attention_d<T, 32>(a, waves, s) : a.D <= 64 ? launch_attention_d<T, 64>(a, waves, s) : launch_attention_d<T, 128>(a, waves, s);
     if (e) return e;
     if (a.splits > 1) {
-        hipLaunchKernelGGL((attention_join_k<T>), dim3((unsigned)((a.Pq * a.Hq + 3) / 4)), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)((a.Pq * a.Hq + 3) / 4));
+        if (a.D <= 64) hipLaunchKernelGGL((attention_join_k<T, 16>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attention_join_k<T, 32>), grid, dim3(256), 0, s, a);
         return check_launch("attention_join_k");
     }
     if (a.seg && a.zero_rest) {

@@ -10,6 +10,10 @@ struct Plan {
 };
 
 // The forms, by the mean lengths (the offsets are on the device).
+//   A block per segment where the queries of a segment fill no half wave and its keys are many; else tiles of positions,
+//   of one wave where segments are short (a tile of four would walk over the keys of several) and four where not.
+//   Keys are split over blocks where the blocks would not fill the card, or would fill it unevenly: rounds of resident
+//   blocks against what writing and joining the parts costs.
 Plan plan_of(const pmg_attention_args& r) {
     Plan p{0, 4, 1};
     if (r.segments < 1) return p;
@@ -18,11 +22,20 @@ Plan plan_of(const pmg_attention_args& r) {
     p.seg = nq * (double)G <= 16.0 && nk >= 128.0;
     p.waves = p.seg || nk < 512.0 ? 1 : 4;
     const int64_t units = p.seg ? r.segments : (r.q_positions * G + 32 * p.waves - 1) / (32 * p.waves);
-    const int64_t waves = units * r.Hk * p.waves;
-    int64_t s = waves > 0 ? 2048 / waves : 1;
-    const int64_t most = (int64_t)(nk / 256.0);
-    s = s < most ? s : most;
-    p.splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    const int64_t blocks = units * r.Hk, resident = p.waves == 1 ? 2048 : 512;
+    // microseconds: a tile of 64 keys takes a resident block about 1.9 (four waves) or 2.5 (one) at D = 64
+    const double round = nk / 64.0 * (p.waves == 1 ? 2.5 : 1.9) * (r.D <= 32 ? 0.7 : r.D <= 64 ? 1.0 : 1.8) * (r.type == PMG_TYPE_F32 ? 4.0 : 1.0);
+    const double part = (double)r.q_positions * (double)r.Hq * (double)r.D * 8.0 / 4.0e6;
+    const int most = nk >= 512.0 ? (int)(nk / 256.0 < 64.0 ? nk / 256.0 : 64.0) : 1;
+    double best = 0.0;
+    for (int s = 1; s <= most; ++s) {
+        const double rounds = (double)((blocks * s + resident - 1) / resident);
+        const double t = rounds / s * round + (s > 1 ? 4.0 + s * part : 0.0);
+        if (s == 1 || t < 0.97 * best) {
+            best = t;
+            p.splits = s;
+        }
+    }
     return p;
 }
 
@@ -63,6 +76,7 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     };
     const int per = 16 / es;
     PMG_REQUIRE(ok(r.q, r.q_row, r.q_head, per) && ok(r.k, r.k_row, r.k_head, per) && ok(r.v, r.v_row, r.v_head, per), "q, k, v: buffers and strides in whole 16 bytes");
+    PMG_REQUIRE(r.k_row >= 0 && r.v_row >= 0 && r.k_row < ((int64_t)1 << 31) / es && r.v_row < ((int64_t)1 << 31) / es, "k, v: rows further than 2 GiB apart");
     PMG_REQUIRE(ok(r.out, r.out_row, r.out_head, 4), "out: buffer and strides in whole groups of 4 elements");
     PMG_REQUIRE(!r.slopes || (aligned16(r.q_coords) && aligned16(r.k_coords)), "coordinates must be 16-byte aligned");
     const Plan pl = plan_of(r);

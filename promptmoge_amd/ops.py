@@ -11,7 +11,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import EPI_ACC, EPI_BIAS, EPI_Q, EPI_QLIN, EPI_R, EPI_RLN, EPI_ROUT, EPI_SILU, ConvEpilogue, call, lib
+from ._lib import EPI_ACC, EPI_BIAS, EPI_Q, EPI_QLIN, EPI_R, EPI_RLN, EPI_ROUT, EPI_SILU, ConvEpilogue, call, check, lib
 
 __all__ = [
     "voxelize", "nmap_column", "nmap_hash", "row_order", "nmap_from_rows", "kmap_compact", "spconv_i8",
@@ -579,51 +579,72 @@ def gauge_poly(depth: torch.Tensor, lidar: torch.Tensor, conf: Optional[torch.Te
 
 
 # ---------------------------------------------------------------------------------- (5) dense operators around the maps
+# (These calls last a few microseconds: the checks below are written so that a valid call passes each in one step.)
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16,
           torch.int8: _lib.TYPE_I8}
 
 
-def _inputs(*named: Tuple[str, Optional[torch.Tensor]]) -> torch.device:
-    """The one device of the given tensors (None: absent); refuses host tensors and tensors that need gradients."""
+def _refuse(**named: Optional[torch.Tensor]) -> None:
+    """Says which of the tensors (None: absent) is not on the first one's GPU or needs a gradient."""
     dev = None
-    for name, t in named:
+    for name, t in named.items():
         if t is None:
             continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"{name} must be a GPU tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        dev = t.device if dev is None else dev
+        if t.device != dev:
             raise ValueError(f"{name} is on {t.device}, the other tensors on {dev}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the libpmg operators are inference-only; run under torch.no_grad()")
-    return dev
 
 
-def _on(dev: torch.device, name: str, *args) -> None:
-    """call() on the tensors' own device (the current one or not), on that device's current stream."""
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, _stream())
+def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
+    """The index of the one GPU that all the tensors (None: absent) are on; -1 if there is none, or one needs a gradient."""
+    grad = torch.is_grad_enabled()
+    d = -1
+    for t in tensors:
+        if t is not None:
+            if not isinstance(t, torch.Tensor) or (grad and t.requires_grad):
+                return -1
+            i = t.get_device()
+            if i != d:
+                if d >= 0:
+                    return -1
+                d = i
+    return d
+
+
+def _on(d: int, name: str, *args) -> None:
+    """call() on GPU d (the current one or not), on its current stream."""
+    if d == torch.cuda.current_device():
+        check(getattr(lib(), name)(*args, torch.cuda.current_stream(d).cuda_stream))
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, _stream())
+        with torch.cuda.device(d):
+            check(getattr(lib(), name)(*args, torch.cuda.current_stream(d).cuda_stream))
 
 
 def _floating(t: torch.Tensor, name: str) -> int:
-    if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    ty = _TYPES.get(t.dtype, _lib.TYPE_I8)
+    if ty == _lib.TYPE_I8:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    return _TYPES[t.dtype]
+    return ty
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor, name: str) -> int:
     """The row stride of an (M, C) tensor whose rows are contiguous and do not overlap."""
     if t.ndim != 2:
         raise ValueError(f"{name} must be 2-D, got {tuple(t.shape)}")
-    if t.shape[0] <= 1 and (t.shape[1] <= 1 or t.stride(1) == 1):
-        return max(t.shape[1], 1)
-    if (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
-    return t.stride(0)
+    (M, width), (row, one) = t.shape, t.stride()
+    if (one == 1 or width <= 1) and row >= width:
+        return max(row, 1)
+    if M <= 1 and (one == 1 or width <= 1):
+        return max(width, 1)
+    raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -636,28 +657,31 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
-    dev = _inputs(("x", x), ("w", w), ("bias", bias), ("w_scale", w_scale), ("residual", residual), ("out", out))
-    if w.ndim != 2 or not w.is_contiguous():
-        raise ValueError("w must be a contiguous (N, K) matrix")
-    if w.dtype != x.dtype:
-        raise ValueError(f"w must be {x.dtype}, got {w.dtype}")
+    d = _one_gpu(x, w, bias, w_scale, residual, out)
+    if d < 0:
+        _refuse(x=x, w=w, bias=bias, w_scale=w_scale, residual=residual, out=out)
     ldx = _rows(x, "x")
     M, K = x.shape
-    N = w.shape[0]
-    if w.shape[1] != K:
-        raise ValueError(f"w expects {w.shape[1]} input channels, x has {K}")
-    for name, t in (("bias", bias), ("w_scale", w_scale)):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (N,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 ({N},) vector")
-    if act not in _lib.ACTS:
+    if w.dtype != x.dtype:
+        raise ValueError(f"w must be {x.dtype}, got {w.dtype}")
+    if w.ndim != 2 or not w.is_contiguous():
+        raise ValueError("w must be a contiguous (N, K) matrix")
+    N, kw = w.shape
+    if kw != K:
+        raise ValueError(f"w expects {kw} input channels, x has {K}")
+    _vector(bias, "bias", N)
+    _vector(w_scale, "w_scale", N)
+    code = _lib.ACTS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(_lib.ACTS)}, got {act!r}")
-    rt, ldr = 0, 0
+    rt = ldr = 0
     if residual is not None:
         rt, ldr = _floating(residual, "residual"), _rows(residual, "residual")
         if residual.shape != (M, N):
             raise ValueError(f"residual must be ({M}, {N}), got {tuple(residual.shape)}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        ldo = N
     else:
         if out.shape != (M, N):
             raise ValueError(f"out must be ({M}, {N}), got {tuple(out.shape)}")
@@ -667,9 +691,10 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
                 out.data_ptr() == residual.data_ptr() and out.dtype == residual.dtype
                 and out.stride() == residual.stride()):
             raise ValueError("out may be residual itself, but not overlap it otherwise")
-    args = _lib.LinearArgs(_TYPES[x.dtype], _p(x), ldx, _p(w), M, K, N, a_scale, _p(w_scale), _p(bias),
-                           _lib.ACTS[act], _p(residual), rt, ldr, _p(out), _floating(out, "out"), _rows(out, "out"))
-    _on(dev, "pmg_linear", C.byref(args))
+        ldo = _rows(out, "out")
+    args = _lib.LINEAR_PACK.pack(_TYPES[x.dtype], x.data_ptr(), ldx, w.data_ptr(), M, K, N, a_scale, _ptr(w_scale),
+                                 _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), _floating(out, "out"), ldo)
+    _on(d, "pmg_linear", args)
     return out
 
 
@@ -680,7 +705,6 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     follows it. x: (M, K) fp32 / fp16 / bf16 (rows may be strided); w: (N, K) of x's type; bias: (N,) fp32; act: "none",
     "relu", "silu", "gelu" (erf) or "gelu_tanh"; residual: (M, N) of any of the three types. Sums in fp32, rounded
     once to out_dtype (default: x's). `out` may be the residual itself. Forward only."""
-    _inputs(("x", x), ("w", w))
     _floating(x, "x")
     return _linear(x, w, bias, 1.0, None, act, residual, out_dtype or (x.dtype if out is None else out.dtype), out)
 
@@ -690,7 +714,6 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = N
               out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """linear on int8 codes: act((acc * a_scale) * w_scale[n] + bias) + residual with the exact int32 sums acc, the
     arithmetic of spconv_i8. x: (M, K) int8; w: (N, K) int8; w_scale, bias: (N,) fp32; result fp32, fp16 or bf16."""
-    _inputs(("x", x), ("w", w))
     if x.dtype != torch.int8:
         raise ValueError(f"x must be torch.int8, got {x.dtype}")
     return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype, out)
@@ -700,8 +723,8 @@ def _heads(t: torch.Tensor, name: str, unit: int) -> torch.Tensor:
     """An (M, H, D) tensor whose heads are contiguous, on `unit` bytes; copied where its strides or address are not."""
     if t.ndim != 3:
         raise ValueError(f"{name} must be (rows, heads, width), got {tuple(t.shape)}")
-    e = t.element_size()
-    if t.stride(2) != 1 or t.data_ptr() % unit or t.stride(0) * e % unit or t.stride(1) * e % unit:
+    row, head, one = t.stride()
+    if one != 1 or (t.data_ptr() | row * t.element_size() | head * t.element_size()) & (unit - 1):
         t = t.contiguous()
     return t
 
@@ -729,9 +752,11 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     (b, x, y, z); freqs: (P, 3) fp32, P <= D / 2: pair p is turned by the angle x f[p, 0] + y f[p, 1] + z f[p, 2], formed in 64
     bits. Pair p is (p, p + D/2), or with interleaved (2p, 2p + 1). Returns (q, k) in new tensors, or in `out` (which
     may be the inputs). Forward only."""
-    dev = _inputs(("q", q), ("k", k), ("coords", coords), ("freqs", freqs), ("q_weight", q_weight),
-                  ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias),
-                  ("out[0]", out[0] if out else None), ("out[1]", out[1] if out else None))
+    qo, ko = out if out is not None else (None, None)
+    d = _one_gpu(q, k, coords, freqs, q_weight, k_weight, q_bias, k_bias, qo, ko)
+    if d < 0:
+        _refuse(q=q, k=k, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias,
+                out_q=qo, out_k=ko)
     ty = _floating(q, "q")
     unit = 4 * q.element_size()
     if norm not in ("rms", "layer"):
@@ -747,10 +772,10 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
         _vector(t, name, D)
     if out is None:
-        qo = torch.empty((M, Hq, D), dtype=q.dtype, device=dev)
-        ko = torch.empty((M, k.shape[1], D), dtype=q.dtype, device=dev) if k is not None else None
+        qo = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
+        if k is not None:
+            ko = torch.empty((M, k.shape[1], D), dtype=q.dtype, device=q.device)
     else:
-        qo, ko = out
         for name, t, o in (("out[0]", q, qo), ("out[1]", k, ko)):
             if (t is None) != (o is None) or (t is not None and (o.shape != t.shape or o.dtype != q.dtype)):
                 raise ValueError(f"{name} must match its input")
@@ -764,12 +789,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
             raise ValueError("out[0] and out[1] must not overlap")
     q = _heads(q, "q", unit)
     k = _heads(k, "k", unit) if k is not None else None
-    args = _lib.RopeArgs(ty, M, Hq, k.shape[1] if k is not None else 0, D, freqs.shape[0], _p(q), q.stride(0),
-                         q.stride(1), _p(k), k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0,
-                         _p(qo), qo.stride(0), qo.stride(1), _p(ko), ko.stride(0) if ko is not None else 0,
-                         ko.stride(1) if ko is not None else 0, _p(coords), _p(freqs), _p(q_weight), _p(k_weight),
-                         _p(q_bias), _p(k_bias), norm == "layer", bool(interleaved), float(eps))
-    _on(dev, "pmg_qk_norm_rope", C.byref(args))
+    Hk, (ks, kh), (kos, koh) = 0, (0, 0), (0, 0)
+    if k is not None:
+        Hk, (ks, kh, _), (kos, koh, _) = k.shape[1], k.stride(), ko.stride()
+    (qs, qh, _), (qos, qoh, _) = q.stride(), qo.stride()
+    args = _lib.ROPE_PACK.pack(ty, M, Hq, Hk, D, freqs.shape[0], q.data_ptr(), qs, qh, _ptr(k), ks, kh, qo.data_ptr(),
+                               qos, qoh, _ptr(ko), kos, koh, coords.data_ptr(), freqs.data_ptr(), _ptr(q_weight),
+                               _ptr(k_weight), _ptr(q_bias), _ptr(k_bias), norm == "layer", bool(interleaved), eps)
+    _on(d, "pmg_qk_norm_rope", args)
     return qo, ko
 
 
@@ -796,9 +823,10 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Rows outside every segment are 0 in a new result and left as they were in a given `out`. Every row should be named
     by at most one query position. Forward only."""
-    dev = _inputs(("q", q), ("k", k), ("v", v), ("offsets", offsets), ("kv_offsets", kv_offsets), ("index", index),
-                  ("kv_index", kv_index), ("coords", coords), ("kv_coords", kv_coords), ("slopes", slopes),
-                  ("kv_mask", kv_mask), ("out", out))
+    d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
+    if d < 0:
+        _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
+                kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask, out=out)
     ty = _floating(q, "q")
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"q must be (Mq, Hq, D), k and v (Mk, Hk, D); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -836,7 +864,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     fresh = out is None
     if fresh:
         whole = index is None or index.numel() == Mq
-        out = (torch.empty if whole else torch.zeros)((Mq, Hq, D), dtype=q.dtype, device=dev)
+        out = (torch.empty if whole else torch.zeros)((Mq, Hq, D), dtype=q.dtype, device=q.device)
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
@@ -845,13 +873,14 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
             raise ValueError("out must not overlap q, k or v")
     q, k, v = _heads(q, "q", 16), _heads(k, "k", 16), _heads(v, "v", 16)
-    args = _lib.AttentionArgs(
-        ty, Hq, Hk, D, _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
-        v.stride(1), _p(out), out.stride(0), out.stride(1), Mq, Mk, Mq if index is None else index.numel(),
-        Mk if kv_index is None else kv_index.numel(), offsets.numel() - 1, _p(offsets), _p(kv_offsets), _p(index),
-        _p(kv_index), _p(coords) if slopes is not None else None, _p(kv_coords) if slopes is not None else None,
-        _p(slopes), _p(kv_mask), D ** -0.5 if scale is None else float(scale), float(cap), fresh)
-    ws_bytes = lib().pmg_attention_workspace_bytes(C.byref(args))
-    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
-    _on(dev, "pmg_attention", C.byref(args), _p(ws), ws_bytes)
+    (qs, qh, _), (ks, kh, _), (vs, vh, _), (os, oh, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    args = _lib.ATTENTION_PACK.pack(
+        ty, Hq, Hk, D, q.data_ptr(), qs, qh, k.data_ptr(), ks, kh, v.data_ptr(), vs, vh, out.data_ptr(), os, oh, Mq, Mk,
+        Mq if index is None else index.shape[0], Mk if kv_index is None else kv_index.shape[0], offsets.shape[0] - 1,
+        offsets.data_ptr(), kv_offsets.data_ptr(), _ptr(index), _ptr(kv_index), _ptr(coords) if slopes is not None else 0,
+        _ptr(kv_coords) if slopes is not None else 0, _ptr(slopes), _ptr(kv_mask), D ** -0.5 if scale is None else scale,
+        cap, fresh)
+    ws_bytes = lib().pmg_attention_workspace_bytes(args)
+    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _on(d, "pmg_attention", args, _ptr(ws), ws_bytes)
     return out
