@@ -11,7 +11,7 @@
 // row-major V by the transposing LDS read (fp32: by plain reads). K and V tiles go from memory straight to LDS, one tile
 // ahead into the other of two buffers: each lane names the 16 bytes it fetches, so rows are gathered by index, the
 // banks' swizzle is made by the choice of chunk, and an absent row (masked, behind its segment, a bad index) is fetched
-// from a line of zeros. The rows' numbers, mask and coordinates run two and three tiles ahead.
+// from a line of zeros. The rows' numbers, mask and coordinates are looked up a key a thread, a group of tiles ahead.
 //
 // Queries are taken in order of position, 32 NW QT / G positions a block, whatever segments they fall in: the block
 // walks over the keys of all its segments, and each lane counts the keys of its own. No work list is needed, and small
@@ -45,7 +45,7 @@ struct AttnArgs {
     float cap2, cap_arg;  // cap log2(e); the factor of tanh's argument (0 cap: none)
     int seg, splits, zero_rest;
     uint32_t blocks;
-    float* part_o;  // [splits][Pq][Hq][D]
+    float* part_o;  // [splits][Hq][Pq][D]; (m, l) [splits][Hq][Pq], l < 0: a position of no segment
     float2* part_ml;
 };
 
@@ -89,52 +89,86 @@ __device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t fi
 // What absent keys and values are fetched from.
 __device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};
 
-// The other half's value (lane l <-> l ^ 32).
-__device__ inline float other_half(float v) {
-    const uint32_t u = f2u(v);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return u2f((threadIdx.x & 32) ? r[0] : r[1]);
+// Maximum / sum over lanes l and l ^ 32.
+__device__ inline float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    return __builtin_fmaxf(u2f(r[0]), u2f(r[1]));
+}
+__device__ inline float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    return u2f(r[0]) + u2f(r[1]);
+}
+// Minimum / maximum over the wave, the same in every lane: rotations within rows of 16 lanes, then across the rows.
+template <bool MAX>
+__device__ inline int32_t wave_extreme(int32_t v) {
+    const auto f = [](int32_t x, int32_t y) { return (MAX ? x > y : x < y) ? x : y; };
+    v = f(v, (int32_t)dpp_u32<0x128, 0xf>((uint32_t)v));
+    v = f(v, (int32_t)dpp_u32<0x124, 0xf>((uint32_t)v));
+    v = f(v, (int32_t)dpp_u32<0x122, 0xf>((uint32_t)v));
+    v = f(v, (int32_t)dpp_u32<0x121, 0xf>((uint32_t)v));
+    const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = f((int32_t)a[0], (int32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = f((int32_t)b[0], (int32_t)b[1]);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The thread's number, hidden from the compiler: what is derived from it is formed where it is used, not kept in registers
+// through the loop over the keys.
+__device__ inline int thread_again() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
 }
 
 // The kernel's arguments, read anew from here on (kept in scalar registers through the loop over the keys they would be
 // spilled to vector registers, lane by lane).
-__device__ inline const AttnArgs& args_again() {
+typedef const __attribute__((address_space(4))) AttnArgs ConstArgs;
+__device__ inline ConstArgs& args_again() {
     auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(p));
-    return *(const AttnArgs*)p;
+    return *(ConstArgs*)p;
+}
+
+// Waves a SIMD the registers are kept to (what the LDS of a block allows, too).
+constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
+    if (NW == 1) return DP == 128 ? 1 : 2;
+    if (ES == 4) return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - BIAS;
+    return DP == 32 ? 4 : DP == 64 ? 4 - BIAS : 2;
 }
 
 // Registers: with at most 256 the matrix instructions' results stay in ordinary vector registers, where the softmax
 // works on them; only the widest fp32 form of one wave needs more.
 template <class T, int DP, int NW, int QT, bool BIAS>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1 : 2) void attention_k(AttnArgs a0) {
+__global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void attention_k(AttnArgs a0) {
     const AttnArgs& a = a0;
     constexpr int ES = sizeof(T), PER = 16 / ES, CPR = DP / PER, NT = 64 * NW;
-    constexpr int BK = (NW == 1 || ES == 4) ? 32 : 64, KB = BK / 32;
+    constexpr int BK = (NW == 1 || ES == 4 || DP == 128) ? 32 : 64, KB = BK / 32;
     constexpr int NCH = BK * CPR / NT;         // 16-byte chunks of K (and of V) a thread stages
     constexpr int NB = DP / 32;                // 32-column blocks of O
+    constexpr bool SEG = NW == 1;               // a block per segment
     constexpr int QC = CPR / 2;                // operand chunks of a query a lane holds
     typedef typename Mat<T>::chunk chunk;
     static_assert(NCH * NT == BK * CPR, "whole chunks");
     __shared__ __attribute__((aligned(16))) char s_k[2][BK * DP * ES];
     __shared__ __attribute__((aligned(16))) char s_v[2][BK * DP * ES];
-    __shared__ uint32_t s_ok[3][KB];  // which keys there are
-    __shared__ int32_t s_row[3][BK];
-    __shared__ __attribute__((aligned(16))) uint2 s_c[3][BIAS ? 3 : 1][BIAS ? BK : 1];
+    constexpr int SB = NT, TPS = SB / BK;  // keys (and tiles) whose numbers are looked up at a time, one a thread
+    __shared__ uint32_t s_ok[2][SB / 32];  // which keys there are
+    __shared__ int32_t s_row[2][SB];
+    __shared__ __attribute__((aligned(16))) uint4 s_xy[2 * (BIAS ? SB : 1) + 1];  // coordinates; their parts' weights
+    __shared__ __attribute__((aligned(16))) uint2 s_z[2 * (BIAS ? SB : 1) + 1];
+    static_assert(TPS >= 2, "a group's numbers are written while its predecessor's first tile is worked on");
     __shared__ int32_t s_r[3][NW];
     __shared__ int s_flag[NW];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // block -> (split, key head, tile or segment): an XCD's blocks are neighbours, on one head's keys
     const uint32_t id = xcd_tile(blockIdx.x, a.blocks);
     const uint32_t per_head = a.blocks / (uint32_t)(a.Hk * a.splits);
     const uint32_t unit = id % per_head;
     const int hk = (int)(id / per_head) % a.Hk, split = (int)(id / per_head) / a.Hk;
 
-    const auto kswz = [](int row, int c) {
-        if constexpr (CPR >= 8) return c ^ ((row ^ (row >> 3)) & 7);
-        else return c ^ (((row >> 1) ^ (row >> 3)) & 3);
-    };
+    const auto kswz = [](int row, int c) { return swizzle<CPR>(row, c); };
     // V: 32-byte units of a row, so that the four rows of a transposing read lie in different banks
     const auto vswz = [](int row, int c) {
         if constexpr (ES == 4) return c;
@@ -144,7 +178,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
     // slots of the block: [slot0, slot1) of all positions' G slots (SEG: of the segment's)
     int64_t slot0, slot1;
     int32_t seg_lo = 0, seg_hi = 0;  // (positions and rows fit 32 bits)
-    if (a.seg) {
+    if constexpr (SEG) {
         const int64_t p0 = clamp64(a.q_off[unit], 0, a.Pq), p1 = clamp64(a.q_off[unit + 1], 0, a.Pq);
         slot0 = p0 * a.G;
         slot1 = p1 * a.G;
@@ -156,8 +190,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
         if (slot1 > a.Pq * a.G) slot1 = a.Pq * a.G;
     }
 
-    for (int64_t base = slot0; base < slot1; base += 32 * NW * QT) {
+    for (int64_t base = slot0; base < slot1; base += SEG ? 32 * NW * QT : (int64_t)1 << 40) {
         // ---- the lane's slots
+        const int tid = thread_again(), lane = tid & 63, half = lane >> 5;
         int32_t pos[QT], lo[QT], hi[QT], row[QT], seg[QT], head[QT];
         int32_t blo = (int32_t)a.Pk, bhi = 0;
         const int64_t wfirst = base + wave * QT * 32;
@@ -171,14 +206,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
             seg[t] = -1;
             lo[t] = hi[t] = 0;
             int32_t sg = (int32_t)unit;
-            if (!a.seg && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos[t] : 0x7ffffffe);
+            if (!SEG && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos[t] : 0x7ffffffe);
             if (in) {
                 const int32_t r = a.q_index ? a.q_index[pos[t]] : pos[t];
                 row[t] = r >= 0 && r < a.Mq ? r : -1;
                 seg[t] = sg;
                 if (seg[t] >= 0) {
-                    lo[t] = a.seg ? seg_lo : (int32_t)clamp64(a.k_off[seg[t]], 0, a.Pk);
-                    hi[t] = a.seg ? seg_hi : (int32_t)clamp64(a.k_off[seg[t] + 1], lo[t], a.Pk);
+                    lo[t] = SEG ? seg_lo : (int32_t)clamp64(a.k_off[seg[t]], 0, a.Pk);
+                    hi[t] = SEG ? seg_hi : (int32_t)clamp64(a.k_off[seg[t] + 1], lo[t], a.Pk);
                     if (hi[t] > lo[t]) {
                         blo = lo[t] < blo ? lo[t] : blo;
                         bhi = hi[t] > bhi ? hi[t] : bhi;
@@ -187,13 +222,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
             }
         }
         // the block's keys, and whether some lane sees only a part of them
-        for (int o = 32; o > 0; o >>= 1) {
-            const int32_t x = __shfl_xor(blo, o, 64), y = __shfl_xor(bhi, o, 64);
-            blo = x < blo ? x : blo;
-            bhi = y > bhi ? y : bhi;
-        }
-        blo = __builtin_amdgcn_readfirstlane(blo);
-        bhi = __builtin_amdgcn_readfirstlane(bhi);
+        blo = wave_extreme<false>(blo);
+        bhi = wave_extreme<true>(bhi);
         const int32_t wlo = blo, whi = bhi;  // the wave's
         if constexpr (NW > 1) {
             __syncthreads();
@@ -218,13 +248,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
                 ilo = lo[t] > ilo ? lo[t] : ilo;
                 ihi = hi[t] < ihi ? hi[t] : ihi;
             }
-        for (int o = 32; o > 0; o >>= 1) {
-            const int32_t x = __shfl_xor(ilo, o, 64), y = __shfl_xor(ihi, o, 64);
-            ilo = x > ilo ? x : ilo;
-            ihi = y < ihi ? y : ihi;
-        }
-        ilo = __builtin_amdgcn_readfirstlane(ilo);
-        ihi = __builtin_amdgcn_readfirstlane(ihi);
+        ilo = wave_extreme<true>(ilo);
+        ihi = wave_extreme<false>(ihi);
         bool part_seen = false;
 #pragma unroll
         for (int t = 0; t < QT; ++t) part_seen = part_seen || (seg[t] >= 0 && hi[t] > lo[t] && (lo[t] != blo || hi[t] != bhi));
@@ -248,8 +273,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
                 if (row[t] >= 0 && cc * PER < a.D) qf[t][c] = *(const chunk*)(qp + cc * PER);
             }
             if constexpr (BIAS) {
-                // the difference of two coordinates as a product: key parts (8 bits each, exact in bf16) times
-                // their weights, minus the weights times the query's parts; exact up to 2^24
+                // The difference of two coordinates as a product of 16 terms: the key's parts (8 bits each, exact in
+                // bf16) times their weights 1, 2^8, 2^16, 2^24 in the lower half's lanes, the weights times the query's
+                // negated parts in the upper half's; exact up to 2^23. The key's operand holds two axes at a time, the
+                // query's is 0 for the other one.
 #pragma unroll
                 for (int x = 0; x < 3; ++x) {
                     const int32_t c = row[t] >= 0 ? a.q_coords[(int64_t)row[t] * 4 + 1 + x] : 0;
@@ -258,15 +285,23 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
                     const float w[4] = {1.0f, 256.0f, 65536.0f, 16777216.0f};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        qc[t][x][i] = (__bf16)(half ? 0.0f : w[i]);
-                        qc[t][x][4 + i] = (__bf16)(half ? 0.0f : -p[i]);
+                        qc[t][x][i] = (__bf16)(x == 1 ? 0.0f : half ? -p[i] : w[i]);
+                        qc[t][x][4 + i] = (__bf16)(x != 1 ? 0.0f : half ? -p[i] : w[i]);
                     }
                 }
+            }
+        }
+        if constexpr (BIAS) {
+            if (tid == 0) {
+                s_xy[2 * SB] = make_uint4(0x43803f80u, 0x4b804780u, 0x43803f80u, 0x4b804780u);
+                s_z[2 * SB] = make_uint2(0x43803f80u, 0x4b804780u);
             }
         }
 
         int32_t only = -1;  // >= 0: the one segment this turn is for
         for (;;) {
+            const int tid = thread_again(), lane = tid & 63, half = lane >> 5;
+            ConstArgs& a = args_again();
             int32_t klo = blo, khi = bhi;
             if (only >= 0) {
                 const int32_t l0 = (int32_t)clamp64(a.k_off[only], 0, a.Pk), h0 = (int32_t)clamp64(a.k_off[only + 1], l0, a.Pk);
@@ -287,38 +322,32 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
                 for (int b = 0; b < NB; ++b) O[t][b] = v16f{};
             }
 
-            // ---- the keys: row numbers three tiles ahead, mask and coordinates two, data one
-            const bool mt = tid < BK;  // a thread that looks after a key of each tile
-            int32_t mi = -1;           // its row in the tile whose mask and coordinates come next
-            const auto number = [&](int32_t t) -> int32_t {
-                if (!mt || t >= nt || tid >= khi - klo - t * BK) return -1;
-                const int32_t p = klo + t * BK + tid, r = a.k_index ? a.k_index[p] : p;
-                return r >= 0 && r < (int32_t)a.Mk ? r : -1;
+            // ---- the keys' numbers, mask and coordinates, by groups of SB
+            int32_t mi = -1;  // the thread's row in the group whose mask and coordinates come next
+            const auto number = [&](int32_t g) -> int32_t {
+                if (g * (int64_t)SB >= khi - klo || tid >= khi - klo - g * SB) return -1;
+                const int32_t p = klo + g * SB + tid;
+                return a.k_index ? a.k_index[p] : p;  // (looked at in about(): nothing waits for it here)
             };
             int4 mc = make_int4(0, 0, 0, 0);
             uint8_t mm = 1;
             const auto about = [&]() {  // of row mi
+                mi = mi < (int32_t)a.Mk ? mi : -1;
                 const int64_t r = mi >= 0 ? mi : 0;
                 if (a.k_mask) mm = a.k_mask[r];
                 if constexpr (BIAS) mc = *(const int4*)(a.k_coords + r * 4);
             };
-            const auto note = [&](int b, int32_t r) {
-                if (wave == 0) {
-                    const bool on = r >= 0 && mm != 0;
-                    const uint64_t w = __ballot(mt && on);
-                    if (tid < KB) s_ok[b][tid] = (uint32_t)(w >> (32 * tid));
-                    if (mt) s_row[b][tid] = on ? r : -1;
-                    if constexpr (BIAS) {
-                        if (mt) {
-                            const int32_t c[3] = {mc.y, mc.z, mc.w};
-#pragma unroll
-                            for (int x = 0; x < 3; ++x) {
-                                const auto b16 = [](int v) { return f2u((float)v) >> 16; };  // (exact: 8 bits)
-                                s_c[b][x][tid] = make_uint2(b16(c[x] & 255) | (b16((c[x] >> 8) & 255) << 16),
-                                                            b16((c[x] >> 16) & 255) | (b16(c[x] >> 24) << 16));
-                            }
-                        }
-                    }
+            const auto note = [&](int b) {
+                const bool on = mi >= 0 && mm != 0;
+                const uint64_t w = __ballot(on);
+                if (lane < 2) s_ok[b][2 * wave + lane] = (uint32_t)(w >> (32 * lane));
+                s_row[b][tid] = on ? mi : -1;
+                if constexpr (BIAS) {
+                    const auto b16 = [](int v) { return f2u((float)v) >> 16; };  // (exact: 8 bits)
+                    const auto p01 = [&](int v) { return b16(v & 255) | (b16((v >> 8) & 255) << 16); };
+                    const auto p23 = [&](int v) { return b16((v >> 16) & 255) | (b16(v >> 24) << 16); };
+                    s_xy[b * SB + tid] = make_uint4(p01(mc.y), p23(mc.y), p01(mc.z), p23(mc.z));
+                    s_z[b * SB + tid] = make_uint2(p01(mc.w), p23(mc.w));
                 }
             };
             // (rows are less than 2^31 bytes apart; a chunk behind the head's width is the line of zeros of every row)
@@ -333,208 +362,183 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
                 ks[i] = ck < a.D ? (uint32_t)a.k_row * ES : 0u;
                 vs[i] = cv < a.D ? (uint32_t)a.v_row * ES : 0u;
             }
-            const auto fetch = [&](int b, int nb) {  // the tile noted in slot nb, into buffer b
+            const auto fetch = [&](int b, uint32_t t) {  // tile t into buffer b
+                const int32_t* rows = &s_row[(t / TPS) & 1][(t % TPS) * BK];
+                const uint32_t* oks = &s_ok[(t / TPS) & 1][(t % TPS) * KB];
+                uint32_t all = oks[0];
+                if constexpr (KB == 2) all &= oks[1];
+                all = __builtin_amdgcn_readfirstlane(all);
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) {
-                    const int32_t row = s_row[nb][((i * NW + wave) * 64 + lane) / CPR];
-                    const char* kp = row >= 0 ? kb[i] + (uint64_t)(uint32_t)row * ks[i] : (const char*)&g_zeros;
-                    const char* vp = row >= 0 ? vb[i] + (uint64_t)(uint32_t)row * vs[i] : (const char*)&g_zeros;
-                    typedef __attribute__((address_space(1))) const void* gp;
-                    typedef __attribute__((address_space(3))) void* lp;
-                    __builtin_amdgcn_global_load_lds((gp)kp, (lp)(s_k[b] + (i * NW + wave) * 1024), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((gp)vp, (lp)(s_v[b] + (i * NW + wave) * 1024), 16, 0, 0);
+                    const int32_t row = rows[((i * NW + wave) * 64 + lane) / CPR];
+                    const char* kp = kb[i] + (uint64_t)(uint32_t)row * ks[i];
+                    const char* vp = vb[i] + (uint64_t)(uint32_t)row * vs[i];
+                    if (all != 0xffffffffu) {
+                        kp = row >= 0 ? kp : (const char*)&g_zeros;
+                        vp = row >= 0 ? vp : (const char*)&g_zeros;
+                    }
+                    load_to_lds(kp, s_k[b] + (i * NW + wave) * 1024);
+                    load_to_lds(vp, s_v[b] + (i * NW + wave) * 1024);
                 }
             };
             if (nt > 0) {
                 mi = number(0);
                 about();
                 const int32_t m1 = number(1);
-                note(0, mi);
+                note(0);
                 mi = m1;
-                about();
-                const int32_t m2 = number(2);
-                note(1, mi);
-                mi = m2;
                 __syncthreads();
                 fetch(0, 0);
+                loads_landed<0>();
             }
             __syncthreads();
 
             for (int32_t it = 0; it < nt; ++it) {
                 const int cur = it & 1;
                 const bool more = it + 1 < nt;
-                const int slot = it % 3, next_slot = (it + 1) % 3;
+                const int slot = ((uint32_t)it / TPS) & 1, k0 = (int)((uint32_t)it % TPS) * BK;  // where its keys' numbers are
+                const bool ahead = k0 == 0 && it + TPS < nt;  // look up the next group
                 int32_t mn = -1;
-                if (more) {
-                    fetch(cur ^ 1, next_slot);
+                if (more) fetch(cur ^ 1, it + 1);
+                if (ahead) {
                     about();
-                    mn = number(it + 3);
+                    mn = number((uint32_t)it / TPS + 2);
                 }
-                const int32_t p0 = klo + it * BK;
-                if (p0 < whi && wlo - p0 < BK) {
+                // 32 keys at a time: more waves on a SIMD are worth more than longer runs of one (a single wave issues
+                // an ordinary instruction every 5 cycles, two or more together one every 2.5, measured)
+#pragma unroll 1
+                for (int b = 0; b < KB; ++b) {
+                    const int32_t p0 = klo + it * BK + 32 * b;
+                    if (p0 >= whi || wlo - p0 >= 32) continue;
+                    const char* sk = s_k[cur] + 32 * b * DP * ES;
+                    const char* sv = s_v[cur] + 32 * b * DP * ES;
+                    const int kn = slot * SB + k0 + 32 * b;  // its keys' numbers
+                    const uint32_t ok = __builtin_amdgcn_readfirstlane((&s_ok[0][0])[kn / 32]);
+                    const bool all = p0 >= ilo && ihi - p0 >= 32 && ok == 0xffffffffu;
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
-                        v16f s[KB];
                         // ---- scores
-#pragma unroll
-                        for (int b = 0; b < KB; ++b) s[b] = v16f{};
+                        v16f s = {};
                         constexpr int QG = QC < 4 ? QC : 4;  // operand chunks at a time
 #pragma unroll
                         for (int c0 = 0; c0 < QC; c0 += QG) {
-                            chunk kf[KB][QG];
+                            chunk kf[QG];
+                            const int r = lane & 31;
 #pragma unroll
-                            for (int c = 0; c < QG; ++c)
+                            for (int c = 0; c < QG; ++c) kf[c] = *(const chunk*)(sk + r * DP * ES + 16 * kswz(r, 2 * (c0 + c) + half));
 #pragma unroll
-                                for (int b = 0; b < KB; ++b) {
-                                    const int kr_ = 32 * b + (lane & 31);
-                                    kf[b][c] = *(const chunk*)(s_k[cur] + kr_ * DP * ES + 16 * kswz(kr_, 2 * (c0 + c) + half));
-                                }
-                            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                            for (int c = 0; c < QG; ++c)
-#pragma unroll
-                                for (int b = 0; b < KB; ++b) s[b] = Mat<T>::mma32(kf[b][c], qf[t][c0 + c], s[b]);
+                            for (int c = 0; c < QG; ++c) s = Mat<T>::mma32(kf[c], qf[t][c0 + c], s);
                         }
                         // less the maximum so far, in powers of two
                         if (a.cap2 != 0.0f) {
 #pragma unroll
-                            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    if constexpr (ES == 4) s[b][e] = a.cap2 * tanhf(s[b][e] * a.cap_arg);
-                                    else s[b][e] = __builtin_fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[b][e] * a.cap_arg)), a.cap2);
-                                }
+                            for (int e = 0; e < 16; ++e) {
+                                if constexpr (ES == 4) s[e] = a.cap2 * tanhf(s[e] * a.cap_arg);
+                                else s[e] = __builtin_fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[e] * a.cap_arg)), a.cap2);
+                            }
                         }
                         if constexpr (BIAS) {
+                            const int kc = half ? 2 * SB : kn + (lane & 31);
+                            const uint2 z = s_z[kc];
+                            const v8bf kxy = __builtin_bit_cast(v8bf, s_xy[kc]), kz = __builtin_bit_cast(v8bf, make_uint4(z.x, z.y, 0u, 0u));
+                            v16f u;
 #pragma unroll
-                            for (int b = 0; b < KB; ++b) {
-                                v16f u;
+                            for (int x = 0; x < 3; ++x) {
+                                const v16f d = Mat<__bf16>::mma32(x < 2 ? kxy : kz, qc[t][x], v16f{});
 #pragma unroll
-                                for (int x = 0; x < 3; ++x) {
-                                    const uint2 kp = s_c[slot][x][32 * b + (lane & 31)];
-                                    // parts, then the weights 1, 2^8, 2^16, 2^24 in bf16
-                                    // (both halves of the wave hold them: the query's are 0 in the upper one)
-                                    const v4i kc = v4i{(int)kp.x, (int)kp.y, (int)0x43803f80u, (int)0x4b804780u};
-                                    const v16f d = Mat<__bf16>::mma32(__builtin_bit_cast(v8bf, kc), qc[t][x], v16f{});
-#pragma unroll
-                                    for (int e = 0; e < 16; ++e) u[e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[t][x], x == 0 ? -m[t] : u[e]);
-                                }
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) s[b][e] = __builtin_fmaf(s[b][e], k2, u[e]);
+                                for (int e = 0; e < 16; ++e) u[e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[t][x], x == 0 ? -m[t] : u[e]);
+                                __builtin_amdgcn_sched_barrier(0);  // (one difference's registers at a time)
                             }
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], k2, u[e]);
                         } else {
 #pragma unroll
-                            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) s[b][e] = __builtin_fmaf(s[b][e], k2, -m[t]);
+                            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], k2, -m[t]);
                         }
                         // ---- the keys that count for the lane's slot
-                        const int jl = lo[t] - p0, jh = hi[t] - p0;
-                        const bool inside = p0 >= ilo && ihi - p0 >= BK;
+                        if (!all) {
+                            const int x = lo[t] - p0, y = hi[t] - p0;
+                            uint32_t w = y >= 32 ? 0xffffffffu : y <= 0 ? 0u : (1u << y) - 1u;
+                            w &= x <= 0 ? 0xffffffffu : x >= 32 ? 0u : ~((1u << x) - 1u);
+                            w = (w & ok) >> (4 * half);
 #pragma unroll
-                        for (int b = 0; b < KB; ++b) {
-                            const uint32_t ok = __builtin_amdgcn_readfirstlane(s_ok[slot][b]);
-                            if (!inside || ok != 0xffffffffu) {
-                                const int x = jl - 32 * b, y = jh - 32 * b;
-                                uint32_t w = y >= 32 ? 0xffffffffu : y <= 0 ? 0u : (1u << y) - 1u;
-                                w &= x <= 0 ? 0xffffffffu : x >= 32 ? 0u : ~((1u << x) - 1u);
-                                w = (w & ok) >> (4 * half);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const uint32_t on = (uint32_t)((int32_t)(w << (31 - ((e & 3) + 8 * (e >> 2)))) >> 31);
-                                    s[b][e] = u2f((on & f2u(s[b][e])) | (~on & 0xff800000u));
-                                }
+                            for (int e = 0; e < 16; ++e) {
+                                const uint32_t on = (uint32_t)((int32_t)(w << (31 - ((e & 3) + 8 * (e >> 2)))) >> 31);
+                                s[e] = u2f((on & f2u(s[e])) | (~on & 0xff800000u));
                             }
                         }
                         // ---- running maximum: set by the first keys, then moved only when it grows by more than
                         // 2^8 for some slot of the wave (weights of up to 2^8 lose nothing)
-                        float mx = s[0][0];
+                        float mx = s[0];
 #pragma unroll
-                        for (int b = 0; b < KB; ++b)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) mx = __builtin_fmaxf(mx, s[b][e]);
-                        mx = __builtin_fmaxf(mx, other_half(mx));
+                        for (int e = 1; e < 16; ++e) mx = __builtin_fmaxf(mx, s[e]);
+                        mx = halves_max(mx);
                         if (__any(mx > grow[t])) {
                             const bool any = mx > -__builtin_inff();  // (a slot without a key so far keeps m = 0)
                             const float up = any && (mx > 0.0f || grow[t] < 0.0f) ? mx : 0.0f;
-                            const float al = __builtin_amdgcn_exp2f(-up);
+                            // (nothing to scale before the first key, whose score may be far below -2^7)
+                            const float al = grow[t] < 0.0f ? 1.0f : __builtin_amdgcn_exp2f(-up);
                             grow[t] = any ? 8.0f : grow[t];
                             m[t] = m[t] + up;
                             l[t] = l[t] * al;
 #pragma unroll
-                            for (int b = 0; b < KB; ++b)
+                            for (int e = 0; e < 16; ++e) s[e] = s[e] - up;
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) s[b][e] = s[b][e] - up;
+                            for (int n = 0; n < NB; ++n)
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) O[t][b][e] = O[t][b][e] * al;
+                                for (int e = 0; e < 16; ++e) O[t][n][e] = O[t][n][e] * al;
                         }
-                        // (the first operands of V are on their way while the exponentials are formed)
-                        chunk vf[2][NB];
-                        const auto values = [&](int b, int f) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            s[e] = __builtin_amdgcn_exp2f(s[e]);
+                            sum = sum + s[e];
+                        }
+                        l[t] = l[t] + sum;
+                        // ---- O^T += V^T P^T
+                        if constexpr (ES == 4) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const int r = (e & 3) + 8 * (e >> 2) + 4 * half;
+#pragma unroll
+                                for (int n = 0; n < NB; ++n) {
+                                    const float vf = *(const float*)(sv + r * DP * 4 + (32 * n + (lane & 31)) * 4);
+                                    O[t][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[e], O[t][n], 0, 0, 0);
+                                }
+                            }
+                        } else {
                             typedef short v4s __attribute__((ext_vector_type(4)));
                             typedef short v8s __attribute__((ext_vector_type(8)));
                             typedef __attribute__((address_space(3))) v4s* lds4;
 #pragma unroll
-                            for (int n = 0; n < NB; ++n) {
-                                const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                                const int r0 = 32 * b + 16 * f + 4 * half + (i >> 2);
-                                const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + r0 * DP * 2 + 16 * vswz(r0, c) + (i & 1) * 8));
-                                const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(s_v[cur] + (r0 + 8) * DP * 2 + 16 * vswz(r0 + 8, c) + (i & 1) * 8));
-                                const v8s vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                                vf[f][n] = __builtin_bit_cast(chunk, vv);
-                            }
-                        };
-                        if constexpr (ES == 2) {
-                            values(0, 0);
-                            values(0, 1);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                        float sum = 0.0f;
+                            for (int f = 0; f < 2; ++f) {
+                                chunk pf;
 #pragma unroll
-                        for (int b = 0; b < KB; ++b)
+                                for (int i = 0; i < 8; ++i) pf[i] = (T)s[8 * f + i];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                s[b][e] = __builtin_amdgcn_exp2f(s[b][e]);
-                                sum = sum + s[b][e];
-                            }
-                        l[t] = l[t] + sum;
-                        // ---- O^T += V^T P^T
-#pragma unroll
-                        for (int b = 0; b < KB; ++b) {
-                            if constexpr (ES == 4) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const int kr_ = 32 * b + (e & 3) + 8 * (e >> 2) + 4 * half;
-#pragma unroll
-                                    for (int n = 0; n < NB; ++n) {
-                                        const float vf = *(const float*)(s_v[cur] + kr_ * DP * 4 + (32 * n + (lane & 31)) * 4);
-                                        O[t][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[b][e], O[t][n], 0, 0, 0);
-                                    }
-                                }
-                            } else {
-#pragma unroll
-                                for (int f = 0; f < 2; ++f) {
-                                    chunk pf;
-#pragma unroll
-                                    for (int i = 0; i < 8; ++i) pf[i] = (T)s[b][8 * f + i];
-#pragma unroll
-                                    for (int n = 0; n < NB; ++n) O[t][n] = Mat<T>::mma32(vf[f][n], pf, O[t][n]);
-                                    if (b + 1 < KB) values(b + 1, f);
+                                for (int n = 0; n < NB; ++n) {
+                                    const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                                    const int r = 16 * f + 4 * half + (i >> 2);
+                                    const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + r * DP * 2 + 16 * vswz(r, c) + (i & 1) * 8));
+                                    const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + (r + 8) * DP * 2 + 16 * vswz(r + 8, c) + (i & 1) * 8));
+                                    const v8s vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                                    O[t][n] = Mat<T>::mma32(__builtin_bit_cast(chunk, vv), pf, O[t][n]);
                                 }
                             }
                         }
                     }
                 }
-                if (more) {
-                    note((it + 2) % 3, mi);
+                if (ahead) {
+                    note(slot ^ 1);
                     mi = mn;
                 }
+                loads_landed<0>();
                 __syncthreads();
             }
 
-            const AttnArgs& a = args_again();
+            {
+            const int tid = thread_again(), lane = tid & 63, half = lane >> 5;
+            ConstArgs& a = args_again();
             // ---- values of other segments that are not finite: once more, segment by segment
             if (only < 0) {
                 float bad = 0.0f;
@@ -560,12 +564,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
             // ---- results (before a second turn: those of no segment only)
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float lt = l[t] + other_half(l[t]);
+                const float lt = halves_sum(l[t]);
                 const bool mine = only == -2 ? seg[t] < 0 : only < 0 || seg[t] == only;
                 if (a.splits > 1) {
+                    const int64_t o = ((int64_t)split * a.Hq + head[t]) * a.Pq + pos[t];
+                    if (mine && pos[t] >= 0 && half == 0)
+                        a.part_ml[o] = make_float2(grow[t] > 0.0f ? m[t] : -__builtin_inff(), seg[t] >= 0 ? lt : -1.0f);
                     if (mine && seg[t] >= 0) {
-                        const int64_t o = ((int64_t)split * a.Pq + pos[t]) * a.Hq + head[t];
-                        if (half == 0) a.part_ml[o] = make_float2(grow[t] > 0.0f ? m[t] : -__builtin_inff(), lt);
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -597,10 +602,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
 #pragma unroll
             for (int t = 0; t < QT; ++t)
                 if (seg[t] >= 0 && seg[t] > only && seg[t] < next) next = seg[t];
-            for (int o = 32; o > 0; o >>= 1) {
-                const int32_t x = __shfl_xor(next, o, 64);
-                next = x < next ? x : next;
-            }
+            next = wave_extreme<false>(next);
             if constexpr (NW > 1) {
                 __syncthreads();
                 if (lane == 0) s_r[2][wave] = next;
@@ -610,41 +612,43 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && DP == 128 && NW == 1 ? 1
             }
             if (next == 0x7fffffff) break;
             only = __builtin_amdgcn_readfirstlane(next);
+            }
         }
     }
 }
 
-// Joins the splits: a wave a (position, head). Its lanes are G groups of 16 or 32, each on every G-th split and 4 columns a
-// lane; the groups' sums are added in order at the end.
-template <class T, int CL>
+// Joins the splits of each (position, head): groups of CL lanes, 4 columns a lane. WIDE (many splits): a wave a position, each
+// group on every (64 / CL)-th split, the groups' sums added in order at the end. Otherwise a group a position, its splits
+// in order.
+template <class T, int CL, bool WIDE>
 __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
-    constexpr int G = 64 / CL;
-    const int lane = threadIdx.x & 63, g = lane / CL, d = 4 * (lane % CL);
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= a.Pq * a.Hq) return;
-    const int64_t pos = item / a.Hq;
-    const int head = (int)(item - pos * a.Hq);
+    constexpr int G = 64 / CL, PER = WIDE ? 4 : 4 * G;  // positions a block
+    const int lane = threadIdx.x & 63, g = lane / CL, d = 4 * (lane % CL), head = blockIdx.y;
+    const int64_t pos = (int64_t)blockIdx.x * PER + (WIDE ? threadIdx.x >> 6 : threadIdx.x / CL);
+    if (pos >= a.Pq) return;
     const int32_t r = a.q_index ? a.q_index[pos] : (int32_t)pos;
-    const bool in = segment_of(a.q_off, a.S, pos) >= 0;
+    const int64_t step = (int64_t)a.Hq * a.Pq, at = (int64_t)head * a.Pq + pos;
+    // (blocks by segment write nothing for positions of no segment)
+    const bool in = a.seg ? segment_of(a.q_off, a.S, pos) >= 0 : a.part_ml[at].y >= 0.0f || a.part_ml[at].y != a.part_ml[at].y;
     if (r < 0 || r >= a.Mq || (!in && !a.zero_rest)) return;
     typedef T v4t __attribute__((ext_vector_type(4)));
     v4t* op = (v4t*)((T*)a.out + (int64_t)r * a.o_row + head * a.o_head + d);
-    const bool mine = g == 0 && d < a.D;
+    const bool mine = (!WIDE || g == 0) && d < a.D;
     if (!in) {
         if (mine) *op = v4t{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
         return;
     }
-    const int64_t step = a.Pq * a.Hq;
     float m = -__builtin_inff();
-    for (int s = lane; s < a.splits; s += 64) m = __builtin_fmaxf(m, a.part_ml[item + s * step].x);
-    for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
+    for (int s = WIDE ? lane : 0; s < a.splits; s += WIDE ? 64 : 1) m = __builtin_fmaxf(m, a.part_ml[at + s * step].x);
+    if constexpr (WIDE)
+        for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
     const float ms = m == -__builtin_inff() ? 0.0f : m;
     float l = 0.0f;
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int s = g; s < a.splits; s += G) {
-        const float2 ml = a.part_ml[item + s * step];
-        const v4f po = d < a.D ? *(const v4f*)(a.part_o + (item + s * step) * a.D + d) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = WIDE ? g : 0; s < a.splits; s += WIDE ? G : 1) {
+        const float2 ml = a.part_ml[at + s * step];
+        const v4f po = d < a.D ? *(const v4f*)(a.part_o + (at + s * step) * a.D + d) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
         const float w = __builtin_amdgcn_exp2f(ml.x - ms);
         if (ml.y != 0.0f) {  // (a part without keys counts for nothing)
             l = __builtin_fmaf(ml.y, w, l);
@@ -652,11 +656,13 @@ __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
             for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(po[i], w, acc[i]);
         }
     }
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int o = CL; o < 64; o <<= 1) {
-        l = l + __shfl_xor(l, o, 64);
+        for (int o = CL; o < 64; o <<= 1) {
+            l = l + __shfl_xor(l, o, 64);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = acc[i] + __shfl_xor(acc[i], o, 64);
+            for (int i = 0; i < 4; ++i) acc[i] = acc[i] + __shfl_xor(acc[i], o, 64);
+        }
     }
     if (!mine) return;
     const float inv = 1.0f / l;
@@ -664,6 +670,16 @@ __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (T)(l == 0.0f ? 0.0f : acc[i] * inv);
     *op = v;
+}
+
+template <class T, int CL>
+static int launch_join(const AttnArgs& a, hipStream_t s) {
+    const bool wide = a.splits >= 16;
+    const int per = wide ? 4 : 4 * (64 / CL);
+    const dim3 grid((unsigned)((a.Pq + per - 1) / per), (unsigned)a.Hq);
+    if (wide) hipLaunchKernelGGL((attention_join_k<T, CL, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_join_k<T, CL, false>), grid, dim3(256), 0, s, a);
+    return check_launch("attention_join_k");
 }
 
 // The rows outside every segment, where blocks go by segment.
@@ -678,32 +694,27 @@ __global__ __launch_bounds__(256) void attention_rest_k(AttnArgs a) {
         for (int d = threadIdx.x & 63; d < a.D; d += 64) ((T*)a.out)[r * a.o_row + h * a.o_head + d] = (T)0.0f;
 }
 
-template <class T, int DP, int NW, int QT>
+template <class T, int DP, int NW>
 static int launch_attention_w(AttnArgs& a, hipStream_t s) {
-    const int64_t units = a.seg ? a.S : (a.Pq * a.G + 32 * NW * QT - 1) / (32 * NW * QT);
+    const int64_t units = NW == 1 ? a.S : (a.Pq * a.G + 32 * NW - 1) / (32 * NW);
     const int64_t blocks = units * a.Hk * a.splits;
     PMG_REQUIRE(blocks < (int64_t)1 << 31, "too many blocks");
     a.blocks = (uint32_t)blocks;
-    if (a.slopes) hipLaunchKernelGGL((attention_k<T, DP, NW, QT, true>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((attention_k<T, DP, NW, QT, false>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
+    if (a.slopes) hipLaunchKernelGGL((attention_k<T, DP, NW, 1, true>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
+    else hipLaunchKernelGGL((attention_k<T, DP, NW, 1, false>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
     return check_launch("attention_k");
 }
 
 template <class T, int DP>
-static int launch_attention_d(AttnArgs& a, int waves, hipStream_t s) {
-    return waves == 1 ? launch_attention_w<T, DP, 1, 1>(a, s) : launch_attention_w<T, DP, 4, 1>(a, s);
+static int launch_attention_d(AttnArgs& a, hipStream_t s) {
+    return a.seg ? launch_attention_w<T, DP, 1>(a, s) : launch_attention_w<T, DP, 4>(a, s);
 }
 
 template <class T>
-int launch_attention_t(AttnArgs& a, int waves, hipStream_t s) {
-    int e = a.D <= 32 ? launch_attention_d<T, 32>(a, waves, s) : a.D <= 64 ? launch_attention_d<T, 64>(a, waves, s) : launch_attention_d<T, 128>(a, waves, s);
+int launch_attention_t(AttnArgs& a, hipStream_t s) {
+    int e = a.D <= 32 ? launch_attention_d<T, 32>(a, s) : a.D <= 64 ? launch_attention_d<T, 64>(a, s) : launch_attention_d<T, 128>(a, s);
     if (e) return e;
-    if (a.splits > 1) {
-        const dim3 grid((unsigned)((a.Pq * a.Hq + 3) / 4));
-        if (a.D <= 64) hipLaunchKernelGGL((attention_join_k<T, 16>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((attention_join_k<T, 32>), grid, dim3(256), 0, s, a);
-        return check_launch("attention_join_k");
-    }
+    if (a.splits > 1) return a.D <= 64 ? launch_join<T, 16>(a, s) : launch_join<T, 32>(a, s);
     if (a.seg && a.zero_rest) {
         hipLaunchKernelGGL((attention_rest_k<T>), dim3((unsigned)((a.Pq + 3) / 4)), dim3(256), 0, s, a);
         return check_launch("attention_rest_k");
@@ -711,8 +722,8 @@ int launch_attention_t(AttnArgs& a, int waves, hipStream_t s) {
     return PMG_OK;
 }
 
-int launch_attention_f16(AttnArgs& a, int waves, hipStream_t s);
-int launch_attention_bf16(AttnArgs& a, int waves, hipStream_t s);
-int launch_attention_f32(AttnArgs& a, int waves, hipStream_t s);
+int launch_attention_f16(AttnArgs& a, hipStream_t s);
+int launch_attention_bf16(AttnArgs& a, hipStream_t s);
+int launch_attention_f32(AttnArgs& a, hipStream_t s);
 
 }  // namespace pmg

@@ -6,31 +6,39 @@ using namespace pmg;
 namespace {
 
 struct Plan {
-    int seg, waves, splits;
+    int seg, splits;
 };
 
-// The forms, by the mean lengths (the offsets are on the device).
-//   A block per segment where the queries of a segment fill no half wave and its keys are many; else tiles of positions,
-//   of one wave where segments are short (a tile of four would walk over the keys of several) and four where not.
-//   Keys are split over blocks where the blocks would not fill the card, or would fill it unevenly: rounds of resident
-//   blocks against what writing and joining the parts costs.
+// The forms, by the mean lengths (the offsets are on the device). A block per segment where the queries of a segment fill no
+// half wave and its keys are many, the keys split so that about 2048 waves (8 a CU) read them. Else tiles of 128 slots;
+// their keys are split where the blocks would lie unevenly on the CUs, or too few on each to hide what they wait for:
+// a CU's share of the blocks against what writing and joining the parts costs. Measured (MI355X): 19200 rows, 4 heads of
+// 64, biased (600 blocks): 1 part 844 us, 2 parts 738 and 20 to join, 4 parts 712 and 25.
 Plan plan_of(const pmg_attention_args& r) {
-    Plan p{0, 4, 1};
+    Plan p{0, 1};
     if (r.segments < 1) return p;
     const int64_t G = r.Hq / r.Hk;
     const double nq = (double)r.q_positions / (double)r.segments, nk = (double)r.k_positions / (double)r.segments;
     p.seg = nq * (double)G <= 16.0 && nk >= 128.0;
-    p.waves = p.seg || nk < 512.0 ? 1 : 4;
-    const int64_t units = p.seg ? r.segments : (r.q_positions * G + 32 * p.waves - 1) / (32 * p.waves);
-    const int64_t blocks = units * r.Hk, resident = p.waves == 1 ? 2048 : 512;
-    // microseconds: a tile of 64 keys takes a resident block about 1.9 (four waves) or 2.5 (one) at D = 64
-    const double round = nk / 64.0 * (p.waves == 1 ? 2.5 : 1.9) * (r.D <= 32 ? 0.7 : r.D <= 64 ? 1.0 : 1.8) * (r.type == PMG_TYPE_F32 ? 4.0 : 1.0);
-    const double part = (double)r.q_positions * (double)r.Hq * (double)r.D * 8.0 / 4.0e6;
-    const int most = nk >= 512.0 ? (int)(nk / 256.0 < 64.0 ? nk / 256.0 : 64.0) : 1;
+    if (p.seg) {
+        const int64_t s = 2048 / (r.segments * r.Hk), most = (int64_t)(nk / 256.0);
+        p.splits = (int)(s < most ? s : most);
+        p.splits = p.splits < 1 ? 1 : p.splits > 256 ? 256 : p.splits;
+        return p;
+    }
+    const int64_t blocks = (r.q_positions * G + 127) / 128 * r.Hk;
+    // a block's keys: its positions' own segment lengths (longer ones hold more of the positions) and what it straddles;
+    // microseconds: 64 keys of a block at a CU's full throughput (and a block's start); the share of that throughput that
+    // 1 .. 4 resident blocks reach; a part's O written and read
+    const double keys = nk >= 1024.0 ? nk : 2.0 * nk < 1024.0 ? 2.0 * nk + 128.0 / (double)G : 1024.0;
+    const double block = keys / 64.0 * (r.D <= 32 ? 0.6 : r.D <= 64 ? 1.0 : 1.8) * (r.type == PMG_TYPE_F32 ? 4.0 : 1.0);
+    const double reach[5] = {1.0, 0.5, 0.68, 0.84, 1.0};
+    const int resident = r.D <= 64 ? (r.slopes ? 3 : 4) : 2;
+    const double part = (double)r.q_positions * (double)r.Hq * (double)r.D * 8.0 / 8.0e6;
     double best = 0.0;
-    for (int s = 1; s <= most; ++s) {
-        const double rounds = (double)((blocks * s + resident - 1) / resident);
-        const double t = rounds / s * round + (s > 1 ? 4.0 + s * part : 0.0);
+    for (int s = 1; s <= 64 && s <= (int)(keys / 128.0) + 1; ++s) {
+        const int64_t each = (blocks * s + 255) / 256;
+        const double t = (double)each * (block / s + 1.0) * reach[resident] / reach[each < resident ? each : resident] + (s > 1 ? 6.0 + s * part : 0.0);
         if (s == 1 || t < 0.97 * best) {
             best = t;
             p.splits = s;
@@ -126,7 +134,7 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
         a.part_ml = (float2*)((char*)workspace + (size_t)pl.splits * (size_t)r.q_positions * (size_t)r.Hq * (size_t)r.D * 4);
     }
     hipStream_t s = (hipStream_t)stream;
-    if (r.type == PMG_TYPE_F32) return launch_attention_f32(a, pl.waves, s);
-    if (r.type == PMG_TYPE_F16) return launch_attention_f16(a, pl.waves, s);
-    return launch_attention_bf16(a, pl.waves, s);
+    if (r.type == PMG_TYPE_F32) return launch_attention_f32(a, s);
+    if (r.type == PMG_TYPE_F16) return launch_attention_f16(a, s);
+    return launch_attention_bf16(a, s);
 }

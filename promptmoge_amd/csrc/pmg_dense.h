@@ -69,8 +69,42 @@ __device__ inline uint32_t xcd_tile(uint32_t id, uint32_t n) {
     return x * q + (x < r ? x : r) + i;
 }
 
-// Which 16-byte slot of its LDS row chunk `c` of row `row` is kept in (an exclusive or within the row's 8 slots):
-// 8, and 16, consecutive rows read at one chunk index lie in different banks.
-__device__ inline int swz8(int row, int c) { return c ^ ((row ^ (row >> 3)) & 7); }
+// Which 16-byte slot of its LDS row (of `CPR` 16-byte chunks) chunk c of row `row` is kept in. The rows that a 16-byte read of
+// 32 rows at one chunk index serves at a time (0-3, 12-15, 20-23, 24-27 and the other half) lie in different banks;
+// rows 32 apart are kept alike.
+template <int CPR>
+__device__ inline int swizzle(int row, int c) {
+    if constexpr (CPR == 4) return c ^ ((row >> 2) & 3);
+    else if constexpr (CPR == 8) return c ^ ((row ^ ((row >> 3) & 3)) & 7);
+    else return c ^ (row & 15);
+}
+
+// 16 bytes a lane from memory to LDS, lane after lane from `to` (the same in every lane) on. Written out, for the compiler
+// would wait for these loads before the next LDS read of any kind; loads_landed() waits until at most N of the wave's
+// loads are still on their way (they land in order).
+__device__ inline uint32_t lds_address(const void* to) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to);
+}
+__device__ inline void load_to_lds(const void* from, const void* to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_address(to)), "v"(from) : "memory", "m0");
+}
+// The same from a buffer: at byte `off` (a lane's) + `more` (the wave's); zeros from its end on.
+__device__ inline void buffer_to_lds(v4i rsrc, uint32_t off, uint32_t more, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(to), "v"(off), "s"(rsrc), "s"(more) : "memory", "m0");
+}
+__device__ inline v4i buffer_of(const void* base, uint32_t bytes) {
+    const uint64_t p = (uint64_t)base;
+    return v4i{(int)(uint32_t)p, (int)(uint32_t)(p >> 32), (int)bytes, 0x00027000};
+}
+template <int N>
+__device__ inline void loads_landed() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// A barrier of the block behind which every wave's loads to LDS but its last N, and every LDS access before, are done.
+template <int N>
+__device__ inline void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
 
 }  // namespace pmg

@@ -2,8 +2,8 @@
 // for fp32, fp16, bf16 (fp32 sums, no scales) and int8 (exact int32 sums).
 //
 // Two kernels, both with w's rows as the matrix instruction's row operand, so that a lane holds four neighbouring n of
-// one m. `linear_tile_k`: a block's BM x BN outputs from tiles of 128 bytes of k in LDS, filled by direct loads to LDS
-// one tile ahead; the sums go through LDS once so that residual and output move as whole rows. `linear_rows_k`: few
+// one m. `linear_tile_k`: a block's BM x BN outputs from tiles of 64 bytes of k in LDS, filled by direct loads to LDS
+// NS - 1 tiles ahead; the sums go through LDS once so that residual and output move as whole rows. `linear_rows_k`: few
 // outputs; the block's waves share out k, operands straight into registers.
 #include "pmg_dense.h"
 
@@ -25,30 +25,48 @@ struct LinearArgs {
 };
 
 // --------------------------------------------------------------------------------------------------------- epilogue
-// erf within 1.5e-7 (Abramowitz and Stegun 7.1.26), an eighth of erff's instructions: for outputs of 16 bits, whose
-// half step is 2^-12 of the value at the least; fp32 outputs take erff.
-__device__ inline float erf_as(float x) {
-    const float a = __builtin_fabsf(x);
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, a, 1.0f));
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f);
-    const float e = __builtin_amdgcn_exp2f(-(a * a) * PMG_LOG2E);
-    return __builtin_copysignf(__builtin_fmaf(-(p * t), e, 1.0f), x);
+// gelu(y) = max(y, 0) - |y| q(|y|), q(a) = erfc(a / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (erf within 1.5e-7, so gelu
+// within 0.75e-7 |y|): for outputs of 16 bits, whose half step is 2^-12 of the value at the least; fp32 outputs take
+// erff, several times as long.
+__device__ inline float gelu_16(float y) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, __builtin_fabsf(y), 1.0f));
+    float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+    p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+    const float q = (p * t) * __builtin_amdgcn_exp2f((y * y) * (-0.5f * PMG_LOG2E));
+    return __builtin_fmaf(-__builtin_fabsf(y), q, y < 0.0f ? 0.0f : y);
 }
 
-__device__ inline float activate(float y, int act, bool wide) {
+// act of 8 values in place; wide: for fp32 outputs.
+__device__ inline void activate8(float (&v)[8], int act, bool wide) {
     switch (act) {
-        case PMG_ACT_RELU: return y < 0.0f ? 0.0f : y;  // (NaN stays)
-        case PMG_ACT_SILU: return silu_fast(y);
-        case PMG_ACT_GELU: return 0.5f * y * (1.0f + (wide ? erff(y * 0.70710678f) : erf_as(y * 0.70710678f)));
-        case PMG_ACT_GELU_TANH: {
-            const float u = 0.7978845608f * __builtin_fmaf(0.044715f * y * y, y, y);
-            // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
-            return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * (-2.0f * PMG_LOG2E)));
-        }
-        default: return y;
+        case PMG_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
+            break;
+        case PMG_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = silu_fast(v[i]);
+            break;
+        case PMG_ACT_GELU:
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = gelu_16(v[i]);
+            }
+            break;
+        case PMG_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = v[i], u = __builtin_fmaf(0.044715f * y * y, y, y);
+                // (1 + tanh(c u)) / 2 = 1 / (1 + exp(-2 c u)), c = sqrt(2 / pi)
+                v[i] = y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * (-2.0f * 0.7978845608f * PMG_LOG2E)));
+            }
+            break;
+        default: break;
     }
 }
 
@@ -87,16 +105,46 @@ __device__ inline void store8(E* p, int n, bool vec, const float (&v)[8]) {
     }
 }
 
-// n <= 8 outputs of row m from column n0 on: v holds scaled sums plus bias.
-__device__ inline void finish8(const LinearArgs& a, int64_t m, int n0, int n, float (&v)[8]) {
-    const bool wide = a.out_type == PMG_TYPE_F32;
-    if (a.act != PMG_ACT_NONE)
+// 8 values of the residual as they lie in memory (16-bit types: the first half), and as numbers.
+struct Raw8 {
+    uint4 a, b;
+};
+__device__ inline Raw8 raw8(const LinearArgs& a, int64_t m, int n0) {
+    Raw8 r{};
+    const int64_t o = m * a.ldr + n0;
+    if (a.res_type == PMG_TYPE_F32) {
+        r.a = *(const uint4*)((const float*)a.res + o);
+        r.b = *(const uint4*)((const float*)a.res + o + 4);
+    } else {
+        r.a = *(const uint4*)((const _Float16*)a.res + o);
+    }
+    return r;
+}
+__device__ inline void numbers8(const LinearArgs& a, const Raw8& r, float (&v)[8]) {
+    if (a.res_type == PMG_TYPE_F32) {
+        const v4f x = __builtin_bit_cast(v4f, r.a), y = __builtin_bit_cast(v4f, r.b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = activate(v[i], a.act, wide);
+        for (int i = 0; i < 8; ++i) v[i] = i < 4 ? x[i & 3] : y[i & 3];
+    } else if (a.res_type == PMG_TYPE_F16) {
+        const v8h x = __builtin_bit_cast(v8h, r.a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    } else {
+        const v8bf x = __builtin_bit_cast(v8bf, r.a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    }
+}
+
+// n <= 8 outputs of row m from column n0 on: v holds scaled sums plus bias. `early`: the residual, if it is there already.
+__device__ inline void finish8(const LinearArgs& a, int64_t m, int n0, int n, float (&v)[8], const Raw8* early = nullptr) {
+    const bool wide = a.out_type == PMG_TYPE_F32;
+    activate8(v, a.act, wide);
     if (a.res) {
         float r[8];
         const int64_t o = m * a.ldr + n0;
-        if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
+        if (early) numbers8(a, *early, r);
+        else if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
         else if (a.res_type == PMG_TYPE_F16) load8((const _Float16*)a.res + o, n, a.vec_res, r);
         else load8((const __bf16*)a.res + o, n, a.vec_res, r);
 #pragma unroll
@@ -131,12 +179,16 @@ __device__ inline typename Mat<T>::chunk load_chunk_any(const T* row, int k, int
 
 // ------------------------------------------------------------------------------------------------------ tile kernel
 // VEC: rows of x and w start on 16 bytes and K is a whole number of 16-byte chunks; the loads go straight to LDS, and
-// a chunk behind K or a row behind M or N is given an offset beyond the buffer's record count, which reads zeros.
-template <class T, int BM, int BN, int WM, int WN, bool VEC>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tile_k(LinearArgs a) {
-    constexpr int NT = 64 * WM * WN, KB = 128, KE = KB / (int)sizeof(T);
+// a chunk behind K or a row behind M or N is given an offset behind the buffer's end, which reads zeros. One barrier a
+// tile.
+constexpr uint32_t kNowhere = 0x7ffffff0u;
+
+template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 1 : 2) void linear_tile_k(LinearArgs a) {
+    constexpr int NW = WM * WN, NT = 64 * NW, KE = KB / (int)sizeof(T), PER = Mat<T>::kPer;
+    constexpr int CPR = KB / 16, RPL = 64 / CPR, STEPS = CPR / 2;  // chunks a row, rows a load, steps a tile
     constexpr int TM = BM / WM, TN = BN / WN, MT = TM / 32, NTL = TN / 32;
-    constexpr int kStage = (BM + BN) * KB;
+    constexpr int NL = ((BM + BN) / RPL + NW - 1) / NW, kStage = VEC ? NL * NW * 1024 : (BM + BN) * KB;  // a wave's loads a tile
     typedef typename Mat<T>::chunk chunk;
     typedef typename Mat<T>::acc32 acc32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -150,77 +202,125 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_k(LinearArgs a) {
     const int rows_m = a.M - m0 < BM ? (int)(a.M - m0) : BM, rows_n = a.N - n0 < BN ? a.N - n0 : BN;
     const int nk = (a.K + KE - 1) / KE;
 
-    auto fill = [&](int t, int buf) {
-        char* base = lds + buf * kStage;
-        if constexpr (VEC) {
-            const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)xb, 0, (int)(((int64_t)(rows_m - 1) * a.ldx + a.K) * (int)sizeof(T)), 0x00027000);
-            const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)wb, 0, (int)(((int64_t)(rows_n - 1) * a.ldw + a.K) * (int)sizeof(T)), 0x00027000);
-#pragma unroll
-            for (int i = 0; i < (BM + BN) / 8 / (WM * WN); ++i) {
-                const int g = i * WM * WN + wave;  // 8 rows of x's or w's tile (uniform over the wave)
-                const int r = (g < BM / 8 ? g : g - BM / 8) * 8 + (lane >> 3);
-                const int c = swz8(r, lane & 7) * Mat<T>::kPer + t * KE;
-                const bool isx = g < BM / 8;
-                const bool in = c < a.K && r < (isx ? rows_m : rows_n);
-                const uint32_t off = in ? (uint32_t)(((int64_t)r * (isx ? a.ldx : (int64_t)a.ldw) + c) * (int)sizeof(T)) : 0x7ffffff0u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(isx ? rx : rw, (__attribute__((address_space(3))) void*)(base + g * 1024), 16, off, 0, 0, 0);
-            }
-        } else {
-            for (int e = tid; e < (BM + BN) * 8; e += NT) {
-                const int r = e >> 3, c = e & 7, k = t * KE + c * Mat<T>::kPer;
-                chunk v{};
-                if (r < BM) {
-                    if (r < rows_m) v = load_chunk_any<T>(xb + r * a.ldx, k, a.K);
-                } else if (r - BM < rows_n) {
-                    v = load_chunk_any<T>(wb + (int64_t)(r - BM) * a.ldw, k, a.K);
-                }
-                const int lr = r < BM ? r : r - BM;
-                *(chunk*)(base + r * KB + 16 * swz8(lr, c)) = v;
-            }
-        }
-    };
-
     acc32 acc[MT][NTL];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NTL; ++j) acc[i][j] = acc32{};
-
-    fill(0, 0);
-    __syncthreads();
-    for (int t = 0; t < nk; ++t) {
-        const char* cur = lds + (t & 1) * kStage;
-        if (t + 1 < nk) fill(t + 1, (t + 1) & 1);
+    // the lane's chunks of a tile's steps (row r of a 32-row operand)
+    const int r = lane & 31;
+    int at[STEPS];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int r = lane & 31, c = 2 * s + (lane >> 5);
-            chunk fx[MT], fw[NTL];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int row = wm * TM + 32 * i + r;
-                fx[i] = *(const chunk*)(cur + row * KB + 16 * swz8(row, c));
-            }
-#pragma unroll
-            for (int j = 0; j < NTL; ++j) {
-                const int row = wn * TN + 32 * j + r;
-                fw[j] = *(const chunk*)(cur + (BM + row) * KB + 16 * swz8(row, c));
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) acc[i][j] = Mat<T>::mma32(fw[j], fx[i], acc[i][j]);
-        }
-        __syncthreads();
-    }
-
-    // Sums through LDS: 32 rows of the wave's TN columns at a time, in fp32.
-    constexpr int LD = TN + 4;
-    float* st = (float*)lds + wave * 32 * LD;
-    constexpr int LPR = TN / 8, RPP = 64 / LPR;  // lanes a row, rows a pass
+    for (int s = 0; s < STEPS; ++s) at[s] = r * KB + 16 * swizzle<CPR>(r, 2 * s + (lane >> 5));
+    // what the epilogue needs is asked for first: scale, bias, and in the small tile the residual
+    constexpr int LPR = TN / 8, RPP = 64 / LPR, NP = 32 / RPP;  // lanes a row, rows a pass, passes
     const int nc = n0 + wn * TN + 8 * (lane % LPR);
     const int left = a.N - nc < 8 ? a.N - nc : 8;
     float sc[8], bs[8];
     columns8<T>(a, nc, sc, bs);
+    Raw8 early[MT == 1 ? NP : 1];
+    const bool ahead = MT == 1 && a.res && a.vec_res && a.N % 8 == 0;
+    if constexpr (MT == 1) {
+        if (ahead) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int64_t m = m0 + wm * TM + p * RPP + lane / LPR;
+                if (m < a.M && left > 0) early[p] = raw8(a, m, nc);
+            }
+        }
+    }
+
+    chunk fx[2][MT], fw[2][NTL];
+    const auto operands = [&](const char* st, int s) {  // step s of the tile at st
+        const char* sx = st + wm * TM * KB + at[s];
+        const char* sw = st + (BM + wn * TN) * KB + at[s];
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) fw[s & 1][j] = *(const chunk*)(sw + j * 32 * KB);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fx[s & 1][i] = *(const chunk*)(sx + i * 32 * KB);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = Mat<T>::mma32(fw[s & 1][j], fx[s & 1][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    if constexpr (VEC) {
+        const v4i rx = buffer_of(xb, (uint32_t)(((int64_t)(rows_m - 1) * a.ldx + a.K) * (int)sizeof(T)));
+        const v4i rw = buffer_of(wb, (uint32_t)(((int64_t)(rows_n - 1) * a.ldw + a.K) * (int)sizeof(T)));
+        uint32_t off[NL];
+        const int kbytes = a.K * (int)sizeof(T);
+        int kc[NL];  // byte of k of the lane's chunk in tile 0
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int row = (i * NW + wave) * RPL + lane / CPR;
+            const bool isx = (i * NW + wave) * RPL < BM;  // (uniform over the wave)
+            const int rr = isx ? row : row - BM;
+            kc[i] = 16 * swizzle<CPR>(rr, lane % CPR);
+            off[i] = rr < (isx ? rows_m : rows_n) ? (uint32_t)((int64_t)rr * (isx ? a.ldx : (int64_t)a.ldw) * (int)sizeof(T)) + kc[i] : kNowhere;
+        }
+        const uint32_t base = lds_address(lds);
+        const auto fill = [&](int t, uint32_t place) {
+            const bool whole = (t + 1) * KB <= kbytes;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const uint32_t o = whole || t * KB + kc[i] < kbytes ? off[i] : kNowhere;
+                buffer_to_lds((i * NW + wave) * RPL < BM ? rx : rw, o, (uint32_t)(t * KB), base + place * kStage + (i * NW + wave) * 1024);
+            }
+        };
+        // While one step's products are formed the next step's operands are read; before the last step of tile t all
+        // waves have its operands in registers, so its place takes tile t + NS.
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+            if (t < nk) fill(t, t);
+        if (NS - 1 < nk) landed_barrier<(NS - 1) * NL>();
+        else landed_barrier<0>();
+        operands(lds, 0);
+        uint32_t place = 0;
+        for (int t = 0; t < nk; ++t) {
+#pragma unroll
+            for (int s = 0; s + 1 < STEPS; ++s) {
+                operands(lds + place * kStage, s + 1);
+                multiply(s);
+            }
+            if (t + 1 < nk) {
+                if (t + NS - 1 < nk) landed_barrier<(NS - 2) * NL>();
+                else landed_barrier<0>();
+                if (t + NS < nk) fill(t + NS, place);
+                place = place + 1 == NS ? 0 : place + 1;
+                operands(lds + place * kStage, 0);
+            }
+            multiply(STEPS - 1);
+        }
+    } else {
+        for (int t = 0; t < nk; ++t) {
+            for (int e = tid; e < (BM + BN) * CPR; e += NT) {
+                const int row = e / CPR, c = e % CPR, k = t * KE + c * PER;
+                chunk v{};
+                if (row < BM) {
+                    if (row < rows_m) v = load_chunk_any<T>(xb + row * a.ldx, k, a.K);
+                } else if (row - BM < rows_n) {
+                    v = load_chunk_any<T>(wb + (int64_t)(row - BM) * a.ldw, k, a.K);
+                }
+                *(chunk*)(lds + row * KB + 16 * swizzle<CPR>(row < BM ? row : row - BM, c)) = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                operands(lds, s);
+                multiply(s);
+            }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+
+    // Sums through LDS: 32 rows of the wave's TN columns at a time, in fp32.
+    constexpr int LD = TN + 4;
+    float* st = (float*)lds + wave * 32 * LD;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -229,26 +329,29 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_k(LinearArgs a) {
             for (int e = 0; e < 4; ++e) {
                 v4f v;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if constexpr (sizeof(T) == 1) v[q] = (float)acc[i][j][4 * e + q];
-                    else v[q] = acc[i][j][4 * e + q];
-                }
-                *(v4f*)(st + (lane & 31) * LD + 32 * j + 8 * e + 4 * (lane >> 5)) = v;
+                for (int q = 0; q < 4; ++q) v[q] = (float)acc[i][j][4 * e + q];
+                *(v4f*)(st + r * LD + 32 * j + 8 * e + 4 * (lane >> 5)) = v;
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int p = 0; p < 32 / RPP; ++p) {
-            const int r = p * RPP + lane / LPR;
-            const int64_t m = m0 + wm * TM + 32 * i + r;
-            const v4f u0 = *(const v4f*)(st + r * LD + 8 * (lane % LPR)), u1 = *(const v4f*)(st + r * LD + 8 * (lane % LPR) + 4);
+        const auto pass = [&](int p, const Raw8* res) {
+            const int row = p * RPP + lane / LPR;
+            const int64_t m = m0 + wm * TM + 32 * i + row;
+            const v4f u0 = *(const v4f*)(st + row * LD + 8 * (lane % LPR)), u1 = *(const v4f*)(st + row * LD + 8 * (lane % LPR) + 4);
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 const float s = q < 4 ? u0[q & 3] : u1[q & 3];
                 v[q] = sizeof(T) == 1 ? (s * a.a_scale) * sc[q] + bs[q] : s + bs[q];
             }
-            if (m < a.M && left > 0) finish8(a, m, nc, left, v);
+            if (m < a.M && left > 0) finish8(a, m, nc, left, v, res);
+        };
+        if (MT == 1 && ahead) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pass(p, &early[MT == 1 ? p : 0]);
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < NP; ++p) pass(p, nullptr);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -330,17 +433,18 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_k(LinearArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- launch
-template <class T, int BM, int BN, int WM, int WN, bool VEC>
+template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC>
 static int launch_tile(LinearArgs& a, hipStream_t s) {
-    constexpr int kStage = (BM + BN) * 128, kOut = WM * WN * 32 * (BN / WN + 4) * 4;
-    const int nk = (a.K * (int)sizeof(T) + 127) / 128;
-    int bytes = kStage * (nk > 1 ? 2 : 1);
+    constexpr int NW = WM * WN, RPL = 1024 / KB;
+    constexpr int kStage = VEC ? ((BM + BN) / RPL + NW - 1) / NW * NW * 1024 : (BM + BN) * KB, kOut = NW * 32 * (BN / WN + 4) * 4;
+    const int nk = (a.K * (int)sizeof(T) + KB - 1) / KB;
+    int bytes = kStage * (!VEC ? 1 : nk < NS ? nk : NS);
     if (bytes < kOut) bytes = kOut;
     const int64_t tm = (a.M + BM - 1) / BM;
     a.tiles_n = (uint32_t)((a.N + BN - 1) / BN);
     PMG_REQUIRE(tm * a.tiles_n < (int64_t)1 << 31, "too many outputs");
     a.tiles = (uint32_t)(tm * a.tiles_n);
-    hipLaunchKernelGGL((linear_tile_k<T, BM, BN, WM, WN, VEC>), dim3(a.tiles), dim3(64 * WM * WN), bytes, s, a);
+    hipLaunchKernelGGL((linear_tile_k<T, BM, BN, WM, WN, KB, NS, VEC>), dim3(a.tiles), dim3(64 * WM * WN), bytes, s, a);
     return check_launch("linear_tile_k");
 }
 
@@ -354,13 +458,40 @@ static int launch_rows(LinearArgs& a, hipStream_t s) {
     return check_launch("linear_rows_k");
 }
 
+// Few outputs (at most a block a CU): the kernel whose waves share out k and whose operands go straight to registers; for
+// fp32, whose products take 16 times as long on the matrix units, up to two. Eight waves where k is long enough to give
+// each two rounds of loads, else four. Measured, K = 1024, fp16: 64 rows to 1024 columns 4.5 us (64 x 64 tiles: 7.3),
+// 1000 rows to 256 columns 8.7 (7.6); fp32: 8.4 (23) and 14 (24).
+//
+// Tiles, by what a CU's share of them costs: k in units of 128 bytes, then the epilogue, in microseconds.
+//   64 x 64     0.27 a unit, 0.4; five blocks a CU. Products bound by memory, and fp32: (76811 x 256) int8 to 256 columns
+//               29 us, the larger tiles 30 to 47.
+//   128 x 128   0.6 and 3, two blocks a CU: 19200 x 256 bf16 to 768 columns 24 us (64 x 64: 26).
+//   256 x 256   2.2 and 16, one block: 8192 x 4096 bf16 to 4096 columns 281 us (980 TFLOP/s; 128 x 128: 310). Its LDS reads
+//               are a quarter fewer a product.
+//   320 x 256   2.4 and 20: where it takes fewer rounds: 4800 x 1024 bf16 to 4096 columns with gelu 61 us (240 tiles on
+//               256 CUs; 128 x 128 67, 256 x 256 83).
 template <class T, bool VEC>
 static int launch_linear(LinearArgs& a, hipStream_t s) {
-    const int64_t t64 = ((a.M + 63) / 64) * ((a.N + 63) / 64), t128 = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (a.M <= 16) return launch_rows<T, 1, 8, VEC>(a, s);
-    if (t64 < 128) return launch_rows<T, 2, 4, VEC>(a, s);
-    if (t128 < 512 || a.N <= 64) return launch_tile<T, 64, 64, 2, 2, VEC>(a, s);
-    return launch_tile<T, 128, 128, 2, 2, VEC>(a, s);
+    const int64_t tn = (a.N + 15) / 16, n1 = (a.M + 15) / 16 * tn, n2 = (a.M + 31) / 32 * tn;
+    const bool lengthy = (int64_t)a.K * (int)sizeof(T) >= 48 * 64;
+    if (n1 <= 256) return lengthy ? launch_rows<T, 1, 8, VEC>(a, s) : launch_rows<T, 1, 4, VEC>(a, s);
+    if (n2 <= (sizeof(T) == 4 ? 512 : 256)) return lengthy ? launch_rows<T, 2, 8, VEC>(a, s) : launch_rows<T, 2, 4, VEC>(a, s);
+    if constexpr (VEC && sizeof(T) < 4) {
+        const double k = (double)((int64_t)a.K * (int)sizeof(T) + 127) / 128;
+        const auto cost = [&](int bm, int bn, double unit, double end) {
+            const int64_t tiles = (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn);
+            return (double)((tiles + 255) / 256) * (k * unit + end);
+        };
+        const double c[4] = {cost(64, 64, 0.27, 0.4), cost(128, 128, 0.6, 3.0), cost(256, 256, 2.2, 16.0), cost(320, 256, 2.4, 20.0)};
+        int best = 0;
+        for (int i = 1; i < 4; ++i)
+            if (c[i] < c[best]) best = i;
+        if (best == 1) return launch_tile<T, 128, 128, 4, 2, 128, 2, VEC>(a, s);
+        if (best == 2) return launch_tile<T, 256, 256, 2, 4, 64, 4, VEC>(a, s);
+        if (best == 3) return launch_tile<T, 320, 256, 2, 4, 64, 3, VEC>(a, s);
+    }
+    return launch_tile<T, 64, 64, 2, 2, 128, 2, VEC>(a, s);
 }
 
 }  // namespace pmg

@@ -27,6 +27,7 @@ struct RopeArgs {
     int layer, interleaved;
     float eps;
     int rows;  // rows a block
+    uint32_t q_magic, k_magic;
 };
 
 template <class T>
@@ -45,88 +46,132 @@ __device__ inline void store4(T* p, const float* v) {
     *(v4t*)p = t;
 }
 
+// Sum over groups of G neighbouring lanes (a power of two up to 16), the same in each of them: neighbours, pairs, then
+// mirrored halves and rows.
+template <int G>
+__device__ inline float group_sum(float v) {
+    if constexpr (G >= 2) v = v + u2f(dpp_u32<0xB1, 0xf>(f2u(v)));
+    if constexpr (G >= 4) v = v + u2f(dpp_u32<0x4E, 0xf>(f2u(v)));
+    if constexpr (G >= 8) v = v + u2f(dpp_u32<0x141, 0xf>(f2u(v)));
+    if constexpr (G >= 16) v = v + u2f(dpp_u32<0x140, 0xf>(f2u(v)));
+    return v;
+}
+
+// The heads of one of the two tensors, rows m0 .. m0 + rows - 1.
+struct RopeSide {
+    const void* x;
+    void* out;
+    int64_t row, head, orow, ohead;
+    int H;
+    uint32_t magic;  // ceil(2^32 / H): item / H for items below 2^16
+    const float* weight;
+    const float* bias;
+};
+
+template <class T, int G, bool INTER, bool LAYER>
+__device__ inline void rope_side(const RopeArgs& a, const RopeSide& s, const float2* turn, int64_t m0, int rows) {
+    const int tid = threadIdx.x, g = tid & (G - 1), D = a.D;
+    // the lane's four pairs: elements pa .. pa + 3 and pb .. pb + 3, or 8 neighbouring ones
+    const bool lane_in = 8 * g < D;
+    const int p0 = lane_in ? 4 * g : 0, pa = INTER ? 2 * p0 : p0, pb = INTER ? pa + 4 : D / 2 + p0;
+    float w[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f}, b[8] = {};
+    if (s.weight) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = s.weight[i < 4 ? pa + i : pb + i - 4];
+    }
+    if (s.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = s.bias[i < 4 ? pa + i : pb + i - 4];
+    }
+    const float inv = 1.0f / (float)D;
+    const T* x0 = (const T*)s.x + m0 * s.row;
+    T* o0 = (T*)s.out + m0 * s.orow;
+    const int items = rows * s.H;
+    for (int at = 0; at < items; at += 256 / G) {  // (every lane of a wave takes part in the sums)
+        const int item = at + tid / G;
+        const bool on = item < items && lane_in;
+        const int r = s.H > 1 ? (int)__umulhi((uint32_t)item, s.magic) : item, h = item - r * s.H;
+        float v[8] = {};
+        if (on) {
+            const T* x = x0 + r * s.row + h * s.head;
+            load4(x + pa, v);
+            load4(x + pb, v + 4);
+        }
+        if constexpr (LAYER) {
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t = t + v[i];
+            const float mean = group_sum<G>(t) * inv;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = on ? v[i] - mean : 0.0f;
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+        const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<G>(ss), inv, a.eps));
+        if (!on) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(v[i] * rstd, w[i], b[i]);
+        if (p0 + 4 <= a.P && a.P % 4 == 0) {
+            const v4f t01 = *(const v4f*)(turn + r * a.P + p0), t23 = *(const v4f*)(turn + r * a.P + p0 + 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float c = j < 2 ? t01[2 * (j & 1)] : t23[2 * (j & 1)], sn = j < 2 ? t01[2 * (j & 1) + 1] : t23[2 * (j & 1) + 1];
+                float& x = v[INTER ? 2 * j : j];
+                float& y = v[INTER ? 2 * j + 1 : 4 + j];
+                const float u = x, z = y;
+                x = __builtin_fmaf(u, c, -(z * sn));
+                y = __builtin_fmaf(u, sn, z * c);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (p0 + j >= a.P) continue;
+                const float2 t = turn[r * a.P + p0 + j];
+                float& x = v[INTER ? 2 * j : j];
+                float& y = v[INTER ? 2 * j + 1 : 4 + j];
+                const float u = x, z = y;
+                x = __builtin_fmaf(u, t.x, -(z * t.y));
+                y = __builtin_fmaf(u, t.y, z * t.x);
+            }
+        }
+        T* o = o0 + r * s.orow + h * s.ohead;
+        store4(o + pa, v);
+        store4(o + pb, v + 4);
+    }
+}
+
 // G lanes a head (a power of two >= D / 8).
-template <class T, int G>
+template <class T, int G, bool INTER, bool LAYER>
 __global__ __launch_bounds__(256) void qk_norm_rope_k(RopeArgs a) {
-    extern __shared__ float2 turn[];  // [rows][P] (cos, sin)
-    const int tid = threadIdx.x, g = tid & (G - 1), D = a.D, h2 = D / 2;
+    extern __shared__ __attribute__((aligned(16))) float2 turn[];  // [rows][P] (cos, sin)
     const int64_t m0 = (int64_t)blockIdx.x * a.rows;
     const int rows = a.M - m0 < a.rows ? (int)(a.M - m0) : a.rows;
-    for (int e = tid; e < rows * a.P; e += 256) {
+    for (int e = threadIdx.x; e < rows * a.P; e += 256) {
         const int r = e / a.P, p = e - r * a.P;
-        const int32_t* c = a.coords + (m0 + r) * 4;
-        double t = (double)c[1] * (double)a.freqs[3 * p];
-        t = __builtin_fma((double)c[2], (double)a.freqs[3 * p + 1], t);
-        t = __builtin_fma((double)c[3], (double)a.freqs[3 * p + 2], t);
+        const int4 c = *(const int4*)(a.coords + (m0 + r) * 4);
+        double t = (double)c.y * (double)a.freqs[3 * p];
+        t = __builtin_fma((double)c.z, (double)a.freqs[3 * p + 1], t);
+        t = __builtin_fma((double)c.w, (double)a.freqs[3 * p + 2], t);
         t = t * 0.15915494309189535;  // turns
         float s, co;
         sincospif((float)(2.0 * (t - __builtin_rint(t))), &s, &co);
         turn[e] = make_float2(co, s);
     }
     __syncthreads();
-    // the lane's four pairs: elements pa .. pa + 3 and pb .. pb + 3, or 8 neighbouring ones
-    const bool lane_in = 8 * g < D;
-    const int p0 = lane_in ? 4 * g : 0, pa = a.interleaved ? 2 * p0 : p0, pb = a.interleaved ? pa + 4 : h2 + p0;
-    float wq[8], wk[8], bq[8], bk[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = i < 4 ? pa + i : pb + i - 4;
-        wq[i] = a.q_weight ? a.q_weight[d] : 1.0f;
-        wk[i] = a.k_weight ? a.k_weight[d] : 1.0f;
-        bq[i] = a.q_bias ? a.q_bias[d] : 0.0f;
-        bk[i] = a.k_bias ? a.k_bias[d] : 0.0f;
-    }
-    const float inv = 1.0f / (float)D;
-    const int heads = a.Hq + a.Hk;
-    const int items = rows * heads, rounds = (items + 256 / G - 1) / (256 / G);
-    for (int it = 0; it < rounds; ++it) {  // (every lane of a wave takes part in the sums)
-        const int item = it * (256 / G) + tid / G;
-        const bool on = item < items && lane_in;
-        const int r = item < items ? item / heads : 0, h = item < items ? item - r * heads : 0;
-        const bool isq = h < a.Hq;
-        const int64_t m = m0 + r;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (on) {
-            const T* x = isq ? (const T*)a.q + m * a.q_row + h * a.q_head : (const T*)a.k + m * a.k_row + (h - a.Hq) * a.k_head;
-            load4(x + pa, v);
-            load4(x + pb, v + 4);
-        }
-        float s = 0.0f, mean = 0.0f;
-        if (a.layer) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s = s + v[i];
-#pragma unroll
-            for (int o = 1; o < G; o <<= 1) s = s + __shfl_xor(s, o, 64);
-            mean = s * inv;
-        }
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] = on ? v[i] - mean : 0.0f;
-            ss = __builtin_fmaf(v[i], v[i], ss);
-        }
-#pragma unroll
-        for (int o = 1; o < G; o <<= 1) ss = ss + __shfl_xor(ss, o, 64);
-        const float rstd = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, inv, a.eps));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(v[i] * rstd, isq ? wq[i] : wk[i], isq ? bq[i] : bk[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (p0 + j < a.P && on) {
-                const float2 t = turn[r * a.P + p0 + j];
-                const int ia = a.interleaved ? 2 * j : j, ib = a.interleaved ? 2 * j + 1 : 4 + j;
-                float& x = v[ia];
-                float& y = v[ib];
-                const float u = x, w = y;
-                x = __builtin_fmaf(u, t.x, -(w * t.y));
-                y = __builtin_fmaf(u, t.y, w * t.x);
-            }
-        }
-        if (on) {
-            T* o = isq ? (T*)a.q_out + m * a.qo_row + h * a.qo_head : (T*)a.k_out + m * a.ko_row + (h - a.Hq) * a.ko_head;
-            store4(o + pa, v);
-            store4(o + pb, v + 4);
-        }
+    rope_side<T, G, INTER, LAYER>(a, RopeSide{a.q, a.q_out, a.q_row, a.q_head, a.qo_row, a.qo_head, a.Hq, a.q_magic, a.q_weight, a.q_bias}, turn, m0, rows);
+    if (a.Hk) rope_side<T, G, INTER, LAYER>(a, RopeSide{a.k, a.k_out, a.k_row, a.k_head, a.ko_row, a.ko_head, a.Hk, a.k_magic, a.k_weight, a.k_bias}, turn, m0, rows);
+}
+
+template <class T, int G>
+static void launch_rope_g(const RopeArgs& a, dim3 grid, size_t lds, hipStream_t s) {
+    const dim3 block(256);
+    if (a.interleaved) {
+        if (a.layer) hipLaunchKernelGGL((qk_norm_rope_k<T, G, true, true>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((qk_norm_rope_k<T, G, true, false>), grid, block, lds, s, a);
+    } else {
+        if (a.layer) hipLaunchKernelGGL((qk_norm_rope_k<T, G, false, true>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((qk_norm_rope_k<T, G, false, false>), grid, block, lds, s, a);
     }
 }
 
@@ -139,13 +184,15 @@ static int launch_rope(RopeArgs& a, hipStream_t s) {
     a.rows = rows;
     const int64_t blocks = (a.M + rows - 1) / rows;
     const size_t lds = sizeof(float2) * (size_t)rows * (size_t)(a.P > 0 ? a.P : 1);
-    const dim3 grid((unsigned)blocks), block(256);
+    a.q_magic = (uint32_t)((((uint64_t)1 << 32) + a.Hq - 1) / (uint64_t)a.Hq);
+    a.k_magic = a.Hk ? (uint32_t)((((uint64_t)1 << 32) + a.Hk - 1) / (uint64_t)a.Hk) : 0;
+    const dim3 grid((unsigned)blocks);
     switch (G) {
-        case 1: hipLaunchKernelGGL((qk_norm_rope_k<T, 1>), grid, block, lds, s, a); break;
-        case 2: hipLaunchKernelGGL((qk_norm_rope_k<T, 2>), grid, block, lds, s, a); break;
-        case 4: hipLaunchKernelGGL((qk_norm_rope_k<T, 4>), grid, block, lds, s, a); break;
-        case 8: hipLaunchKernelGGL((qk_norm_rope_k<T, 8>), grid, block, lds, s, a); break;
-        default: hipLaunchKernelGGL((qk_norm_rope_k<T, 16>), grid, block, lds, s, a); break;
+        case 1: launch_rope_g<T, 1>(a, grid, lds, s); break;
+        case 2: launch_rope_g<T, 2>(a, grid, lds, s); break;
+        case 4: launch_rope_g<T, 4>(a, grid, lds, s); break;
+        case 8: launch_rope_g<T, 8>(a, grid, lds, s); break;
+        default: launch_rope_g<T, 16>(a, grid, lds, s); break;
     }
     return check_launch("qk_norm_rope_k");
 }
@@ -166,6 +213,7 @@ extern "C" int pmg_qk_norm_rope(const pmg_rope_args* p, void* stream) {
     if (r.M == 0) return PMG_OK;
     PMG_REQUIRE(r.q && r.q_out && (r.Hk == 0 || (r.k && r.k_out)), "null buffer");
     PMG_REQUIRE(r.pairs == 0 || (r.coords && r.freqs), "rotation needs coords and freqs");
+    PMG_REQUIRE(aligned16(r.coords), "coords must be 16-byte aligned");
     const int es = r.type == PMG_TYPE_F32 ? 4 : 2;
     auto ok = [&](const void* b, int64_t row, int64_t head) {
         return (reinterpret_cast<uintptr_t>(b) & (uintptr_t)(4 * es - 1)) == 0 && row % 4 == 0 && head % 4 == 0;

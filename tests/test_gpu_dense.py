@@ -46,6 +46,21 @@ def test_linear_sizes(gpu, dt, M, K, N):
     check_linear(gpu, M, K, N, dt, seed=M + K + N)
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M,K,N", [(4099, 200, 1030), (4800, 1024, 4096), (8200, 1024, 2056), (20_000, 264, 776), (33_000, 64, 520)])
+def test_linear_large(gpu, dt, M, K, N):
+    """Every tile shape, with rows, columns and k that end inside a tile; checked on a sample of rows in 64 bits."""
+    g = torch.Generator(device=gpu).manual_seed(M)
+    x = torch.randn((M, K), device=gpu, generator=g).to(dt)
+    w = (torch.randn((N, K), device=gpu, generator=g) / math.sqrt(K)).to(dt)
+    b, r = torch.randn(N, device=gpu, generator=g), torch.randn((M, N), device=gpu, generator=g).to(dt)
+    announce(f"linear large {dt} {M} {K} {N}")
+    got = ops.linear(x, w, b, act="gelu", residual=r)
+    rows = torch.cat([torch.arange(0, M, 37), torch.arange(M - 70, M)]).to(gpu)
+    want, tol = ref.linear(x[rows], w, b, act="gelu", residual=r[rows], out_dtype=dt)
+    ref.assert_within(got[rows], want, tol)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (5, 3, 64), (300, 7, 33), (9000, 3, 64), (2000, 65, 1), (4097, 130, 129), (70, 1021, 77)])
 def test_linear_odd_widths(gpu, dt, M, K, N):
@@ -317,6 +332,19 @@ def test_attention_rising_scores(gpu, dt):
         edit(q, kv, kw)
         kv[:, 0] = kv[:, 0].flip(0)
     check_attention(gpu, dt, [600], 2, 2, 32, scale=0.5, edit=down)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_attention_first_keys_far_away(gpu, dt):
+    """The first keys' scores lie thousands below the later ones' (and below 2^-128 of anything): they set the running
+    maximum first and then count for nothing."""
+    def edit(q, kv, kw):
+        kw["coords"][:, 1:] = 5
+        kw["coords"][:96, 1] = 20_000  # keys 0 .. 95 of the first segment, queries there included
+        kw["coords"][500:560, 3] = -30_000
+    check_attention(gpu, dt, [400, 300], 2, 2, 32, bias=True, edit=edit)
+    check_attention(gpu, dt, [3, 2], 2, 2, 64, kv_lengths=[3000, 900], bias=True, top=5, edit=lambda q, kv, kw: (
+        kw["kv_coords"].__setitem__((slice(0, 2900), 2), 9_000), kw["kv_coords"].__setitem__((slice(3000, 3500), 2), 9_000)))
 
 
 @pytest.mark.parametrize("dt", TYPES)
