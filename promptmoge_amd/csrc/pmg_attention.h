@@ -4,7 +4,7 @@
 //          cap(scale q_i . k_j) - sum over axes of slope[head][axis] |c_i - c_j|[axis],   cap(x) = cap tanh(x / cap)
 //
 // One pass over the keys with the running maximum m and sum l of the softmax (fp32, in powers of two). A wave owns 32
-// slots (QT times): a slot is a query position and one of the G query heads that share a key head. The products are
+// slots: a slot is a query position and one of the G query heads that share a key head. The products are
 // formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds 16 scores of ONE slot: maximum and sum are
 // taken in the lane and once across the two halves of the wave, and the scores, rounded to the inputs' type (the
 // weights of the second product; l sums the unrounded ones), are that product's operand as they lie. V^T comes from
@@ -13,7 +13,7 @@
 // banks' swizzle is made by the choice of chunk, and an absent row (masked, behind its segment, a bad index) is fetched
 // from a line of zeros. The rows' numbers, mask and coordinates are looked up a key a thread, a group of tiles ahead.
 //
-// Queries are taken in order of position, 32 NW QT / G positions a block, whatever segments they fall in: the block
+// Queries are taken in order of position, 32 NW / G positions a block, whatever segments they fall in: the block
 // walks over the keys of all its segments, and each lane counts the keys of its own. No work list is needed, and small
 // cells share a wave. A weight of 0 times a value that is infinite or NaN is NaN: where outputs of a block over
 // several segments are not finite, the block goes over its segments one by one. (SEG: a block per segment, for few
@@ -44,6 +44,8 @@ struct AttnArgs {
     float scale2;         // scale log2(e)
     float cap2, cap_arg;  // cap log2(e); the factor of tanh's argument (0 cap: none)
     int seg, splits, zero_rest;
+    int whole;  // blocks of one segment each
+    int near;   // K and V each below 4 GiB, heads of full width: rows are fetched by 32-bit byte offsets
     uint32_t blocks;
     float* part_o;  // [splits][Hq][Pq][D]; (m, l) [splits][Hq][Pq], l < 0: a position of no segment
     float2* part_ml;
@@ -84,6 +86,29 @@ __device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t fi
     if (c == 64) return segment_of(off, S, p);
     const int64_t s = lo + c - 1;
     return s < S ? (int32_t)s : -1;
+}
+
+// Blocks that hold one segment each: interval j of S + 2 (the rows before the segments, the segments, the rows behind) from
+// starts(j) on has the blocks from floor(G starts(j) / per) + j on, which are enough for its slots, one too many at most;
+// so block `unit` finds its interval, and its slots [slot0, slot1), by a search in the offsets alone. Returns the segment, or -1.
+__device__ inline int32_t unit_segment(const int64_t* off, int64_t S, int64_t P, int G, int per, uint32_t unit, int64_t& slot0, int64_t& slot1) {
+    const int lane = threadIdx.x & 63;
+    const auto starts = [&](int64_t j) { return j == 0 ? 0 : clamp64(off[j - 1], 0, P); };
+    const auto first = [&](int64_t j) { return starts(j) * G / per + j; };
+    int64_t lo = 0, n = S + 2;  // intervals before lo start at or before the block, those from lo + n on do not
+    while (n > 0) {
+        const int64_t step = (n + 63) >> 6, j = (lane + 1) * step - 1;
+        const bool le = j < n && first(lo + j) <= (int64_t)unit;
+        const int t = __popcll(__ballot(le));
+        lo += t * step;
+        n -= t * step;
+        n = n < step - 1 ? n : step - 1;
+    }
+    const int64_t j = lo > 0 ? lo - 1 : 0;
+    slot0 = starts(j) * G + ((int64_t)unit - first(j)) * per;
+    slot1 = j <= S ? starts(j + 1) * G : P * G;
+    slot1 = slot0 + per < slot1 ? slot0 + per : slot1;
+    return j >= 1 && j <= S ? (int32_t)(j - 1) : -1;
 }
 
 // What absent keys and values are fetched from.
@@ -139,7 +164,8 @@ constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
 
 // Registers: with at most 256 the matrix instructions' results stay in ordinary vector registers, where the softmax
 // works on them; only the widest fp32 form of one wave needs more.
-template <class T, int DP, int NW, int QT, bool BIAS>
+// MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use).
+template <class T, int DP, int NW, bool BIAS, bool MASK>
 __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void attention_k(AttnArgs a0) {
     const AttnArgs& a = a0;
     constexpr int ES = sizeof(T), PER = 16 / ES, CPR = DP / PER, NT = 64 * NW;
@@ -154,7 +180,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     __shared__ __attribute__((aligned(16))) char s_v[2][BK * DP * ES];
     constexpr int SB = NT, TPS = SB / BK;  // keys (and tiles) whose numbers are looked up at a time, one a thread
     __shared__ uint32_t s_ok[2][SB / 32];  // which keys there are
-    __shared__ int32_t s_row[2][SB];
+    __shared__ uint2 s_row[2][SB];         // their rows of K and V: byte offsets (near), or the row's number
     __shared__ __attribute__((aligned(16))) uint4 s_xy[2 * (BIAS ? SB : 1) + 1];  // coordinates; their parts' weights
     __shared__ __attribute__((aligned(16))) uint2 s_z[2 * (BIAS ? SB : 1) + 1];
     static_assert(TPS >= 2, "a group's numbers are written while its predecessor's first tile is worked on");
@@ -177,6 +203,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
 
     // slots of the block: [slot0, slot1) of all positions' G slots (SEG: of the segment's)
     int64_t slot0, slot1;
+    int32_t own = -1;  // the block's segment, with blocks of one segment each
     int32_t seg_lo = 0, seg_hi = 0;  // (positions and rows fit 32 bits)
     if constexpr (SEG) {
         const int64_t p0 = clamp64(a.q_off[unit], 0, a.Pq), p1 = clamp64(a.q_off[unit + 1], 0, a.Pq);
@@ -184,40 +211,40 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
         slot1 = p1 * a.G;
         seg_lo = (int32_t)clamp64(a.k_off[unit], 0, a.Pk);
         seg_hi = (int32_t)clamp64(a.k_off[unit + 1], seg_lo, a.Pk);
+    } else if (a.whole) {
+        own = unit_segment(a.q_off, a.S, a.Pq, a.G, 32 * NW, unit, slot0, slot1);
     } else {
-        slot0 = (int64_t)unit * (32 * NW * QT);
-        slot1 = slot0 + 32 * NW * QT;
+        slot0 = (int64_t)unit * (32 * NW);
+        slot1 = slot0 + 32 * NW;
         if (slot1 > a.Pq * a.G) slot1 = a.Pq * a.G;
     }
 
-    for (int64_t base = slot0; base < slot1; base += SEG ? 32 * NW * QT : (int64_t)1 << 40) {
+    if (slot0 >= slot1) return;
+    for (int64_t base = slot0;;) {
         // ---- the lane's slots
         const int tid = thread_again(), lane = tid & 63, half = lane >> 5;
-        int32_t pos[QT], lo[QT], hi[QT], row[QT], seg[QT], head[QT];
+        int32_t pos, lo, hi, row, seg, head;
         int32_t blo = (int32_t)a.Pk, bhi = 0;
-        const int64_t wfirst = base + wave * QT * 32;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int64_t slot = base + (wave * QT + t) * 32 + (lane & 31);
-            const bool in = slot < slot1;
-            pos[t] = in ? (int32_t)(slot / a.G) : -1;
-            head[t] = hk * a.G + (in ? (int)(slot - (int64_t)pos[t] * a.G) : 0);
-            row[t] = -1;
-            seg[t] = -1;
-            lo[t] = hi[t] = 0;
-            int32_t sg = (int32_t)unit;
-            if (!SEG && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos[t] : 0x7ffffffe);
-            if (in) {
-                const int32_t r = a.q_index ? a.q_index[pos[t]] : pos[t];
-                row[t] = r >= 0 && r < a.Mq ? r : -1;
-                seg[t] = sg;
-                if (seg[t] >= 0) {
-                    lo[t] = SEG ? seg_lo : (int32_t)clamp64(a.k_off[seg[t]], 0, a.Pk);
-                    hi[t] = SEG ? seg_hi : (int32_t)clamp64(a.k_off[seg[t] + 1], lo[t], a.Pk);
-                    if (hi[t] > lo[t]) {
-                        blo = lo[t] < blo ? lo[t] : blo;
-                        bhi = hi[t] > bhi ? hi[t] : bhi;
-                    }
+        const int64_t wfirst = base + wave * 32;
+        const int64_t slot = base + wave * 32 + (lane & 31);
+        const bool in = slot < slot1;
+        pos = in ? (int32_t)(slot / a.G) : -1;
+        head = hk * a.G + (in ? (int)(slot - (int64_t)pos * a.G) : 0);
+        row = -1;
+        seg = -1;
+        lo = hi = 0;
+        int32_t sg = SEG ? (int32_t)unit : own;
+        if (!SEG && !a.whole && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos : 0x7ffffffe);
+        if (in) {
+            const int32_t r = a.q_index ? a.q_index[pos] : pos;
+            row = r >= 0 && r < a.Mq ? r : -1;
+            seg = sg;
+            if (seg >= 0) {
+                lo = SEG ? seg_lo : (int32_t)clamp64(a.k_off[seg], 0, a.Pk);
+                hi = SEG ? seg_hi : (int32_t)clamp64(a.k_off[seg + 1], lo, a.Pk);
+                if (hi > lo) {
+                    blo = lo < blo ? lo : blo;
+                    bhi = hi > bhi ? hi : bhi;
                 }
             }
         }
@@ -242,17 +269,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
         }
         // keys that every slot of the wave sees (slots of no segment take whatever comes)
         int32_t ilo = 0, ihi = 0x7fffffff;
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-            if (seg[t] >= 0) {
-                ilo = lo[t] > ilo ? lo[t] : ilo;
-                ihi = hi[t] < ihi ? hi[t] : ihi;
-            }
+        if (seg >= 0) {
+            ilo = lo;
+            ihi = hi;
+        }
         ilo = wave_extreme<true>(ilo);
         ihi = wave_extreme<false>(ihi);
-        bool part_seen = false;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) part_seen = part_seen || (seg[t] >= 0 && hi[t] > lo[t] && (lo[t] != blo || hi[t] != bhi));
+        const bool part_seen = seg >= 0 && hi > lo && (lo != blo || hi != bhi);
         if (a.splits > 1 && bhi > blo) {
             const int64_t each = (((int64_t)bhi - blo + a.splits - 1) / a.splits + BK - 1) / BK * BK;
             blo = (int32_t)(blo + split * each < bhi ? blo + split * each : bhi);
@@ -260,34 +283,31 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
         }
 
         // ---- the queries, and their coordinates' operands
-        chunk qf[QT][QC];
-        v8bf qc[QT][3];
-        float sl[QT][3];
+        chunk qf[QC];
+        v8bf qc[3];
+        float sl[3];
+        const T* qp = (const T*)a.q + (int64_t)(row >= 0 ? row : 0) * a.q_row + head * a.q_head;
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const T* qp = (const T*)a.q + (int64_t)(row[t] >= 0 ? row[t] : 0) * a.q_row + head[t] * a.q_head;
+        for (int c = 0; c < QC; ++c) {
+            const int cc = 2 * c + half;
+            qf[c] = chunk{};
+            if (row >= 0 && cc * PER < a.D) qf[c] = *(const chunk*)(qp + cc * PER);
+        }
+        if constexpr (BIAS) {
+            // The difference of two coordinates as a product of 16 terms: the key's parts (8 bits each, exact in
+            // bf16) times their weights 1, 2^8, 2^16, 2^24 in the lower half's lanes, the weights times the query's
+            // negated parts in the upper half's; exact up to 2^23. The key's operand holds two axes at a time, the
+            // query's is 0 for the other one.
 #pragma unroll
-            for (int c = 0; c < QC; ++c) {
-                const int cc = 2 * c + half;
-                qf[t][c] = chunk{};
-                if (row[t] >= 0 && cc * PER < a.D) qf[t][c] = *(const chunk*)(qp + cc * PER);
-            }
-            if constexpr (BIAS) {
-                // The difference of two coordinates as a product of 16 terms: the key's parts (8 bits each, exact in
-                // bf16) times their weights 1, 2^8, 2^16, 2^24 in the lower half's lanes, the weights times the query's
-                // negated parts in the upper half's; exact up to 2^23. The key's operand holds two axes at a time, the
-                // query's is 0 for the other one.
+            for (int x = 0; x < 3; ++x) {
+                const int32_t c = row >= 0 ? a.q_coords[(int64_t)row * 4 + 1 + x] : 0;
+                sl[x] = -a.slopes[head * 3 + x] * PMG_LOG2E;
+                const float p[4] = {(float)(c & 255), (float)((c >> 8) & 255), (float)((c >> 16) & 255), (float)(c >> 24)};
+                const float w[4] = {1.0f, 256.0f, 65536.0f, 16777216.0f};
 #pragma unroll
-                for (int x = 0; x < 3; ++x) {
-                    const int32_t c = row[t] >= 0 ? a.q_coords[(int64_t)row[t] * 4 + 1 + x] : 0;
-                    sl[t][x] = -a.slopes[head[t] * 3 + x] * PMG_LOG2E;
-                    const float p[4] = {(float)(c & 255), (float)((c >> 8) & 255), (float)((c >> 16) & 255), (float)(c >> 24)};
-                    const float w[4] = {1.0f, 256.0f, 65536.0f, 16777216.0f};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        qc[t][x][i] = (__bf16)(x == 1 ? 0.0f : half ? -p[i] : w[i]);
-                        qc[t][x][4 + i] = (__bf16)(x != 1 ? 0.0f : half ? -p[i] : w[i]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    qc[x][i] = (__bf16)(x == 1 ? 0.0f : half ? -p[i] : w[i]);
+                    qc[x][4 + i] = (__bf16)(x != 1 ? 0.0f : half ? -p[i] : w[i]);
                 }
             }
         }
@@ -310,17 +330,16 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
             }
             const int32_t nt = khi > klo ? (khi - klo + (BK - 1)) / BK : 0;
 
-            v16f O[QT][NB];
-            float m[QT], l[QT], grow[QT];
+            v16f O[NB];
+            float m, l, grow;
+            bool look;  // the maximum is looked for: some slot of the wave has none yet, or a weight grew too large
             const float k2 = a.cap2 != 0.0f ? 1.0f : a.scale2;
+            m = 0.0f;
+            grow = -__builtin_inff();
+            l = 0.0f;
+            look = true;
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                m[t] = 0.0f;
-                grow[t] = -__builtin_inff();
-                l[t] = 0.0f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) O[t][b] = v16f{};
-            }
+            for (int b = 0; b < NB; ++b) O[b] = v16f{};
 
             // ---- the keys' numbers, mask and coordinates, by groups of SB
             int32_t mi = -1;  // the thread's row in the group whose mask and coordinates come next
@@ -341,7 +360,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 const bool on = mi >= 0 && mm != 0;
                 const uint64_t w = __ballot(on);
                 if (lane < 2) s_ok[b][2 * wave + lane] = (uint32_t)(w >> (32 * lane));
-                s_row[b][tid] = on ? mi : -1;
+                // (absent: behind the buffer's end, whichever chunk is added; or -1)
+                s_row[b][tid] = !on ? make_uint2(0xffff0000u, 0xffff0000u)
+                                    : make_uint2((uint32_t)mi * (a.near ? (uint32_t)a.k_row * ES : 1u), (uint32_t)mi * (a.near ? (uint32_t)a.v_row * ES : 1u));
                 if constexpr (BIAS) {
                     const auto b16 = [](int v) { return f2u((float)v) >> 16; };  // (exact: 8 bits)
                     const auto p01 = [&](int v) { return b16(v & 255) | (b16((v >> 8) & 255) << 16); };
@@ -350,35 +371,37 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                     s_z[b * SB + tid] = make_uint2(p01(mc.w), p23(mc.w));
                 }
             };
-            // (rows are less than 2^31 bytes apart; a chunk behind the head's width is the line of zeros of every row)
-            const char *kb[NCH], *vb[NCH];
-            uint32_t ks[NCH], vs[NCH];
+            // Tile t into buffer b. Near: a load behind the buffer's end is a row of zeros. Otherwise 64-bit addresses (rows
+            // are less than 2^31 bytes apart); absent rows and chunks behind the head's width come from a line of zeros.
+            const bool near = a.near;
+            const v4i kr = buffer_of((const T*)a.k + hk * a.k_head, (uint32_t)((a.Mk - 1) * a.k_row + DP) * ES);
+            const v4i vr = buffer_of((const T*)a.v + hk * a.v_head, (uint32_t)((a.Mk - 1) * a.v_row + DP) * ES);
+            const uint32_t lk = lds_address(s_k[0]) + wave * 1024, lv = lds_address(s_v[0]) + wave * 1024;
+            const auto fetch = [&](int b, uint32_t t) {
+                const uint2* rows = &s_row[(t / TPS) & 1][(t % TPS) * BK];
+                if (near) {
 #pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int e = (i * NW + wave) * 64 + lane, r = e / CPR, p = e % CPR;
-                const int ck = kswz(r, p) * PER, cv = vswz(r, p) * PER;
-                kb[i] = ck < a.D ? (const char*)((const T*)a.k + hk * a.k_head + ck) : (const char*)&g_zeros;
-                vb[i] = cv < a.D ? (const char*)((const T*)a.v + hk * a.v_head + cv) : (const char*)&g_zeros;
-                ks[i] = ck < a.D ? (uint32_t)a.k_row * ES : 0u;
-                vs[i] = cv < a.D ? (uint32_t)a.v_row * ES : 0u;
-            }
-            const auto fetch = [&](int b, uint32_t t) {  // tile t into buffer b
-                const int32_t* rows = &s_row[(t / TPS) & 1][(t % TPS) * BK];
-                const uint32_t* oks = &s_ok[(t / TPS) & 1][(t % TPS) * KB];
-                uint32_t all = oks[0];
-                if constexpr (KB == 2) all &= oks[1];
-                all = __builtin_amdgcn_readfirstlane(all);
-#pragma unroll
-                for (int i = 0; i < NCH; ++i) {
-                    const int32_t row = rows[((i * NW + wave) * 64 + lane) / CPR];
-                    const char* kp = kb[i] + (uint64_t)(uint32_t)row * ks[i];
-                    const char* vp = vb[i] + (uint64_t)(uint32_t)row * vs[i];
-                    if (all != 0xffffffffu) {
-                        kp = row >= 0 ? kp : (const char*)&g_zeros;
-                        vp = row >= 0 ? vp : (const char*)&g_zeros;
+                    for (int i = 0; i < NCH; ++i) {
+                        const int e = (i * NW + wave) * 64 + lane, r = e / CPR, p = e % CPR;
+                        const uint2 row = rows[r];
+                        const uint32_t to = b * (BK * DP * ES) + i * NW * 1024;
+                        buffer_to_lds(kr, row.x + kswz(r, p) * 16, 0, lk + to);
+                        buffer_to_lds(vr, row.y + vswz(r, p) * 16, 0, lv + to);
                     }
-                    load_to_lds(kp, s_k[b] + (i * NW + wave) * 1024);
-                    load_to_lds(vp, s_v[b] + (i * NW + wave) * 1024);
+                } else {
+                    const int lane = thread_again() & 63;  // (its addresses are not kept in registers)
+#pragma unroll
+                    for (int i = 0; i < NCH; ++i) {
+                        const int e = (i * NW + wave) * 64 + lane, r = e / CPR, p = e % CPR;
+                        const int ck = kswz(r, p) * 16, cv = vswz(r, p) * 16;
+                        const uint2 row = rows[r];
+                        const uint32_t to = b * (BK * DP * ES) + i * NW * 1024;
+                        const bool on = (int32_t)row.x >= 0;
+                        const char* kp = (const char*)((const T*)a.k + hk * a.k_head) + (uint64_t)row.x * ((uint32_t)a.k_row * ES) + ck;
+                        const char* vp = (const char*)((const T*)a.v + hk * a.v_head) + (uint64_t)row.y * ((uint32_t)a.v_row * ES) + cv;
+                        load_to_lds(on && ck < a.D * ES ? kp : (const char*)&g_zeros, lk + to);
+                        load_to_lds(on && cv < a.D * ES ? vp : (const char*)&g_zeros, lv + to);
+                    }
                 }
             };
             if (nt > 0) {
@@ -391,6 +414,20 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 fetch(0, 0);
                 loads_landed<0>();
             }
+            // Keys can be taken out by a product with -inf where no query is infinite or NaN (an absent key's zeros times
+            // that) and no cap makes it finite.
+            uint32_t minus = 0xffffffffu;
+            if constexpr (MASK) {
+                bool odd = a.cap2 != 0.0f;
+                v16f z = {};
+#pragma unroll
+                for (int c = 0; c < QC; ++c) z = Mat<T>::mma32(chunk{}, qf[c], z);
+                odd = odd || z[0] != 0.0f;
+                if (__any(odd)) minus = 0u;
+            }
+            // (vmcnt(0) as the compiler counts: else it waits for the queries, and with them for the next tile, at their
+            // every use in the loop)
+            __builtin_amdgcn_s_waitcnt(0x0f70);
             __syncthreads();
 
             for (int32_t it = 0; it < nt; ++it) {
@@ -414,11 +451,19 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                     const char* sv = s_v[cur] + 32 * b * DP * ES;
                     const int kn = slot * SB + k0 + 32 * b;  // its keys' numbers
                     const uint32_t ok = __builtin_amdgcn_readfirstlane((&s_ok[0][0])[kn / 32]);
-                    const bool all = p0 >= ilo && ihi - p0 >= 32 && ok == 0xffffffffu;
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) {
-                        // ---- scores
-                        v16f s = {};
+                    const bool inside = p0 >= ilo && ihi - p0 >= 32;  // every slot's keys
+                    // ---- scores
+                    v16f s;
+                    const auto scores = [&]() {
+                        s = v16f{};
+                        // keys that are absent for every slot: -inf from one more product, of (0 or -inf) x 1. The select
+                        // below costs two instructions a score
+                        if constexpr (MASK) {
+                            const uint32_t off = ((half ? 0u : ~ok & minus) >> (lane & 31)) & 1u;
+                            typedef short v4s __attribute__((ext_vector_type(4)));
+                            const v4s kx = {(short)(off * 0xff80u), 0, 0, 0}, qx = {(short)(half ? 0 : 0x3f80), 0, 0, 0};
+                            s = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(kx, qx, s, 0, 0, 0);
+                        }
                         constexpr int QG = QC < 4 ? QC : 4;  // operand chunks at a time
 #pragma unroll
                         for (int c0 = 0; c0 < QC; c0 += QG) {
@@ -427,7 +472,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
 #pragma unroll
                             for (int c = 0; c < QG; ++c) kf[c] = *(const chunk*)(sk + r * DP * ES + 16 * kswz(r, 2 * (c0 + c) + half));
 #pragma unroll
-                            for (int c = 0; c < QG; ++c) s = Mat<T>::mma32(kf[c], qf[t][c0 + c], s);
+                            for (int c = 0; c < QG; ++c) s = Mat<T>::mma32(kf[c], qf[c0 + c], s);
                         }
                         // less the maximum so far, in powers of two
                         if (a.cap2 != 0.0f) {
@@ -444,20 +489,20 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                             v16f u;
 #pragma unroll
                             for (int x = 0; x < 3; ++x) {
-                                const v16f d = Mat<__bf16>::mma32(x < 2 ? kxy : kz, qc[t][x], v16f{});
+                                const v16f d = Mat<__bf16>::mma32(x < 2 ? kxy : kz, qc[x], v16f{});
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) u[e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[t][x], x == 0 ? -m[t] : u[e]);
+                                for (int e = 0; e < 16; ++e) u[e] = __builtin_fmaf(__builtin_fabsf(d[e]), sl[x], x == 0 ? -m : u[e]);
                                 __builtin_amdgcn_sched_barrier(0);  // (one difference's registers at a time)
                             }
 #pragma unroll
                             for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], k2, u[e]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], k2, -m[t]);
+                            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], k2, -m);
                         }
                         // ---- the keys that count for the lane's slot
-                        if (!all) {
-                            const int x = lo[t] - p0, y = hi[t] - p0;
+                        if (!inside || (ok | (MASK ? minus : 0u)) != 0xffffffffu) {
+                            const int x = lo - p0, y = hi - p0;
                             uint32_t w = y >= 32 ? 0xffffffffu : y <= 0 ? 0u : (1u << y) - 1u;
                             w &= x <= 0 ? 0xffffffffu : x >= 32 ? 0u : ~((1u << x) - 1u);
                             w = (w & ok) >> (4 * half);
@@ -467,64 +512,79 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                                 s[e] = u2f((on & f2u(s[e])) | (~on & 0xff800000u));
                             }
                         }
-                        // ---- running maximum: set by the first keys, then moved only when it grows by more than
-                        // 2^8 for some slot of the wave (weights of up to 2^8 lose nothing)
+                    };
+                    // ---- weights; the running maximum is set by the first keys, then moved only when a weight grows beyond 2^8
+                    // (up to 2^12 nothing is lost). That shows in the sum of a lane's 16 weights: only then the
+                    // scores are formed again and their maximum looked for.
+                    float sum;
+                    const auto weights = [&]() {
+                        float part[4];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            s[e] = __builtin_amdgcn_exp2f(s[e]);
+                            part[e & 3] = e < 4 ? s[e] : part[e & 3] + s[e];
+                        }
+                        sum = (part[0] + part[1]) + (part[2] + part[3]);
+                    };
+                    if (!look) {
+                        scores();
+                        weights();
+                        look = __any(sum > 4096.0f);
+                    }
+                    if (look) {
+                        scores();
                         float mx = s[0];
 #pragma unroll
                         for (int e = 1; e < 16; ++e) mx = __builtin_fmaxf(mx, s[e]);
                         mx = halves_max(mx);
-                        if (__any(mx > grow[t])) {
+                        if (__any(mx > grow)) {
                             const bool any = mx > -__builtin_inff();  // (a slot without a key so far keeps m = 0)
-                            const float up = any && (mx > 0.0f || grow[t] < 0.0f) ? mx : 0.0f;
+                            const float up = any && (mx > 0.0f || grow < 0.0f) ? mx : 0.0f;
                             // (nothing to scale before the first key, whose score may be far below -2^7)
-                            const float al = grow[t] < 0.0f ? 1.0f : __builtin_amdgcn_exp2f(-up);
-                            grow[t] = any ? 8.0f : grow[t];
-                            m[t] = m[t] + up;
-                            l[t] = l[t] * al;
+                            const float al = grow < 0.0f ? 1.0f : __builtin_amdgcn_exp2f(-up);
+                            grow = any ? 8.0f : grow;
+                            m = m + up;
+                            l = l * al;
 #pragma unroll
                             for (int e = 0; e < 16; ++e) s[e] = s[e] - up;
 #pragma unroll
                             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) O[t][n][e] = O[t][n][e] * al;
+                                for (int e = 0; e < 16; ++e) O[n][e] = O[n][e] * al;
                         }
-                        float sum = 0.0f;
+                        weights();
+                        look = __any(grow < 0.0f);
+                    }
+                    l = l + sum;
+                    typedef short v4s __attribute__((ext_vector_type(4)));
+                    typedef short v8s __attribute__((ext_vector_type(8)));
+                    typedef __attribute__((address_space(3))) v4s* lds4;
+                    const auto values = [&](int f, int n) {  // V^T: columns 32 n on, keys 16 f on
+                        const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                        const int r = 16 * f + 4 * half + (i >> 2);
+                        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + r * DP * 2 + 16 * vswz(r, c) + (i & 1) * 8));
+                        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + (r + 8) * DP * 2 + 16 * vswz(r + 8, c) + (i & 1) * 8));
+                        return __builtin_bit_cast(chunk, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    };
+                    // ---- O^T += V^T P^T
+                    if constexpr (ES == 4) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            s[e] = __builtin_amdgcn_exp2f(s[e]);
-                            sum = sum + s[e];
+                            const int r = (e & 3) + 8 * (e >> 2) + 4 * half;
+#pragma unroll
+                            for (int n = 0; n < NB; ++n) {
+                                const float vf = *(const float*)(sv + r * DP * 4 + (32 * n + (lane & 31)) * 4);
+                                O[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[e], O[n], 0, 0, 0);
+                            }
                         }
-                        l[t] = l[t] + sum;
-                        // ---- O^T += V^T P^T
-                        if constexpr (ES == 4) {
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int r = (e & 3) + 8 * (e >> 2) + 4 * half;
+                        for (int f = 0; f < 2; ++f) {
+                            chunk pf;
 #pragma unroll
-                                for (int n = 0; n < NB; ++n) {
-                                    const float vf = *(const float*)(sv + r * DP * 4 + (32 * n + (lane & 31)) * 4);
-                                    O[t][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[e], O[t][n], 0, 0, 0);
-                                }
-                            }
-                        } else {
-                            typedef short v4s __attribute__((ext_vector_type(4)));
-                            typedef short v8s __attribute__((ext_vector_type(8)));
-                            typedef __attribute__((address_space(3))) v4s* lds4;
+                            for (int i = 0; i < 8; ++i) pf[i] = (T)s[8 * f + i];
 #pragma unroll
-                            for (int f = 0; f < 2; ++f) {
-                                chunk pf;
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) pf[i] = (T)s[8 * f + i];
-#pragma unroll
-                                for (int n = 0; n < NB; ++n) {
-                                    const int i = lane & 15, c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                                    const int r = 16 * f + 4 * half + (i >> 2);
-                                    const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + r * DP * 2 + 16 * vswz(r, c) + (i & 1) * 8));
-                                    const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(sv + (r + 8) * DP * 2 + 16 * vswz(r + 8, c) + (i & 1) * 8));
-                                    const v8s vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                                    O[t][n] = Mat<T>::mma32(__builtin_bit_cast(chunk, vv), pf, O[t][n]);
-                                }
-                            }
+                            for (int n = 0; n < NB; ++n) O[n] = Mat<T>::mma32(values(f, n), pf, O[n]);
                         }
                     }
                 }
@@ -543,11 +603,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
             if (only < 0) {
                 float bad = 0.0f;
 #pragma unroll
-                for (int t = 0; t < QT; ++t)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) bad = __builtin_fmaf(O[t][b][e], 0.0f, bad);
+                    for (int e = 0; e < 16; ++e) bad = __builtin_fmaf(O[b][e], 0.0f, bad);
                 // (a wave that sees part of the keys: its own lanes; each wave's keys are the block's)
                 bool again = __any(part_seen) && __any(bad != 0.0f);
                 if constexpr (NW > 1) {
@@ -562,46 +620,41 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 }
             }
             // ---- results (before a second turn: those of no segment only)
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                const float lt = halves_sum(l[t]);
-                const bool mine = only == -2 ? seg[t] < 0 : only < 0 || seg[t] == only;
-                if (a.splits > 1) {
-                    const int64_t o = ((int64_t)split * a.Hq + head[t]) * a.Pq + pos[t];
-                    if (mine && pos[t] >= 0 && half == 0)
-                        a.part_ml[o] = make_float2(grow[t] > 0.0f ? m[t] : -__builtin_inff(), seg[t] >= 0 ? lt : -1.0f);
-                    if (mine && seg[t] >= 0) {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int g = 0; g < 4; ++g) {
-                                const int d = 32 * b + 8 * g + 4 * half;
-                                if (d < a.D) *(float4*)(a.part_o + o * a.D + d) = make_float4(O[t][b][4 * g], O[t][b][4 * g + 1], O[t][b][4 * g + 2], O[t][b][4 * g + 3]);
-                            }
-                    }
-                } else if (mine && row[t] >= 0 && (seg[t] >= 0 || a.zero_rest)) {
-                    const bool none = lt == 0.0f || seg[t] < 0;  // no key left
-                    const float inv = 1.0f / lt;
-                    T* op = (T*)a.out + (int64_t)row[t] * a.o_row + head[t] * a.o_head;
+            const float lt = halves_sum(l);
+            const bool mine = only == -2 ? seg < 0 : only < 0 || seg == only;
+            if (a.splits > 1) {
+                const int64_t o = ((int64_t)split * a.Hq + head) * a.Pq + pos;
+                if (mine && pos >= 0 && half == 0)
+                    a.part_ml[o] = make_float2(grow > 0.0f ? m : -__builtin_inff(), seg >= 0 ? lt : -1.0f);
+                if (mine && seg >= 0) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
                             const int d = 32 * b + 8 * g + 4 * half;
-                            typedef T v4t __attribute__((ext_vector_type(4)));
-                            v4t v;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.0f : O[t][b][4 * g + i] * inv);
-                            if (d < a.D) *(v4t*)(op + d) = v;
+                            if (d < a.D) *(float4*)(a.part_o + o * a.D + d) = make_float4(O[b][4 * g], O[b][4 * g + 1], O[b][4 * g + 2], O[b][4 * g + 3]);
                         }
                 }
+            } else if (mine && row >= 0 && (seg >= 0 || a.zero_rest)) {
+                const bool none = lt == 0.0f || seg < 0;  // no key left
+                const float inv = 1.0f / lt;
+                T* op = (T*)a.out + (int64_t)row * a.o_row + head * a.o_head;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int d = 32 * b + 8 * g + 4 * half;
+                        typedef T v4t __attribute__((ext_vector_type(4)));
+                        v4t v;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = (T)(none ? 0.0f : O[b][4 * g + i] * inv);
+                        if (d < a.D) *(v4t*)(op + d) = v;
+                    }
             }
             if (only == -1) break;
             // the next segment of the block
             int32_t next = 0x7fffffff;
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-                if (seg[t] >= 0 && seg[t] > only && seg[t] < next) next = seg[t];
+            if (seg >= 0 && seg > only && seg < next) next = seg;
             next = wave_extreme<false>(next);
             if constexpr (NW > 1) {
                 __syncthreads();
@@ -614,6 +667,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
             only = __builtin_amdgcn_readfirstlane(next);
             }
         }
+        if constexpr (!SEG) break;
+        base += 32 * NW;
+        if (base >= slot1) break;
     }
 }
 
@@ -696,12 +752,14 @@ __global__ __launch_bounds__(256) void attention_rest_k(AttnArgs a) {
 
 template <class T, int DP, int NW>
 static int launch_attention_w(AttnArgs& a, hipStream_t s) {
-    const int64_t units = NW == 1 ? a.S : (a.Pq * a.G + 32 * NW - 1) / (32 * NW);
+    const int64_t units = NW == 1 ? a.S : a.whole ? a.Pq * a.G / (32 * NW) + a.S + 2 : (a.Pq * a.G + 32 * NW - 1) / (32 * NW);
     const int64_t blocks = units * a.Hk * a.splits;
     PMG_REQUIRE(blocks < (int64_t)1 << 31, "too many blocks");
     a.blocks = (uint32_t)blocks;
-    if (a.slopes) hipLaunchKernelGGL((attention_k<T, DP, NW, 1, true>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((attention_k<T, DP, NW, 1, false>), dim3(a.blocks), dim3(64 * NW), 0, s, a);
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), 0, s, a); };
+    if (a.slopes) launch(attention_k<T, DP, NW, true, false>);
+    else if (a.k_mask) launch(attention_k<T, DP, NW, false, true>);
+    else launch(attention_k<T, DP, NW, false, false>);
     return check_launch("attention_k");
 }
 

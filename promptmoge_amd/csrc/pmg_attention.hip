@@ -6,40 +6,52 @@ using namespace pmg;
 namespace {
 
 struct Plan {
-    int seg, splits;
+    int seg, whole, splits;
 };
 
-// The forms, by the mean lengths (the offsets are on the device). A block per segment where the queries of a segment fill no
-// half wave and its keys are many, the keys split so that about 2048 waves (8 a CU) read them. Else tiles of 128 slots;
-// their keys are split where the blocks would lie unevenly on the CUs, or too few on each to hide what they wait for:
-// a CU's share of the blocks against what writing and joining the parts costs. Measured (MI355X): 19200 rows, 4 heads of
-// 64, biased (600 blocks): 1 part 844 us, 2 parts 738 and 20 to join, 4 parts 712 and 25.
+// The forms, by the mean lengths (the offsets are on the device).
+//
+// A block per segment (seg) where the queries of a segment fill no half wave and its keys are many, the keys split so that
+// about 2048 waves (8 a CU) read them.
+//
+// Else tiles of 128 slots, from each segment's start on (whole) where segments have more than 160 slots, else through all
+// segments: a tile of two segments goes over the keys of both. Measured (MI355X, 40,000 rows, 8 heads of 64, bf16, segments of
+// about L rows; through all against whole): L = 32: 46 and 78 us, 64: 48 and 54, 100: 53 and 48, 128: 54 and 57, 192: 60 and
+// 53, 512: 97 and 76, 2048: 262 and 222; 4 frames of 2745 rows: 168 and 102.
+//
+// Tiles' keys are split where the tiles would lie unevenly on the CUs, or too few on each to hide what they wait for. 19200
+// rows in one segment, 4 heads of 64 (600 tiles), 1 .. 6 parts: 617, 558, 534, 521, 502, 519 us; 4 frames of 2745 rows, 8
+// heads (688 tiles): 102, 119, 122, 120, 131, 140.
 Plan plan_of(const pmg_attention_args& r) {
-    Plan p{0, 1};
+    Plan p{0, 0, 1};
     if (r.segments < 1) return p;
-    const int64_t G = r.Hq / r.Hk;
+    const double G = (double)(r.Hq / r.Hk);
     const double nq = (double)r.q_positions / (double)r.segments, nk = (double)r.k_positions / (double)r.segments;
-    p.seg = nq * (double)G <= 16.0 && nk >= 128.0;
+    p.seg = nq * G <= 16.0 && nk >= 128.0;
     if (p.seg) {
         const int64_t s = 2048 / (r.segments * r.Hk), most = (int64_t)(nk / 256.0);
         p.splits = (int)(s < most ? s : most);
         p.splits = p.splits < 1 ? 1 : p.splits > 256 ? 256 : p.splits;
         return p;
     }
-    const int64_t blocks = (r.q_positions * G + 127) / 128 * r.Hk;
-    // a block's keys: its positions' own segment lengths (longer ones hold more of the positions) and what it straddles;
-    // microseconds: 64 keys of a block at a CU's full throughput (and a block's start); the share of that throughput that
-    // 1 .. 4 resident blocks reach; a part's O written and read
-    const double keys = nk >= 1024.0 ? nk : 2.0 * nk < 1024.0 ? 2.0 * nk + 128.0 / (double)G : 1024.0;
-    const double block = keys / 64.0 * (r.D <= 32 ? 0.6 : r.D <= 64 ? 1.0 : 1.8) * (r.type == PMG_TYPE_F32 ? 4.0 : 1.0);
-    const double reach[5] = {1.0, 0.5, 0.68, 0.84, 1.0};
-    const int resident = r.D <= 64 ? (r.slopes ? 3 : 4) : 2;
+    p.whole = nq * G > 160.0;
+    const int64_t slots = r.q_positions * (r.Hq / r.Hk);
+    const int64_t blocks = (p.whole ? slots / 128 + r.segments + 2 : (slots + 127) / 128) * r.Hk;
+    // Microseconds, as measured: 64 keys of a tile at a CU's full throughput; a block's start; the share of that
+    // throughput that 1 .. 4 blocks on a CU reach; a part's O written and read.
+    const double keys = p.whole ? nk : nk + (nq > 0.0 ? 128.0 / G / nq : 0.0) * nk;
+    const bool f32 = r.type == PMG_TYPE_F32;
+    const double tile = (f32 ? 0.07 * (r.D <= 32 ? 32 : r.D <= 64 ? 64 : 128) : r.D <= 32 ? 0.52 : r.D <= 64 ? 0.66 : 1.37) + (r.slopes ? 0.3 : 0.0);
+    const double reach[5] = {1.0, 0.5, 0.81, 0.91, 1.0};
+    const int resident = f32 || r.D > 64 ? 2 : r.slopes && r.D > 32 ? 3 : 4;
     const double part = (double)r.q_positions * (double)r.Hq * (double)r.D * 8.0 / 8.0e6;
     double best = 0.0;
     for (int s = 1; s <= 64 && s <= (int)(keys / 128.0) + 1; ++s) {
-        const int64_t each = (blocks * s + 255) / 256;
-        const double t = (double)each * (block / s + 1.0) * reach[resident] / reach[each < resident ? each : resident] + (s > 1 ? 6.0 + s * part : 0.0);
-        if (s == 1 || t < 0.97 * best) {
+        const int64_t each = (blocks * s + 255) / 256, rem = each % resident;  // a CU's blocks; those that do not fill it
+        const double slow = rem == 0 || f32 ? 1.0 : reach[resident] / reach[rem];
+        const double rounds = (double)(each - rem) + (double)rem * (each < resident ? slow : 0.5 + 0.5 * slow);
+        const double t = rounds * (keys / 64.0 * tile / s + 1.5) + (s > 1 ? 6.0 + s * part : 0.0);
+        if (s == 1 || t < 0.99 * best) {
             best = t;
             p.splits = s;
         }
@@ -127,8 +139,11 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
         a.cap_arg = (float)((double)r.scale / (double)r.cap * (r.type == PMG_TYPE_F32 ? 1.0 : 2.0 * log2e));
     }
     a.seg = pl.seg;
+    a.whole = pl.whole;
     a.splits = pl.splits;
     a.zero_rest = r.zero_rest;
+    const int64_t end = (a.Mk - 1) * (r.k_row > r.v_row ? r.k_row : r.v_row) * es + (int64_t)r.D * es;
+    a.near = (r.D == 32 || r.D == 64 || r.D == 128) && end <= 0xffff0000;
     if (pl.splits > 1) {
         a.part_o = (float*)workspace;
         a.part_ml = (float2*)((char*)workspace + (size_t)pl.splits * (size_t)r.q_positions * (size_t)r.Hq * (size_t)r.D * 4);

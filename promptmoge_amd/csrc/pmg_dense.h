@@ -85,8 +85,8 @@ __device__ inline int swizzle(int row, int c) {
 __device__ inline uint32_t lds_address(const void* to) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to);
 }
-__device__ inline void load_to_lds(const void* from, const void* to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_address(to)), "v"(from) : "memory", "m0");
+__device__ inline void load_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
 }
 // The same from a buffer: at byte `off` (a lane's) + `more` (the wave's); zeros from its end on.
 __device__ inline void buffer_to_lds(v4i rsrc, uint32_t off, uint32_t more, uint32_t to) {

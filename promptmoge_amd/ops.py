@@ -604,24 +604,36 @@ def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
     grad = torch.is_grad_enabled()
     d = -1
     for t in tensors:
-        if t is not None:
-            if not isinstance(t, torch.Tensor) or (grad and t.requires_grad):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or (grad and t.requires_grad):
+            return -1
+        i = t.get_device()
+        if i != d:
+            if d >= 0:
                 return -1
-            i = t.get_device()
-            if i != d:
-                if d >= 0:
-                    return -1
-                d = i
+            d = i
     return d
+
+
+# The current stream's handle without building a torch.cuda.Stream (1 us); what the compiled torch code itself calls.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda d: torch.cuda.current_stream(d).cuda_stream)
+_ENTRIES: dict = {}
 
 
 def _on(d: int, name: str, *args) -> None:
     """call() on GPU d (the current one or not), on its current stream."""
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        entry = _ENTRIES[name] = getattr(lib(), name)
     if d == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream(d).cuda_stream))
+        code = entry(*args, _raw_stream(d))
     else:
         with torch.cuda.device(d):
-            check(getattr(lib(), name)(*args, torch.cuda.current_stream(d).cuda_stream))
+            code = entry(*args, _raw_stream(d))
+    if code:
+        check(code)
 
 
 def _floating(t: torch.Tensor, name: str) -> int:
@@ -669,8 +681,10 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
     N, kw = w.shape
     if kw != K:
         raise ValueError(f"w expects {kw} input channels, x has {K}")
-    _vector(bias, "bias", N)
-    _vector(w_scale, "w_scale", N)
+    if bias is not None:
+        _vector(bias, "bias", N)
+    if w_scale is not None:
+        _vector(w_scale, "w_scale", N)
     code = _lib.ACTS.get(act)
     if code is None:
         raise ValueError(f"act must be one of {sorted(_lib.ACTS)}, got {act!r}")
@@ -680,7 +694,7 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
         if residual.shape != (M, N):
             raise ValueError(f"residual must be ({M}, {N}), got {tuple(residual.shape)}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        out = x.new_empty((M, N), dtype=out_dtype) if out_dtype != x.dtype else x.new_empty((M, N))
         ldo = N
     else:
         if out.shape != (M, N):
@@ -735,8 +749,8 @@ def _coords(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _vector(t: Optional[torch.Tensor], name: str, n: int) -> None:
-    if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+def _vector(t: torch.Tensor, name: str, n: int) -> None:
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 ({n},) vector")
 
 
@@ -770,11 +784,12 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     if freqs.dtype != torch.float32 or freqs.ndim != 2 or freqs.shape[1] != 3 or not freqs.is_contiguous():
         raise ValueError("freqs must be a contiguous (pairs, 3) float32 tensor")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
-        _vector(t, name, D)
+        if t is not None:
+            _vector(t, name, D)
     if out is None:
-        qo = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
+        qo = q.new_empty((M, Hq, D))
         if k is not None:
-            ko = torch.empty((M, k.shape[1], D), dtype=q.dtype, device=q.device)
+            ko = q.new_empty((M, k.shape[1], D))
     else:
         for name, t, o in (("out[0]", q, qo), ("out[1]", k, ko)):
             if (t is None) != (o is None) or (t is not None and (o.shape != t.shape or o.dtype != q.dtype)):
@@ -864,7 +879,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     fresh = out is None
     if fresh:
         whole = index is None or index.numel() == Mq
-        out = (torch.empty if whole else torch.zeros)((Mq, Hq, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((Mq, Hq, D)) if whole else q.new_zeros((Mq, Hq, D))
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
