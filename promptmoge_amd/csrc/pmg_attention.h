@@ -111,6 +111,11 @@ __device__ inline int32_t unit_segment(const int64_t* off, int64_t S, int64_t P,
     return j >= 1 && j <= S ? (int32_t)(j - 1) : -1;
 }
 
+// slot / G (a 64-bit division is some hundred instructions).
+__device__ inline int32_t position_of(int64_t slot, int G) {
+    return (int32_t)(G == 1 ? slot : slot >> 32 ? slot / G : (int64_t)((uint32_t)slot / (uint32_t)G));
+}
+
 // What absent keys and values are fetched from.
 __device__ const uint4 g_zeros = {0u, 0u, 0u, 0u};
 
@@ -174,6 +179,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     constexpr int NB = DP / 32;                // 32-column blocks of O
     constexpr bool SEG = NW == 1;               // a block per segment
     constexpr int QC = CPR / 2;                // operand chunks of a query a lane holds
+    constexpr bool LOOK = BIAS && DP == 32;  // the maximum is looked for every time: the test's registers would be spilled
     typedef typename Mat<T>::chunk chunk;
     static_assert(NCH * NT == BK * CPR, "whole chunks");
     __shared__ __attribute__((aligned(16))) char s_k[2][BK * DP * ES];
@@ -223,46 +229,53 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     for (int64_t base = slot0;;) {
         // ---- the lane's slots
         const int tid = thread_again(), lane = tid & 63, half = lane >> 5;
-        int32_t pos, lo, hi, row, seg, head;
         int32_t blo = (int32_t)a.Pk, bhi = 0;
         const int64_t wfirst = base + wave * 32;
         const int64_t slot = base + wave * 32 + (lane & 31);
         const bool in = slot < slot1;
-        pos = in ? (int32_t)(slot / a.G) : -1;
-        head = hk * a.G + (in ? (int)(slot - (int64_t)pos * a.G) : 0);
-        row = -1;
-        seg = -1;
-        lo = hi = 0;
-        int32_t sg = SEG ? (int32_t)unit : own;
-        if (!SEG && !a.whole && wfirst < slot1) sg = wave_segment(a.q_off, a.S, (int32_t)(wfirst / a.G), in ? pos : 0x7ffffffe);
-        if (in) {
-            const int32_t r = a.q_index ? a.q_index[pos] : pos;
-            row = r >= 0 && r < a.Mq ? r : -1;
-            seg = sg;
+        const int32_t pos = in ? position_of(slot, a.G) : -1;
+        const int head = hk * a.G + (in ? (int)(slot - (int64_t)pos * a.G) : 0);
+        int32_t row = in ? pos : -1, seg = -1, lo = 0, hi = 0;
+        if (in && a.q_index) row = a.q_index[pos];  // (looked at below: nothing waits for it here)
+        int32_t wlo, whi;  // the wave's keys
+        if (SEG || a.whole) {
+            if constexpr (!SEG) {
+                seg_lo = own >= 0 ? (int32_t)clamp64(a.k_off[own], 0, a.Pk) : 0;
+                seg_hi = own >= 0 ? (int32_t)clamp64(a.k_off[own + 1], seg_lo, a.Pk) : 0;
+            }
+            if (in) {
+                seg = SEG ? (int32_t)unit : own;
+                lo = seg_lo;
+                hi = seg_hi;
+            }
+            blo = wlo = seg_lo;
+            bhi = whi = seg_hi;
+        } else {
+            if (wfirst < slot1) seg = wave_segment(a.q_off, a.S, position_of(wfirst, a.G), in ? pos : 0x7ffffffe);
+            if (!in) seg = -1;
             if (seg >= 0) {
-                lo = SEG ? seg_lo : (int32_t)clamp64(a.k_off[seg], 0, a.Pk);
-                hi = SEG ? seg_hi : (int32_t)clamp64(a.k_off[seg + 1], lo, a.Pk);
+                lo = (int32_t)clamp64(a.k_off[seg], 0, a.Pk);
+                hi = (int32_t)clamp64(a.k_off[seg + 1], lo, a.Pk);
                 if (hi > lo) {
-                    blo = lo < blo ? lo : blo;
-                    bhi = hi > bhi ? hi : bhi;
+                    blo = lo;
+                    bhi = hi;
                 }
             }
-        }
-        // the block's keys, and whether some lane sees only a part of them
-        blo = wave_extreme<false>(blo);
-        bhi = wave_extreme<true>(bhi);
-        const int32_t wlo = blo, whi = bhi;  // the wave's
-        if constexpr (NW > 1) {
-            __syncthreads();
-            if (lane == 0) {
-                s_r[0][wave] = blo;
-                s_r[1][wave] = bhi;
-            }
-            __syncthreads();
+            // the block's keys, and whether some lane sees only a part of them
+            blo = wlo = wave_extreme<false>(blo);
+            bhi = whi = wave_extreme<true>(bhi);
+            if constexpr (NW > 1) {
+                __syncthreads();
+                if (lane == 0) {
+                    s_r[0][wave] = blo;
+                    s_r[1][wave] = bhi;
+                }
+                __syncthreads();
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                blo = s_r[0][w] < blo ? s_r[0][w] : blo;
-                bhi = s_r[1][w] > bhi ? s_r[1][w] : bhi;
+                for (int w = 0; w < NW; ++w) {
+                    blo = s_r[0][w] < blo ? s_r[0][w] : blo;
+                    bhi = s_r[1][w] > bhi ? s_r[1][w] : bhi;
+                }
             }
             blo = __builtin_amdgcn_readfirstlane(blo);
             bhi = __builtin_amdgcn_readfirstlane(bhi);
@@ -282,7 +295,16 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
             bhi = (int32_t)(blo + each < bhi ? blo + each : bhi);
         }
 
+        // the first keys' numbers, on their way with the queries' own
+        const auto number = [](const int32_t* k_index, int tid, int32_t g, int32_t from, int32_t to) -> int32_t {
+            if (g * (int64_t)SB >= to - from || tid >= to - from - g * SB) return -1;
+            const int32_t p = from + g * SB + tid;
+            return k_index ? k_index[p] : p;  // (looked at in about(): nothing waits for it here)
+        };
+        const int32_t first0 = number(a.k_index, tid, 0, blo, bhi), first1 = number(a.k_index, tid, 1, blo, bhi);
+
         // ---- the queries, and their coordinates' operands
+        row = row >= 0 && row < a.Mq ? row : -1;
         chunk qf[QC];
         v8bf qc[3];
         float sl[3];
@@ -343,11 +365,6 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
 
             // ---- the keys' numbers, mask and coordinates, by groups of SB
             int32_t mi = -1;  // the thread's row in the group whose mask and coordinates come next
-            const auto number = [&](int32_t g) -> int32_t {
-                if (g * (int64_t)SB >= khi - klo || tid >= khi - klo - g * SB) return -1;
-                const int32_t p = klo + g * SB + tid;
-                return a.k_index ? a.k_index[p] : p;  // (looked at in about(): nothing waits for it here)
-            };
             int4 mc = make_int4(0, 0, 0, 0);
             uint8_t mm = 1;
             const auto about = [&]() {  // of row mi
@@ -363,6 +380,8 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 // (absent: behind the buffer's end, whichever chunk is added; or -1)
                 s_row[b][tid] = !on ? make_uint2(0xffff0000u, 0xffff0000u)
                                     : make_uint2((uint32_t)mi * (a.near ? (uint32_t)a.k_row * ES : 1u), (uint32_t)mi * (a.near ? (uint32_t)a.v_row * ES : 1u));
+            };
+            const auto note_where = [&](int b) {
                 if constexpr (BIAS) {
                     const auto b16 = [](int v) { return f2u((float)v) >> 16; };  // (exact: 8 bits)
                     const auto p01 = [&](int v) { return b16(v & 255) | (b16((v >> 8) & 255) << 16); };
@@ -405,13 +424,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 }
             };
             if (nt > 0) {
-                mi = number(0);
+                mi = only < 0 ? first0 : number(a.k_index, tid, 0, klo, khi);
                 about();
-                const int32_t m1 = number(1);
                 note(0);
-                mi = m1;
                 __syncthreads();
                 fetch(0, 0);
+                note_where(0);
+                mi = only < 0 ? first1 : number(a.k_index, tid, 1, klo, khi);
                 loads_landed<0>();
             }
             // Keys can be taken out by a product with -inf where no query is infinite or NaN (an absent key's zeros times
@@ -439,7 +458,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 if (more) fetch(cur ^ 1, it + 1);
                 if (ahead) {
                     about();
-                    mn = number((uint32_t)it / TPS + 2);
+                    mn = number(a.k_index, tid, (uint32_t)it / TPS + 2, klo, khi);
                 }
                 // 32 keys at a time: more waves on a SIMD are worth more than longer runs of one (a single wave issues
                 // an ordinary instruction every 5 cycles, two or more together one every 2.5, measured)
@@ -526,12 +545,12 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                         }
                         sum = (part[0] + part[1]) + (part[2] + part[3]);
                     };
-                    if (!look) {
+                    if (!LOOK && !look) {
                         scores();
                         weights();
                         look = __any(sum > 4096.0f);
                     }
-                    if (look) {
+                    if (LOOK || look) {
                         scores();
                         float mx = s[0];
 #pragma unroll
@@ -590,6 +609,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 }
                 if (ahead) {
                     note(slot ^ 1);
+                    note_where(slot ^ 1);
                     mi = mn;
                 }
                 loads_landed<0>();
