@@ -143,6 +143,18 @@ __device__ inline int32_t wave_extreme(int32_t v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
+// tanh without branches, within 2 ulp: below 0.55 y + y^3 P(y^2), P of degree 4 through (tanh(y) / y - 1) / y^2 at the
+// Chebyshev nodes of that range (2^-24 of the value, coefficients and evaluation in fp32); above 1 - 2 / (e^2y + 1).
+__device__ inline float tanh_f32(float y) {
+    const float z = y * y;
+    float p = __builtin_fmaf(-0.00661022774875164f, z, 0.021309388801455498f);
+    p = __builtin_fmaf(p, z, -0.05390942841768265f);
+    p = __builtin_fmaf(p, z, 0.13333113491535187f);
+    p = __builtin_fmaf(p, z, -0.3333333134651184f);
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * PMG_LOG2E * __builtin_fabsf(y)));
+    return __builtin_fabsf(y) < 0.55f ? __builtin_fmaf(y * z, p, y) : __builtin_copysignf(__builtin_fmaf(-2.0f, r, 1.0f), y);
+}
+
 // The thread's number, hidden from the compiler: what is derived from it is formed where it is used, not kept in registers
 // through the loop over the keys.
 __device__ inline int thread_again() {
@@ -249,7 +261,8 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                 hi = seg_hi;
             }
             blo = wlo = seg_lo;
-            bhi = whi = seg_hi;
+            bhi = seg_hi;
+            whi = wfirst < slot1 ? seg_hi : seg_lo;  // (a wave without slots does nothing)
         } else {
             if (wfirst < slot1) seg = wave_segment(a.q_off, a.S, position_of(wfirst, a.G), in ? pos : 0x7ffffffe);
             if (!in) seg = -1;
@@ -491,13 +504,14 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
 #pragma unroll
                             for (int c = 0; c < QG; ++c) kf[c] = *(const chunk*)(sk + r * DP * ES + 16 * kswz(r, 2 * (c0 + c) + half));
 #pragma unroll
-                            for (int c = 0; c < QG; ++c) s = Mat<T>::mma32(kf[c], qf[c0 + c], s);
+                            for (int c = 0; c < QG; ++c)  // (fp32: 256 cycles a chunk, not spent behind the head's width)
+                                if (ES == 2 || 2 * (c0 + c) * PER < a.D) s = Mat<T>::mma32(kf[c], qf[c0 + c], s);
                         }
                         // less the maximum so far, in powers of two
                         if (a.cap2 != 0.0f) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                if constexpr (ES == 4) s[e] = a.cap2 * tanhf(s[e] * a.cap_arg);
+                                if constexpr (ES == 4) s[e] = a.cap2 * tanh_f32(s[e] * a.cap_arg);
                                 else s[e] = __builtin_fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[e] * a.cap_arg)), a.cap2);
                             }
                         }

@@ -39,7 +39,10 @@ Plan plan_of(const pmg_attention_args& r) {
     const int64_t blocks = (p.whole ? slots / 128 + r.segments + 2 : (slots + 127) / 128) * r.Hk;
     // Microseconds, as measured: 64 keys of a tile at a CU's full throughput; a block's start; the share of that
     // throughput that 1 .. 4 blocks on a CU reach; a part's O written and read.
-    const double keys = p.whole ? nk : nk + (nq > 0.0 ? 128.0 / G / nq : 0.0) * nk;
+    // (a tile's keys: more than a few segments are taken to be ragged, their rows in segments of 1.5 times the mean
+    // length, the longest of 2.5 times, whose tiles are at work last and alone)
+    const bool ragged = r.segments > 4;
+    const double keys = (ragged ? 1.5 : 1.0) * nk * (p.whole || nq <= 0.0 ? 1.0 : 1.0 + 128.0 / G / nq);
     const bool f32 = r.type == PMG_TYPE_F32;
     const double tile = (f32 ? 0.07 * (r.D <= 32 ? 32 : r.D <= 64 ? 64 : 128) : r.D <= 32 ? 0.52 : r.D <= 64 ? 0.66 : 1.37) + (r.slopes ? 0.3 : 0.0);
     const double reach[5] = {1.0, 0.5, 0.81, 0.91, 1.0};
@@ -50,7 +53,9 @@ Plan plan_of(const pmg_attention_args& r) {
         const int64_t each = (blocks * s + 255) / 256, rem = each % resident;  // a CU's blocks; those that do not fill it
         const double slow = rem == 0 || f32 ? 1.0 : reach[resident] / reach[rem];
         const double rounds = (double)(each - rem) + (double)rem * (each < resident ? slow : 0.5 + 0.5 * slow);
-        const double t = rounds * (keys / 64.0 * tile / s + 1.5) + (s > 1 ? 6.0 + s * part : 0.0);
+        const double alone = (ragged ? 2.5 : 1.0) * nk / 64.0 * tile / s / (f32 && !r.slopes && r.cap == 0.0f ? 0.9 : 0.5) + 1.5;
+        const double all = rounds * (keys / 64.0 * tile / s + 1.5);
+        const double t = (all > alone ? all : alone) + (s > 1 ? 6.0 + s * part : 0.0);
         if (s == 1 || t < 0.99 * best) {
             best = t;
             p.splits = s;
