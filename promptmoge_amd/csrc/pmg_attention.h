@@ -69,7 +69,7 @@ __device__ inline int32_t segment_of(const int64_t* off, int64_t S, int64_t p) {
 // search with 64 probes a round for `first`, then among the 64 offsets that follow.
 __device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t first, int32_t p) {
     const int lane = threadIdx.x & 63;
-    int64_t lo = 0, n = S + 1;  // entries before lo are <= first, those from lo + n on are not
+    int64_t lo = 0, n = S < 64 ? 0 : S + 1;  // entries before lo are <= first, those from lo + n on are not; (few: all are read)
     while (n > 0) {
         const int64_t step = (n + 63) >> 6, j = (lane + 1) * step - 1;
         const bool le = j < n && off[lo + j] <= first;
@@ -104,9 +104,9 @@ __device__ inline int32_t unit_segment(const int64_t* off, int64_t S, int64_t P,
         n -= t * step;
         n = n < step - 1 ? n : step - 1;
     }
-    const int64_t j = lo > 0 ? lo - 1 : 0;
-    slot0 = starts(j) * G + ((int64_t)unit - first(j)) * per;
+    const int64_t j = lo > 0 ? lo - 1 : 0, nth = (int64_t)unit - first(j);
     slot1 = j <= S ? starts(j + 1) * G : P * G;
+    slot0 = nth >= 0 ? starts(j) * G + nth * per : slot1;  // (negative: offsets that decrease)
     slot1 = slot0 + per < slot1 ? slot0 + per : slot1;
     return j >= 1 && j <= S ? (int32_t)(j - 1) : -1;
 }
@@ -709,44 +709,58 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
 
 // Joins the splits of each (position, head): groups of CL lanes, 4 columns a lane. WIDE (many splits): a wave a position, each
 // group on every (64 / CL)-th split, the groups' sums added in order at the end. Otherwise a group a position, its splits
-// in order.
+// in order. One pass with the running maximum, the loads of U splits under way at once with the row's number: such a small
+// kernel is a chain of loads (8 positions of 16 heads of 64, 64 splits: X us; 19200 rows of 4 heads, 5 splits: Y us, Z TB/s).
 template <class T, int CL, bool WIDE>
 __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
     constexpr int G = 64 / CL, PER = WIDE ? 4 : 4 * G;  // positions a block
+    constexpr int U = WIDE ? 8 : 4, EACH = WIDE ? G : 1;
     const int lane = threadIdx.x & 63, g = lane / CL, d = 4 * (lane % CL), head = blockIdx.y;
-    const int64_t pos = (int64_t)blockIdx.x * PER + (WIDE ? threadIdx.x >> 6 : threadIdx.x / CL);
-    if (pos >= a.Pq) return;
-    const int32_t r = a.q_index ? a.q_index[pos] : (int32_t)pos;
-    const int64_t step = (int64_t)a.Hq * a.Pq, at = (int64_t)head * a.Pq + pos;
-    // (blocks by segment write nothing for positions of no segment)
-    const bool in = a.seg ? segment_of(a.q_off, a.S, pos) >= 0 : a.part_ml[at].y >= 0.0f || a.part_ml[at].y != a.part_ml[at].y;
-    if (r < 0 || r >= a.Mq || (!in && !a.zero_rest)) return;
-    typedef T v4t __attribute__((ext_vector_type(4)));
-    v4t* op = (v4t*)((T*)a.out + (int64_t)r * a.o_row + head * a.o_head + d);
-    const bool mine = (!WIDE || g == 0) && d < a.D;
-    if (!in) {
-        if (mine) *op = v4t{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-        return;
-    }
-    float m = -__builtin_inff();
-    for (int s = WIDE ? lane : 0; s < a.splits; s += WIDE ? 64 : 1) m = __builtin_fmaxf(m, a.part_ml[at + s * step].x);
-    if constexpr (WIDE)
-        for (int o = 32; o > 0; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
-    const float ms = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f;
+    const int64_t first = (int64_t)blockIdx.x * PER + (WIDE ? threadIdx.x >> 6 : (threadIdx.x >> 6) * G);  // the wave's
+    const int64_t pos = WIDE ? first : first + g;
+    if (first >= a.Pq) return;
+    const bool there = pos < a.Pq;
+    const int64_t step = (int64_t)a.Hq * a.Pq, at = (int64_t)head * a.Pq + (there ? pos : first);
+    int32_t r = there ? a.q_index ? a.q_index[pos] : (int32_t)pos : -1;
+    const float y0 = a.part_ml[at].y;
+    float m = -__builtin_inff(), l = 0.0f;
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = WIDE ? g : 0; s < a.splits; s += WIDE ? G : 1) {
-        const float2 ml = a.part_ml[at + s * step];
-        const v4f po = d < a.D ? *(const v4f*)(a.part_o + (at + s * step) * a.D + d) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        const float w = __builtin_amdgcn_exp2f(ml.x - ms);
-        if (ml.y != 0.0f) {  // (a part without keys counts for nothing)
-            l = __builtin_fmaf(ml.y, w, l);
+    for (int s0 = WIDE ? g : 0; s0 < a.splits; s0 += U * EACH) {
+        float2 ml[U];
+        v4f po[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(po[i], w, acc[i]);
+        for (int u = 0; u < U; ++u) {
+            const int64_t s = at + (s0 + u * EACH < a.splits ? s0 + u * EACH : s0) * step;
+            ml[u] = a.part_ml[s];
+            po[u] = *(const v4f*)(a.part_o + s * a.D + (d < a.D ? d : 0));
+            if (s0 + u * EACH >= a.splits) ml[u] = make_float2(-__builtin_inff(), 0.0f);
+        }
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = __builtin_fmaxf(mx, ml[u].x);
+        const float ms = mx == -__builtin_inff() ? 0.0f : mx, was = __builtin_amdgcn_exp2f(m - ms);
+        m = mx;
+        l = l * was;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * was;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = __builtin_amdgcn_exp2f(ml[u].x - ms);
+            if (ml[u].y != 0.0f) {  // (a part without keys counts for nothing)
+                l = __builtin_fmaf(ml[u].y, w, l);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(po[u][i], w, acc[i]);
+            }
         }
     }
     if constexpr (WIDE) {
+        float mx = m;
+#pragma unroll
+        for (int o = CL; o < 64; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
+        const float w = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+        l = l * w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * w;
 #pragma unroll
         for (int o = CL; o < 64; o <<= 1) {
             l = l + __shfl_xor(l, o, 64);
@@ -754,12 +768,15 @@ __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
             for (int i = 0; i < 4; ++i) acc[i] = acc[i] + __shfl_xor(acc[i], o, 64);
         }
     }
-    if (!mine) return;
+    // (blocks by segment write nothing for positions of no segment)
+    const bool in = a.seg ? wave_segment(a.q_off, a.S, (int32_t)first, there ? (int32_t)pos : (int32_t)first) >= 0 : y0 >= 0.0f || y0 != y0;
+    if (r < 0 || r >= a.Mq || (!in && !a.zero_rest) || (WIDE && g != 0) || d >= a.D) return;
+    typedef T v4t __attribute__((ext_vector_type(4)));
     const float inv = 1.0f / l;
     v4t v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (T)(l == 0.0f ? 0.0f : acc[i] * inv);
-    *op = v;
+    for (int i = 0; i < 4; ++i) v[i] = (T)(!in || l == 0.0f ? 0.0f : acc[i] * inv);
+    *(v4t*)((T*)a.out + (int64_t)r * a.o_row + head * a.o_head + d) = v;
 }
 
 template <class T, int CL>
