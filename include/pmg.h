@@ -628,7 +628,8 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  *   x_j = scale q_i . k_j;  cap > 0: x_j = cap tanh(x_j / cap);  x_j -= sum over axes of slopes[h][axis] |c_i - c_j|[axis]
  *   out_i = sum_j softmax(x)_j v_j, 0 where no key is left. Key head of h: h / (Hq / Hk).
  * Sums and statistics in fp32; the softmax's weights enter the second product rounded to `type`.
- * Offsets are held to [0, positions]; a position whose index lies outside the rows is absent. Query rows outside every
+ * Offsets are held to [0, positions] (where they fall, query rows may be left as they were); a position whose index
+ * lies outside the rows is absent. Query rows outside every
  * segment are left as they were, or zeroed with zero_rest (those that a position names). A row named by two query
  * positions gets either's result. Differences of coordinates are exact up to 2^23.
  * D a multiple of 8 up to 128; q, k, v: buffers and strides (elements) in whole 16 bytes, out in groups of 4 elements;

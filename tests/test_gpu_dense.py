@@ -335,6 +335,18 @@ def test_attention_rising_scores(gpu, dt):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attention_scores_that_jump(gpu, dt, D):
+    """Runs of keys whose scores lie up to 2^60 weights above the ones before, under a mask and under a bias."""
+    def edit(q, kv, kw):
+        n = kv.shape[0]
+        q[:] = 1
+        kv[:, 0] = (torch.arange(n, device=q.device) // 45 % 7 * 5.0).to(dt).view(n, 1, 1)
+    check_attention(gpu, dt, [500], 2, 2, D, scale=1.0 / D, mask=0.2, edit=edit)
+    check_attention(gpu, dt, [500, 300], 2, 2, D, scale=1.0 / D, bias=True, edit=edit)
+
+
+@pytest.mark.parametrize("dt", TYPES)
 def test_attention_first_keys_far_away(gpu, dt):
     """The first keys' scores lie thousands below the later ones' (and below 2^-128 of anything): they set the running
     maximum first and then count for nothing."""
@@ -475,6 +487,63 @@ def test_attention_offsets_beyond_32_bits(gpu):
     want, tol, _ = ref.attention(q[1:], kv[0, -400:], kv[1, -400:], torch.tensor([0, 1]), torch.tensor([0, 400]))
     ref.assert_within(got[1:], want, tol)
     assert not bool(got[0].any())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lengths,Hq,Hk,D", [([200, 0, 385, 128, 256, 1], 2, 1, 32), ([1000], 1, 1, 64), ([129, 300, 90, 300], 3, 3, 40),
+                                             ([2600, 1, 0, 2300], 1, 1, 64), ([500] * 70, 1, 1, 32)])
+def test_attention_long_segments_with_rows_around(gpu, dt, lengths, Hq, Hk, D):
+    """Segments of many rows, whose tiles start where they start, with rows before, between masked keys and behind."""
+    check_attention(gpu, dt, lengths, Hq, Hk, D, start=37, tail=300, mask=0.2, seed=D)
+    check_attention(gpu, dt, lengths, Hq, Hk, D, start=128, tail=1, perm=True, bias=True, seed=D + 1)
+
+
+def test_attention_falling_offsets_of_long_segments(gpu):
+    g = gen(8)
+    M, H, D = 900, 2, 32
+    q, kv = randn(g, M, H, D).to(F16).to(gpu), randn(g, M, 2, H, D).to(F16).to(gpu)
+    for off in ([700, 100, 650, 2 ** 62], [900, -1, 2 ** 40, 0], [-(2 ** 62), 2 ** 62, 5, 880]):
+        for dt in TYPES:
+            announce(f"attention falling offsets {off} {dt}")
+            # (offsets have to rise: rows that these miss may be left as they were, but nothing else happens)
+            out = torch.full((M + 64, H, D), 7.0, dtype=dt, device=gpu)
+            ops.sparse_attention(q.to(dt), kv[:, 0].to(dt), kv[:, 1].to(dt), torch.tensor(off, device=gpu), out=out[32:-32])
+            assert bool(torch.isfinite(out).all()) and bool((out[:32] == 7).all()) and bool((out[-32:] == 7).all())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_attention_one_query_not_finite(gpu, dt, value):
+    """Every other row of its tile is what it is without it, masked keys or not."""
+    g = gen(9)
+    M, H, D = 300, 2, 64
+    q, kv = randn(g, M, H, D).to(dt).to(gpu), randn(g, M, 2, H, D).to(dt).to(gpu)
+    off, mask = torch.tensor([0, 300]), torch.rand(M, generator=g) > 0.3
+    want, tol, _ = ref.attention(q, kv[:, 0], kv[:, 1], off, kv_mask=mask)
+    bad = q.clone()
+    bad[7, :, 3], bad[200, 1] = value, value
+    announce(f"attention query {value} {dt}")
+    got = ops.sparse_attention(bad, kv[:, 0], kv[:, 1], off.to(gpu), kv_mask=mask.to(gpu))
+    rest = torch.ones(M, dtype=torch.bool)
+    rest[[7, 200]] = False
+    ref.assert_within(got[rest.to(gpu)], want[rest], tol[rest])
+    assert bool(torch.isnan(got[7]).any()) and bool(torch.isnan(got[200, 1]).any())
+
+
+def test_attention_keys_of_almost_4_gib(gpu):
+    Mk, D = 16_700_000, 128
+    announce("attention keys of 4.28e9 bytes")
+    kv = torch.zeros((2, Mk, 1, D), dtype=F16, device=gpu)
+    g = gen(2)
+    kv[:, -400:] = randn(g, 2, 400, 1, D).to(F16).to(gpu)
+    kv[:, -100] = float("nan")
+    q = randn(g, 200, 1, D).to(F16).to(gpu)
+    mask = torch.ones(Mk, dtype=torch.bool, device=gpu)
+    mask[-100] = False
+    off, koff = torch.tensor([0, 200], device=gpu), torch.tensor([Mk - 400, Mk], device=gpu)
+    got = ops.sparse_attention(q, kv[0], kv[1], off, koff, kv_mask=mask)
+    want, tol, _ = ref.attention(q, kv[0, -400:], kv[1, -400:], torch.tensor([0, 200]), torch.tensor([0, 400]), kv_mask=mask[-400:])
+    ref.assert_within(got, want, tol)
 
 
 def test_attention_refusals(gpu):
