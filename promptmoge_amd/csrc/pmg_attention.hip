@@ -64,6 +64,10 @@ Plan plan_of(const pmg_attention_args& r) {
     return p;
 }
 
+size_t parts_bytes(const pmg_attention_args& r, const Plan& p) {
+    return p.splits <= 1 ? 0 : (size_t)p.splits * (size_t)r.q_positions * (size_t)r.Hq * ((size_t)r.D * 4 + 8);
+}
+
 int attention_args(const pmg_attention_args& r) {
     PMG_REQUIRE(r.type >= PMG_TYPE_F32 && r.type <= PMG_TYPE_BF16, "type must be f32, f16 or bf16");
     PMG_REQUIRE(r.Hq >= 1 && r.Hk >= 1 && r.Hq <= 4096 && r.Hq % r.Hk == 0, "query heads must be a multiple of key heads (up to 4096)");
@@ -82,9 +86,7 @@ int attention_args(const pmg_attention_args& r) {
 
 extern "C" size_t pmg_attention_workspace_bytes(const pmg_attention_args* p) {
     if (!p || attention_args(*p) != PMG_OK) return 0;
-    const Plan pl = plan_of(*p);
-    if (pl.splits <= 1) return 0;
-    return (size_t)pl.splits * (size_t)p->q_positions * (size_t)p->Hq * ((size_t)p->D * 4 + 8);
+    return parts_bytes(*p, plan_of(*p));
 }
 
 extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -105,7 +107,7 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     PMG_REQUIRE(ok(r.out, r.out_row, r.out_head, 4), "out: buffer and strides in whole groups of 4 elements");
     PMG_REQUIRE(!r.slopes || (aligned16(r.q_coords) && aligned16(r.k_coords)), "coordinates must be 16-byte aligned");
     const Plan pl = plan_of(r);
-    const size_t need = pmg_attention_workspace_bytes(p);
+    const size_t need = parts_bytes(r, pl);
     PMG_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), "workspace too small, null or not 16-byte aligned");
     AttnArgs a{};
     a.q = r.q;

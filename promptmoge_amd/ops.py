@@ -837,7 +837,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     kv_mask (Mk,) bool / uint8: rows with 0 are not attended to. A query with no key left gets 0.
 
     Rows outside every segment are 0 in a new result and left as they were in a given `out`. Every row should be named
-    by at most one query position. Forward only."""
+    by at most one query position; an index as long as q has to name every row (in a new result, rows that it misses are
+    not written). offsets that fall leave rows unwritten, too. Forward only."""
     d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
     if d < 0:
         _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
