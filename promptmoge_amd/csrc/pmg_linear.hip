@@ -2,9 +2,14 @@
 // for fp32, fp16, bf16 (fp32 sums, no scales) and int8 (exact int32 sums).
 //
 // Two kernels, both with w's rows as the matrix instruction's row operand, so that a lane holds four neighbouring n of
-// one m. `linear_tile_k`: a block's BM x BN outputs from tiles of 64 bytes of k in LDS, filled by direct loads to LDS
-// NS - 1 tiles ahead; the sums go through LDS once so that residual and output move as whole rows. `linear_rows_k`: few
-// outputs; the block's waves share out k, operands straight into registers.
+// one m. `linear_tile_k`: a block's BM x BN outputs from tiles of KB bytes of k (64 or 128) in NS LDS buffers, filled by
+// direct loads to LDS several tiles ahead; the sums go through LDS once so that residual and output move as whole rows.
+// `linear_rows_k`: few outputs; the block's waves share out k, operands straight into registers.
+//
+// Measured (MI355X), and what bounds it: 4800 x 1024 bf16 to 4096 columns, gelu: 54 us, 745 TFLOP/s (the 16-bit tiles take
+// what the chip's power leaves of the matrix units' rate, and the epilogue after them; a library's product without an
+// epilogue takes 50); one row of 1024 fp16 to 1024: 4.2 us, a load's latency four times over; 76,800 rows of 64 fp32 to
+// 128: 21 us (59 MB; matrix units 8 us, loads and epilogue of blocks of two tiles of k lie one behind the other).
 #include "pmg_dense.h"
 
 namespace pmg {

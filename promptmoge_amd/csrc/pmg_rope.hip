@@ -7,6 +7,8 @@
 // two). The angles are the same for every head: a block forms those of its rows once, in 64 bits (the product of a
 // 32-bit coordinate and an fp32 frequency is exact there, and the reduction to one turn loses nothing an fp32 sine
 // could show), and keeps their sines and cosines in LDS.
+//
+// Bound by memory: 76,800 rows, 8 and 8 heads of 32, fp16: 157 MB in 32.6 us, 4.8 TB/s (a copy reaches 5.0).
 #include "pmg_dense.h"
 
 namespace pmg {
