@@ -468,14 +468,18 @@ static int launch_rows(LinearArgs& a, hipStream_t s) {
 // each two rounds of loads, else four. Measured, K = 1024, fp16: 64 rows to 1024 columns 4.5 us (64 x 64 tiles: 7.3),
 // 1000 rows to 256 columns 8.7 (7.6); fp32: 8.4 (23) and 14 (24).
 //
-// Tiles, by what a CU's share of them costs: k in units of 128 bytes, then the epilogue, in microseconds.
-//   64 x 64     0.27 a unit, 0.4; five blocks a CU. Products bound by memory, and fp32: (76811 x 256) int8 to 256 columns
-//               29 us, the larger tiles 30 to 47.
-//   128 x 128   0.6 and 3, two blocks a CU: 19200 x 256 bf16 to 768 columns 24 us (64 x 64: 26).
-//   256 x 256   2.2 and 16, one block: 8192 x 4096 bf16 to 4096 columns 281 us (980 TFLOP/s; 128 x 128: 310). Its LDS reads
-//               are a quarter fewer a product.
-//   320 x 256   2.4 and 20: where it takes fewer rounds: 4800 x 1024 bf16 to 4096 columns with gelu 61 us (240 tiles on
-//               256 CUs; 128 x 128 67, 256 x 256 83).
+// Tiles, by what a CU's share of them costs, fitted to the times of 20 products: k in units of 128 bytes, then the epilogue,
+// in microseconds. Measured, us:
+//                                          64 x 64   128 x 64   128 x 128   256 x 256   320 x 256
+//   11213 x 512 to 256, fp16                  10        11.4        11.3
+//   76800 x 256 to 256, fp16                  32        30          32          49          33
+//   4800 x 1024 to 1024, bf16                 23        20          21          41          50
+//   4800 x 4096 to 1024, bf16                 76        62          53          109         137
+//   19200 x 1024 to 1024, int8                45        47          41          65          43
+//   4800 x 1024 to 4096, bf16, gelu           77        67          62          82          56
+//   8192 x 4096 to 4096, bf16                                       310         281
+// A CU holds five blocks of 64 x 64, three of 128 x 64, two of 128 x 128 (where it has two at most the chip clocks higher) and
+// one of the largest, whose LDS reads are a quarter fewer a product. fp32 takes 64 x 64: its products are 16 times as long.
 template <class T, bool VEC>
 static int launch_linear(LinearArgs& a, hipStream_t s) {
     const int64_t tn = (a.N + 15) / 16, n1 = (a.M + 15) / 16 * tn, n2 = (a.M + 31) / 32 * tn;
@@ -484,17 +488,18 @@ static int launch_linear(LinearArgs& a, hipStream_t s) {
     if (n2 <= (sizeof(T) == 4 ? 512 : 256)) return lengthy ? launch_rows<T, 2, 8, VEC>(a, s) : launch_rows<T, 2, 4, VEC>(a, s);
     if constexpr (VEC && sizeof(T) < 4) {
         const double k = (double)((int64_t)a.K * (int)sizeof(T) + 127) / 128;
-        const auto cost = [&](int bm, int bn, double unit, double end) {
-            const int64_t tiles = (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn);
-            return (double)((tiles + 255) / 256) * (k * unit + end);
-        };
-        const double c[4] = {cost(64, 64, 0.27, 0.4), cost(128, 128, 0.6, 3.0), cost(256, 256, 2.2, 16.0), cost(320, 256, 2.4, 20.0)};
+        const auto rounds = [&](int bm, int bn) { return (double)(((a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) + 255) / 256); };
+        const double r = rounds(128, 128);
+        const double c[5] = {rounds(64, 64) * (0.24 * k + 0.6), rounds(128, 64) * (0.31 * k + 1.5),
+                             r > 2.0 ? r * (0.55 * k + 3.5) : (r < 2.0 ? 1.5 : r) * (0.36 * k + 4.7),
+                             rounds(256, 256) * (2.0 * k + 15.0), rounds(320, 256) * (2.4 * k + 20.0)};
         int best = 0;
-        for (int i = 1; i < 4; ++i)
+        for (int i = 1; i < 5; ++i)
             if (c[i] < c[best]) best = i;
-        if (best == 1) return launch_tile<T, 128, 128, 4, 2, 128, 2, VEC>(a, s);
-        if (best == 2) return launch_tile<T, 256, 256, 2, 4, 64, 4, VEC>(a, s);
-        if (best == 3) return launch_tile<T, 320, 256, 2, 4, 64, 3, VEC>(a, s);
+        if (best == 1) return launch_tile<T, 128, 64, 4, 2, 128, 2, VEC>(a, s);
+        if (best == 2) return launch_tile<T, 128, 128, 4, 2, 128, 2, VEC>(a, s);
+        if (best == 3) return launch_tile<T, 256, 256, 2, 4, 64, 4, VEC>(a, s);
+        if (best == 4) return launch_tile<T, 320, 256, 2, 4, 64, 3, VEC>(a, s);
     }
     return launch_tile<T, 64, 64, 2, 2, 128, 2, VEC>(a, s);
 }

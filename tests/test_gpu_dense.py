@@ -61,6 +61,29 @@ def test_linear_large(gpu, dt, M, K, N):
     ref.assert_within(got[rows], want, tol)
 
 
+@pytest.mark.parametrize("dt", [F16, BF16, torch.int8])
+@pytest.mark.parametrize("M,K,N", [(9_700, 1024, 1000), (30_001, 272, 264), (19_300, 816, 200), (4_777, 4096, 520)])
+def test_linear_large_of_middle_tiles(gpu, dt, M, K, N):
+    """Tiles of 128 rows, with and without a residual read ahead; checked on a sample of rows in 64 bits."""
+    g = torch.Generator(device=gpu).manual_seed(M)
+    i8 = dt == torch.int8
+    if i8:
+        x = torch.randint(-127, 128, (M, K), device=gpu, generator=g, dtype=dt)
+        w = torch.randint(-127, 128, (N, K), device=gpu, generator=g, dtype=dt)
+        kw = dict(a_scale=4.0 / 127, w_scale=(0.5 + torch.rand(N, device=gpu, generator=g)) / (74 * math.sqrt(K)), out_dtype=F16)
+    else:
+        x = torch.randn((M, K), device=gpu, generator=g).to(dt)
+        w = (torch.randn((N, K), device=gpu, generator=g) / math.sqrt(K)).to(dt)
+        kw = dict(out_dtype=dt)
+    b = torch.randn(N, device=gpu, generator=g)
+    rows = torch.cat([torch.arange(0, M, 41), torch.arange(M - 130, M)]).to(gpu)
+    for r in (None, torch.randn((M, N), device=gpu, generator=g).to(F16)):
+        announce(f"linear middle tiles {dt} {M} {K} {N} residual={r is not None}")
+        got = (ops.linear_i8 if i8 else ops.linear)(x, w, b, act="silu", residual=r, **kw)
+        want, tol = ref.linear(x[rows], w, b, act="silu", residual=None if r is None else r[rows], **kw)
+        ref.assert_within(got[rows], want, tol)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (5, 3, 64), (300, 7, 33), (9000, 3, 64), (2000, 65, 1), (4097, 130, 129), (70, 1021, 77)])
 def test_linear_odd_widths(gpu, dt, M, K, N):
