@@ -487,7 +487,7 @@ static int launch_linear(LinearArgs& a, hipStream_t s) {
     if (n1 <= 256) return lengthy ? launch_rows<T, 1, 8, VEC>(a, s) : launch_rows<T, 1, 4, VEC>(a, s);
     if (n2 <= (sizeof(T) == 4 ? 512 : 256)) return lengthy ? launch_rows<T, 2, 8, VEC>(a, s) : launch_rows<T, 2, 4, VEC>(a, s);
     if constexpr (VEC && sizeof(T) < 4) {
-        const double k = (double)((int64_t)a.K * (int)sizeof(T) + 127) / 128;
+        const double k = (double)(((int64_t)a.K * (int)sizeof(T) + 127) / 128);
         const auto rounds = [&](int bm, int bn) { return (double)(((a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) + 255) / 256); };
         const double r = rounds(128, 128);
         const double c[5] = {rounds(64, 64) * (0.24 * k + 0.6), rounds(128, 64) * (0.31 * k + 1.5),
