@@ -602,11 +602,12 @@ def _refuse(**named: Optional[torch.Tensor]) -> None:
 def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
     """The index of the one GPU that all the tensors (None: absent) are on; -1 if there is none, or one needs a gradient."""
     grad = torch.is_grad_enabled()
+    tensor = torch.Tensor
     d = -1
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or (grad and t.requires_grad):
+        if not isinstance(t, tensor) or (grad and t.requires_grad):
             return -1
         i = t.get_device()
         if i != d:
@@ -619,15 +620,21 @@ def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
 # The current stream's handle without building a torch.cuda.Stream (1 us); what the compiled torch code itself calls.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda d: torch.cuda.current_stream(d).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _ENTRIES: dict = {}
 
 
-def _on(d: int, name: str, *args) -> None:
-    """call() on GPU d (the current one or not), on its current stream."""
+def _entry(name: str):
     entry = _ENTRIES.get(name)
     if entry is None:
         entry = _ENTRIES[name] = getattr(lib(), name)
-    if d == torch.cuda.current_device():
+    return entry
+
+
+def _on(d: int, name: str, *args) -> None:
+    """call() on GPU d (the current one or not; there are tensors on it), on its current stream."""
+    entry = _ENTRIES.get(name) or _entry(name)
+    if d == _current_device():
         code = entry(*args, _raw_stream(d))
     else:
         with torch.cuda.device(d):
@@ -783,9 +790,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     coords = _coords(coords, "coords", M)
     if freqs.dtype != torch.float32 or freqs.ndim != 2 or freqs.shape[1] != 3 or not freqs.is_contiguous():
         raise ValueError("freqs must be a contiguous (pairs, 3) float32 tensor")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
-        if t is not None:
-            _vector(t, name, D)
+    if q_weight is not None:
+        _vector(q_weight, "q_weight", D)
+    if k_weight is not None:
+        _vector(k_weight, "k_weight", D)
+    if q_bias is not None:
+        _vector(q_bias, "q_bias", D)
+    if k_bias is not None:
+        _vector(k_bias, "k_bias", D)
     if out is None:
         qo = q.new_empty((M, Hq, D))
         if k is not None:
@@ -815,9 +827,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     return qo, ko
 
 
-def _index(t: Optional[torch.Tensor], name: str) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous()):
+def _index(t: torch.Tensor, name: str) -> None:
+    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+
+
+def _offsets(t: torch.Tensor, name: str) -> None:
+    if t.dtype != torch.int64 or t.ndim != 1 or t.numel() < 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous (segments + 1,) int64 tensor")
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
@@ -859,13 +876,15 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         if Mk != Mq:
             raise ValueError(f"without kv_offsets the keys are the queries' rows: {Mq} and {Mk}")
         kv_offsets, kv_index, kv_coords = offsets, index, coords
-    for name, t in (("offsets", offsets), ("kv_offsets", kv_offsets)):
-        if t.dtype != torch.int64 or t.ndim != 1 or t.numel() < 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous (segments + 1,) int64 tensor")
-    if kv_offsets.numel() != offsets.numel():
-        raise ValueError("offsets and kv_offsets must have the same length")
-    _index(index, "index")
-    _index(kv_index, "kv_index")
+    _offsets(offsets, "offsets")
+    if index is not None:
+        _index(index, "index")
+    if not own:
+        _offsets(kv_offsets, "kv_offsets")
+        if kv_offsets.numel() != offsets.numel():
+            raise ValueError("offsets and kv_offsets must have the same length")
+        if kv_index is not None:
+            _index(kv_index, "kv_index")
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (Hq, 3) or not slopes.is_contiguous():
             raise ValueError(f"slopes must be a contiguous ({Hq}, 3) float32 tensor")
@@ -896,7 +915,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         offsets.data_ptr(), kv_offsets.data_ptr(), _ptr(index), _ptr(kv_index), _ptr(coords) if slopes is not None else 0,
         _ptr(kv_coords) if slopes is not None else 0, _ptr(slopes), _ptr(kv_mask), D ** -0.5 if scale is None else scale,
         cap, fresh)
-    ws_bytes = lib().pmg_attention_workspace_bytes(args)
-    ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+    ws_bytes = _entry("pmg_attention_workspace_bytes")(args)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _on(d, "pmg_attention", args, _ptr(ws), ws_bytes)
     return out
