@@ -9,6 +9,10 @@ struct Plan {
     int seg, whole, splits;
 };
 
+size_t parts_bytes(const pmg_attention_args& r, const Plan& p) {
+    return p.splits <= 1 ? 0 : (size_t)p.splits * (size_t)r.q_positions * (size_t)r.Hq * ((size_t)r.D * 4 + 8);
+}
+
 // The forms, by the mean lengths (the offsets are on the device).
 //
 // A block per segment (seg) where the queries of a segment fill no half wave and its keys are many, the keys split so that
@@ -56,16 +60,13 @@ Plan plan_of(const pmg_attention_args& r) {
         const double alone = (ragged ? 2.5 : 1.0) * nk / 64.0 * tile / s / (f32 && !r.slopes && r.cap == 0.0f ? 0.9 : 0.5) + 1.5;
         const double all = rounds * (keys / 64.0 * tile / s + 1.5);
         const double t = (all > alone ? all : alone) + (s > 1 ? 6.0 + s * part : 0.0);
-        if (s == 1 || t < 0.99 * best) {
+        if (s > 1 && parts_bytes(r, Plan{0, 0, s}) > (size_t)1 << 28) break;  // (256 MB of parts at most)
+        if (s == 1 || t < 0.98 * best) {
             best = t;
             p.splits = s;
         }
     }
     return p;
-}
-
-size_t parts_bytes(const pmg_attention_args& r, const Plan& p) {
-    return p.splits <= 1 ? 0 : (size_t)p.splits * (size_t)r.q_positions * (size_t)r.Hq * ((size_t)r.D * 4 + 8);
 }
 
 int attention_args(const pmg_attention_args& r) {

@@ -85,6 +85,12 @@ def test_attention_workspace_is_asked_for_and_checked(libpmg):
     assert libpmg.pmg_attention_workspace_bytes(None) == 0
 
 
+@pytest.mark.parametrize("rows,heads,width,segments", [(19_200, 4, 64, 1), (76_800, 8, 64, 1), (300_000, 8, 128, 1), (1_000_000, 32, 128, 3), (5_000, 8, 96, 20)])
+def test_attention_workspace_stays_small(libpmg, rows, heads, width, segments):
+    a = attention_args(Hq=heads, Hk=heads, D=width, q_rows=rows, q_positions=rows, k_rows=rows, k_positions=rows, segments=segments)
+    assert libpmg.pmg_attention_workspace_bytes(C.byref(a)) <= 1 << 28
+
+
 def test_null_args_and_empty_calls(libpmg):
     for f in (lambda p: libpmg.pmg_linear(p, None), lambda p: libpmg.pmg_qk_norm_rope(p, None),
               lambda p: libpmg.pmg_attention(p, None, 0, None)):
