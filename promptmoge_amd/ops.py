@@ -600,10 +600,11 @@ def _refuse(**named: Optional[torch.Tensor]) -> None:
 
 
 def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
-    """The index of the one GPU that all the tensors (None: absent) are on; -1 if there is none, or one needs a gradient."""
+    """The index of the one GPU that all the tensors (None: absent) are on; negative if there is none, one is
+    not on a GPU, or one needs a gradient."""
     grad = torch.is_grad_enabled()
     tensor = torch.Tensor
-    d = -1
+    d = -2  # (none seen; a host tensor's is -1)
     for t in tensors:
         if t is None:
             continue
@@ -611,7 +612,7 @@ def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
             return -1
         i = t.get_device()
         if i != d:
-            if d >= 0:
+            if i < 0 or d >= 0:
                 return -1
             d = i
     return d
