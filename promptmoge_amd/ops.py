@@ -741,14 +741,17 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = N
     return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype, out)
 
 
+def _off_units(t: torch.Tensor, unit: int) -> bool:
+    """Whether an (M, H, D) tensor's heads are not contiguous, or some not on `unit` bytes."""
+    row, head, one = t.stride()
+    return one != 1 or (t.data_ptr() | row * t.element_size() | head * t.element_size()) & (unit - 1) != 0
+
+
 def _heads(t: torch.Tensor, name: str, unit: int) -> torch.Tensor:
     """An (M, H, D) tensor whose heads are contiguous, on `unit` bytes; copied where its strides or address are not."""
     if t.ndim != 3:
         raise ValueError(f"{name} must be (rows, heads, width), got {tuple(t.shape)}")
-    row, head, one = t.stride()
-    if one != 1 or (t.data_ptr() | row * t.element_size() | head * t.element_size()) & (unit - 1):
-        t = t.contiguous()
-    return t
+    return t.clone(memory_format=torch.contiguous_format) if _off_units(t, unit) else t  # (contiguous() keeps an odd address)
 
 
 def _coords(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
@@ -807,7 +810,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
         for name, t, o in (("out[0]", q, qo), ("out[1]", k, ko)):
             if (t is None) != (o is None) or (t is not None and (o.shape != t.shape or o.dtype != q.dtype)):
                 raise ValueError(f"{name} must match its input")
-            if o is not None and _heads(o, name, unit) is not o:
+            if o is not None and _off_units(o, unit):
                 raise ValueError(f"{name}: strides and address must be whole groups of 4 elements")
             for other in (q, k):  # (the inputs themselves are fine: each head is read whole before it is written)
                 if o is not None and other is not None and _overlap(o, other) and not (
@@ -904,7 +907,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
-        if _heads(out, "out", 4 * q.element_size()) is not out:
+        if _off_units(out, 4 * q.element_size()):
             raise ValueError("out: strides and address must be whole groups of 4 elements")
         if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
             raise ValueError("out must not overlap q, k or v")

@@ -82,3 +82,32 @@ def test_the_places_are_all_there_are():
         named = set(inspect.signature(getattr(ops, name)).parameters)
         rest = {"act", "out_dtype", "a_scale", "norm", "eps", "interleaved", "cap", "scale"}
         assert named - rest == set(args)
+
+
+@pytest.mark.parametrize("make", [
+    lambda b: b[1:97].view(3, 2, 16),                                       # contiguous, but at an odd element
+    lambda b: b[:96].view(3, 2, 16)[:, :1].as_strided((3, 1, 16), (32, 17, 1)),  # one head, whose stride means nothing
+    lambda b: b[4:52].view(1, 3, 16).as_strided((1, 3, 16), (51, 16, 1)),    # one row
+    lambda b: b[:102].view(3, 34)[:, 1:33].unflatten(1, (2, 16)),            # odd columns
+    lambda b: b[:96].view(3, 16, 2).transpose(1, 2),                         # heads not contiguous
+])
+def test_heads_off_their_units_are_copied(make):
+    t = make(torch.arange(128, dtype=torch.float32).to(F16))
+    for unit in (8, 16):
+        c = ops._heads(t, "q", unit)
+        assert torch.equal(c, t) and c.data_ptr() % unit == 0 and c.stride(2) == 1
+        assert c.stride(0) * 2 % unit == 0 and c.stride(1) * 2 % unit == 0
+    straight = torch.zeros(3, 2, 16, dtype=F16)
+    assert ops._heads(straight, "q", 16) is straight
+
+
+def test_an_out_off_its_units_is_refused(no_launch):
+    for shape in ((5, 2, 16), (5, 1, 16)):
+        n = shape[0] * shape[1] * 16
+        x = on_gpu(zeros(*shape))
+        c, f = on_gpu(zeros(5, 4, dtype=torch.int32)), on_gpu(zeros(8, 3, dtype=F32))
+        odd = on_gpu(zeros(n + 8)[1:n + 1].view(shape))
+        with pytest.raises(ValueError, match="groups of 4"):
+            ops.qk_norm_rope(x, None, c, f, out=(odd, None))
+        with pytest.raises(ValueError, match="groups of 4"):
+            ops.sparse_attention(x, x, x, on_gpu(torch.tensor([0, 5])), out=odd)

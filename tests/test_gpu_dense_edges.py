@@ -1,0 +1,38 @@
+"""The dense operators (ops.linear, linear_i8, qk_norm_rope, sparse_attention) where calls are unusual: addresses, extremes,
+tables that do not hold what they should, launches larger than a grid."""
+import math
+
+import pytest
+import torch
+
+import dense_ref as ref
+from conftest import announce
+from promptmoge_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F16, BF16, F32]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("H", [1, 2])
+def test_heads_at_odd_addresses(gpu, dt, H):
+    """Contiguous tensors that start at an odd element: the results of their aligned copies, bit for bit."""
+    g = gen(3)
+    M, D = 70, 32
+    off = torch.tensor([0, 30, 70], device=gpu)
+    c, f = torch.randint(0, 50, (M, 4), generator=g, dtype=torch.int32).to(gpu), torch.rand((D // 2, 3), generator=g).to(gpu)
+    q, k, v = (randn(g, M * H * D + 1).to(dt).to(gpu)[1:].view(M, H, D) for _ in range(3))
+    announce(f"heads at odd addresses {dt} {H}")
+    got, want = ops.qk_norm_rope(q, k, c, f), ops.qk_norm_rope(q.clone(), k.clone(), c, f)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(ops.sparse_attention(q, k, v, off), ops.sparse_attention(q.clone(), k.clone(), v.clone(), off))
