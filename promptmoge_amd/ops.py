@@ -667,13 +667,31 @@ def _rows(t: torch.Tensor, name: str) -> int:
     raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
 
 
+def _layout(t: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(address, end, period, width) in bytes: `width` bytes from the address on, and again every `period` bytes (the
+    widest stride; 0: once), hold all of a tensor that is not empty."""
+    axes = [(st, n - 1) for st, n in zip(t.stride(), t.shape) if n > 1]
+    span, (period, more) = sum(st * n for st, n in axes) + 1, max(axes, default=(0, 0))
+    es = t.element_size()
+    return t.data_ptr(), t.data_ptr() + span * es, period * es, (span - period * more) * es
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    """Whether two tensors share memory. Columns of one buffer (equal widest strides) are told apart; of other tensors
+    laced into each other it is taken that they do."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1, pa, wa), (b0, b1, pb, wb) = _layout(a), _layout(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if pa != pb and a1 - a0 <= pb:  # (all of a in one of b's periods, as one row)
+        pa, wa = pb, a1 - a0
+    elif pa != pb and b1 - b0 <= pa:
+        pb, wb = pa, b1 - b0
+    if pa != pb or wa > pa or wb > pb:
+        return True
+    ahead = (b0 - a0) % pa
+    return ahead < wa or ahead + wb > pa
 
 
 def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
@@ -807,16 +825,16 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
         if k is not None:
             ko = q.new_empty((M, k.shape[1], D))
     else:
-        for name, t, o in (("out[0]", q, qo), ("out[1]", k, ko)):
+        for i, (name, t, o) in enumerate((("out[0]", q, qo), ("out[1]", k, ko))):
             if (t is None) != (o is None) or (t is not None and (o.shape != t.shape or o.dtype != q.dtype)):
                 raise ValueError(f"{name} must match its input")
             if o is not None and _off_units(o, unit):
                 raise ValueError(f"{name}: strides and address must be whole groups of 4 elements")
-            for other in (q, k):  # (the inputs themselves are fine: each head is read whole before it is written)
+            for j, other in enumerate((q, k)):  # (its input itself is fine: each head is read whole before it is written)
                 if o is not None and other is not None and _overlap(o, other) and not (
-                        o.data_ptr() == t.data_ptr() and o.stride() == t.stride()):
+                        i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()):
                     raise ValueError(f"{name} may be its input itself, but not overlap the inputs otherwise")
-        if ko is not None and _overlap(qo, ko) and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
+        if ko is not None and _overlap(qo, ko):
             raise ValueError("out[0] and out[1] must not overlap")
     q = _heads(q, "q", unit)
     k = _heads(k, "k", unit) if k is not None else None

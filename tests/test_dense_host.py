@@ -111,3 +111,52 @@ def test_an_out_off_its_units_is_refused(no_launch):
             ops.qk_norm_rope(x, None, c, f, out=(odd, None))
         with pytest.raises(ValueError, match="groups of 4"):
             ops.sparse_attention(x, x, x, on_gpu(torch.tensor([0, 5])), out=odd)
+
+
+def test_overlap_of_strided_tensors_is_that_of_their_elements():
+    """Against the sets of bytes themselves, over slices of one buffer; a doubtful pair may count as overlapping only where rows
+    of different strides (or more than one axis that leaves gaps) are laced into each other."""
+    buf = torch.zeros(4, 6, 10)
+    views = [buf[:, a:b] for a, b in ((0, 2), (2, 4), (1, 3), (5, 6))] + [buf[:, :, 2:4], buf[:, :, 4:8], buf[1:2], buf[:0], buf[2:, 1:3],
+             buf.view(24, 10)[:, :5], buf.view(24, 10)[:, 5:], buf.view(24, 10)[3:9, 4:6], buf.view(-1)[7:30],
+             buf.permute(1, 0, 2)[:3], buf.permute(1, 0, 2)[3:], buf.view(4, 60)[:, 12:40], buf.view(4, 60)[:, 40:], buf.view(4, 60)[:1, :40]]
+    sets = [{v.data_ptr() + 4 * sum(i * s for i, s in zip(at, v.stride())) for at in torch.cartesian_prod(*[torch.arange(n) for n in v.shape]).view(-1, v.ndim).tolist()}
+            if v.numel() else set() for v in views]
+    for a, sa in zip(views, sets):
+        for b, sb in zip(views, sets):
+            truth = bool(sa & sb)
+            assert ops._overlap(a, b) or not truth
+            wide = [max((s for n, s in zip(v.shape, v.stride()) if n > 1), default=0) for v in (a, b)]
+            if not truth and a.ndim == 2 and b.ndim == 2 and wide[0] == wide[1]:
+                assert not ops._overlap(a, b), (a.shape, a.stride(), b.shape, b.stride())
+
+
+def test_disjoint_columns_of_one_buffer_are_taken(no_launch):
+    buf = on_gpu(zeros(5, 64))
+    w = on_gpu(zeros(32, 32))
+    with pytest.raises(Reached):
+        ops.linear(buf[:, :32], w, out=buf[:, 32:])
+    with pytest.raises(Reached):
+        ops.linear(buf[:, :32], on_gpu(zeros(16, 32)), residual=buf[:, 32:48], out=buf[:, 48:])
+    for a, b in ((0, 31), (1, 0), (8, 24)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.linear(buf[:, a:a + 32], w, out=buf[:, b:b + 32])
+    qk = on_gpu(zeros(5, 6, 16))
+    c, f = on_gpu(zeros(5, 4, dtype=torch.int32)), on_gpu(zeros(8, 3, dtype=F32))
+    with pytest.raises(Reached):  # q and k side by side, in and out
+        ops.qk_norm_rope(qk[:, :2], qk[:, 2:3], c, f, out=(qk[:, 3:5], qk[:, 5:]))
+    with pytest.raises(Reached):  # the same in place
+        ops.qk_norm_rope(qk[:, :2], qk[:, 2:3], c, f, out=(qk[:, :2], qk[:, 2:3]))
+    hq = on_gpu(zeros(3, 5, 16)).permute(1, 0, 2)  # heads first
+    with pytest.raises(Reached):
+        ops.qk_norm_rope(hq[:, :2], hq[:, 2:], c, f, out=(hq[:, :2], hq[:, 2:]))
+    with pytest.raises(Reached):
+        ops.sparse_attention(qk[:, :2], qk[:, 2:4], qk[:, 2:4], on_gpu(torch.tensor([0, 5])), out=qk[:, 4:])
+    with pytest.raises(ValueError, match="overlap"):
+        ops.sparse_attention(qk[:, :2], qk[:, 2:4], qk[:, 2:4], on_gpu(torch.tensor([0, 5])), out=qk[:, 3:5])
+    with pytest.raises(ValueError, match="overlap"):  # k would be read while q, the same rows, is written
+        ops.qk_norm_rope(qk[:, :2], qk[:, :2], c, f, out=(qk[:, :2], on_gpu(zeros(5, 2, 16))))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.qk_norm_rope(qk[:, :2], qk[:, 2:4], c, f, out=(qk[:, 2:4], qk[:, :2]))
+    with pytest.raises(ValueError, match="must not overlap"):
+        ops.qk_norm_rope(qk[:, :2], qk[:, 2:4], c, f, out=(on_gpu(zeros(5, 2, 16)),) * 2)

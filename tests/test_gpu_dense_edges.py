@@ -36,3 +36,29 @@ def test_heads_at_odd_addresses(gpu, dt, H):
     got, want = ops.qk_norm_rope(q, k, c, f), ops.qk_norm_rope(q.clone(), k.clone(), c, f)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(ops.sparse_attention(q, k, v, off), ops.sparse_attention(q.clone(), k.clone(), v.clone(), off))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_results_beside_their_inputs_in_one_buffer(gpu, dt):
+    """Outputs in other columns of the inputs' own rows; what lies beside them stays."""
+    g = gen(4)
+    M, D = 90, 32
+    announce(f"results beside inputs {dt}")
+    buf = randn(g, M, 160).to(dt).to(gpu)
+    w = randn(g, 64, 64).to(dt).to(gpu)
+    want = ops.linear(buf[:, 16:80].clone(), w)
+    keep = buf.clone()
+    ops.linear(buf[:, 16:80], w, out=buf[:, 80:144])
+    assert torch.equal(buf[:, 80:144], want) and torch.equal(buf[:, :80], keep[:, :80]) and torch.equal(buf[:, 144:], keep[:, 144:])
+    x = randn(g, M, 8, D).to(dt).to(gpu)
+    c, f = torch.randint(0, 50, (M, 4), generator=g, dtype=torch.int32).to(gpu), torch.rand((D // 2, 3), generator=g).to(gpu)
+    keep = x.clone()
+    want = ops.qk_norm_rope(keep[:, :2], keep[:, 2:3], c, f)
+    ops.qk_norm_rope(x[:, :2], x[:, 2:3], c, f, out=(x[:, 4:6], x[:, 6:7]))
+    assert torch.equal(x[:, 4:6], want[0]) and torch.equal(x[:, 6:7], want[1])
+    assert torch.equal(x[:, :4], keep[:, :4]) and torch.equal(x[:, 7:], keep[:, 7:])
+    off = torch.tensor([0, 40, M], device=gpu)
+    want = ops.sparse_attention(keep[:, :2], keep[:, 2:4], keep[:, 4:6], off)
+    x = keep.clone()
+    ops.sparse_attention(x[:, :2], x[:, 2:4], x[:, 4:6], off, out=x[:, 6:])
+    assert torch.equal(x[:, 6:], want) and torch.equal(x[:, :6], keep[:, :6])
