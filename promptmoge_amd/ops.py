@@ -694,6 +694,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return ahead < wa or ahead + wb > pa
 
 
+def _apart(out: torch.Tensor, name: str, **others: Optional[torch.Tensor]) -> None:
+    """Refuses a result on an argument that other blocks still read when it is written."""
+    for other, t in others.items():
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{name} must not overlap {other}")
+
+
 def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
     d = _one_gpu(x, w, bias, w_scale, residual, out)
     if d < 0:
@@ -725,8 +732,7 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
     else:
         if out.shape != (M, N):
             raise ValueError(f"out must be ({M}, {N}), got {tuple(out.shape)}")
-        if _overlap(out, x) or _overlap(out, w):
-            raise ValueError("out must not overlap x or w")
+        _apart(out, "out", x=x, w=w, bias=bias, w_scale=w_scale)
         if residual is not None and _overlap(out, residual) and not (
                 out.data_ptr() == residual.data_ptr() and out.dtype == residual.dtype
                 and out.stride() == residual.stride()):
@@ -834,6 +840,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
                 if o is not None and other is not None and _overlap(o, other) and not (
                         i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()):
                     raise ValueError(f"{name} may be its input itself, but not overlap the inputs otherwise")
+            if o is not None:
+                _apart(o, name, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias)
         if ko is not None and _overlap(qo, ko):
             raise ValueError("out[0] and out[1] must not overlap")
     q = _heads(q, "q", unit)
@@ -927,8 +935,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
         if _off_units(out, 4 * q.element_size()):
             raise ValueError("out: strides and address must be whole groups of 4 elements")
-        if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
-            raise ValueError("out must not overlap q, k or v")
+        _apart(out, "out", q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index,
+               coords=coords, kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask)
     q, k, v = _heads(q, "q", 16), _heads(k, "k", 16), _heads(v, "v", 16)
     (qs, qh, _), (ks, kh, _), (vs, vh, _), (os, oh, _) = q.stride(), k.stride(), v.stride(), out.stride()
     args = _lib.ATTENTION_PACK.pack(

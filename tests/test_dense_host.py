@@ -160,3 +160,23 @@ def test_disjoint_columns_of_one_buffer_are_taken(no_launch):
         ops.qk_norm_rope(qk[:, :2], qk[:, 2:4], c, f, out=(qk[:, 2:4], qk[:, :2]))
     with pytest.raises(ValueError, match="must not overlap"):
         ops.qk_norm_rope(qk[:, :2], qk[:, 2:4], c, f, out=(on_gpu(zeros(5, 2, 16)),) * 2)
+
+
+@pytest.mark.parametrize("name,place", [
+    ("linear", "bias"), ("linear_i8", "bias"), ("linear_i8", "w_scale"), ("qk_norm_rope", "coords"), ("qk_norm_rope", "freqs"),
+    ("qk_norm_rope", "q_weight"), ("qk_norm_rope", "k_weight"), ("qk_norm_rope", "q_bias"), ("qk_norm_rope", "k_bias"),
+    ("sparse_attention", "offsets"), ("sparse_attention", "kv_offsets"), ("sparse_attention", "index"), ("sparse_attention", "kv_index"),
+    ("sparse_attention", "coords"), ("sparse_attention", "kv_coords"), ("sparse_attention", "slopes"), ("sparse_attention", "kv_mask")])
+def test_an_out_on_another_argument_is_refused(no_launch, name, place):
+    """A block would write what another one still reads."""
+    args = next(a for n, a, _ in calls() if n == name)
+    args = {n: everywhere(v) for n, v in args.items()}
+    bytes_ = torch.zeros(4096, dtype=torch.uint8)
+    t = args[place]
+    args[place] = on_gpu(bytes_[:t.numel() * t.element_size()].view(t.dtype).view(t.shape))
+    lay = lambda o: on_gpu(bytes_[:o.numel() * o.element_size()].view(o.dtype).view(o.shape))  # noqa: E731
+    for which in range(len(args["out"])) if isinstance(args["out"], tuple) else [None]:
+        out = args["out"]
+        out = lay(out) if which is None else tuple(lay(o) if i == which else o for i, o in enumerate(out))
+        with pytest.raises(ValueError, match="overlap"):
+            getattr(ops, name)(**{**args, "out": out})
