@@ -778,6 +778,14 @@ def _heads(t: torch.Tensor, name: str, unit: int) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format) if _off_units(t, unit) else t  # (contiguous() keeps an odd address)
 
 
+def _laced(t: torch.Tensor) -> bool:
+    """Whether an (M, H, D) tensor's heads may overlap one another: neither its rows lie apart within a head's stride nor its
+    heads within a row's."""
+    (M, H, D), (row, head, _) = t.shape, t.stride()
+    apart = lambda n, near, m, far: (n <= 1 or near >= D) and (m <= 1 or far >= (n - 1) * near * (n > 1) + D)  # noqa: E731
+    return t.numel() > 0 and not (apart(H, head, M, row) or apart(M, row, H, head))
+
+
 def _coords(t: torch.Tensor, name: str, rows: int) -> torch.Tensor:
     if t.dtype != torch.int32 or t.shape != (rows, 4):
         raise ValueError(f"{name} must be ({rows}, 4) int32, got {tuple(t.shape)} {t.dtype}")
@@ -836,6 +844,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
                 raise ValueError(f"{name} must match its input")
             if o is not None and _off_units(o, unit):
                 raise ValueError(f"{name}: strides and address must be whole groups of 4 elements")
+            if o is not None and _laced(o):
+                raise ValueError(f"{name}: its own rows and heads must not overlap")
             for j, other in enumerate((q, k)):  # (its input itself is fine: each head is read whole before it is written)
                 if o is not None and other is not None and _overlap(o, other) and not (
                         i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()):
@@ -935,6 +945,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")
         if _off_units(out, 4 * q.element_size()):
             raise ValueError("out: strides and address must be whole groups of 4 elements")
+        if _laced(out):
+            raise ValueError("out: its own rows and heads must not overlap")
         _apart(out, "out", q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index,
                coords=coords, kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask)
     q, k, v = _heads(q, "q", 16), _heads(k, "k", 16), _heads(v, "v", 16)

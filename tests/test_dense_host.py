@@ -180,3 +180,27 @@ def test_an_out_on_another_argument_is_refused(no_launch, name, place):
         out = lay(out) if which is None else tuple(lay(o) if i == which else o for i, o in enumerate(out))
         with pytest.raises(ValueError, match="overlap"):
             getattr(ops, name)(**{**args, "out": out})
+
+
+def test_an_out_whose_own_rows_overlap_is_refused(no_launch):
+    """Different results would be written to one place."""
+    x, off = on_gpu(zeros(6, 2, 16)), on_gpu(torch.tensor([0, 6]))
+    c, f = on_gpu(zeros(6, 4, dtype=torch.int32)), on_gpu(zeros(8, 3, dtype=F32))
+    big = zeros(512)
+    for strides in ((0, 16, 1), (16, 16, 1), (32, 0, 1), (24, 12, 1), (8, 96, 1), (16, 80, 1)):
+        out = on_gpu(big.as_strided((6, 2, 16), strides))
+        with pytest.raises(ValueError, match="overlap"):
+            ops.sparse_attention(x, x, x, off, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            ops.qk_norm_rope(x, None, c, f, out=(out, None))
+        with pytest.raises(ValueError, match="overlap"):
+            ops.qk_norm_rope(x, x, c, f, out=(on_gpu(zeros(6, 2, 16)), out))
+    for strides in ((32, 16, 1), (48, 20, 1), (16, 96, 1), (20, 120, 1)):
+        out = on_gpu(big.as_strided((6, 2, 16), strides))
+        with pytest.raises(Reached):
+            ops.sparse_attention(x, x, x, off, out=out)
+        with pytest.raises(Reached):
+            ops.qk_norm_rope(x, None, c, f, out=(out, None))
+    one = on_gpu(big.as_strided((1, 2, 16), (0, 16, 1)))
+    with pytest.raises(Reached):
+        ops.sparse_attention(x[:1], x[:1], x[:1], off, out=one)
