@@ -732,6 +732,8 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
     else:
         if out.shape != (M, N):
             raise ValueError(f"out must be ({M}, {N}), got {tuple(out.shape)}")
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise ValueError(f"out_dtype is {out_dtype}, out has {out.dtype}")
         _apart(out, "out", x=x, w=w, bias=bias, w_scale=w_scale)
         if residual is not None and _overlap(out, residual) and not (
                 out.data_ptr() == residual.data_ptr() and out.dtype == residual.dtype
@@ -750,19 +752,20 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     """act(x w^T + bias) + residual in one kernel: nn.Linear of the U-Net's PoolDown, NearestUp and projections with what
     follows it. x: (M, K) fp32 / fp16 / bf16 (rows may be strided); w: (N, K) of x's type; bias: (N,) fp32; act: "none",
     "relu", "silu", "gelu" (erf) or "gelu_tanh"; residual: (M, N) of any of the three types. Sums in fp32, rounded
-    once to out_dtype (default: x's). `out` may be the residual itself. Forward only."""
+    once to out_dtype (default: out's, or x's). `out` may be the residual itself. Forward only."""
     _floating(x, "x")
-    return _linear(x, w, bias, 1.0, None, act, residual, out_dtype or (x.dtype if out is None else out.dtype), out)
+    return _linear(x, w, bias, 1.0, None, act, residual, out_dtype or (x.dtype if out is None else None), out)
 
 
 def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, a_scale: float = 1.0,
               w_scale: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
-              out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """linear on int8 codes: act((acc * a_scale) * w_scale[n] + bias) + residual with the exact int32 sums acc, the
-    arithmetic of spconv_i8. x: (M, K) int8; w: (N, K) int8; w_scale, bias: (N,) fp32; result fp32, fp16 or bf16."""
+    arithmetic of spconv_i8. x: (M, K) int8; w: (N, K) int8; w_scale, bias: (N,) fp32; result fp32 (default), fp16 or
+    bf16."""
     if x.dtype != torch.int8:
         raise ValueError(f"x must be torch.int8, got {x.dtype}")
-    return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype, out)
+    return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype or (torch.float32 if out is None else None), out)
 
 
 def _off_units(t: torch.Tensor, unit: int) -> bool:

@@ -204,3 +204,16 @@ def test_an_out_whose_own_rows_overlap_is_refused(no_launch):
     one = on_gpu(big.as_strided((1, 2, 16), (0, 16, 1)))
     with pytest.raises(Reached):
         ops.sparse_attention(x[:1], x[:1], x[:1], off, out=one)
+
+
+def test_out_dtype_has_to_be_that_of_out(no_launch):
+    x, w, q, u = on_gpu(zeros(4, 16)), on_gpu(zeros(8, 16)), on_gpu(zeros(4, 16, dtype=torch.int8)), on_gpu(zeros(8, 16, dtype=torch.int8))
+    for out in (F16, F32, torch.bfloat16):
+        o = on_gpu(zeros(4, 8, dtype=out))
+        for want in (F16, F32, torch.bfloat16):
+            for f in (lambda: ops.linear(x, w, out_dtype=want, out=o), lambda: ops.linear_i8(q, u, out_dtype=want, out=o)):
+                with pytest.raises(Reached if want == out else ValueError, match=None if want == out else "out_dtype"):
+                    f()
+        for f in (lambda: ops.linear(x, w, out=o), lambda: ops.linear_i8(q, u, out=o)):  # out says it
+            with pytest.raises(Reached):
+                f()
