@@ -9,6 +9,7 @@ import ctypes as C
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import EPI_ACC, EPI_BIAS, EPI_Q, EPI_QLIN, EPI_R, EPI_RLN, EPI_ROUT, EPI_SILU, ConvEpilogue, call, check, lib
@@ -584,8 +585,12 @@ _TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bflo
           torch.int8: _lib.TYPE_I8}
 
 
-def _refuse(**named: Optional[torch.Tensor]) -> None:
-    """Says which of the tensors (None: absent) is not on the first one's GPU or needs a gradient."""
+def _in_forward_ad() -> bool:
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def _refuse(**named: Optional[torch.Tensor]) -> int:
+    """Says which of the tensors (None: absent) is not on the first one's GPU or needs a gradient; that GPU's index if none."""
     dev = None
     for name, t in named.items():
         if t is None:
@@ -595,13 +600,17 @@ def _refuse(**named: Optional[torch.Tensor]) -> None:
         dev = t.device if dev is None else dev
         if t.device != dev:
             raise ValueError(f"{name} is on {t.device}, the other tensors on {dev}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the libpmg operators are inference-only; run under torch.no_grad()")
+        if (t.requires_grad and torch.is_grad_enabled()) or (
+                _in_forward_ad() and forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError("the libpmg operators are inference-only; run under torch.no_grad(), without tangents")
+    if dev is None:
+        raise ValueError("no tensors")
+    return dev.index
 
 
 def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
-    """The index of the one GPU that all the tensors (None: absent) are on; negative if there is none, one is
-    not on a GPU, or one needs a gradient."""
+    """The index of the one GPU that all the tensors (None: absent) are on; negative if that takes a closer look (_refuse):
+    one may not be on a GPU, on another one, or need a gradient."""
     grad = torch.is_grad_enabled()
     tensor = torch.Tensor
     d = -2  # (none seen; a host tensor's is -1)
@@ -615,7 +624,7 @@ def _one_gpu(*tensors: Optional[torch.Tensor]) -> int:
             if i < 0 or d >= 0:
                 return -1
             d = i
-    return d
+    return -1 if _in_forward_ad() else d
 
 
 # The current stream's handle without building a torch.cuda.Stream (1 us); what the compiled torch code itself calls.
@@ -704,7 +713,7 @@ def _apart(out: torch.Tensor, name: str, **others: Optional[torch.Tensor]) -> No
 def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
     d = _one_gpu(x, w, bias, w_scale, residual, out)
     if d < 0:
-        _refuse(x=x, w=w, bias=bias, w_scale=w_scale, residual=residual, out=out)
+        d = _refuse(x=x, w=w, bias=bias, w_scale=w_scale, residual=residual, out=out)
     ldx = _rows(x, "x")
     M, K = x.shape
     if w.dtype != x.dtype:
@@ -815,8 +824,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     qo, ko = out if out is not None else (None, None)
     d = _one_gpu(q, k, coords, freqs, q_weight, k_weight, q_bias, k_bias, qo, ko)
     if d < 0:
-        _refuse(q=q, k=k, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias,
-                out_q=qo, out_k=ko)
+        d = _refuse(q=q, k=k, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias,
+                    out_q=qo, out_k=ko)
     ty = _floating(q, "q")
     unit = 4 * q.element_size()
     if norm not in ("rms", "layer"):
@@ -901,8 +910,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     not written). offsets that fall leave rows unwritten, too. Forward only."""
     d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
     if d < 0:
-        _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
-                kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask, out=out)
+        d = _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
+                    kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask, out=out)
     ty = _floating(q, "q")
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"q must be (Mq, Hq, D), k and v (Mk, Hk, D); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")

@@ -217,3 +217,20 @@ def test_out_dtype_has_to_be_that_of_out(no_launch):
         for f in (lambda: ops.linear(x, w, out=o), lambda: ops.linear_i8(q, u, out=o)):  # out says it
             with pytest.raises(Reached):
                 f()
+
+
+@pytest.mark.parametrize("name,place", [(n, p) for n, args, _ in calls() for p, v in args.items() if p != "out" and v.is_floating_point()])
+def test_forward_mode_tangents_are_refused(no_launch, name, place):
+    """They would be lost in silence. Without a tangent, or outside its level, the call is made."""
+    args = next(a for n, a, _ in calls() if n == name)
+    every = {n: everywhere(v) for n, v in args.items()}
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(Reached):
+            getattr(ops, name)(**every)
+        dual = torch.autograd.forward_ad.make_dual(args[place], torch.ones_like(args[place]))
+        with pytest.raises(RuntimeError, match="inference-only"):
+            getattr(ops, name)(**{**every, place: on_gpu(dual)})
+        with pytest.raises(ValueError, match="GPU tensor"):  # on the host as well
+            getattr(ops, name)(**{**every, "out": args["out"]})
+    with pytest.raises(Reached):
+        getattr(ops, name)(**every)
