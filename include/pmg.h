@@ -570,8 +570,9 @@ enum { PMG_ACT_NONE = 0, PMG_ACT_RELU = 1, PMG_ACT_SILU = 2, PMG_ACT_GELU = 3 /*
  *   type: of x and w. fp32, fp16, bf16: fp32 sums, the scales are not read. int8: exact int32 sums, the int8 arithmetic of
  *   pmg_spconv_i8. One rounding, to out_type, at the end. x: rows of ldx >= K elements; w [N][K]; residual and out: rows
  *   of ldr, ldo >= N elements. out may be residual (same type and ldr = ldo); it must not overlap x or w.
- *   K 1 .. 131072, N 1 .. 2^24, M 0 .. 2^31 - 1, ldx at most 4 MiB; any alignment of whole elements (rows of x and w on
- *   16 bytes with K a whole number of 16 bytes are read 16 bytes at a time, others element by element). */
+ *   K 1 .. 131072 (int8: 131071, so that no sum passes 32 bits), N 1 .. 2^24, M 0 .. 2^31 - 1, ldx at most 4 MiB; any
+ *   alignment of whole elements (rows of x and w on 16 bytes with K a whole number of 16 bytes are read 16 bytes at a time,
+ *   others element by element). */
 typedef struct {
     int type;
     const void* x;

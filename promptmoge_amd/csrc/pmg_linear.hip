@@ -516,7 +516,8 @@ extern "C" int pmg_linear(const pmg_linear_args* p, void* stream) {
     PMG_REQUIRE(q.out_type >= PMG_TYPE_F32 && q.out_type <= PMG_TYPE_BF16, "out_type must be f32, f16 or bf16");
     PMG_REQUIRE(q.act >= PMG_ACT_NONE && q.act <= PMG_ACT_GELU_TANH, "unknown activation");
     PMG_REQUIRE(q.M >= 0 && q.M < (int64_t)1 << 31, "M out of range");
-    PMG_REQUIRE(q.K >= 1 && q.K <= 131072 && q.N >= 1 && q.N <= (1 << 24), "K must be 1 .. 131072 and N 1 .. 2^24");
+    // (int8: 131072 products of -128 by -128 are 2^31)
+    PMG_REQUIRE(q.K >= 1 && q.K <= (q.type == PMG_TYPE_I8 ? 131071 : 131072) && q.N >= 1 && q.N <= (1 << 24), "K must be 1 .. 131072 (int8: 131071) and N 1 .. 2^24");
     const int es = bytes(q.type);
     PMG_REQUIRE(q.ldx >= q.K && q.ldx <= (1 << 22) / es && q.ldo >= q.N && (!q.residual || q.ldr >= q.N), "row strides must cover the row (x: at most 4 MiB)");
     if (q.M == 0) return PMG_OK;

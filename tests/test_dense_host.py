@@ -1,11 +1,13 @@
 """What the dense operators' Python entries decide on the host before anything is launched. The tensors here say that they
 are on a GPU and are not; nothing may reach a kernel."""
+import ctypes as C
 import inspect
 
 import pytest
 import torch
 
-from promptmoge_amd import ops
+from promptmoge_amd import _lib, ops
+from test_dense_abi import linear_args
 
 F16, F32 = torch.float16, torch.float32
 
@@ -234,3 +236,13 @@ def test_forward_mode_tangents_are_refused(no_launch, name, place):
             getattr(ops, name)(**{**every, "out": args["out"]})
     with pytest.raises(Reached):
         getattr(ops, name)(**every)
+
+
+def test_int8_sums_that_could_pass_32_bits_are_refused(libpmg):
+    """131,072 products of -128 by -128 are 2^31; one fewer fit."""
+    i8 = dict(type=_lib.TYPE_I8, ldx=1 << 18)
+    assert (-128) ** 2 * 131_072 > 2 ** 31 - 1 >= (-128) ** 2 * 131_071
+    assert libpmg.pmg_linear(C.byref(linear_args(K=131_072, **i8)), None) == _lib.PMG_E_INVALID
+    assert b"K must" in libpmg.pmg_last_error()
+    assert libpmg.pmg_linear(C.byref(linear_args(K=131_071, M=0, **i8)), None) == _lib.PMG_OK
+    assert libpmg.pmg_linear(C.byref(linear_args(K=131_072, M=0, ldx=1 << 18)), None) == _lib.PMG_OK

@@ -62,3 +62,14 @@ def test_results_beside_their_inputs_in_one_buffer(gpu, dt):
     x = keep.clone()
     ops.sparse_attention(x[:, :2], x[:, 2:4], x[:, 4:6], off, out=x[:, 6:])
     assert torch.equal(x[:, 6:], want) and torch.equal(x[:, :6], keep[:, :6])
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_linear_i8_largest_sums(gpu, M):
+    """All codes -128 over the longest k: sums of 2^31 - 2^14, exact in fp32 (17 bits times 2^14)."""
+    announce(f"linear_i8 largest sums, M={M}")
+    x = torch.full((M, 131_071), -128, dtype=torch.int8, device=gpu)
+    w = torch.full((70, 131_071), -128, dtype=torch.int8, device=gpu)
+    w[::2] = 127
+    got = ops.linear_i8(x, w)
+    assert bool((got[:, 1::2] == float(2 ** 31 - 2 ** 14)).all()) and bool((got[:, ::2] == float(-128 * 127 * 131_071)).all())
