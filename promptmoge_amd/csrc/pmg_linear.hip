@@ -34,13 +34,14 @@ struct LinearArgs {
 // within 0.75e-7 |y|): for outputs of 16 bits, whose half step is 2^-12 of the value at the least; fp32 outputs take
 // erff, several times as long.
 __device__ inline float gelu_16(float y) {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, __builtin_fabsf(y), 1.0f));
+    const float x = __builtin_fminf(y, 3.0e38f);  // (+inf: 0 times it would be NaN; -inf and NaN give NaN, as -inf times 0 does)
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, __builtin_fabsf(x), 1.0f));
     float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
     p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
     p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
     p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
-    const float q = (p * t) * __builtin_amdgcn_exp2f((y * y) * (-0.5f * PMG_LOG2E));
-    return __builtin_fmaf(-__builtin_fabsf(y), q, y < 0.0f ? 0.0f : y);
+    const float q = (p * t) * __builtin_amdgcn_exp2f((x * x) * (-0.5f * PMG_LOG2E));
+    return __builtin_fmaf(-__builtin_fabsf(x), q, y < 0.0f ? 0.0f : y);
 }
 
 // act of 8 values in place; wide: for fp32 outputs.

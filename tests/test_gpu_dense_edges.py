@@ -73,3 +73,23 @@ def test_linear_i8_largest_sums(gpu, M):
     w[::2] = 127
     got = ops.linear_i8(x, w)
     assert bool((got[:, 1::2] == float(2 ** 31 - 2 ** 14)).all()) and bool((got[:, ::2] == float(-128 * 127 * 131_071)).all())
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("M", [5, 700])
+def test_linear_activations_of_infinities(gpu, act, out, M):
+    """What the formula gives for +-inf and NaN, whatever the result's type and the kernel's form."""
+    announce(f"linear activations of infinities {act} {out} {M}")
+    x = torch.zeros(M, 64, device=gpu)
+    x[:, 0] = torch.tensor([math.inf, -math.inf, math.nan, 1e30, -1e30], device=gpu).repeat(M // 5)
+    w = torch.zeros(48, 64, device=gpu)
+    w[:, 0] = 1
+    want = {"none": [math.inf, -math.inf, math.nan, math.inf, -math.inf], "relu": [math.inf, 0, math.nan, math.inf, 0]}.get(
+        act, [math.inf, math.nan, math.nan, math.inf, 0])  # (-inf times 0)
+    if out != F16:  # (1e30 is finite there)
+        big = float(torch.tensor(1e30).to(out))
+        want = [w_ if i < 3 or w_ == 0 else math.copysign(big, w_) for i, w_ in enumerate(want)]
+    got = ops.linear(x, w, act=act, out_dtype=out).cpu()
+    want = torch.tensor(want).repeat(M // 5).view(M, 1).expand(M, 48).to(out)
+    assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0)), (got[:5, 0], want[:5, 0])
