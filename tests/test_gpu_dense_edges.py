@@ -93,3 +93,19 @@ def test_linear_activations_of_infinities(gpu, act, out, M):
     got = ops.linear(x, w, act=act, out_dtype=out).cpu()
     want = torch.tensor(want).repeat(M // 5).view(M, 1).expand(M, 48).to(out)
     assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0)), (got[:5, 0], want[:5, 0])
+
+
+@pytest.mark.parametrize("out", [F16, BF16])
+def test_linear_gelu_in_the_negative_tail(gpu, out):
+    """gelu of each number from -14 to 9 in 16-bit results: within 0.6 of a step (half a step for the rounding, and an evaluation
+    of a tenth of a step at most) of the value, subnormal steps included. In bf16, whose subnormal numbers are fp32's, values
+    below the smallest normal one may be 0: the exponential has none."""
+    announce(f"gelu tail {out}")
+    y = torch.linspace(-14.0, 9.0, 64 * 4096).view(-1, 64)
+    eye = torch.eye(64, device=gpu)
+    got = ops.linear(y.to(gpu), eye, act="gelu", out_dtype=out).cpu().double()
+    want = ref.act64(y.double(), "gelu")
+    step = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=1e-300)))) * torch.finfo(out).eps
+    least = torch.finfo(out).tiny * (torch.finfo(out).eps if out == F16 else 1 / 0.6)
+    far = (got - want).abs() / step.clamp(min=least)
+    assert float(far.max()) <= 0.6, (float(far.max()), float(y.flatten()[far.argmax()]))
