@@ -9,7 +9,7 @@
 // Measured (MI355X), and what bounds it: 4800 x 1024 bf16 to 4096 columns, gelu: 54 us, 745 TFLOP/s (the 16-bit tiles take
 // what the chip's power leaves of the matrix units' rate, and the epilogue after them; a library's product without an
 // epilogue takes 50); one row of 1024 fp16 to 1024: 4.2 us, a load's latency four times over; 76,800 rows of 64 fp32 to
-// 128: 21 us (59 MB; matrix units 8 us, loads and epilogue of blocks of two tiles of k lie one behind the other).
+// 128, silu: 22.3 us (59 MB; matrix units 8 us, loads and epilogue of blocks of two tiles of k lie one behind the other).
 #include "pmg_dense.h"
 
 namespace pmg {
@@ -47,6 +47,16 @@ __device__ inline float gelu_16(float y) {
     return __builtin_fmaf(-__builtin_fabsf(x), q, y < 0.0f ? 0.0f : y);
 }
 
+// 1 / (1 + exp(-z)) for fp32 outputs, within 2^-22 of its value: the exponential of -|z|, which cannot overflow, its argument in two
+// parts (in one, as silu_fast has it, |z| 2^-24 of the result is lost: 20 times the rest at -80), then 1 ulp each for exp2 and
+// reciprocal. Values below 2^-126 may be 0.
+__device__ inline float sigmoid_wide(float z) {
+    const float a = __builtin_fminf(__builtin_fabsf(z), 200.0f), hi = a * -PMG_LOG2E;  // (infinity times the second part would be NaN)
+    const float lo = __builtin_fmaf(a, -1.92596299e-8f, __builtin_fmaf(a, -PMG_LOG2E, -hi));
+    const float e2 = __builtin_amdgcn_exp2f(hi), e = __builtin_fmaf(e2, lo * 0.69314718f, e2), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return z < 0.0f ? e * r : r;
+}
+
 // act of 8 values in place; wide: for fp32 outputs.
 __device__ inline void activate8(float (&v)[8], int act, bool wide) {
     switch (act) {
@@ -55,8 +65,13 @@ __device__ inline void activate8(float (&v)[8], int act, bool wide) {
             for (int i = 0; i < 8; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
             break;
         case PMG_ACT_SILU:
+            if (wide) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = silu_fast(v[i]);
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * sigmoid_wide(v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = silu_fast(v[i]);
+            }
             break;
         case PMG_ACT_GELU:
             if (wide) {
@@ -67,14 +82,18 @@ __device__ inline void activate8(float (&v)[8], int act, bool wide) {
                 for (int i = 0; i < 8; ++i) v[i] = gelu_16(v[i]);
             }
             break;
-        case PMG_ACT_GELU_TANH:
+        case PMG_ACT_GELU_TANH: {  // (1 + tanh(c u)) / 2 = 1 / (1 + exp(-2 c u)), c = sqrt(2 / pi)
+            constexpr float c2 = 2.0f * 0.7978845608f;
+            const auto u = [](float y) { return __builtin_fmaf(0.044715f * y * y, y, y); };
+            if (wide) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = v[i], u = __builtin_fmaf(0.044715f * y * y, y, y);
-                // (1 + tanh(c u)) / 2 = 1 / (1 + exp(-2 c u)), c = sqrt(2 / pi)
-                v[i] = y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * (-2.0f * 0.7978845608f * PMG_LOG2E)));
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * sigmoid_wide(u(v[i]) * c2);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u(v[i]) * (-c2 * PMG_LOG2E)));
             }
             break;
+        }
         default: break;
     }
 }

@@ -109,3 +109,21 @@ def test_linear_gelu_in_the_negative_tail(gpu, out):
     least = torch.finfo(out).tiny * (torch.finfo(out).eps if out == F16 else 1 / 0.6)
     far = (got - want).abs() / step.clamp(min=least)
     assert float(far.max()) <= 0.6, (float(far.max()), float(y.flatten()[far.argmax()]))
+
+
+def test_linear_fp32_activations_far_out(gpu):
+    """silu and gelu_tanh in fp32 results, relative to their own value from -85 (-8.5) to 40: y / (1 + exp(-z)) with an
+    exponential and a reciprocal of 1 ulp (2 x 2^-24) and four more roundings, 2^-21 together; gelu_tanh's z is up to five roundings
+    off (constants counted half), |z| 5 x 2^-24 of the exponential."""
+    y = torch.linspace(-85.0, 40.0, 64 * 4096).view(-1, 64)
+    eye = torch.eye(64, device=gpu)
+    announce("linear fp32 silu, gelu_tanh far out")
+    got = ops.linear(y.to(gpu), eye, act="silu").cpu().double()
+    want = ref.act64(y.double(), "silu")
+    assert float(((got - want).abs() / want.abs()).max()) <= 2.0 ** -21
+    y = (y / 10).float()
+    got = ops.linear(y.to(gpu), eye, act="gelu_tanh").cpu().double()
+    yd = y.double()
+    z = 2 * math.sqrt(2 / math.pi) * (yd + 0.044715 * yd ** 3)
+    want = yd / (1 + torch.exp(-z))
+    assert float(((got - want).abs() / (want.abs() * (2.0 ** -21 + 5 * 2.0 ** -24 * z.abs()))).max()) <= 1.0
