@@ -628,6 +628,8 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  * seg_indices). For query row i and head h, over the keys j of i's segment with k_mask[j] != 0 (row-indexed, or NULL):
  *   x_j = scale q_i . k_j;  cap > 0: x_j = cap tanh(x_j / cap);  x_j -= sum over axes of slopes[h][axis] |c_i - c_j|[axis]
  *   out_i = sum_j softmax(x)_j v_j, 0 where no key is left. Key head of h: h / (Hq / Hk).
+ * scale up to 1e30; cap 0 or up to 1e30, scale / cap up to 1e37; a capped score is accurate relative to itself (16-bit types, caps
+ * up to 256: within 3e-7 cap).
  * Sums and statistics in fp32; the softmax's weights enter the second product rounded to `type`.
  * Offsets are held to [0, positions] (where they fall, query rows may be left as they were); a position whose index
  * lies outside the rows is absent. Query rows outside every

@@ -42,7 +42,7 @@ struct AttnArgs {
     const uint8_t* k_mask;
     int Hq, Hk, G, D;
     float scale2;         // scale log2(e)
-    float cap2, cap_arg;  // cap log2(e); the factor of tanh's argument (0 cap: none)
+    float cap2, cap_arg;  // cap log2(e) (0: none); what its argument is multiplied by: 1 / cap for tanh, 2 log2(e) / cap for the exponential
     int seg, splits, zero_rest;
     int whole;  // blocks of one segment each
     int near;   // K and V each below 4 GiB, heads of full width: rows are fetched by 32-bit byte offsets
@@ -50,6 +50,10 @@ struct AttnArgs {
     float* part_o;  // [splits][Hq][Pq][D]; (m, l) [splits][Hq][Pq], l < 0: a position of no segment
     float2* part_ml;
 };
+
+// 16-bit types: caps (times log2 e) up to which cap tanh(x / cap) is formed as cap - 2 cap / (1 + e^(2 x / cap)), whose error is
+// that of the cap itself: 3e-7 of it, so weights within 8e-5, a sixth of a half step of fp16. Above, as in fp32.
+constexpr float kFineCap = 256.0f * 1.44269504f;
 
 __device__ inline int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -187,8 +191,9 @@ constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
 //
 // Registers: with at most 256 the matrix instructions' results stay in ordinary vector registers, where the softmax
 // works on them; only the widest fp32 form of one wave needs more.
-// MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use).
-template <class T, int DP, int NW, bool BIAS, bool MASK>
+// MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use). FINE: caps by tanh_f32 (fp32, and
+// large caps of the 16-bit types; a kernel of its own, for a branch inside the loop spills 2 to 8 registers).
+template <class T, int DP, int NW, bool BIAS, bool MASK, bool FINE>
 __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void attention_k(AttnArgs a0) {
     const AttnArgs& a = a0;
     constexpr int ES = sizeof(T), PER = 16 / ES, CPR = DP / PER, NT = 64 * NW;
@@ -519,7 +524,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                         if (a.cap2 != 0.0f) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                if constexpr (ES == 4) s[e] = a.cap2 * tanh_f32(s[e] * a.cap_arg);
+                                if constexpr (FINE) s[e] = a.cap2 * tanh_f32(s[e] * a.cap_arg);
                                 else s[e] = __builtin_fmaf(-2.0f * a.cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[e] * a.cap_arg)), a.cap2);
                             }
                         }
@@ -816,9 +821,13 @@ static int launch_attention_w(AttnArgs& a, hipStream_t s) {
     PMG_REQUIRE(blocks < (int64_t)1 << 31, "too many blocks");
     a.blocks = (uint32_t)blocks;
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), 0, s, a); };
-    if (a.slopes) launch(attention_k<T, DP, NW, true, false>);
-    else if (a.k_mask) launch(attention_k<T, DP, NW, false, true>);
-    else launch(attention_k<T, DP, NW, false, false>);
+    constexpr bool F32 = sizeof(T) == 4;
+    if (!F32 && a.cap2 > kFineCap) {
+        if (a.slopes) launch(attention_k<T, DP, NW, true, false, true>);
+        else launch(attention_k<T, DP, NW, false, false, true>);
+    } else if (a.slopes) launch(attention_k<T, DP, NW, true, false, F32>);
+    else if (a.k_mask) launch(attention_k<T, DP, NW, false, true, F32>);
+    else launch(attention_k<T, DP, NW, false, false, F32>);
     return check_launch("attention_k");
 }
 

@@ -78,8 +78,9 @@ int attention_args(const pmg_attention_args& r) {
     PMG_REQUIRE(r.q_rows < big && r.k_rows < big && r.q_positions < big && r.k_positions < big && r.segments < big - 1, "2^31 rows, positions or segments");
     PMG_REQUIRE(r.q_index || r.q_positions <= r.q_rows, "more query positions than rows");
     PMG_REQUIRE(r.k_index || r.k_positions <= r.k_rows, "more key positions than rows");
-    PMG_REQUIRE(r.scale > 0.0f && r.scale < 3.0e38f, "scale must be positive");
-    PMG_REQUIRE(r.cap >= 0.0f && r.cap < 3.0e38f, "cap must not be negative");
+    PMG_REQUIRE(r.scale > 0.0f && r.scale <= 1.0e30f, "scale must be positive, up to 1e30");
+    PMG_REQUIRE(r.cap >= 0.0f && r.cap <= 1.0e30f, "cap must not be negative, nor above 1e30");
+    PMG_REQUIRE(r.cap == 0.0f || (double)r.scale / (double)r.cap <= 1.0e37, "cap is too small for the scale");
     return PMG_OK;
 }
 
@@ -144,7 +145,7 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     a.scale2 = (float)((double)r.scale * log2e);
     if (r.cap > 0.0f) {
         a.cap2 = (float)((double)r.cap * log2e);
-        a.cap_arg = (float)((double)r.scale / (double)r.cap * (r.type == PMG_TYPE_F32 ? 1.0 : 2.0 * log2e));
+        a.cap_arg = (float)((double)r.scale / (double)r.cap * (r.type == PMG_TYPE_F32 || a.cap2 > kFineCap ? 1.0 : 2.0 * log2e));
     }
     a.seg = pl.seg;
     a.whole = pl.whole;

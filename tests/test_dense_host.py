@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from promptmoge_amd import _lib, ops
-from test_dense_abi import linear_args
+from test_dense_abi import attention_args, linear_args
 
 F16, F32 = torch.float16, torch.float32
 
@@ -246,3 +246,11 @@ def test_int8_sums_that_could_pass_32_bits_are_refused(libpmg):
     assert b"K must" in libpmg.pmg_last_error()
     assert libpmg.pmg_linear(C.byref(linear_args(K=131_071, M=0, **i8)), None) == _lib.PMG_OK
     assert libpmg.pmg_linear(C.byref(linear_args(K=131_072, M=0, ldx=1 << 18)), None) == _lib.PMG_OK
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(scale=2e30), "scale"), (dict(cap=2e30), "cap"), (dict(cap=float("nan")), "cap"), (dict(cap=float("inf")), "cap"),
+                                    (dict(cap=1e-38), "too small"), (dict(cap=1e-8, scale=1e30), "too small")])
+def test_attention_scales_and_caps_out_of_range_are_refused(libpmg, kw, msg):
+    """Products of them with log2 e, and their quotient, have to be numbers of fp32."""
+    assert libpmg.pmg_attention(C.byref(attention_args(**kw)), None, 0, None) == _lib.PMG_E_INVALID
+    assert msg in libpmg.pmg_last_error().decode()

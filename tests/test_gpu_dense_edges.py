@@ -127,3 +127,32 @@ def test_linear_fp32_activations_far_out(gpu):
     z = 2 * math.sqrt(2 / math.pi) * (yd + 0.044715 * yd ** 3)
     want = yd / (1 + torch.exp(-z))
     assert float(((got - want).abs() / (want.abs() * (2.0 ** -21 + 5 * 2.0 ** -24 * z.abs()))).max()) <= 1.0
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cap", [0.5, 30.0, 200.0, 256.0, 300.0, 1e4, 1e6, 1e8, 1e30])
+@pytest.mark.parametrize("few", [False, True])
+def test_attention_caps_of_any_size(gpu, dt, cap, few):
+    """One query on two keys whose scores are 0 and x: the result tells the capped score, for x from far below the cap to beyond
+    it. The weight e^t / (1 + e^t) of t = cap tanh(x / cap) is off by a quarter of t's error at most: |x| 2^-20 for its few
+    roundings, and below a cap of 256, where the 16-bit types take a form whose error is the cap's, 2^-21 cap for these."""
+    g = gen(2)
+    n = 64
+    x = (torch.rand(n, generator=g) * 12 - 6).to(dt)
+    x[:6] = torch.tensor([0.0, 1e-3, -1e-3, 0.25, 6.0, -6.0]).to(dt)
+    q = torch.zeros(n, 1, 32, dtype=dt)
+    q[:, 0, 0] = x
+    k, v = torch.zeros(2 * n, 1, 32, dtype=dt), torch.zeros(2 * n, 1, 32, dtype=dt)
+    k[1::2, 0, 0], v[1::2] = 1, 1
+    off, koff = torch.arange(n + 1), torch.arange(n + 1) * 2
+    if few:  # (a block per segment: long segments, the same key again and again)
+        k, v = k.view(n, 2, 1, 32).repeat(1, 100, 1, 1).view(-1, 1, 32), v.view(n, 2, 1, 32).repeat(1, 100, 1, 1).view(-1, 1, 32)
+        koff = torch.arange(n + 1) * 200
+    announce(f"attention cap {cap} {dt} few={few}")
+    got = ops.sparse_attention(q.to(gpu), k.to(gpu), v.to(gpu), off.to(gpu), koff.to(gpu), cap=cap, scale=1.0).cpu().double()
+    xd = x.double()
+    want = torch.sigmoid(cap * torch.tanh(xd / cap)).view(n, 1, 1).expand(n, 1, 32)
+    terr = xd.abs() * 2.0 ** -20 + (2.0 ** -21 * cap if cap < 256 and dt != F32 else 0.0)
+    # each weight is rounded to the type, and the result; sums of 2 or 200 weights
+    tol = want * (1 - want) * 1.01 * terr.view(n, 1, 1) + want * (2 * ref.U[dt] + 2.0 ** -20 + (200 if few else 2) * 2.0 ** -22) + ref.TINY[dt]
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
