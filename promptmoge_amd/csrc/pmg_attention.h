@@ -19,6 +19,8 @@
 // several segments are not finite, the block goes over its segments one by one. (SEG: a block per segment, for few
 // queries on many keys.) The keys of a block can be split over gridDim blocks, whose (m, l, O) a second kernel joins.
 #pragma once
+#include <type_traits>
+
 #include "pmg_dense.h"
 
 namespace pmg {
@@ -559,9 +561,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                             }
                         }
                     };
-                    // ---- weights; the running maximum is set by the first keys, then moved only when a weight grows beyond 2^8
-                    // (up to 2^12 nothing is lost). That shows in the sum of a lane's 16 weights: only then the
-                    // scores are formed again and their maximum looked for.
+                    // ---- weights, in units that put the running maximum at 2^kTop. It is set by the first keys, then moved only when
+                    // a weight grows beyond 2^kMost (up to 2^(kMost + 4) nothing is lost). That shows in the sum of a lane's 16
+                    // weights: only then the scores are formed again and their maximum looked for. fp16, whose numbers end
+                    // at 2^-24, has the maximum at 2^7: a weight is off by at most 2^-32 of it, a million small ones by 2^-12 (at 1
+                    // they would lose 2^-25 each: 150,000 keys 0.4 % of the result).
+                    constexpr bool HALF = std::is_same<T, _Float16>::value;
+                    constexpr float kTop = HALF ? 7.0f : 0.0f, kMost = HALF ? 11.0f : 8.0f, kSum = HALF ? 32768.0f : 4096.0f;
                     float sum;
                     const auto weights = [&]() {
                         float part[4];
@@ -575,7 +581,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                     if (!LOOK && !look) {
                         scores();
                         weights();
-                        look = __any(sum > 4096.0f);
+                        look = __any(sum > kSum);
                     }
                     if (LOOK || look) {
                         scores();
@@ -585,10 +591,10 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                         mx = halves_max(mx);
                         if (__any(mx > grow)) {
                             const bool any = mx > -__builtin_inff();  // (a slot without a key so far keeps m = 0)
-                            const float up = any && (mx > 0.0f || grow < 0.0f) ? mx : 0.0f;
+                            const float up = any && (mx > kTop || grow < 0.0f) ? mx - kTop : 0.0f;
                             // (nothing to scale before the first key, whose score may be far below -2^7)
                             const float al = grow < 0.0f ? 1.0f : __builtin_amdgcn_exp2f(-up);
-                            grow = any ? 8.0f : grow;
+                            grow = any ? kMost : grow;
                             m = m + up;
                             l = l * al;
 #pragma unroll

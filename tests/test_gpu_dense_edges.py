@@ -156,3 +156,37 @@ def test_attention_caps_of_any_size(gpu, dt, cap, few):
     # each weight is rounded to the type, and the result; sums of 2 or 200 weights
     tol = want * (1 - want) * 1.01 * terr.view(n, 1, 1) + want * (2 * ref.U[dt] + 2.0 ** -20 + (200 if few else 2) * 2.0 ** -22) + ref.TINY[dt]
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("D,bias,mask", [(32, False, False), (64, False, True), (64, True, False), (128, False, False)])
+@pytest.mark.parametrize("queries", [1, 70, 8192])
+def test_attention_many_small_weights(gpu, dt, D, bias, mask, queries):
+    """One key of weight 1 and 150,000 of 2^-25.3, values all 1: the result is 1 within the type's half step and the roundings of
+    the two sums in fp32, which hold 1: a matrix step of 16 keys (fp32: 2) and a lane's sum of 32 round by 2^-24 each. (fp16
+    holds numbers down to 2^-25: small weights kept as such would all be lost, 0.36 % of the sum, three times that, where the
+    keys are not split over blocks: the 16 heads of the most queries.)"""
+    n = 150_000
+    announce(f"attention small weights {dt} D={D} bias={bias} mask={mask} queries={queries}")
+    k, v = torch.zeros(n, 1, D, dtype=dt), torch.ones(n, 1, D, dtype=dt)
+    low = -25.3 / 1.4426950408889634
+    queries = 20_000 if D == 128 and queries > 100 else queries
+    heads = 16 if queries > 100 else 1
+    q = torch.ones(queries, heads, D, dtype=dt)
+    kw = dict(scale=1.0 / D)
+    if bias:
+        kc = torch.zeros(n, 4, dtype=torch.int32)
+        kc[:, 1] = 5
+        kc[77, 1] = 0
+        kw |= dict(coords=torch.zeros(queries, 4, dtype=torch.int32).to(gpu), kv_coords=kc.to(gpu), slopes=torch.tensor([[-low / 5, 0.0, 0.0]] * heads, device=gpu))
+    else:
+        k[:] = low
+        k[77] = 0
+    if mask:
+        m = torch.ones(n, dtype=torch.bool)
+        m[1000:2000] = False
+        kw["kv_mask"] = m.to(gpu)
+    off, koff = torch.tensor([0, queries]), torch.tensor([0, n])
+    got = ops.sparse_attention(q.to(gpu), k.to(gpu), v.to(gpu), off.to(gpu), koff.to(gpu), **kw).double()
+    # (and half a step of the small weights' own share, 2^-8)
+    assert float((got - 1).abs().max()) <= ref.U[dt] * (1 + 2.0 ** -8) + (n / (2 if dt == F32 else 16) + n / 32) * 2.0 ** -24
