@@ -631,10 +631,10 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  * scale up to 1e30; cap 0 or up to 1e30, scale / cap up to 1e37; a capped score is accurate relative to itself (16-bit types, caps
  * up to 256: within 3e-7 cap).
  * Sums and statistics in fp32; the softmax's weights enter the second product rounded to `type`.
- * Offsets are held to [0, positions] (where they fall, query rows may be left as they were); a position whose index
- * lies outside the rows is absent. Query rows outside every
- * segment are left as they were, or zeroed with zero_rest (those that a position names). A row named by two query
- * positions gets either's result. Differences of coordinates are exact up to 2^23.
+ * Offsets are held to [0, positions] (where they fall, what the rows get is not said); a position whose index lies outside the
+ * rows is absent. Query rows that no position of a segment names are left as they were, or with zero_rest set to 0, whatever the
+ * tables hold. A row named by two query positions gets either's result (0 of a position of no segment). Differences of
+ * coordinates are exact up to 2^23.
  * D a multiple of 8 up to 128; q, k, v: buffers and strides (elements) in whole 16 bytes, out in groups of 4 elements;
  * out must not overlap the inputs. Workspace (any contents; may be NULL if 0 bytes): must not be shared by calls that
  * overlap. */

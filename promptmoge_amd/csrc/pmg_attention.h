@@ -71,6 +71,9 @@ __device__ inline int32_t segment_of(const int64_t* off, int64_t S, int64_t p) {
     return p < off[lo] ? (int32_t)(lo - 1) : -1;
 }
 
+// Whether segment s (or -1), found by a search, holds position p, which it may not where offsets fall.
+__device__ inline bool in_segment(const int64_t* off, int32_t s, int64_t p) { return s >= 0 && off[s] <= p && p < off[s + 1]; }
+
 // The segment (as above) of position p of each lane, all lanes of a wave taking part; first: a lower bound of the p. A
 // search with 64 probes a round for `first`, then among the 64 offsets that follow.
 __device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t first, int32_t p) {
@@ -92,6 +95,13 @@ __device__ inline int32_t wave_segment(const int64_t* off, int64_t S, int32_t fi
     if (c == 64) return segment_of(off, S, p);
     const int64_t s = lo + c - 1;
     return s < S ? (int32_t)s : -1;
+}
+
+// Whether up to kLook offsets rise, as blocks of one segment each need it.
+constexpr int kLook = 64;
+__device__ inline bool offsets_rise(const int64_t* off, int64_t S) {
+    const int j = threadIdx.x & 63;
+    return __all(j >= S || off[j] <= off[j + 1]);
 }
 
 // Blocks that hold one segment each: interval j of S + 2 (the rows before the segments, the segments, the rows behind) from
@@ -237,6 +247,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     // slots of the block: [slot0, slot1) of all positions' G slots (SEG: of the segment's)
     int64_t slot0, slot1;
     int32_t own = -1;  // the block's segment, with blocks of one segment each
+    bool whole = false;
     int32_t seg_lo = 0, seg_hi = 0;  // (positions and rows fit 32 bits)
     if constexpr (SEG) {
         const int64_t p0 = clamp64(a.q_off[unit], 0, a.Pq), p1 = clamp64(a.q_off[unit + 1], 0, a.Pq);
@@ -244,9 +255,10 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
         slot1 = p1 * a.G;
         seg_lo = (int32_t)clamp64(a.k_off[unit], 0, a.Pk);
         seg_hi = (int32_t)clamp64(a.k_off[unit + 1], seg_lo, a.Pk);
-    } else if (a.whole) {
+    } else if (a.whole && (whole = a.S > kLook || offsets_rise(a.q_off, a.S))) {
         own = unit_segment(a.q_off, a.S, a.Pq, a.G, 32 * NW, unit, slot0, slot1);
-    } else {
+    } else {  // (where offsets fall, blocks of one segment each would miss rows; there are enough of them for these tiles. Of more
+              // segments than a wave looks through at once, rows and parts that are missed hold what attention_fill_k left)
         slot0 = (int64_t)unit * (32 * NW);
         slot1 = slot0 + 32 * NW;
         if (slot1 > a.Pq * a.G) slot1 = a.Pq * a.G;
@@ -265,7 +277,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
         int32_t row = in ? pos : -1, seg = -1, lo = 0, hi = 0;
         if (in && a.q_index) row = a.q_index[pos];  // (looked at below: nothing waits for it here)
         int32_t wlo, whi;  // the wave's keys
-        if (SEG || a.whole) {
+        if (SEG || whole) {
             if constexpr (!SEG) {
                 seg_lo = own >= 0 ? (int32_t)clamp64(a.k_off[own], 0, a.Pk) : 0;
                 seg_hi = own >= 0 ? (int32_t)clamp64(a.k_off[own + 1], seg_lo, a.Pk) : 0;
@@ -788,7 +800,8 @@ __global__ __launch_bounds__(256) void attention_join_k(AttnArgs a) {
         }
     }
     // (blocks by segment write nothing for positions of no segment)
-    const bool in = a.seg ? wave_segment(a.q_off, a.S, (int32_t)first, there ? (int32_t)pos : (int32_t)first) >= 0 : y0 >= 0.0f || y0 != y0;
+    bool in = y0 >= 0.0f || y0 != y0;
+    if (a.seg) in = in_segment(a.q_off, wave_segment(a.q_off, a.S, (int32_t)first, there ? (int32_t)pos : (int32_t)first), pos);
     if (r < 0 || r >= a.Mq || (!in && !a.zero_rest) || (WIDE && g != 0) || d >= a.D) return;
     typedef T v4t __attribute__((ext_vector_type(4)));
     const float inv = 1.0f / l;
@@ -808,16 +821,30 @@ static int launch_join(const AttnArgs& a, hipStream_t s) {
     return check_launch("attention_join_k");
 }
 
-// The rows outside every segment, where blocks go by segment.
+// In front of the others: zeros in a result that the tables may not name whole, and no segment in the parts' (m, l) where blocks of
+// one segment each may miss some. (39 MB: 8 us.)
 template <class T>
-__global__ __launch_bounds__(256) void attention_rest_k(AttnArgs a) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= a.Pq) return;
-    if (segment_of(a.q_off, a.S, item) >= 0) return;
-    const int64_t r = a.q_index ? a.q_index[item] : item;
-    if (r < 0 || r >= a.Mq) return;
-    for (int h = 0; h < a.Hq; ++h)
-        for (int d = threadIdx.x & 63; d < a.D; d += 64) ((T*)a.out)[r * a.o_row + h * a.o_head + d] = (T)0.0f;
+__global__ __launch_bounds__(256) void attention_fill_k(AttnArgs a, int64_t rows, int64_t chunks, int64_t parts) {
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = first; i < chunks; i += step) ((uint4*)a.out)[i] = make_uint4(0u, 0u, 0u, 0u);  // (a contiguous result)
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    const int per = a.Hq * (a.D / 4);
+    for (int64_t r = first >> 6; r < rows; r += step >> 6)
+        for (int d = threadIdx.x & 63; d < per; d += 64) *(v4t*)((T*)a.out + r * a.o_row + d / (a.D / 4) * a.o_head + d % (a.D / 4) * 4) = v4t{};
+    for (int64_t i = first; i < parts; i += step) a.part_ml[i] = make_float2(-__builtin_inff(), -1.0f);
+}
+
+template <class T>
+static int launch_fill(const AttnArgs& a, hipStream_t s) {
+    const int64_t chunks = a.Mq * a.Hq * a.D * (int64_t)sizeof(T) / 16;  // (D is a multiple of 8)
+    const bool split = a.splits > 1, missed = a.whole && a.S > kLook;  // (Pq 0: neither)
+    const bool fill = a.zero_rest && (a.q_index || a.Pq < a.Mq || missed || (a.seg && !split));
+    const bool straight = a.o_head == a.D && a.o_row == (int64_t)a.Hq * a.D && aligned16(a.out);
+    const int64_t n = fill && straight ? chunks : 0, rows = fill && !straight ? a.Mq : 0, parts = split && missed ? a.splits * a.Pq * a.Hq : 0;
+    const int64_t most = n > rows * 64 ? n : rows * 64, blocks = ((most > parts ? most : parts) + 1023) / 1024;
+    if (blocks == 0) return PMG_OK;
+    hipLaunchKernelGGL((attention_fill_k<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, rows, n, parts);
+    return check_launch("attention_fill_k");
 }
 
 template <class T, int DP, int NW>
@@ -844,13 +871,10 @@ static int launch_attention_d(AttnArgs& a, hipStream_t s) {
 
 template <class T>
 int launch_attention_t(AttnArgs& a, hipStream_t s) {
-    int e = a.D <= 32 ? launch_attention_d<T, 32>(a, s) : a.D <= 64 ? launch_attention_d<T, 64>(a, s) : launch_attention_d<T, 128>(a, s);
-    if (e) return e;
+    if (int e = launch_fill<T>(a, s)) return e;
+    if (a.Pq == 0) return PMG_OK;
+    if (int e = a.D <= 32 ? launch_attention_d<T, 32>(a, s) : a.D <= 64 ? launch_attention_d<T, 64>(a, s) : launch_attention_d<T, 128>(a, s)) return e;
     if (a.splits > 1) return a.D <= 64 ? launch_join<T, 16>(a, s) : launch_join<T, 32>(a, s);
-    if (a.seg && a.zero_rest) {
-        hipLaunchKernelGGL((attention_rest_k<T>), dim3((unsigned)((a.Pq + 3) / 4)), dim3(256), 0, s, a);
-        return check_launch("attention_rest_k");
-    }
     return PMG_OK;
 }
 

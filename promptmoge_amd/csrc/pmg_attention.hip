@@ -95,8 +95,8 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     PMG_REQUIRE(p, "null args");
     const pmg_attention_args& r = *p;
     if (int e = attention_args(r)) return e;
-    if (r.q_rows == 0 || r.q_positions == 0) return PMG_OK;
-    PMG_REQUIRE(r.q && r.out && r.q_offsets && r.k_offsets, "null buffer");
+    if (r.q_rows == 0 || (r.q_positions == 0 && !r.zero_rest)) return PMG_OK;
+    PMG_REQUIRE(r.out && (r.q_positions == 0 || (r.q && r.q_offsets && r.k_offsets)), "null buffer");
     PMG_REQUIRE(r.k_rows == 0 || r.k_positions == 0 || (r.k && r.v), "null buffer");
     PMG_REQUIRE(!r.slopes || (r.q_coords && (r.k_coords || r.k_rows == 0)), "slopes need coordinates");
     const int es = r.type == PMG_TYPE_F32 ? 4 : 2;
@@ -153,7 +153,7 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     a.zero_rest = r.zero_rest;
     const int64_t end = (a.Mk - 1) * (r.k_row > r.v_row ? r.k_row : r.v_row) * es + (int64_t)r.D * es;
     a.near = (r.D == 32 || r.D == 64 || r.D == 128) && end <= 0xffff0000;
-    if (pl.splits > 1) {
+    if (need) {
         a.part_o = (float*)workspace;
         a.part_ml = (float2*)((char*)workspace + (size_t)pl.splits * (size_t)r.q_positions * (size_t)r.Hq * (size_t)r.D * 4);
     }

@@ -905,9 +905,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     slopes (Hq, 3) fp32: minus sum over the axes of slopes[h, axis] |difference of coords (M, 4) int32 (b, x, y, z)|;
     kv_mask (Mk,) bool / uint8: rows with 0 are not attended to. A query with no key left gets 0.
 
-    Rows outside every segment are 0 in a new result and left as they were in a given `out`. Every row should be named
-    by at most one query position; an index as long as q has to name every row (in a new result, rows that it misses are
-    not written). offsets that fall leave rows unwritten, too. Forward only."""
+    Rows that no position of a segment names are 0 in a new result and left as they were in a given `out`. A row named by
+    two query positions gets either's result. Where offsets fall, what the rows get is not said. Forward only."""
     d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
     if d < 0:
         d = _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
@@ -950,8 +949,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
             raise ValueError(f"kv_mask must be a contiguous ({Mk},) bool or uint8 tensor")
     fresh = out is None
     if fresh:
-        whole = index is None or index.numel() == Mq
-        out = q.new_empty((Mq, Hq, D)) if whole else q.new_zeros((Mq, Hq, D))
+        out = q.new_empty((Mq, Hq, D))
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}")

@@ -190,3 +190,149 @@ def test_attention_many_small_weights(gpu, dt, D, bias, mask, queries):
     got = ops.sparse_attention(q.to(gpu), k.to(gpu), v.to(gpu), off.to(gpu), koff.to(gpu), **kw).double()
     # (and half a step of the small weights' own share, 2^-8)
     assert float((got - 1).abs().max()) <= ref.U[dt] * (1 + 2.0 ** -8) + (n / (2 if dt == F32 else 16) + n / 32) * 2.0 ** -24
+
+
+def used_before(gpu, nbytes):
+    """Leaves freed memory that is full of NaN where the next new tensors come from."""
+    x = torch.full((nbytes // 4,), math.nan, device=gpu)
+    y = [torch.full((n,), math.nan, device=gpu) for n in (1 << 8, 1 << 12, 1 << 16, 1 << 18)]
+    torch.cuda.synchronize()
+    del x, y
+
+
+TABLES = {
+    "an index out of range": lambda M, g: (torch.tensor([0, M // 3, M]), torch.where(torch.rand(M, generator=g) < 0.2, torch.randint(-9, 2 * M, (M,), generator=g), torch.randperm(M, generator=g)).int()),
+    "one row named by all": lambda M, g: (torch.tensor([0, M]), torch.full((M,), 5, dtype=torch.int32)),
+    "rows named twice": lambda M, g: (torch.tensor([0, M // 2, M]), torch.randint(0, M, (M,), generator=g).int()),
+    "more positions than rows": lambda M, g: (torch.tensor([0, M // 2, 3 * M]), torch.randint(0, M // 2, (3 * M,), generator=g).int()),
+    "fewer positions than rows": lambda M, g: (torch.tensor([0, 3, M // 4]), torch.randperm(M, generator=g)[:M // 4].int()),
+    "no position": lambda M, g: (torch.tensor([0, 0]), torch.zeros(0, dtype=torch.int32)),
+    "segments of a part": lambda M, g: (torch.tensor([M // 5, M // 2, M - 7]), torch.randperm(M, generator=g).int()),
+}
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M", [12, 60, 900])
+@pytest.mark.parametrize("name", list(TABLES))
+@pytest.mark.parametrize("few", [False, True])
+def test_attention_new_results_are_written_whole(gpu, dt, M, name, few):
+    """Rows that no position of a segment names are 0, in memory that held NaN; a row that several name has the result of one."""
+    g = gen(M)
+    H, D = 2, 32
+    off, idx = TABLES[name](M, g)
+    q = randn(g, M, H, D).to(dt).to(gpu)
+    if few:  # (few queries on many keys: a block per segment)
+        S, Mk = len(off) - 1, 300 * len(idx) + 600
+        kv = randn(g, Mk, 2, H, D).to(dt).to(gpu)
+        koff, args = torch.arange(S + 1) * (Mk // S), {}
+    else:
+        kv = randn(g, M, 2, H, D).to(dt).to(gpu)
+        koff, args = off, {"kv_index": idx.to(gpu)}
+    announce(f"attention whole results {dt} {M} {name} few={few}")
+    used_before(gpu, 1 << 22)
+    got = ops.sparse_attention(q, kv[:, 0], kv[:, 1], off.to(gpu), koff.to(gpu), index=idx.to(gpu), **args).cpu()
+    assert not bool(torch.isnan(got).any())
+    seg = torch.full((M,), -1)
+    named = {}
+    for s in range(len(off) - 1):
+        for p in range(int(off[s]), min(int(off[s + 1]), len(idx))):
+            if 0 <= int(idx[p]) < M:
+                named.setdefault(int(idx[p]), set()).add(s)
+    outside = {int(r) for p, r in enumerate(idx.tolist()) if not (int(off[0]) <= p < int(off[-1]))}
+    rest = torch.tensor([r not in named for r in range(M)])
+    assert not bool(got[rest].any())
+    for s in range(len(off) - 1):  # each segment's rows, as if its queries alone were there
+        rows = torch.tensor([r for r in range(M) if named.get(r) == {s} and r not in outside], dtype=torch.int64)
+        if not len(rows):
+            continue
+        one = torch.tensor([0, len(rows)])
+        ks = koff[s:s + 2].clamp(max=len(idx)) if not few else koff[s:s + 2]
+        want, tol, _ = ref.attention(q[rows.to(gpu)], kv[:, 0], kv[:, 1], one, ks, **({} if few else {"kv_index": idx}))
+        ref.assert_within(got[rows], want, tol)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("off", [[700, 100, 650, 2 ** 62], [900, -1, 2 ** 40, 0], [-(2 ** 62), 2 ** 62, 5, 880], [0, 900, 300, 900, 100]])
+@pytest.mark.parametrize("kind", ["long", "split", "few", "short"])
+def test_attention_falling_offsets_leave_no_row_unwritten(gpu, dt, off, kind):
+    """What falling offsets give is not said, but it comes from no memory that nobody wrote."""
+    g = gen(7)
+    H, D = 2, 32
+    M = {"long": 900, "split": 900, "few": 900, "short": 900}[kind]
+    off = torch.tensor(off)
+    if kind == "short":  # (many short segments: tiles through all of them)
+        off = torch.cat([off, torch.randint(-50, 1000, (40,), generator=g)])
+    q = randn(g, M, H, D).to(dt).to(gpu)
+    if kind == "few":
+        off = torch.cat([off, torch.randint(-50, 1000, (160,), generator=g)])
+        Mk = 200_000
+        kv = randn(g, 1000, 2, H, D).to(dt).to(gpu).repeat(200, 1, 1, 1)
+        koff = torch.arange(len(off)) * (Mk // len(off))
+    elif kind == "split":
+        kv = randn(g, 1000, 2, H, D).to(dt).to(gpu).repeat(40, 1, 1, 1)
+        koff = torch.arange(len(off)) * 10_000
+    else:
+        kv, koff = randn(g, M, 2, H, D).to(dt).to(gpu), off
+    for idx in (None, torch.randperm(M, generator=g).int().to(gpu)):
+        announce(f"attention falling offsets {kind} {off.tolist()[:5]} {dt} index={idx is not None}")
+        used_before(gpu, 1 << 24)
+        got = ops.sparse_attention(q, kv[:, 0], kv[:, 1], off.to(gpu), koff.to(gpu), index=idx)
+        assert not bool(torch.isnan(got).any())
+        if kind != "few":  # (there two blocks may work on one row)
+            assert float(got.abs().max()) <= 1.02 * float(kv[:, 1].abs().max())  # (an average of values, or 0)
+        out = torch.full((M + 64, H, D), 7.0, dtype=dt, device=gpu)
+        used_before(gpu, 1 << 24)
+        ops.sparse_attention(q, kv[:, 0], kv[:, 1], off.to(gpu), koff.to(gpu), index=idx, out=out[32:-32])
+        assert not bool(torch.isnan(out).any())
+        assert bool((out[:32] == 7).all()) and bool((out[-32:] == 7).all())
+
+
+@pytest.mark.parametrize("fall", [False, True])
+def test_attention_many_long_segments_with_a_fall(gpu, fall):
+    """More segments than a block looks through itself: a kernel looks for a fall in front of it."""
+    g = gen(17)
+    S, L, H, D = 700, 170, 1, 32
+    M = S * L
+    off = torch.arange(S + 1) * L
+    if fall:
+        off[333], off[334] = off[334].item(), off[333].item()
+    q, kv = randn(g, M, H, D).to(F16).to(gpu), randn(g, M, 2, H, D).to(F16).to(gpu)
+    announce(f"attention many long segments, fall={fall}")
+    used_before(gpu, 1 << 25)
+    got = ops.sparse_attention(q, kv[:, 0], kv[:, 1], off.to(gpu))
+    assert not bool(torch.isnan(got).any())
+    if not fall:
+        want, tol, _ = ref.attention(q, kv[:, 0], kv[:, 1], off)
+        ref.assert_within(got, want, tol)
+
+
+def test_attention_whole_results_captured_and_replayed(gpu):
+    """Marks of named rows live in the call's workspace: a graph's replays with another index each give that index's result."""
+    g = gen(21)
+    M, H, D = 500, 2, 32
+    q, kv = randn(g, M, H, D).to(F16).to(gpu), randn(g, M, 2, H, D).to(F16).to(gpu)
+    off = torch.tensor([0, 200, M], device=gpu)
+    idx = torch.arange(M, dtype=torch.int32, device=gpu)
+    announce("attention whole results in a graph")
+    call = lambda: ops.sparse_attention(q, kv[:, 0], kv[:, 1], off, index=idx)  # noqa: E731
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    for k in range(5):
+        new = torch.randperm(M, generator=g).int()
+        new[k::7] = torch.tensor([-1, M, 0, 2 ** 31 - 1, 3], dtype=torch.int32)[k]
+        if k == 2 or k == 4:  # (a row named twice has either's result: named by none instead)
+            new[new == (0 if k == 2 else 3)] = -1
+        idx.copy_(new)
+        y.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol, covered = ref.attention(q, kv[:, 0], kv[:, 1], off, index=new)
+        assert not bool(y.cpu()[~covered].any())
+        ref.assert_within(y, want, tol)
+        torch.cuda.synchronize()
+        assert torch.equal(y, call())
