@@ -635,6 +635,8 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  * rows is absent. Query rows that no position of a segment names are left as they were, or with zero_rest set to 0, whatever the
  * tables hold. A row named by two query positions gets either's result (0 of a position of no segment). Differences of
  * coordinates are exact up to 2^23.
+ * Rows, positions and segments below 2^31 - 64; query positions times Hq (and segments times 128 Hk) below 2^31, else the call
+ * may be refused: a grid holds 2^32 threads.
  * D a multiple of 8 up to 128; q, k, v: buffers and strides (elements) in whole 16 bytes, out in groups of 4 elements;
  * out must not overlap the inputs. Workspace (any contents; may be NULL if 0 bytes): must not be shared by calls that
  * overlap. */

@@ -851,7 +851,7 @@ template <class T, int DP, int NW>
 static int launch_attention_w(AttnArgs& a, hipStream_t s) {
     const int64_t units = NW == 1 ? a.S : a.whole ? a.Pq * a.G / (32 * NW) + a.S + 2 : (a.Pq * a.G + 32 * NW - 1) / (32 * NW);
     const int64_t blocks = units * a.Hk * a.splits;
-    PMG_REQUIRE(blocks < (int64_t)1 << 31, "too many blocks");
+    PMG_REQUIRE(blocks <= grid_blocks(64 * NW), "too many slots or segments for one launch");
     a.blocks = (uint32_t)blocks;
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), 0, s, a); };
     constexpr bool F32 = sizeof(T) == 4;

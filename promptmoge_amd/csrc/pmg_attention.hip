@@ -74,8 +74,8 @@ int attention_args(const pmg_attention_args& r) {
     PMG_REQUIRE(r.Hq >= 1 && r.Hk >= 1 && r.Hq <= 4096 && r.Hq % r.Hk == 0, "query heads must be a multiple of key heads (up to 4096)");
     PMG_REQUIRE(r.D >= 8 && r.D <= 128 && r.D % 8 == 0, "head width must be a multiple of 8 up to 128");
     PMG_REQUIRE(r.q_rows >= 0 && r.k_rows >= 0 && r.q_positions >= 0 && r.k_positions >= 0 && r.segments >= 0, "negative size");
-    const int64_t big = (int64_t)1 << 31;
-    PMG_REQUIRE(r.q_rows < big && r.k_rows < big && r.q_positions < big && r.k_positions < big && r.segments < big - 1, "2^31 rows, positions or segments");
+    const int64_t big = ((int64_t)1 << 31) - 64;  // (a tile behind the last key still counts in 32 bits)
+    PMG_REQUIRE(r.q_rows < big && r.k_rows < big && r.q_positions < big && r.k_positions < big && r.segments < big, "2^31 - 64 rows, positions or segments");
     PMG_REQUIRE(r.q_index || r.q_positions <= r.q_rows, "more query positions than rows");
     PMG_REQUIRE(r.k_index || r.k_positions <= r.k_rows, "more key positions than rows");
     PMG_REQUIRE(r.scale > 0.0f && r.scale <= 1.0e30f, "scale must be positive, up to 1e30");

@@ -62,6 +62,9 @@ struct Mat<float> {
     }
 };
 
+// A grid's threads are counted in 32 bits (a larger launch is cut off without an error): blocks of `threads` it may have.
+constexpr int64_t grid_blocks(int threads) { return 0xffffffffll / threads; }
+
 // The XCD a block runs on is its index modulo 8: blocks of one XCD take consecutive tiles, which share operands in
 // that XCD's L2. Tile of block `id` of n (a permutation of 0 .. n - 1).
 __device__ inline uint32_t xcd_tile(uint32_t id, uint32_t n) {

@@ -468,20 +468,25 @@ static int launch_tile(LinearArgs& a, hipStream_t s) {
     const int nk = (a.K * (int)sizeof(T) + KB - 1) / KB;
     int bytes = kStage * (!VEC ? 1 : nk < NS ? nk : NS);
     if (bytes < kOut) bytes = kOut;
-    const int64_t tm = (a.M + BM - 1) / BM;
     a.tiles_n = (uint32_t)((a.N + BN - 1) / BN);
-    PMG_REQUIRE(tm * a.tiles_n < (int64_t)1 << 31, "too many outputs");
-    a.tiles = (uint32_t)(tm * a.tiles_n);
-    hipLaunchKernelGGL((linear_tile_k<T, BM, BN, WM, WN, KB, NS, VEC>), dim3(a.tiles), dim3(64 * WM * WN), bytes, s, a);
-    return check_launch("linear_tile_k");
+    const int64_t most = grid_blocks(64 * NW) / a.tiles_n * BM;  // rows a launch
+    for (int64_t m0 = 0; m0 < a.M; m0 += most) {
+        LinearArgs b = a;
+        b.M = a.M - m0 < most ? a.M - m0 : most;
+        b.x = (const T*)a.x + m0 * a.ldx;
+        if (a.res) b.res = (const char*)a.res + m0 * a.ldr * (a.res_type == PMG_TYPE_F32 ? 4 : 2);
+        b.out = (char*)a.out + m0 * a.ldo * (a.out_type == PMG_TYPE_F32 ? 4 : 2);
+        b.tiles = (uint32_t)((b.M + BM - 1) / BM) * a.tiles_n;
+        hipLaunchKernelGGL((linear_tile_k<T, BM, BN, WM, WN, KB, NS, VEC>), dim3(b.tiles), dim3(64 * NW), bytes, s, b);
+        if (int e = check_launch("linear_tile_k")) return e;
+    }
+    return PMG_OK;
 }
 
 template <class T, int MT, int NW, bool VEC>
 static int launch_rows(LinearArgs& a, hipStream_t s) {
-    const int64_t tm = (a.M + 16 * MT - 1) / (16 * MT);
     a.tiles_n = (uint32_t)((a.N + 15) / 16);
-    PMG_REQUIRE(tm * a.tiles_n < (int64_t)1 << 31, "too many outputs");
-    a.tiles = (uint32_t)(tm * a.tiles_n);
+    a.tiles = (uint32_t)((a.M + 16 * MT - 1) / (16 * MT)) * a.tiles_n;  // (512 at most)
     hipLaunchKernelGGL((linear_rows_k<T, MT, NW, VEC>), dim3(a.tiles), dim3(64 * NW), 0, s, a);
     return check_launch("linear_rows_k");
 }

@@ -184,19 +184,31 @@ static int launch_rope(RopeArgs& a, hipStream_t s) {
     int rows = a.P > 0 ? 256 / a.P : 32;
     rows = rows < 1 ? 1 : rows > 32 ? 32 : rows;
     a.rows = rows;
-    const int64_t blocks = (a.M + rows - 1) / rows;
     const size_t lds = sizeof(float2) * (size_t)rows * (size_t)(a.P > 0 ? a.P : 1);
     a.q_magic = (uint32_t)((((uint64_t)1 << 32) + a.Hq - 1) / (uint64_t)a.Hq);
     a.k_magic = a.Hk ? (uint32_t)((((uint64_t)1 << 32) + a.Hk - 1) / (uint64_t)a.Hk) : 0;
-    const dim3 grid((unsigned)blocks);
-    switch (G) {
-        case 1: launch_rope_g<T, 1>(a, grid, lds, s); break;
-        case 2: launch_rope_g<T, 2>(a, grid, lds, s); break;
-        case 4: launch_rope_g<T, 4>(a, grid, lds, s); break;
-        case 8: launch_rope_g<T, 8>(a, grid, lds, s); break;
-        default: launch_rope_g<T, 16>(a, grid, lds, s); break;
+    const int64_t most = grid_blocks(256) * rows;  // rows a launch
+    for (int64_t m0 = 0; m0 < a.M; m0 += most) {
+        RopeArgs b = a;
+        b.M = a.M - m0 < most ? a.M - m0 : most;
+        b.q = (const T*)a.q + m0 * a.q_row;
+        b.q_out = (T*)a.q_out + m0 * a.qo_row;
+        if (a.Hk) {
+            b.k = (const T*)a.k + m0 * a.k_row;
+            b.k_out = (T*)a.k_out + m0 * a.ko_row;
+        }
+        if (a.P > 0) b.coords = a.coords + m0 * 4;
+        const dim3 grid((unsigned)((b.M + rows - 1) / rows));
+        switch (G) {
+            case 1: launch_rope_g<T, 1>(b, grid, lds, s); break;
+            case 2: launch_rope_g<T, 2>(b, grid, lds, s); break;
+            case 4: launch_rope_g<T, 4>(b, grid, lds, s); break;
+            case 8: launch_rope_g<T, 8>(b, grid, lds, s); break;
+            default: launch_rope_g<T, 16>(b, grid, lds, s); break;
+        }
+        if (int e = check_launch("qk_norm_rope_k")) return e;
     }
-    return check_launch("qk_norm_rope_k");
+    return PMG_OK;
 }
 
 }  // namespace pmg

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from promptmoge_amd import _lib, ops
-from test_dense_abi import attention_args, linear_args
+from test_dense_abi import D16, attention_args, linear_args
 
 F16, F32 = torch.float16, torch.float32
 
@@ -254,3 +254,22 @@ def test_attention_scales_and_caps_out_of_range_are_refused(libpmg, kw, msg):
     """Products of them with log2 e, and their quotient, have to be numbers of fp32."""
     assert libpmg.pmg_attention(C.byref(attention_args(**kw)), None, 0, None) == _lib.PMG_E_INVALID
     assert msg in libpmg.pmg_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [dict(q_rows=1 << 30, q_positions=1 << 30, segments=1), dict(q_rows=1 << 27, q_positions=1 << 27, segments=1 << 26, k_rows=(1 << 31) - 65, k_positions=(1 << 31) - 65)])
+def test_attention_of_more_blocks_than_a_grid_holds_is_refused(libpmg, kw):
+    """(before a launch fails) A grid holds fewer than 2^32 threads."""
+    a = attention_args(Hq=32, Hk=32, D=8, k_row=256, v_row=256, **{k: v for k, v in kw.items() if not k.startswith("k_")})
+    a.k_rows, a.k_positions = kw.get("k_rows", 1 << 30), kw.get("k_positions", 1 << 30)
+    need = libpmg.pmg_attention_workspace_bytes(C.byref(a))
+    assert libpmg.pmg_attention(C.byref(a), D16, need, None) == _lib.PMG_E_INVALID
+    assert b"too many" in libpmg.pmg_last_error()
+
+
+def test_attention_positions_close_to_32_bits_are_refused(libpmg):
+    """A tile of 64 keys behind the last whole one would count past 2^31."""
+    for name in ("q", "k"):
+        for n in ((1 << 31) - 1, (1 << 31) - 63):
+            a = attention_args(**{f"{name}_rows": n, f"{name}_positions": n})
+            assert libpmg.pmg_attention(C.byref(a), None, 0, None) == _lib.PMG_E_INVALID
+            assert b"2^31" in libpmg.pmg_last_error()

@@ -336,3 +336,36 @@ def test_attention_whole_results_captured_and_replayed(gpu):
         ref.assert_within(y, want, tol)
         torch.cuda.synchronize()
         assert torch.equal(y, call())
+
+
+def test_linear_more_rows_than_a_grid_holds(gpu):
+    """2^30 rows in tiles of 64 would be 2^32 threads."""
+    M = 2 ** 30 + 77
+    announce(f"linear of {M} rows")
+    x = torch.zeros((M, 1), dtype=F16, device=gpu)
+    at = torch.tensor([0, 1, 63, 64, 2 ** 29, 2 ** 30 - 65, 2 ** 30 - 64, 2 ** 30 - 1, 2 ** 30, M - 1], device=gpu)
+    x[at, 0] = torch.arange(1, 11, dtype=F16, device=gpu)
+    r = torch.zeros((M, 1), dtype=F16, device=gpu)
+    r[at, 0] = 0.5
+    got = ops.linear(x, torch.full((1, 1), 3.0, dtype=F16, device=gpu), residual=r, out=r)
+    assert torch.equal(got[at, 0].cpu(), 3 * torch.arange(1, 11, dtype=F16) + 0.5)
+    got[at] = 0
+    assert not any(bool(part.any()) for part in got.split(2 ** 28))
+
+
+def test_rope_more_rows_than_a_grid_holds(gpu):
+    """2^26 rows of 64 pairs, four a block, would be 2^32 threads."""
+    M, D = 2 ** 26 + 70, 128
+    announce(f"rope of {M} rows")
+    q = torch.zeros((M, 1, D), dtype=F16, device=gpu)
+    c = torch.zeros((M, 4), dtype=torch.int32, device=gpu)
+    at = torch.tensor([0, 3, 4, 2 ** 25, 2 ** 26 - 5, 2 ** 26 - 4, 2 ** 26 - 1, 2 ** 26, M - 1], device=gpu)
+    g = gen(1)
+    q[at] = randn(g, 9, 1, D).to(F16).to(gpu)
+    c[at] = torch.randint(0, 500, (9, 4), generator=g, dtype=torch.int32).to(gpu)
+    f = torch.rand((D // 2, 3), generator=g).to(gpu)
+    want, tol = ref.norm_rope(q[at], None, None, c[at], f, layer=False, interleaved=False)
+    ops.qk_norm_rope(q, None, c, f, out=(q, None))
+    ref.assert_within(q[at], want, tol)
+    q[at] = 0
+    assert not any(bool(part.any()) for part in q.split(2 ** 23))
