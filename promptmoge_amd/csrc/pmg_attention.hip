@@ -43,9 +43,13 @@ Plan plan_of(const pmg_attention_args& r) {
     const int64_t blocks = (p.whole ? slots / 128 + r.segments + 2 : (slots + 127) / 128) * r.Hk;
     // Microseconds, as measured: 64 keys of a tile at a CU's full throughput; a block's start; the share of that
     // throughput that 1 .. 4 blocks on a CU reach; a part's O written and read.
-    // (a tile's keys: more than a few segments are taken to be ragged, their rows in segments of 1.5 times the mean
-    // length, the longest of 2.5 times, whose tiles are at work last and alone)
-    const bool ragged = r.segments > 4;
+    // (a tile's keys: segments with an index are taken for pool cells, which are ragged. Cells of 16, 24 and 32 voxels of depth maps
+    // of 61 x 83 to 480 x 640: their rows lie in cells of 1.1 to 1.6 times the mean length, the longest has 1.2 to 2.7 times,
+    // whose tiles are at work last and alone. Rows in order are taken for frames of about one length: 12 of 800 rows, 4 heads
+    // of 128, in one part 39 us, in two 54, as ragged ones would be; 8 of 300, 4 heads of 64, biased: 1 .. 4 parts 17.7, 17.5,
+    // 17.6, 18.1. A block alone on its CU reaches half of the throughput; fp32 without bias or cap, bound by the matrix
+    // units, 0.9 of it: 8 frames of 600, 4 heads of 64: 1 .. 5 parts 56, 60, 62, 51, 60)
+    const bool ragged = r.q_index != nullptr;
     const double keys = (ragged ? 1.5 : 1.0) * nk * (p.whole || nq <= 0.0 ? 1.0 : 1.0 + 128.0 / G / nq);
     const bool f32 = r.type == PMG_TYPE_F32;
     const double tile = (f32 ? 0.07 * (r.D <= 32 ? 32 : r.D <= 64 ? 64 : 128) : r.D <= 32 ? 0.52 : r.D <= 64 ? 0.66 : 1.37) + (r.slopes ? 0.3 : 0.0);

@@ -273,3 +273,10 @@ def test_attention_positions_close_to_32_bits_are_refused(libpmg):
             a = attention_args(**{f"{name}_rows": n, f"{name}_positions": n})
             assert libpmg.pmg_attention(C.byref(a), None, 0, None) == _lib.PMG_E_INVALID
             assert b"2^31" in libpmg.pmg_last_error()
+
+
+def test_attention_of_equal_frames_is_not_planned_as_ragged_cells(libpmg):
+    """Twelve frames of 800 rows fill the CUs evenly: split, they take a third longer. Ragged cells have an index."""
+    rows = dict(type=_lib.TYPE_BF16, Hk=4, D=128, q_rows=9600, q_positions=9600, k_rows=9600, k_positions=9600, segments=12)
+    assert libpmg.pmg_attention_workspace_bytes(C.byref(attention_args(**rows))) == 0
+    assert libpmg.pmg_attention_workspace_bytes(C.byref(attention_args(q_index=D16, k_index=D16, **rows))) > 0
