@@ -112,6 +112,7 @@ class AttentionArgs(C.Structure):
         ("out_head", i64), ("q_rows", i64), ("k_rows", i64), ("q_positions", i64), ("k_positions", i64),
         ("segments", i64), ("q_offsets", vp), ("k_offsets", vp), ("q_index", vp), ("k_index", vp), ("q_coords", vp),
         ("k_coords", vp), ("slopes", vp), ("k_mask", vp), ("scale", f32), ("cap", f32), ("zero_rest", i32),
+        ("precise", i32),
     ]
 
 

@@ -45,7 +45,7 @@ struct AttnArgs {
     int Hq, Hk, G, D;
     float scale2;         // scale log2(e)
     float cap2, cap_arg;  // cap log2(e) (0: none); what its argument is multiplied by: 1 / cap for tanh, 2 log2(e) / cap for the exponential
-    int seg, splits, zero_rest;
+    int seg, splits, zero_rest, fine;
     int whole;  // blocks of one segment each
     int near;   // K and V each below 4 GiB, heads of full width: rows are fetched by 32-bit byte offsets
     uint32_t blocks;
@@ -203,8 +203,12 @@ constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
 //
 // Registers: with at most 256 the matrix instructions' results stay in ordinary vector registers, where the softmax
 // works on them; only the widest fp32 form of one wave needs more.
-// MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use). FINE: caps by tanh_f32 (fp32, and
-// large caps of the 16-bit types; a kernel of its own, for a branch inside the loop spills 2 to 8 registers).
+// MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use). FINE: caps by tanh_f32 (a branch
+// inside the loop spills 2 to 8 registers), and 16-bit weights in two parts. Rounded to 8 or 11 bits as one, they add as much error
+// as the result's own rounding (2.3e-3 of the result's size for 1.7e-3 in bf16, 2.8e-4 for 2.1e-4 in fp16); in two parts they add
+// nothing that shows, for 10 % more time (cells, 8 heads of 32 fp16, biased: 115 -> 127 us), 37 % (4 frames of 2745 rows, 8 heads of
+// 64 bf16, masked: 111 -> 151), 24 % (19200 rows, 4 heads of 64 bf16, biased: 657 -> 814), 6 % (pooled queries: 34 -> 36): the
+// caller's choice. (Times without the host, calls in one graph.)
 template <class T, int DP, int NW, bool BIAS, bool MASK, bool FINE>
 __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void attention_k(AttnArgs a0) {
     const AttnArgs& a = a0;
@@ -647,6 +651,13 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                             chunk pf;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) pf[i] = (T)s[8 * f + i];
+                            if constexpr (FINE) {  // what the rounding left, in a product of its own
+                                chunk pr;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) pr[i] = (T)(s[8 * f + i] - (float)pf[i]);
+#pragma unroll
+                                for (int n = 0; n < NB; ++n) O[n] = Mat<T>::mma32(values(f, n), pr, O[n]);
+                            }
 #pragma unroll
                             for (int n = 0; n < NB; ++n) O[n] = Mat<T>::mma32(values(f, n), pf, O[n]);
                         }
@@ -855,7 +866,7 @@ static int launch_attention_w(AttnArgs& a, hipStream_t s) {
     a.blocks = (uint32_t)blocks;
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), 0, s, a); };
     constexpr bool F32 = sizeof(T) == 4;
-    if (!F32 && a.cap2 > kFineCap) {
+    if (!F32 && a.fine) {
         if (a.slopes) launch(attention_k<T, DP, NW, true, false, true>);
         else launch(attention_k<T, DP, NW, false, false, true>);
     } else if (a.slopes) launch(attention_k<T, DP, NW, true, false, F32>);

@@ -147,9 +147,11 @@ extern "C" int pmg_attention(const pmg_attention_args* p, void* workspace, size_
     a.D = r.D;
     const double log2e = 1.4426950408889634;
     a.scale2 = (float)((double)r.scale * log2e);
+    a.fine = r.type == PMG_TYPE_F32 || r.precise;
     if (r.cap > 0.0f) {
         a.cap2 = (float)((double)r.cap * log2e);
-        a.cap_arg = (float)((double)r.scale / (double)r.cap * (r.type == PMG_TYPE_F32 || a.cap2 > kFineCap ? 1.0 : 2.0 * log2e));
+        if (a.cap2 > kFineCap) a.fine = 1;
+        a.cap_arg = (float)((double)r.scale / (double)r.cap * (a.fine ? 1.0 : 2.0 * log2e));
     }
     a.seg = pl.seg;
     a.whole = pl.whole;

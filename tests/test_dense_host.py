@@ -82,7 +82,7 @@ def test_one_host_tensor_is_refused_in_every_place(no_launch, name, place, part)
 def test_the_places_are_all_there_are():
     for name, args, kw in calls():
         named = set(inspect.signature(getattr(ops, name)).parameters)
-        rest = {"act", "out_dtype", "a_scale", "norm", "eps", "interleaved", "cap", "scale"}
+        rest = {"act", "out_dtype", "a_scale", "norm", "eps", "interleaved", "cap", "scale", "precise"}
         assert named - rest == set(args)
 
 

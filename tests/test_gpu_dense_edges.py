@@ -369,3 +369,29 @@ def test_rope_more_rows_than_a_grid_holds(gpu):
     ref.assert_within(q[at], want, tol)
     q[at] = 0
     assert not any(bool(part.any()) for part in q.split(2 ** 23))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("D", [16, 64, 96])
+@pytest.mark.parametrize("kw", [dict(), dict(bias=True), dict(mask=True), dict(cap=5.0, mask=True), dict(bias=True, cap=1e4), dict(few=True, mask=True)])
+def test_attention_precise(gpu, dt, D, kw):
+    """precise: the fp32 form's bounds on the same numbers, and one rounding to the type at the end. The weights' two parts leave 2^-16 of
+    a weight in bf16 (2^-9 of a part that is 2^-8 of it, rounded up) and less in fp16."""
+    g = gen(D)
+    lengths = torch.tensor([0, 3, 300, 700, 1000]) if not kw.get("few") else torch.tensor([0, 1, 3])
+    M = int(lengths[-1])
+    Mk = 20_000 if kw.get("few") else M
+    koff = torch.tensor([0, 9000, Mk]) if kw.get("few") else lengths
+    q, k, v = (randn(g, m, 2, D).to(dt) for m in (M, Mk, Mk))
+    a = dict(cap=kw.get("cap", 0.0))
+    if kw.get("bias"):
+        a |= dict(coords=torch.randint(0, 40, (M, 4), generator=g, dtype=torch.int32), slopes=0.2 * torch.rand((2, 3), generator=g))
+        a["kv_coords"] = a["coords"]
+    if kw.get("mask"):
+        a["kv_mask"] = torch.rand(Mk, generator=g) > 0.3
+    announce(f"attention precise {dt} {D} {kw}")
+    dev = {n: t.to(gpu) if isinstance(t, torch.Tensor) else t for n, t in a.items()}
+    got = ops.sparse_attention(q.to(gpu), k.to(gpu), v.to(gpu), lengths.to(gpu), koff.to(gpu), precise=True, **dev)
+    want, tol, _ = ref.attention(q.float(), k.float(), v.float(), lengths, koff, **a)
+    size, _, _ = ref.attention(q.float(), k.float(), v.float().abs(), lengths, koff, **a)  # sum of p |v|
+    ref.assert_within(got, want, tol + 2.0 ** -16 * size * (dt != F32) + ref.U[dt] * want.abs() * 1.01 + ref.TINY[dt])
