@@ -631,7 +631,7 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  * scale up to 1e30; cap 0 or up to 1e30, scale / cap up to 1e37; a capped score is accurate relative to itself (16-bit types, caps
  * up to 256: within 3e-7 cap).
  * Sums and statistics in fp32; the softmax's weights enter the second product rounded to `type` (half a step of it each: about the
- * error that the result's own rounding adds), or with precise in two parts (fp32's error; 6 to 37 % more time).
+ * error that the result's own rounding adds), or with precise in two parts (fp32's error; 7 to 41 % more time).
  * Offsets are held to [0, positions] (where they fall, what the rows get is not said); a position whose index lies outside the
  * rows is absent. Query rows that no position of a segment names are left as they were, or with zero_rest set to 0, whatever the
  * tables hold. A row named by two query positions gets either's result (0 of a position of no segment). Differences of

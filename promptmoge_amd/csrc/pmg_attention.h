@@ -206,9 +206,9 @@ constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
 // MASK: absent keys are taken out by a product (not with BIAS, whose registers are all in use). FINE: caps by tanh_f32 (a branch
 // inside the loop spills 2 to 8 registers), and 16-bit weights in two parts. Rounded to 8 or 11 bits as one, they add as much error
 // as the result's own rounding (2.3e-3 of the result's size for 1.7e-3 in bf16, 2.8e-4 for 2.1e-4 in fp16); in two parts they add
-// nothing that shows, for 10 % more time (cells, 8 heads of 32 fp16, biased: 115 -> 127 us), 37 % (4 frames of 2745 rows, 8 heads of
-// 64 bf16, masked: 111 -> 151), 24 % (19200 rows, 4 heads of 64 bf16, biased: 657 -> 814), 6 % (pooled queries: 34 -> 36): the
-// caller's choice. (Times without the host, calls in one graph.)
+// nothing that shows, for 16 % more time (cells, 8 heads of 32 fp16, biased: 115 -> 133 us), 41 % (4 frames of 2745 rows, 8 heads of
+// 64 bf16, masked: 108 -> 152), 29 % (19200 rows, 4 heads of 64 bf16, biased: 643 -> 833), 7 % (pooled queries: 34 -> 37): the
+// caller's choice, or with a large cap. (Times without the host, calls in one graph.)
 template <class T, int DP, int NW, bool BIAS, bool MASK, bool FINE>
 __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void attention_k(AttnArgs a0) {
     const AttnArgs& a = a0;
@@ -635,6 +635,9 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                         return __builtin_bit_cast(chunk, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
                     };
                     // ---- O^T += V^T P^T
+                    // (two parts: the first one less than the weight by more than its rounding, so that the second one is
+                    // positive and an infinite value stays infinite)
+                    constexpr float kLess = 1.0f - (HALF ? 1.0f / 1024 : 1.0f / 128);
                     if constexpr (ES == 4) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
@@ -650,8 +653,8 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
                         for (int f = 0; f < 2; ++f) {
                             chunk pf;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) pf[i] = (T)s[8 * f + i];
-                            if constexpr (FINE) {  // what the rounding left, in a product of its own
+                            for (int i = 0; i < 8; ++i) pf[i] = (T)(FINE ? s[8 * f + i] * kLess : s[8 * f + i]);
+                            if constexpr (FINE) {  // what that left, in a product of its own
                                 chunk pr;
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) pr[i] = (T)(s[8 * f + i] - (float)pf[i]);
