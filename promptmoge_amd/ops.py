@@ -589,11 +589,12 @@ def _in_forward_ad() -> bool:
     return getattr(forward_ad, "_current_level", 0) >= 0
 
 
-def _refuse(**named: Optional[torch.Tensor]) -> int:
-    """Says which of the tensors (None: absent) is not on the first one's GPU or needs a gradient; that GPU's index if none."""
+def _refuse(needed: str, **named: Optional[torch.Tensor]) -> int:
+    """Says which of the tensors (None: absent, but those needed) is not on the first one's GPU or needs a gradient; that
+    GPU's index if none."""
     dev = None
     for name, t in named.items():
-        if t is None:
+        if t is None and name not in needed.split():
             continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"{name} must be a GPU tensor")
@@ -603,8 +604,6 @@ def _refuse(**named: Optional[torch.Tensor]) -> int:
         if (t.requires_grad and torch.is_grad_enabled()) or (
                 _in_forward_ad() and forward_ad.unpack_dual(t).tangent is not None):
             raise RuntimeError("the libpmg operators are inference-only; run under torch.no_grad(), without tangents")
-    if dev is None:
-        raise ValueError("no tensors")
     return dev.index
 
 
@@ -711,9 +710,9 @@ def _apart(out: torch.Tensor, name: str, **others: Optional[torch.Tensor]) -> No
 
 
 def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torch.Tensor:
-    d = _one_gpu(x, w, bias, w_scale, residual, out)
+    d = _one_gpu(x, w, bias, w_scale, residual, out) if x is not None and w is not None else -1
     if d < 0:
-        d = _refuse(x=x, w=w, bias=bias, w_scale=w_scale, residual=residual, out=out)
+        d = _refuse("x w", x=x, w=w, bias=bias, w_scale=w_scale, residual=residual, out=out)
     ldx = _rows(x, "x")
     M, K = x.shape
     if w.dtype != x.dtype:
@@ -736,6 +735,8 @@ def _linear(x, w, bias, a_scale, w_scale, act, residual, out_dtype, out) -> torc
         if residual.shape != (M, N):
             raise ValueError(f"residual must be ({M}, {N}), got {tuple(residual.shape)}")
     if out is None:
+        if out_dtype is None:
+            out_dtype = x.dtype if x.dtype != torch.int8 else torch.float32
         out = x.new_empty((M, N), dtype=out_dtype) if out_dtype != x.dtype else x.new_empty((M, N))
         ldo = N
     else:
@@ -762,8 +763,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     follows it. x: (M, K) fp32 / fp16 / bf16 (rows may be strided); w: (N, K) of x's type; bias: (N,) fp32; act: "none",
     "relu", "silu", "gelu" (erf) or "gelu_tanh"; residual: (M, N) of any of the three types. Sums in fp32, rounded
     once to out_dtype (default: out's, or x's). `out` may be the residual itself. Forward only."""
-    _floating(x, "x")
-    return _linear(x, w, bias, 1.0, None, act, residual, out_dtype or (x.dtype if out is None else None), out)
+    if isinstance(x, torch.Tensor):
+        _floating(x, "x")
+    return _linear(x, w, bias, 1.0, None, act, residual, out_dtype, out)
 
 
 def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, a_scale: float = 1.0,
@@ -772,9 +774,9 @@ def linear_i8(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = N
     """linear on int8 codes: act((acc * a_scale) * w_scale[n] + bias) + residual with the exact int32 sums acc, the
     arithmetic of spconv_i8. x: (M, K) int8; w: (N, K) int8; w_scale, bias: (N,) fp32; result fp32 (default), fp16 or
     bf16."""
-    if x.dtype != torch.int8:
+    if isinstance(x, torch.Tensor) and x.dtype != torch.int8:
         raise ValueError(f"x must be torch.int8, got {x.dtype}")
-    return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype or (torch.float32 if out is None else None), out)
+    return _linear(x, w, bias, float(a_scale), w_scale, act, residual, out_dtype, out)
 
 
 def _off_units(t: torch.Tensor, unit: int) -> bool:
@@ -822,10 +824,10 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], coords: torch.Tenso
     bits. Pair p is (p, p + D/2), or with interleaved (2p, 2p + 1). Returns (q, k) in new tensors, or in `out` (which
     may be the inputs). Forward only."""
     qo, ko = out if out is not None else (None, None)
-    d = _one_gpu(q, k, coords, freqs, q_weight, k_weight, q_bias, k_bias, qo, ko)
+    d = _one_gpu(q, k, coords, freqs, q_weight, k_weight, q_bias, k_bias, qo, ko) if q is not None else -1
     if d < 0:
-        d = _refuse(q=q, k=k, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias,
-                    out_q=qo, out_k=ko)
+        d = _refuse("q coords freqs", q=q, k=k, coords=coords, freqs=freqs, q_weight=q_weight, k_weight=k_weight,
+                    q_bias=q_bias, k_bias=k_bias, out_q=qo, out_k=ko)
     ty = _floating(q, "q")
     unit = 4 * q.element_size()
     if norm not in ("rms", "layer"):
@@ -910,10 +912,12 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Rows that no position of a segment names are 0 in a new result and left as they were in a given `out`. A row named by
     two query positions gets either's result. Where offsets fall, what the rows get is not said. Forward only."""
-    d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
+    d = -1
+    if q is not None:
+        d = _one_gpu(q, k, v, offsets, kv_offsets, index, kv_index, coords, kv_coords, slopes, kv_mask, out)
     if d < 0:
-        d = _refuse(q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index, kv_index=kv_index, coords=coords,
-                    kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask, out=out)
+        d = _refuse("q k v offsets", q=q, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, index=index,
+                    kv_index=kv_index, coords=coords, kv_coords=kv_coords, slopes=slopes, kv_mask=kv_mask, out=out)
     ty = _floating(q, "q")
     if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"q must be (Mq, Hq, D), k and v (Mk, Hk, D); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -968,7 +972,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         ty, Hq, Hk, D, q.data_ptr(), qs, qh, k.data_ptr(), ks, kh, v.data_ptr(), vs, vh, out.data_ptr(), os, oh, Mq, Mk,
         Mq if index is None else index.shape[0], Mk if kv_index is None else kv_index.shape[0], offsets.shape[0] - 1,
         offsets.data_ptr(), kv_offsets.data_ptr(), _ptr(index), _ptr(kv_index), _ptr(coords) if slopes is not None else 0,
-        _ptr(kv_coords) if slopes is not None else 0, _ptr(slopes), _ptr(kv_mask), D ** -0.5 if scale is None else scale,
+        _ptr(kv_coords) if slopes is not None else 0, _ptr(slopes), _ptr(kv_mask), (D or 1) ** -0.5 if scale is None else scale,
         cap, fresh, bool(precise))
     ws_bytes = _entry("pmg_attention_workspace_bytes")(args)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None

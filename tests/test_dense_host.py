@@ -280,3 +280,22 @@ def test_attention_of_equal_frames_is_not_planned_as_ragged_cells(libpmg):
     rows = dict(type=_lib.TYPE_BF16, Hk=4, D=128, q_rows=9600, q_positions=9600, k_rows=9600, k_positions=9600, segments=12)
     assert libpmg.pmg_attention_workspace_bytes(C.byref(attention_args(**rows))) == 0
     assert libpmg.pmg_attention_workspace_bytes(C.byref(attention_args(q_index=D16, k_index=D16, **rows))) > 0
+
+
+def test_heads_of_no_width_are_refused_as_other_widths(no_launch, monkeypatch):
+    """(by the entry itself: D^-1/2 is not formed)"""
+    q, off = on_gpu(zeros(4, 2, 0)), on_gpu(torch.tensor([0, 4]))
+    with pytest.raises(Reached):
+        ops.sparse_attention(q, q, q, off)
+    with pytest.raises(Reached):
+        ops.sparse_attention(q, q, q, off, scale=1.0)
+
+
+@pytest.mark.parametrize("bad", [None, 1.0, [1.0]])
+def test_what_is_no_tensor_is_refused_by_name(no_launch, bad):
+    every = {n: {m: everywhere(v) for m, v in args.items()} for n, args, _ in calls()}
+    for name, first in (("linear", "x"), ("linear_i8", "x"), ("qk_norm_rope", "q"), ("sparse_attention", "q")):
+        for place in (first, "out") if bad is not None else (first,):
+            wrong = (bad, bad) if (name, place) == ("qk_norm_rope", "out") else bad
+            with pytest.raises(ValueError, match="GPU tensor"):
+                getattr(ops, name)(**{**every[name], place: wrong})
