@@ -639,8 +639,8 @@ int pmg_qk_norm_rope(const pmg_rope_args* args, void* stream);
  * Rows, positions and segments below 2^31 - 64; query positions times Hq (and segments times 128 Hk) below 2^31, else the call
  * may be refused: a grid holds 2^32 threads.
  * D a multiple of 8 up to 128; q, k, v: buffers and strides (elements) in whole 16 bytes, out in groups of 4 elements;
- * out must not overlap the inputs. Workspace (any contents; may be NULL if 0 bytes): must not be shared by calls that
- * overlap. */
+ * out must not overlap the inputs. Workspace (any contents; of the same args, pointers included; may be NULL if 0 bytes):
+ * must not be shared by calls that overlap. */
 typedef struct {
     int type; /* f32, f16 or bf16 */
     int Hq, Hk, D;
