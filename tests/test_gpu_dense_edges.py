@@ -415,3 +415,33 @@ def test_attention_infinite_values_that_count(gpu, dt, D, kw):
     tol = torch.nan_to_num(tol, nan=0.0, posinf=0.0)
     assert bool(torch.isinf(want[:150, 0, 3]).all()) and bool(torch.isnan(want[:150, 0, 6]).all())
     ref.assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("straight", [True, False])
+@pytest.mark.parametrize("positions", [0, 1, 40, 64])
+def test_attention_zero_rest_of_the_c_entry(gpu, dt, straight, positions):
+    """Fewer positions than rows without an index, and results of any stride: the other rows are 0, what lies between them stays."""
+    import ctypes as C
+    g = gen(positions)
+    M, H, D = 64, 2, 40
+    code, es = {F32: _lib.TYPE_F32, F16: _lib.TYPE_F16, BF16: _lib.TYPE_BF16}[dt], torch.finfo(dt).bits // 8
+    q, k, v = (randn(g, M, H, D).to(dt).to(gpu) for _ in range(3))
+    buf = torch.full((M, H + 1, D + 4), math.nan, dtype=dt, device=gpu)
+    out = torch.full((M, H, D), math.nan, dtype=dt, device=gpu) if straight else buf[:, :H, :D]
+    off = torch.tensor([0, positions // 2, max(positions - 3, positions // 2)], device=gpu)
+    a = _lib.AttentionArgs(type=code, Hq=H, Hk=H, D=D, q=q.data_ptr(), q_row=H * D, q_head=D, k=k.data_ptr(), k_row=H * D, k_head=D,
+                           v=v.data_ptr(), v_row=H * D, v_head=D, out=out.data_ptr(), out_row=out.stride(0), out_head=out.stride(1),
+                           q_rows=M, k_rows=M, q_positions=positions, k_positions=positions, segments=2, q_offsets=off.data_ptr(),
+                           k_offsets=off.data_ptr(), scale=D ** -0.5, zero_rest=1)
+    lib = _lib.lib()
+    need = lib.pmg_attention_workspace_bytes(C.byref(a))
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu)
+    announce(f"attention zero_rest {dt} straight={straight} positions={positions}")
+    _lib.check(lib.pmg_attention(C.byref(a), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    want, tol, covered = ref.attention(q, k, v, off)
+    assert not bool(out.cpu()[~covered].any())
+    ref.assert_within(out, want, tol)
+    if not straight:
+        assert bool(torch.isnan(buf[:, H]).all()) and bool(torch.isnan(buf[:, :, D:]).all())
