@@ -47,7 +47,7 @@ __device__ inline float gelu_16(float y) {
     return __builtin_fmaf(-__builtin_fabsf(x), q, y < 0.0f ? 0.0f : y);
 }
 
-// 1 / (1 + exp(-z)) for fp32 outputs, within 2^-22 of its value: the exponential of -|z|, which cannot overflow, its argument in two
+// 1 / (1 + exp(-z)) for fp32 outputs, within 2^-21 of its value: the exponential of -|z|, which cannot overflow, its argument in two
 // parts (in one, as silu_fast has it, |z| 2^-24 of the result is lost: 20 times the rest at -80), then 1 ulp each for exp2 and
 // reciprocal. Values below 2^-126 may be 0.
 __device__ inline float sigmoid_wide(float z) {
