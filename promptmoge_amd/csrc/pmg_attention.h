@@ -49,6 +49,7 @@ struct AttnArgs {
     int whole;  // blocks of one segment each
     int near;   // K and V each below 4 GiB, heads of full width: rows are fetched by 32-bit byte offsets
     uint32_t blocks;
+    uint32_t sweep;  // blocks in front of them, which look after what the tables miss
     float* part_o;  // [splits][Hq][Pq][D]; (m, l) [splits][Hq][Pq], l < 0: a position of no segment
     float2* part_ml;
 };
@@ -188,6 +189,76 @@ __device__ inline ConstArgs& args_again() {
     return *(ConstArgs*)p;
 }
 
+// Zeros in the rows of a wave's lanes that want it.
+template <class T>
+__device__ inline void zero_rows(ConstArgs& a, bool want, int64_t row) {
+    typedef T v4t __attribute__((ext_vector_type(4)));
+    const int quads = a.D / 4;
+    for (uint64_t todo = __ballot(want); todo; todo &= todo - 1) {
+        const int64_t r = __shfl(row, __ffsll((unsigned long long)todo) - 1, 64);
+        for (int d = threadIdx.x & 63; d < a.Hq * quads; d += 64) *(v4t*)((T*)a.out + r * a.o_row + d / quads * a.o_head + d % quads * 4) = v4t{};
+    }
+}
+
+// What a block of the sweep does, beside the blocks that compute: its share of the rows and positions is looked through for rows
+// that no position names (they are set to 0: nobody else writes them), and where the offsets of blocks of one segment each fall,
+// for slots that no block has (set to 0, or marked as of no segment for the join). Two passes over the index (in L2) of the share's
+// 1 / 8 to 1 / 32 a block cost next to nothing beside the others; a kernel in front costs a launch, 3 us, or 7.5 for 39 MB.
+constexpr int kSweepBits = 32768;  // the share: a bit each, in LDS
+template <class T, int NT>
+__device__ inline void attention_sweep(uint32_t* bits, int per_block) {
+    ConstArgs& a = args_again();  // (read here: kept from the kernel's start, they cost the other blocks registers)
+    const int tid = thread_again();
+    const int64_t n = a.Mq > a.Pq ? a.Mq : a.Pq, share = (n + a.sweep - 1) / a.sweep, lo = blockIdx.x * share;
+    const auto clear = [&]() {
+        __syncthreads();
+        for (int i = tid; i < kSweepBits / 32; i += NT) bits[i] = 0;
+        __syncthreads();
+    };
+    const auto set = [&](int64_t i) { atomicOr(&bits[i >> 5], 1u << (i & 31)); };
+    const auto is = [&](int64_t i) { return (bits[i >> 5] >> (i & 31) & 1u) != 0; };
+    if (a.q_index && a.zero_rest) {
+        const int64_t hi = lo + share < a.Mq ? lo + share : a.Mq;
+        clear();
+#pragma unroll 16
+        for (int64_t p = tid; p < a.Pq; p += NT) {
+            const int64_t r = a.q_index[p];
+            if (r >= lo && r < hi) set(r - lo);
+        }
+        __syncthreads();
+        for (int64_t r0 = lo; r0 < hi; r0 += NT) zero_rows<T>(a, r0 + tid < hi && !is(r0 + tid - lo), r0 + tid);
+    }
+    if (!a.whole || a.S <= kLook) return;
+    bool fall = false;
+#pragma unroll 8
+    for (int64_t j = tid; j < a.S; j += NT) fall = fall || a.q_off[j] > a.q_off[j + 1];
+    if (!__syncthreads_or(fall)) return;
+    const int64_t end = (lo + share < a.Pq ? lo + share : a.Pq) * a.G;
+    const uint32_t units = a.blocks / (uint32_t)(a.Hk * a.splits);
+    for (int64_t s0 = lo * a.G; s0 < end; s0 += kSweepBits) {
+        const int64_t s1 = s0 + kSweepBits < end ? s0 + kSweepBits : end;
+        clear();
+        for (uint32_t u = tid >> 6; u < units; u += NT / 64) {
+            int64_t from, to;
+            unit_segment(a.q_off, a.S, a.Pq, a.G, per_block, u, from, to);
+            for (int64_t i = from + (tid & 63); i < to; i += 64)
+                if (i >= s0 && i < s1) set(i - s0);
+        }
+        __syncthreads();
+        for (int64_t i = s0 + tid; i < s1; i += NT) {
+            if (is(i - s0)) continue;
+            const int64_t pos = i / a.G;
+            const int64_t row = a.q_index ? a.q_index[pos] : pos;
+            for (int hk = 0; hk < a.Hk; ++hk) {
+                const int head = hk * a.G + (int)(i - pos * a.G);
+                if (a.splits > 1) a.part_ml[(int64_t)head * a.Pq + pos] = make_float2(-__builtin_inff(), -1.0f);
+                else if (a.zero_rest && row >= 0 && row < a.Mq)
+                    for (int d = 0; d < a.D; ++d) ((T*)a.out)[row * a.o_row + head * a.o_head + d] = (T)0.0f;
+            }
+        }
+    }
+}
+
 // Waves a SIMD the registers are kept to (what the LDS of a block allows, too).
 constexpr int waves_of(int DP, int NW, int ES, bool BIAS) {
     if (NW == 1) return DP == 128 ? 1 : 2;
@@ -234,9 +305,14 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     __shared__ int32_t s_r[3][NW];
     __shared__ int s_flag[NW];
 
+    if (blockIdx.x < a.sweep) {
+        static_assert(sizeof(s_k) >= kSweepBits / 8, "the share's bits");
+        attention_sweep<T, NT>((uint32_t*)s_k, 32 * NW);
+        return;
+    }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // block -> (split, key head, tile or segment): an XCD's blocks are neighbours, on one head's keys
-    const uint32_t id = xcd_tile(blockIdx.x, a.blocks);
+    const uint32_t id = xcd_tile(blockIdx.x - a.sweep, a.blocks);  // (a.sweep is a multiple of 8)
     const uint32_t per_head = a.blocks / (uint32_t)(a.Hk * a.splits);
     const uint32_t unit = id % per_head;
     const int hk = (int)(id / per_head) % a.Hk, split = (int)(id / per_head) / a.Hk;
@@ -262,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, waves_of(DP, NW, sizeof(T), BIAS)) void at
     } else if (a.whole && (whole = a.S > kLook || offsets_rise(a.q_off, a.S))) {
         own = unit_segment(a.q_off, a.S, a.Pq, a.G, 32 * NW, unit, slot0, slot1);
     } else {  // (where offsets fall, blocks of one segment each would miss rows; there are enough of them for these tiles. Of more
-              // segments than a wave looks through at once, rows and parts that are missed hold what attention_fill_k left)
+              // segments than a wave looks through at once the sweep or attention_fill_k sees to what is missed)
         slot0 = (int64_t)unit * (32 * NW);
         slot1 = slot0 + 32 * NW;
         if (slot1 > a.Pq * a.G) slot1 = a.Pq * a.G;
@@ -835,8 +911,8 @@ static int launch_join(const AttnArgs& a, hipStream_t s) {
     return check_launch("attention_join_k");
 }
 
-// In front of the others: zeros in a result that the tables may not name whole, and no segment in the parts' (m, l) where blocks of
-// one segment each may miss some. (39 MB: 8 us.)
+// In front of the others, where a sweep would take too long or there is none: zeros in a result that the tables may not name whole,
+// and no segment in the parts' (m, l) where blocks of one segment each may miss some.
 template <class T>
 __global__ __launch_bounds__(256) void attention_fill_k(AttnArgs a, int64_t rows, int64_t chunks, int64_t parts) {
     const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
@@ -849,15 +925,19 @@ __global__ __launch_bounds__(256) void attention_fill_k(AttnArgs a, int64_t rows
 }
 
 template <class T>
-static int launch_fill(const AttnArgs& a, hipStream_t s) {
+static int launch_fill(AttnArgs& a, hipStream_t s) {
     const int64_t chunks = a.Mq * a.Hq * a.D * (int64_t)sizeof(T) / 16;  // (D is a multiple of 8)
-    const bool split = a.splits > 1, missed = a.whole && a.S > kLook;  // (Pq 0: neither)
-    const bool fill = a.zero_rest && (a.q_index || a.Pq < a.Mq || missed || (a.seg && !split));
+    const bool split = a.splits > 1, unnamed = a.zero_rest && a.q_index, missed = a.whole && a.S > kLook && (a.zero_rest || split);
+    // The sweep's blocks read the index as often as there are shares: up to a million rows that is 134 MB.
+    const int64_t n = a.Mq > a.Pq ? a.Mq : a.Pq, shares = (n + 2047) / 2048;
+    const bool sweep = (unnamed || missed) && a.Pq > 0 && n <= 32 * (int64_t)kSweepBits;
+    if (sweep) a.sweep = (uint32_t)(shares < 32 ? (shares + 7) / 8 * 8 : 32);
+    const bool fill = a.zero_rest && (a.Pq < a.Mq && !a.q_index || a.seg && !split || !sweep && (unnamed || missed));
     const bool straight = a.o_head == a.D && a.o_row == (int64_t)a.Hq * a.D && aligned16(a.out);
-    const int64_t n = fill && straight ? chunks : 0, rows = fill && !straight ? a.Mq : 0, parts = split && missed ? a.splits * a.Pq * a.Hq : 0;
-    const int64_t most = n > rows * 64 ? n : rows * 64, blocks = ((most > parts ? most : parts) + 1023) / 1024;
+    const int64_t wide = fill && straight ? chunks : 0, rows = fill && !straight ? a.Mq : 0, parts = split && missed && !sweep ? a.splits * a.Pq * a.Hq : 0;
+    const int64_t most = wide > rows * 64 ? wide : rows * 64, blocks = ((most > parts ? most : parts) + 1023) / 1024;
     if (blocks == 0) return PMG_OK;
-    hipLaunchKernelGGL((attention_fill_k<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, rows, n, parts);
+    hipLaunchKernelGGL((attention_fill_k<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, rows, wide, parts);
     return check_launch("attention_fill_k");
 }
 
@@ -865,9 +945,9 @@ template <class T, int DP, int NW>
 static int launch_attention_w(AttnArgs& a, hipStream_t s) {
     const int64_t units = NW == 1 ? a.S : a.whole ? a.Pq * a.G / (32 * NW) + a.S + 2 : (a.Pq * a.G + 32 * NW - 1) / (32 * NW);
     const int64_t blocks = units * a.Hk * a.splits;
-    PMG_REQUIRE(blocks <= grid_blocks(64 * NW), "too many slots or segments for one launch");
+    PMG_REQUIRE(blocks + a.sweep <= grid_blocks(64 * NW), "too many slots or segments for one launch");
     a.blocks = (uint32_t)blocks;
-    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), 0, s, a); };
+    const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.blocks + a.sweep), dim3(64 * NW), 0, s, a); };
     constexpr bool F32 = sizeof(T) == 4;
     if (!F32 && a.fine) {
         if (a.slopes) launch(attention_k<T, DP, NW, true, false, true>);

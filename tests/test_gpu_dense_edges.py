@@ -445,3 +445,51 @@ def test_attention_zero_rest_of_the_c_entry(gpu, dt, straight, positions):
     ref.assert_within(out, want, tol)
     if not straight:
         assert bool(torch.isnan(buf[:, H]).all()) and bool(torch.isnan(buf[:, :, D:]).all())
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("S,L,Lk,Hq,Hk,index", [
+    (100, 800, 800, 16, 1, True),      # shares of the rows that take several rounds of bits
+    (70, 200, 3000, 1, 1, False),      # keys split: parts that nobody wrote
+    (90, 200, 2000, 2, 1, True),
+    (1100, 1000, 40, 1, 1, True),      # more rows than a sweep goes through: filled first
+    (1100, 1000, 40, 1, 1, False),
+    (70, 20_000, 300, 1, 1, False)])
+@pytest.mark.parametrize("fall", [False, True])
+def test_attention_many_segments_with_tables_that_miss_rows(gpu, dt, S, L, Lk, Hq, Hk, index, fall):
+    """More segments than a block looks through, with offsets that fall and an index that does not name every row."""
+    g = torch.Generator(device=gpu).manual_seed(S + L)
+    D = 32
+    M, Mk = S * L, S * Lk
+    off, koff = torch.arange(S + 1, device=gpu) * L, torch.arange(S + 1, device=gpu) * Lk
+    if fall:
+        off[S // 2], off[S // 2 + 1] = off[S // 2 + 1].item(), off[S // 2].item()
+        off[5] = M
+        off[S - 3] = -7
+    q = torch.randn((M, Hq, D), device=gpu, generator=g).to(dt)
+    k, v = (torch.randn((Mk, Hk, D), device=gpu, generator=g).to(dt) for _ in range(2))
+    kw = {}
+    if index:
+        idx = torch.randperm(M, device=gpu, generator=g).int()
+        idx[::9] = -1
+        idx[1::50] = 2 ** 31 - 1
+        kw["index"] = idx
+    announce(f"attention tables that miss rows {dt} {S} x {L} on {Lk}, {Hq}/{Hk}, index={index} fall={fall}")
+    used_before(gpu, M * Hq * D * q.element_size())
+    got = ops.sparse_attention(q, k, v, off, koff, **kw)
+    assert not bool(torch.isnan(got).any())
+    assert float(got.abs().max()) <= 1.02 * float(v.abs().max())
+    if index:
+        named = torch.zeros(M, dtype=torch.bool, device=gpu)
+        named[idx[(idx >= 0) & (idx < M)].long()] = True
+        assert not bool(got[~named].any()) and (fall or bool(got[named].any(-1).all()))
+    if not fall:  # some segments' rows
+        for s in (0, 1, S // 2, S - 1):
+            rows = torch.arange(s * L, (s + 1) * L, device=gpu)
+            if index:
+                rows = idx[rows]
+                rows = rows[(rows >= 0) & (rows < M)].long()
+            rows = rows[:200]
+            ks = slice(s * Lk, (s + 1) * Lk)
+            want, tol, _ = ref.attention(q[rows], k[ks], v[ks], torch.tensor([0, len(rows)]), torch.tensor([0, Lk]))
+            ref.assert_within(got[rows], want, tol)
