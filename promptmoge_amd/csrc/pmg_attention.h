@@ -202,8 +202,9 @@ __device__ inline void zero_rows(ConstArgs& a, bool want, int64_t row) {
 
 // What a block of the sweep does, beside the blocks that compute: its share of the rows and positions is looked through for rows
 // that no position names (they are set to 0: nobody else writes them), and where the offsets of blocks of one segment each fall,
-// for slots that no block has (set to 0, or marked as of no segment for the join). Two passes over the index (in L2) of the share's
-// 1 / 8 to 1 / 32 a block cost next to nothing beside the others; a kernel in front costs a launch, 3 us, or 7.5 for 39 MB.
+// for slots that no block has (set to 0, or marked as of no segment for the join). Each of the 8 to 32 blocks reads the whole index
+// for it, mostly from L2. 76,800 rows in 433 cells: 107.8 us without, 110.6 with it; with a kernel of zeros in front 115.0, and
+// small calls 3 us longer for its launch.
 constexpr int kSweepBits = 32768;  // the share: a bit each, in LDS
 template <class T, int NT>
 __device__ inline void attention_sweep(uint32_t* bits, int per_block) {
