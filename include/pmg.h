@@ -670,6 +670,138 @@ typedef struct {
 size_t pmg_attention_workspace_bytes(const pmg_attention_args* args);
 int pmg_attention(const pmg_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------ *
+ * A conditional layer on rows: group norm, a router, its experts' products, and low-rank adapters beside a shared
+ * projection (no counterpart in the reference's flex_gemm). Forward only. None of them allocates or synchronises; all can be
+ * captured into a HIP graph. Segments: offsets is a device table, int64 [segments + 1], rising; segment s holds the positions (rows)
+ * offsets[s] .. offsets[s + 1] - 1. Offsets are held to the positions there are; where they fall, what the rows get is not
+ * said. Workspaces: any contents, on 16 bytes; must not be shared by calls that overlap.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum { PMG_SCORE_SOFTMAX = 0, PMG_SCORE_SIGMOID = 1 };
+
+/* pmg_group_norm -- out[m][c] = act((x[m][c] - mean) rsqrt(var + eps) weight[c] + bias[c]), mean and var (of the values there are,
+ *   not less one) over the rows of m's segment and the C / groups channels of c's group; sums in 64 bits, one rounding, to
+ *   out_type. Rows of no segment are left as they were, or with zero_rest set to 0. out may be x (same type and stride). C 1 ..
+ *   4096, M 0 .. 2^31 - 513, any alignment of whole elements. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    const void* x;
+    int64_t ldx; /* >= C */
+    int64_t M;
+    int C, groups;
+    const float* weight; /* [C] or NULL: ones */
+    const float* bias;   /* [C] or NULL */
+    const int64_t* offsets; /* or NULL: one segment (segments = 1) of all rows */
+    int64_t segments;
+    float eps;
+    int act;
+    void* out;
+    int out_type; /* f32, f16 or bf16 */
+    int64_t ldo;
+    int zero_rest;
+} pmg_group_norm_args;
+size_t pmg_group_norm_workspace_bytes(const pmg_group_norm_args* args);
+int pmg_group_norm(const pmg_group_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* pmg_route -- each row's k experts of largest logit (equal ones: the lowest index first; -inf and NaN are not chosen), and the pairs
+ *   m k + slot in the order of their experts, equal ones in their own order.
+ *   weights [M][k]: the chosen experts' softmax over the row's E logits, or sigmoid; normalize: over the sum of the row's (0 where
+ *   that is 0). experts [M][k]: -1 (weight 0) for a slot without an expert, and in rows with mask[m] = 0. offsets [E + 1]: where
+ *   each expert's pairs start; pairs [M k] and rows [M k] (pair / k): -1 from offsets[E] on.
+ *   fp32 arithmetic on the logits of any type. E 1 .. 1024, k 1 .. 32 and at most E, M k below 2^31 - 512. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    const void* logits;
+    int64_t ld; /* >= E */
+    int64_t M;
+    int E, k;
+    int score, normalize;
+    const uint8_t* mask; /* [M] or NULL */
+    float* weights;
+    int32_t* experts;
+    int64_t* offsets;
+    int32_t* pairs;
+    int32_t* rows;
+} pmg_route_args;
+size_t pmg_route_workspace_bytes(const pmg_route_args* args);
+int pmg_route(const pmg_route_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* pmg_grouped_linear -- position p of segment s reads row i = index[p] of x (or row p) and gives row o = out_index[p] of the result (or
+ *   row p): out[o] = act(x[i] w[s]^T + bias[s]) + residual[o], products, sums and rounding as in pmg_linear. Positions of no
+ *   segment, and those whose row lies outside x or the result, write nothing; with zero_rest (without out_index) their rows are
+ *   set to 0. Two positions with one result row: it gets either's (with residual = out: not said). Limits as in pmg_linear; N to
+ *   2^22, positions, rows of x and of the result 0 .. 2^31 - 513, segments below 2^24. Indexed rows of x that span 2 GiB and more are read
+ *   element by element. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    const void* x;
+    int64_t ldx, x_rows;
+    const void* w; /* [segments][N][K] */
+    int64_t positions, segments;
+    int K, N;
+    const int64_t* offsets;
+    const int32_t* index;     /* [positions] or NULL */
+    const int32_t* out_index; /* [positions] or NULL */
+    const float* bias;        /* [segments][N] or NULL */
+    int act;
+    const void* residual; /* [out_rows] rows of ldr, or NULL */
+    int residual_type;
+    int64_t ldr;
+    void* out;
+    int out_type;
+    int64_t ldo, out_rows;
+    int zero_rest;
+} pmg_grouped_linear_args;
+int pmg_grouped_linear(const pmg_grouped_linear_args* args, void* stream);
+
+/* pmg_combine -- out[m] = sum over the slots j of weights[m][j] y[m][j] + residual[m] in fp32, slots in order, one rounding. A slot of
+ *   weight 0 is not read (its y may hold anything). y[m][j] starts m y_row + j y_slot elements on. out may be residual. */
+typedef struct {
+    int type; /* f32, f16 or bf16 */
+    const void* y;
+    int64_t y_row, y_slot;
+    int64_t M;
+    int k, N;             /* k 1 .. 32, N 1 .. 2^24 */
+    const float* weights; /* [M][k] */
+    const void* residual; /* or NULL */
+    int residual_type;
+    int64_t ldr;
+    void* out;
+    int out_type;
+    int64_t ldo;
+} pmg_combine_args;
+int pmg_combine(const pmg_combine_args* args, void* stream);
+
+/* pmg_lora_linear -- out[m] = act(x[m] w^T + bias + scale[i] (x[m] down[i]^T) up[i]^T) + residual[m], i = adapter[s] of row m's segment
+ *   s; rows of no segment, or with an adapter outside 0 .. adapters - 1, have the projection alone. offsets NULL: every row is a
+ *   segment (segments = M). The low products are held to fp32's accuracy for the second one (16-bit types: in two parts, bf16
+ *   three). Limits as in pmg_linear; N to 2^22, rank 1 .. 128, M 0 .. 2^31 - 513. out may be residual. */
+typedef struct {
+    int type; /* f32, f16 or bf16: of x, w, down and up */
+    const void* x;
+    int64_t ldx;
+    int64_t M;
+    int K, N;
+    const void* w;    /* [N][K] */
+    const void* down; /* [adapters][rank][K] */
+    const void* up;   /* [adapters][N][rank] */
+    int rank, adapters;
+    const float* scale;     /* [adapters] or NULL: ones */
+    const int32_t* adapter; /* [segments] */
+    const int64_t* offsets;
+    int64_t segments;
+    const float* bias; /* [N] or NULL */
+    int act;
+    const void* residual;
+    int residual_type;
+    int64_t ldr;
+    void* out;
+    int out_type;
+    int64_t ldo;
+} pmg_lora_linear_args;
+size_t pmg_lora_linear_workspace_bytes(const pmg_lora_linear_args* args);
+int pmg_lora_linear(const pmg_lora_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@ PMG_OK, PMG_E_INVALID, PMG_E_HIP, PMG_E_OVERFLOW, PMG_E_DEVICE = 0, 1, 2, 3, 4
 EPI_ACC, EPI_Q, EPI_R, EPI_BIAS, EPI_SILU, EPI_RLN, EPI_ROUT, EPI_QLIN = 0, 1, 2, 3, 4, 5, 6, 7
 PREC_INT8, PREC_FP16 = 0, 1
 TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
+SCORES = {"softmax": 0, "sigmoid": 1}
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
@@ -116,6 +117,46 @@ class AttentionArgs(C.Structure):
     ]
 
 
+class GroupNormArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("x", vp), ("ldx", i64), ("M", i64), ("C", i32), ("groups", i32), ("weight", vp), ("bias", vp),
+        ("offsets", vp), ("segments", i64), ("eps", f32), ("act", i32), ("out", vp), ("out_type", i32), ("ldo", i64),
+        ("zero_rest", i32),
+    ]
+
+
+class RouteArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("logits", vp), ("ld", i64), ("M", i64), ("E", i32), ("k", i32), ("score", i32),
+        ("normalize", i32), ("mask", vp), ("weights", vp), ("experts", vp), ("offsets", vp), ("pairs", vp), ("rows", vp),
+    ]
+
+
+class GroupedLinearArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("x", vp), ("ldx", i64), ("x_rows", i64), ("w", vp), ("positions", i64), ("segments", i64),
+        ("K", i32), ("N", i32), ("offsets", vp), ("index", vp), ("out_index", vp), ("bias", vp), ("act", i32),
+        ("residual", vp), ("residual_type", i32), ("ldr", i64), ("out", vp), ("out_type", i32), ("ldo", i64),
+        ("out_rows", i64), ("zero_rest", i32),
+    ]
+
+
+class CombineArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("y", vp), ("y_row", i64), ("y_slot", i64), ("M", i64), ("k", i32), ("N", i32), ("weights", vp),
+        ("residual", vp), ("residual_type", i32), ("ldr", i64), ("out", vp), ("out_type", i32), ("ldo", i64),
+    ]
+
+
+class LoraLinearArgs(C.Structure):
+    _fields_ = [
+        ("type", i32), ("x", vp), ("ldx", i64), ("M", i64), ("K", i32), ("N", i32), ("w", vp), ("down", vp), ("up", vp),
+        ("rank", i32), ("adapters", i32), ("scale", vp), ("adapter", vp), ("offsets", vp), ("segments", i64),
+        ("bias", vp), ("act", i32), ("residual", vp), ("residual_type", i32), ("ldr", i64), ("out", vp),
+        ("out_type", i32), ("ldo", i64),
+    ]
+
+
 def packer(cls) -> struct.Struct:
     """The layout of a C struct as a struct.Struct: its values are packed in one call, a quarter of the time that
     filling the ctypes class takes (the dense operators' calls last a few microseconds)."""
@@ -126,6 +167,8 @@ def packer(cls) -> struct.Struct:
 
 
 LINEAR_PACK, ROPE_PACK, ATTENTION_PACK = packer(LinearArgs), packer(RopeArgs), packer(AttentionArgs)
+GROUP_NORM_PACK, ROUTE_PACK, GROUPED_PACK = packer(GroupNormArgs), packer(RouteArgs), packer(GroupedLinearArgs)
+COMBINE_PACK, LORA_PACK = packer(CombineArgs), packer(LoraLinearArgs)
 
 UNET_COUNTS, UNET_COORDS, UNET_PARENT, UNET_NMAP, UNET_TILE_MASK, UNET_DOWN, UNET_UP, UNET_ENC_TOKENS, \
     UNET_COL_OFFSETS, UNET_STEP_ST = range(10)
@@ -198,6 +241,14 @@ SIGNATURES = {
     "pmg_qk_norm_rope": (i32, [vp, vp]),  # RopeArgs
     "pmg_attention_workspace_bytes": (sz, [vp]),  # AttentionArgs
     "pmg_attention": (i32, [vp, vp, sz, vp]),
+    "pmg_group_norm_workspace_bytes": (sz, [vp]),  # GroupNormArgs
+    "pmg_group_norm": (i32, [vp, vp, sz, vp]),
+    "pmg_route_workspace_bytes": (sz, [vp]),  # RouteArgs
+    "pmg_route": (i32, [vp, vp, sz, vp]),
+    "pmg_grouped_linear": (i32, [vp, vp]),  # GroupedLinearArgs
+    "pmg_combine": (i32, [vp, vp]),  # CombineArgs
+    "pmg_lora_linear_workspace_bytes": (sz, [vp]),  # LoraLinearArgs
+    "pmg_lora_linear": (i32, [vp, vp, sz, vp]),
 }
 
 _lib: C.CDLL | None = None

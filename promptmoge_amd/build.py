@@ -24,7 +24,8 @@ BUILD = HERE / "_build"
 LIB = HERE / "libpmg.so"
 SOURCES = ["pmg_api.hip", "pmg_structure.hip", "pmg_conv.hip", "pmg_conv_col.hip", "pmg_rowops.hip", "pmg_fit.hip", "pmg_fill.hip", "pmg_order.hip", "pmg_probe.hip", "pmg_pool.hip", "pmg_gauge.hip", "pmg_unet.hip",
            "pmg_linear.hip", "pmg_rope.hip", "pmg_attention.hip", "pmg_attention_f16.hip", "pmg_attention_bf16.hip",
-           "pmg_attention_f32.hip"]
+           "pmg_attention_f32.hip", "pmg_norm.hip", "pmg_route.hip", "pmg_grouped.hip", "pmg_grouped_f16.hip",
+           "pmg_grouped_bf16.hip", "pmg_grouped_f32.hip"]
 ARCH = "gfx950"
 
 FLAGS = [

@@ -1,0 +1,531 @@
+// Kernels of the grouped products; both have w's rows as the matrix instruction's row operand, so that a lane holds four
+// neighbouring columns of one row of the result.
+#pragma once
+#include "pmg_grouped.h"
+
+namespace pmg {
+
+constexpr uint32_t kBehind = 0x7ffffff0u;  // an offset behind every buffer's end: reads zeros
+
+// ------------------------------------------------------------------------------------------------------------ tiles
+// A block's BM positions by BN columns from tiles of KB bytes of k in NS LDS buffers, filled by direct loads to LDS several
+// tiles ahead (VEC: rows of x and w on 16 bytes, K whole 16-byte chunks, gathered rows below 2 GiB; else element by element).
+// Tiles start where a segment starts (kRowAdapters: every BM rows), so that a tile has one w (one adapter).
+// kAdapters: the low products come in front, as more k: rows of x's parts against `up` as often, their sums multiplied
+// by the row's factor before the k of x and w.
+template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC, int KIND>
+__global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 1 : 2) void grouped_tile_k(GroupArgs a) {
+    static_assert(KIND != kAdapters || VEC, "parts are read 16 bytes at a time");
+    constexpr int NW = WM * WN, NT = 64 * NW, KE = KB / (int)sizeof(T), PER = Mat<T>::kPer, ES = (int)sizeof(T);
+    constexpr int CPR = KB / 16, RPL = 64 / CPR, STEPS = CPR / 2;  // chunks a row, rows a load, steps a tile
+    constexpr int TM = BM / WM, TN = BN / WN, MT = TM / 32, NTL = TN / 32;
+    constexpr int NL = ((BM + BN) / RPL + NW - 1) / NW, kStage = VEC ? NL * NW * 1024 : (BM + BN) * KB;  // a wave's loads a tile
+    typedef typename Mat<T>::chunk chunk;
+    typedef typename Mat<T>::acc32 acc32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int to[BM];                   // each row's place in the result
+    __shared__ int from[VEC ? 1 : BM];       // and in x
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const uint32_t tile = xcd_tile(blockIdx.x, a.tiles);
+    const int n0 = (int)(tile % a.tiles_n) * BN;
+    const uint32_t id = a.id0 + tile / a.tiles_n;
+    Piece pc;
+    if constexpr (KIND == kRowAdapters) {
+        pc.first = (int)(id * BM);
+        pc.n = a.P - pc.first < BM ? a.P - pc.first : BM;
+        pc.s = 0;
+    } else {
+        pc = piece_of<BM>(a, id);
+    }
+    if (pc.n < 1) return;
+    const int rows_n = a.N - n0 < BN ? a.N - n0 : BN;
+    if (KIND == kExperts && pc.s < 0) {  // positions of no segment
+        if (a.fresh) {
+            constexpr int G = BN / 8;
+            for (int e = tid; e < pc.n * G; e += NT) {
+                const int c = 8 * (e % G);
+                if (c < rows_n) zero8(a, pc.first + e / G, n0 + c, rows_n - c < 8 ? rows_n - c : 8);
+            }
+        }
+        return;
+    }
+    const int seg = KIND == kExperts ? pc.s : 0;
+    const int ad = KIND == kAdapters ? adapter_of(a, pc.s) : -1;
+    const bool gather = KIND == kExperts && a.index;
+    const T* xb = (const T*)a.x + (gather ? 0 : (int64_t)pc.first * a.ldx);
+    const T* wb = (const T*)a.w + (int64_t)seg * a.w_next + (int64_t)n0 * a.K;
+    const int nk = (a.K + KE - 1) / KE;
+    for (int e = tid; e < BM; e += NT) {
+        to[e] = e >= pc.n ? -1 : KIND == kExperts ? row_out(a, pc.first + e) : pc.first + e;
+        if constexpr (!VEC) from[e] = e >= pc.n ? -1 : gather ? (int)row_in(a, pc.first + e) : e;
+    }
+    if constexpr (!VEC) __syncthreads();
+
+    acc32 acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = acc32{};
+    // the lane's chunks of a tile's steps (row r of a 32-row operand)
+    const int r = lane & 31;
+    int at[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) at[s] = r * KB + 16 * swizzle<CPR>(r, 2 * s + (lane >> 5));
+    constexpr int LPR = TN / 8, RPP = 64 / LPR, NP = 32 / RPP;  // lanes a row, rows a pass, passes
+    const int nc = n0 + wn * TN + 8 * (lane % LPR);
+    const int left = a.N - nc < 8 ? a.N - nc : 8;
+    float bs[8];
+    bias8(a, seg, nc, bs);
+
+    chunk fx[2][MT], fw[2][NTL];
+    const auto operands = [&](const char* st, int s) {  // step s of the tile at st
+        const char* sx = st + wm * TM * KB + at[s];
+        const char* sw = st + (BM + wn * TN) * KB + at[s];
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) fw[s & 1][j] = *(const chunk*)(sw + j * 32 * KB);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fx[s & 1][i] = *(const chunk*)(sx + i * 32 * KB);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = Mat<T>::mma32(fw[s & 1][j], fx[s & 1][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    if constexpr (VEC) {
+        const int kbytes = a.K * ES, lowbytes = kParts<T> * a.r * ES;
+        const int ne = ad >= 0 ? (lowbytes + KB - 1) / KB : 0, nt = ne + nk;  // tiles of parts, tiles in all
+        const int64_t xspan = ((gather ? a.x_rows : (int64_t)pc.n) - 1) * a.ldx + a.K;
+        const v4i rx = buffer_of(xb, (uint32_t)(xspan * ES));
+        const v4i rw = buffer_of(wb, (uint32_t)(((int64_t)(rows_n - 1) * a.K + a.K) * ES));
+        v4i rl = rx, ru = rw;
+        if (KIND == kAdapters && ad >= 0) {
+            rl = buffer_of((const char*)a.low + (int64_t)pc.first * lowbytes, (uint32_t)(pc.n * lowbytes));
+            ru = buffer_of((const T*)a.up + ((int64_t)ad * a.N + n0) * a.r, (uint32_t)(rows_n * a.r * ES));
+        }
+        uint32_t off[NL];
+        int kc[NL];  // byte of k of the lane's chunk in tile 0
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int row = (i * NW + wave) * RPL + lane / CPR;
+            const bool isx = (i * NW + wave) * RPL < BM;  // (uniform over the wave)
+            const int rr = isx ? row : row - BM;
+            kc[i] = 16 * swizzle<CPR>(rr, lane % CPR);
+            if (isx) {
+                int64_t m = rr < pc.n ? rr : -1;
+                if (gather && rr < pc.n) m = row_in(a, pc.first + rr);
+                off[i] = m >= 0 ? (uint32_t)(m * a.ldx * ES) + kc[i] : kBehind;
+            } else {
+                off[i] = rr < rows_n ? (uint32_t)((int64_t)rr * a.K * ES) + kc[i] : kBehind;
+            }
+        }
+        const uint32_t base = lds_address(lds);
+        const auto fill = [&](int t, uint32_t place) {
+            if (KIND == kAdapters && t < ne) {
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const int row = (i * NW + wave) * RPL + lane / CPR;
+                    const bool isx = (i * NW + wave) * RPL < BM;
+                    const int rr = isx ? row : row - BM, b = t * KB + kc[i], rb = a.r * ES;
+                    const int ub = b >= 2 * rb ? b - 2 * rb : b >= rb ? b - rb : b;
+                    const bool there = b < lowbytes && rr < (isx ? pc.n : rows_n);
+                    const uint32_t o = !there ? kBehind : isx ? (uint32_t)(rr * lowbytes + b) : (uint32_t)(rr * rb + ub);
+                    buffer_to_lds(isx ? rl : ru, o, 0, base + place * kStage + (i * NW + wave) * 1024);
+                }
+                return;
+            }
+            const int tk = t - ne;
+            const bool whole = (tk + 1) * KB <= kbytes;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const uint32_t o = whole || tk * KB + kc[i] < kbytes ? off[i] : kBehind;
+                buffer_to_lds((i * NW + wave) * RPL < BM ? rx : rw, o, (uint32_t)(tk * KB), base + place * kStage + (i * NW + wave) * 1024);
+            }
+        };
+        // While one step's products are formed the next step's operands are read; before the last step of tile t all
+        // waves have its operands in registers, so its place takes tile t + NS.
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+            if (t < nt) fill(t, t);
+        if (NS - 1 < nt) landed_barrier<(NS - 1) * NL>();
+        else landed_barrier<0>();
+        operands(lds, 0);
+        uint32_t place = 0;
+        for (int t = 0; t < nt; ++t) {
+#pragma unroll
+            for (int s = 0; s + 1 < STEPS; ++s) {
+                operands(lds + place * kStage, s + 1);
+                multiply(s);
+            }
+            if (t + 1 < nt) {
+                if (t + NS - 1 < nt) landed_barrier<(NS - 2) * NL>();
+                else landed_barrier<0>();
+                if (t + NS < nt) fill(t + NS, place);
+                place = place + 1 == NS ? 0 : place + 1;
+                operands(lds + place * kStage, 0);
+            }
+            multiply(STEPS - 1);
+            if constexpr (KIND == kAdapters && __is_same(T, _Float16)) {
+                if (t + 1 == ne) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const int row = wm * TM + 32 * i + r;
+                        const float f = row < pc.n ? a.low_factor[pc.first + row] : 1.0f;
+#pragma unroll
+                        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[i][j][e] = acc[i][j][e] * f;
+                    }
+                }
+            }
+        }
+    } else {
+        for (int t = 0; t < nk; ++t) {
+            for (int e = tid; e < (BM + BN) * CPR; e += NT) {
+                const int row = e / CPR, c = e % CPR, k = t * KE + c * PER;
+                chunk v{};
+                if (row < BM) {
+                    if (from[row] >= 0) v = load_chunk_any<T>(xb + from[row] * a.ldx, k, a.K);
+                } else if (row - BM < rows_n) {
+                    v = load_chunk_any<T>(wb + (int64_t)(row - BM) * a.K, k, a.K);
+                }
+                *(chunk*)(lds + row * KB + 16 * swizzle<CPR>(row < BM ? row : row - BM, c)) = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                operands(lds, s);
+                multiply(s);
+            }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+
+    // Sums through LDS: 32 rows of the wave's TN columns at a time, in fp32.
+    constexpr int LD = TN + 4;
+    float* st = (float*)lds + wave * 32 * LD;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v4f v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] = acc[i][j][4 * e + q];
+                *(v4f*)(st + r * LD + 32 * j + 8 * e + 4 * (lane >> 5)) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int p = 0; p < NP; ++p) {
+            const int row = p * RPP + lane / LPR;
+            const int m = to[wm * TM + 32 * i + row];
+            const v4f u0 = *(const v4f*)(st + row * LD + 8 * (lane % LPR)), u1 = *(const v4f*)(st + row * LD + 8 * (lane % LPR) + 4);
+            if (m == -1 || left <= 0) continue;
+            if (KIND == kExperts && m < 0) {
+                zero8(a, -2 - m, nc, left);
+                continue;
+            }
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (q < 4 ? u0[q & 3] : u1[q & 3]) + bs[q];
+            if constexpr (KIND == kRowAdapters) add_low<T>(a, m, nc, left, v);
+            finish8(a, m, nc, left, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- few rows
+// 16 positions of a segment (kRowAdapters: 16 rows) by 16 NC columns a block, k shared out over the block's NW waves in steps
+// of 64 bytes, operands straight to registers; the waves' sums are added in wave order through LDS.
+template <class T, int NC, int NW, bool VEC, int KIND>
+__global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
+    typedef typename Mat<T>::chunk chunk;
+    typedef typename Mat<T>::acc16 acc16;
+    constexpr int PER = Mat<T>::kPer, U = 4 / NC < 1 ? 1 : 4 / NC;
+    __shared__ float red[NW][16][16 * NC + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const uint32_t id = a.id0 + blockIdx.x / a.tiles_n;
+    const int n0 = (int)(blockIdx.x % a.tiles_n) * 16 * NC;
+    Piece pc;
+    if constexpr (KIND == kRowAdapters) {
+        pc.first = (int)(id * 16);
+        pc.n = a.P - pc.first < 16 ? a.P - pc.first : 16;
+        pc.s = 0;
+    } else {
+        pc = piece_of<16>(a, id);
+    }
+    if (pc.n < 1) return;
+    const int t = threadIdx.x, row = t / (2 * NC), c = n0 + 8 * (t % (2 * NC));  // 8 outputs a thread
+    const int left = a.N - c < 8 ? a.N - c : 8;
+    const bool out = t < 32 * NC && row < pc.n && left > 0;
+    if (KIND == kExperts && pc.s < 0) {
+        if (a.fresh && out) zero8(a, pc.first + row, c, left);
+        return;
+    }
+    const int seg = KIND == kExperts ? pc.s : 0;
+    const T* wr[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        const int n = n0 + 16 * j + r;
+        wr[j] = (const T*)a.w + (int64_t)seg * a.w_next + (int64_t)(n < a.N ? n : a.N - 1) * a.K;
+    }
+    const int64_t m = KIND == kExperts ? row_in(a, pc.first + (r < pc.n ? r : pc.n - 1)) : pc.first + (r < pc.n ? r : pc.n - 1);
+    const T* xr = (const T*)a.x + (m < 0 ? 0 : m) * a.ldx;  // (an absent position's sums are not used)
+    const int place = !out ? -1 : KIND == kExperts ? row_out(a, pc.first + row) : pc.first + row;
+    const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
+    acc16 acc[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[j] = acc16{};
+    auto get = [&](const T* p, int k) -> chunk {
+        if constexpr (VEC) {
+            // (a chunk behind K reads the row's first one instead and counts as zeros)
+            const chunk v = *(const chunk*)(p + (k < a.K ? k : 0));
+            return k < a.K ? v : chunk{};
+        } else {
+            return load_chunk_any<T>(p, k, a.K);
+        }
+    };
+    for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
+        chunk fw[U][NC], fx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (4 * (s0 + u * NW) + g) * PER;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) fw[u][j] = get(wr[j], k);
+            fx[u] = get(xr, k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
+    __syncthreads();
+    if (place == -1) return;
+    if (KIND == kExperts && place < 0) {
+        zero8(a, -2 - place, c, left);
+        return;
+    }
+    float v[8];
+    bias8(a, seg, c, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) s = s + red[w][row][8 * (t % (2 * NC)) + q];
+        v[q] = s + v[q];
+    }
+    if constexpr (KIND == kRowAdapters) add_low<T>(a, place, c, left, v);
+    finish8(a, place, c, left, v);
+}
+
+// ------------------------------------------------------------------------------------------------- the adapters' first half
+// low[m][j] = scale[i] sum_k x[m][k] down[i][j][k], i the adapter of row m's segment, for 16 rows of a segment (a row, where each
+// row is a segment) and all r <= 16 NR of its values: x is read once. For grouped_tile_k's kAdapters (PARTS) as [m][part][r] in T, fp16's
+// multiplied by a power of two that brings the row's largest value to 2^14 .. 2^15 (low_factor: its inverse), which
+// neither overflows nor is lost below 2^-24; else as [m][r] in fp32, with each row's adapter.
+template <class T, int NR, int NW, bool VEC, bool PARTS>
+__global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
+    typedef typename Mat<T>::chunk chunk;
+    typedef typename Mat<T>::acc16 acc16;
+    constexpr int PER = Mat<T>::kPer, U = 4 / NR < 1 ? 1 : 4 / NR;
+    __shared__ float red[NW][16][16 * NR + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const uint32_t id = a.id0 + blockIdx.x;
+    Piece pc;
+    if (a.offsets) pc = piece_of<16>(a, id);
+    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id};
+    if (pc.n < 1) return;
+    const int ad = adapter_of(a, pc.s);
+    const int t = threadIdx.x, row = t >> 4, c = t & 15;
+    if (!PARTS && t < pc.n) a.row_adapter[pc.first + t] = ad;
+    if (ad < 0) return;  // (nothing reads its rows' low products)
+    const T* xr = (const T*)a.x + (int64_t)(pc.first + (r < pc.n ? r : pc.n - 1)) * a.ldx;
+    const T* wr[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int n = 16 * j + r;
+        wr[j] = (const T*)a.down + ((int64_t)ad * a.r + (n < a.r ? n : a.r - 1)) * a.K;
+    }
+    const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
+    acc16 acc[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) acc[j] = acc16{};
+    auto get = [&](const T* p, int k) -> chunk {
+        if constexpr (VEC) {
+            const chunk v = *(const chunk*)(p + (k < a.K ? k : 0));
+            return k < a.K ? v : chunk{};
+        } else {
+            return load_chunk_any<T>(p, k, a.K);
+        }
+    };
+    for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
+        chunk fw[U][NR], fx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (4 * (s0 + u * NW) + g) * PER;
+#pragma unroll
+            for (int j = 0; j < NR; ++j) fw[u][j] = get(wr[j], k);
+            fx[u] = get(xr, k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NR; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
+    __syncthreads();
+    if (t >= 256) return;
+    const float sc = a.scale ? a.scale[ad] : 1.0f;
+    const int m = pc.first + row;
+    float v[NR], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) s = s + red[w][row][16 * j + c];
+        v[j] = 16 * j + c < a.r ? s * sc : 0.0f;
+        top = __builtin_fmaxf(top, __builtin_fabsf(v[j]));
+    }
+    if constexpr (!PARTS) {
+        if (row >= pc.n) return;
+        float* h = (float*)a.low + (int64_t)m * a.r;
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+            if (16 * j + c < a.r) h[16 * j + c] = v[j];
+    } else {
+        float f = 1.0f;
+        if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 16));
+            const int e = (int)(f2u(top) >> 23);  // (0: zero or subnormal, 255: infinite)
+            const int up = 127 + 14 + 127 - e;    // exponent field of 2^14 / 2^(e - 127)
+            f = e == 255 || top == 0.0f ? 1.0f : u2f((uint32_t)(up > 247 ? 247 : up) << 23);
+            if (c == 0 && row < pc.n) a.low_factor[m] = 1.0f / f;
+        }
+        if (row >= pc.n) return;
+        T* h = (T*)a.low + (int64_t)m * kParts<T> * a.r;
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            float x = v[j] * f;
+            const bool ends = !(__builtin_fabsf(x) < 3.0e38f);  // (infinity less itself would be NaN)
+#pragma unroll
+            for (int p = 0; p < kParts<T>; ++p) {
+                const T y = (T)x;
+                if (16 * j + c < a.r) h[p * a.r + 16 * j + c] = y;
+                x = ends ? 0.0f : x - (float)y;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- launch
+template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC, int KIND>
+static int launch_grouped_tile(GroupArgs& a, hipStream_t s) {
+    constexpr int NW = WM * WN, RPL = 1024 / KB;
+    constexpr int kStage = VEC ? ((BM + BN) / RPL + NW - 1) / NW * NW * 1024 : (BM + BN) * KB, kOut = NW * 32 * (BN / WN + 4) * 4;
+    const int nk = (a.K * (int)sizeof(T) + KB - 1) / KB + (KIND == kAdapters ? (kParts<T> * a.r * (int)sizeof(T) + KB - 1) / KB : 0);
+    int bytes = kStage * (!VEC ? 1 : nk < NS ? nk : NS);
+    if (bytes < kOut) bytes = kOut;
+    a.tiles_n = (uint32_t)((a.N + BN - 1) / BN);
+    const uint32_t ids = KIND == kRowAdapters ? (uint32_t)(((int64_t)a.P + BM - 1) / BM) : piece_tiles(a.P, a.S, BM);
+    const uint32_t most = (uint32_t)(grid_blocks(64 * NW) / a.tiles_n);  // (N is at most 2^16 tiles of 64)
+    for (uint32_t i = 0; i < ids; i += most) {
+        a.id0 = i;
+        a.tiles = (ids - i < most ? ids - i : most) * a.tiles_n;
+        hipLaunchKernelGGL((grouped_tile_k<T, BM, BN, WM, WN, KB, NS, VEC, KIND>), dim3(a.tiles), dim3(64 * NW), bytes, s, a);
+        if (int e = check_launch("grouped_tile_k")) return e;
+        if (ids - i <= most) break;
+    }
+    return PMG_OK;
+}
+
+template <class T, int NC, int NW, bool VEC, int KIND>
+static int launch_grouped_rows(GroupArgs& a, hipStream_t s) {
+    a.tiles_n = (uint32_t)((a.N + 16 * NC - 1) / (16 * NC));
+    const uint32_t ids = KIND == kRowAdapters ? (uint32_t)(((int64_t)a.P + 15) / 16) : piece_tiles(a.P, a.S, 16);
+    const uint32_t most = (uint32_t)(grid_blocks(64 * NW) / a.tiles_n);
+    for (uint32_t i = 0; i < ids; i += most) {
+        a.id0 = i;
+        a.tiles = (ids - i < most ? ids - i : most) * a.tiles_n;
+        hipLaunchKernelGGL((grouped_rows_k<T, NC, NW, VEC, KIND>), dim3(a.tiles), dim3(64 * NW), 0, s, a);
+        if (int e = check_launch("grouped_rows_k")) return e;
+        if (ids - i <= most) break;
+    }
+    return PMG_OK;
+}
+
+template <class T, bool VEC, bool PARTS>
+static int launch_low(GroupArgs& a, hipStream_t s) {
+    const uint32_t ids = a.offsets ? piece_tiles(a.P, a.S, 16) : (uint32_t)a.P;
+    const uint32_t most = (uint32_t)grid_blocks(512);
+    for (uint32_t i = 0; i < ids; i += most) {
+        a.id0 = i;
+        const dim3 grid(ids - i < most ? ids - i : most);
+        if (a.r <= 16) hipLaunchKernelGGL((lora_low_k<T, 1, 8, VEC, PARTS>), grid, dim3(512), 0, s, a);
+        else if (a.r <= 32) hipLaunchKernelGGL((lora_low_k<T, 2, 8, VEC, PARTS>), grid, dim3(512), 0, s, a);
+        else if (a.r <= 64) hipLaunchKernelGGL((lora_low_k<T, 4, 4, VEC, PARTS>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((lora_low_k<T, 8, 4, VEC, PARTS>), grid, dim3(256), 0, s, a);
+        if (int e = check_launch("lora_low_k")) return e;
+        if (ids - i <= most) break;
+    }
+    return PMG_OK;
+}
+
+template <class T, bool VEC, int KIND>
+static int launch_tiles(GroupArgs& a, hipStream_t s) {
+    if constexpr (VEC && sizeof(T) < 4) {
+        const double k = (double)(((int64_t)a.K * (int)sizeof(T) + 127) / 128);
+        const double half = KIND == kRowAdapters ? 0.0 : 0.5 * (double)a.S;  // segments end inside a tile
+        const auto rounds = [&](int bm, int bn) {
+            const double t = ((double)a.P / bm + half) * ((a.N + bn - 1) / bn) / 256.0;
+            return t < 1.0 ? 1.0 : __builtin_ceil(t);
+        };
+        const double r = rounds(128, 128);
+        const double c[4] = {rounds(64, 64) * (0.24 * k + 0.6), rounds(128, 64) * (0.31 * k + 1.5),
+                             r > 2.0 ? r * (0.55 * k + 3.5) : (r < 2.0 ? 1.5 : r) * (0.36 * k + 4.7),
+                             rounds(256, 256) * (2.0 * k + 15.0)};
+        int best = 0;
+        for (int i = 1; i < 4; ++i)
+            if (c[i] < c[best]) best = i;
+        if (best == 1) return launch_grouped_tile<T, 128, 64, 4, 2, 128, 2, VEC, KIND>(a, s);
+        if (best == 2) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
+        if (best == 3) return launch_grouped_tile<T, 256, 256, 2, 4, 64, 4, VEC, KIND>(a, s);
+    }
+    return launch_grouped_tile<T, 64, 64, 2, 2, 128, 2, VEC, KIND>(a, s);
+}
+
+template <class T>
+int launch_experts(GroupArgs& a, bool vec, hipStream_t s) {
+    if ((int64_t)a.P <= 16 * a.S) return vec ? launch_grouped_rows<T, 1, 8, true, kExperts>(a, s) : launch_grouped_rows<T, 1, 4, false, kExperts>(a, s);
+    return vec ? launch_tiles<T, true, kExperts>(a, s) : launch_tiles<T, false, kExperts>(a, s);
+}
+
+template <class T>
+int launch_lora(GroupArgs& a, bool vec, bool by_segment, hipStream_t s) {
+    if (by_segment) {
+        if (int e = launch_low<T, true, true>(a, s)) return e;
+        return launch_tiles<T, true, kAdapters>(a, s);
+    }
+    if (int e = vec ? launch_low<T, true, false>(a, s) : launch_low<T, false, false>(a, s)) return e;
+    if (((int64_t)a.P + 15) / 16 * ((a.N + 15) / 16) <= 512)
+        return vec ? launch_grouped_rows<T, 1, 8, true, kRowAdapters>(a, s) : launch_grouped_rows<T, 1, 4, false, kRowAdapters>(a, s);
+    return vec ? launch_tiles<T, true, kRowAdapters>(a, s) : launch_tiles<T, false, kRowAdapters>(a, s);
+}
+
+}  // namespace pmg

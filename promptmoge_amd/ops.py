@@ -6,7 +6,7 @@ Inputs are validated here (device, dtype, shape, contiguity) before the C ABI va
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -22,6 +22,7 @@ __all__ = [
     "math_device", "gauge_poly",
     "nearest_fill",
     "linear", "linear_i8", "qk_norm_rope", "sparse_attention",
+    "group_norm", "route", "Routes", "grouped_linear", "combine", "lora_linear",
     "EPI_ACC", "EPI_Q", "EPI_R", "EPI_BIAS", "EPI_SILU", "EPI_RLN", "EPI_ROUT", "EPI_QLIN",
 ]
 
@@ -977,4 +978,264 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     ws_bytes = _entry("pmg_attention_workspace_bytes")(args)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _on(d, "pmg_attention", args, _ptr(ws), ws_bytes)
+    return out
+
+
+# ------------------------------------------------------------------------------------- (6) a conditional layer on rows
+def _act(act: str) -> int:
+    code = _lib.ACTS.get(act)
+    if code is None:
+        raise ValueError(f"act must be one of {sorted(_lib.ACTS)}, got {act!r}")
+    return code
+
+
+def _residual(residual: Optional[torch.Tensor], rows: int, N: int) -> Tuple[int, int]:
+    """The type and row stride of a (rows, N) residual (None: 0, 0)."""
+    if residual is None:
+        return 0, 0
+    rt, ldr = _floating(residual, "residual"), _rows(residual, "residual")
+    if residual.shape != (rows, N):
+        raise ValueError(f"residual must be ({rows}, {N}), got {tuple(residual.shape)}")
+    return rt, ldr
+
+
+def _result(out: Optional[torch.Tensor], out_dtype: Optional[torch.dtype], like: torch.Tensor, rows: int, N: int, same: str,
+            same_as: Optional[torch.Tensor], **others: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int, int]:
+    """The (rows, N) result, its type and its row stride: a new one, or `out`, which may be `same_as` (named `same`) itself but lie
+    on nothing else of the call."""
+    if out is None:
+        out = like.new_empty((rows, N), dtype=like.dtype if out_dtype is None else out_dtype)
+        return out, _floating(out, "out"), N
+    if out.shape != (rows, N):
+        raise ValueError(f"out must be ({rows}, {N}), got {tuple(out.shape)}")
+    if out_dtype is not None and out_dtype != out.dtype:
+        raise ValueError(f"out_dtype is {out_dtype}, out has {out.dtype}")
+    if same_as is not None and _overlap(out, same_as) and not (
+            out.data_ptr() == same_as.data_ptr() and out.dtype == same_as.dtype and out.stride() == same_as.stride()):
+        raise ValueError(f"out may be {same} itself, but not overlap it otherwise")
+    _apart(out, "out", **others)
+    return out, _floating(out, "out"), _rows(out, "out")
+
+
+def _workspace(entry: str, like: torch.Tensor, args: bytes) -> Tuple[Optional[torch.Tensor], int]:
+    n = _entry(entry)(args)
+    return (like.new_empty((n,), dtype=torch.uint8) if n else None), n
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+               offsets: Optional[torch.Tensor] = None, eps: float = 1e-5, act: str = "none",
+               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Group norm with channels last, then the activation: act((x - mean) / sqrt(var + eps) * weight + bias), mean and var over
+    a segment's rows and a group's C / groups channels (torch's GroupNorm on a frame's (C, rows)).
+
+    x: (M, C) fp32 / fp16 / bf16, C up to 4096 (rows may be strided); weight, bias: (C,) fp32; offsets: (S + 1,) int64, rising:
+    segment s holds the rows offsets[s] .. offsets[s + 1] - 1 (a batch's frames); without, all rows are one segment. act:
+    as for linear. Sums in 64 bits, one rounding, to out_dtype (default: out's, or x's). Rows of no segment are 0 in a new
+    result and left as they were in a given `out`, which may be x itself. Where offsets fall, what the rows get is
+    not said. Forward only."""
+    d = _one_gpu(x, weight, bias, offsets, out) if x is not None else -1
+    if d < 0:
+        d = _refuse("x", x=x, weight=weight, bias=bias, offsets=offsets, out=out)
+    ty, ldx = _floating(x, "x"), _rows(x, "x")
+    M, C_ = x.shape
+    if groups < 1 or C_ % groups or C_ < 1:
+        raise ValueError(f"{C_} channels are not a multiple of {groups} groups")
+    if weight is not None:
+        _vector(weight, "weight", C_)
+    if bias is not None:
+        _vector(bias, "bias", C_)
+    if offsets is not None:
+        _offsets(offsets, "offsets")
+    code = _act(act)
+    fresh = out is None
+    out, ot, ldo = _result(out, out_dtype, x, M, C_, "x", x, weight=weight, bias=bias, offsets=offsets)
+    args = _lib.GROUP_NORM_PACK.pack(ty, x.data_ptr(), ldx, M, C_, groups, _ptr(weight), _ptr(bias), _ptr(offsets),
+                                     1 if offsets is None else offsets.shape[0] - 1, eps, code, out.data_ptr(), ot, ldo, fresh)
+    ws, n = _workspace("pmg_group_norm_workspace_bytes", x, args)
+    _on(d, "pmg_group_norm", args, _ptr(ws), n)
+    return out
+
+
+class Routes(NamedTuple):
+    """Which experts the rows go to, and the tables that group the pairs m k + slot of a row and its slot by expert."""
+
+    weights: torch.Tensor  # (M, k) fp32: 0 for a slot without an expert
+    experts: torch.Tensor  # (M, k) int32: -1 for a slot without an expert
+    offsets: torch.Tensor  # (E + 1,) int64: expert e's pairs are pairs[offsets[e]:offsets[e + 1]]
+    pairs: torch.Tensor    # (M k,) int32: in the order of the experts, then their own; -1 from offsets[E] on
+    rows: torch.Tensor     # (M k,) int32: pairs // k
+
+
+def route(logits: torch.Tensor, k: int, *, score: str = "softmax", normalize: bool = False,
+          mask: Optional[torch.Tensor] = None) -> Routes:
+    """The k experts of largest logit of each row (equal ones: the lowest index first), their weights, and the pairs in the
+    order of the experts, for grouped_linear and combine:
+
+        r = route(logits, k)
+        h = grouped_linear(x, w_up, r.offsets, index=r.rows, act="gelu")
+        y = grouped_linear(h, w_down, r.offsets, out_index=r.pairs, out=h.new_empty((M * k, N)))
+        z = combine(y.view(M, k, N), r.weights, residual=x)
+
+    logits: (M, E) fp32 / fp16 / bf16 (rows may be strided), E up to 1024, k up to 32; score: "softmax" over the row's
+    logits, or "sigmoid"; normalize: the weights over the sum of the row's (0 where that is 0). An expert whose logit is -inf
+    or NaN is not chosen: the slot holds -1 and weight 0. So do the rows with 0 in mask, (M,) bool / uint8, whose pairs come
+    in no segment. Forward only."""
+    d = _one_gpu(logits, mask) if logits is not None else -1
+    if d < 0:
+        d = _refuse("logits", logits=logits, mask=mask)
+    ty, ld = _floating(logits, "logits"), _rows(logits, "logits")
+    M, E = logits.shape
+    if not 1 <= E <= 1024 or not 1 <= k <= min(E, 32):
+        raise ValueError(f"{k} of {E} experts: there may be 1 to 1024, and 1 to 32 a row")
+    code = _lib.SCORES.get(score)
+    if code is None:
+        raise ValueError(f"score must be one of {sorted(_lib.SCORES)}, got {score!r}")
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (M,) or not mask.is_contiguous()):
+        raise ValueError(f"mask must be a contiguous ({M},) bool or uint8 tensor")
+    weights = logits.new_empty((M, k), dtype=torch.float32)
+    tables = logits.new_empty((3 * M * k,), dtype=torch.int32)
+    offsets = logits.new_empty((E + 1,), dtype=torch.int64)
+    experts, pairs, rows = tables[:M * k].view(M, k), tables[M * k:2 * M * k], tables[2 * M * k:]
+    args = _lib.ROUTE_PACK.pack(ty, logits.data_ptr(), ld, M, E, k, code, bool(normalize), _ptr(mask), weights.data_ptr(),
+                                experts.data_ptr(), offsets.data_ptr(), pairs.data_ptr(), rows.data_ptr())
+    ws, n = _workspace("pmg_route_workspace_bytes", logits, args)
+    _on(d, "pmg_route", args, _ptr(ws), n)
+    return Routes(weights, experts, offsets, pairs, rows)
+
+
+def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                   index: Optional[torch.Tensor] = None, out_index: Optional[torch.Tensor] = None, act: str = "none",
+                   residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear with a matrix per segment: act(x w[s]^T + bias[s]) + residual for the rows of segment s (an expert's rows, or a
+    frame's).
+
+    x: (Mx, K) fp32 / fp16 / bf16 (rows may be strided); w: (S, N, K) of x's type; bias: (S, N) fp32; offsets: (S + 1,) int64,
+    rising: segment s holds the positions offsets[s] .. offsets[s + 1] - 1. Position p reads row index[p] of x (int32), or row p,
+    and gives row out_index[p] of the result (int32; needs `out`), or row p; residual is added row by row of the result. Sums in
+    fp32, one rounding, to out_dtype (default: out's, or x's).
+
+    Positions of no segment and those whose index lies outside the rows give nothing: their rows are 0 in a new result and
+    left as they were in a given `out`, which may be the residual itself. A row named by two positions of out_index gets
+    either's result. Where offsets fall, what the rows get is not said. Forward only."""
+    d = -1
+    if x is not None and w is not None and offsets is not None:
+        d = _one_gpu(x, w, offsets, bias, index, out_index, residual, out)
+    if d < 0:
+        d = _refuse("x w offsets", x=x, w=w, offsets=offsets, bias=bias, index=index, out_index=out_index,
+                    residual=residual, out=out)
+    ty, ldx = _floating(x, "x"), _rows(x, "x")
+    Mx, K = x.shape
+    if w.dtype != x.dtype:
+        raise ValueError(f"w must be {x.dtype}, got {w.dtype}")
+    if w.ndim != 3 or not w.is_contiguous():
+        raise ValueError("w must be a contiguous (S, N, K) tensor")
+    S, N, kw = w.shape
+    if kw != K:
+        raise ValueError(f"w expects {kw} input channels, x has {K}")
+    _offsets(offsets, "offsets")
+    if offsets.shape[0] != S + 1:
+        raise ValueError(f"offsets of {offsets.shape[0] - 1} segments, w of {S}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (S, N) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 ({S}, {N}) tensor")
+    P = Mx
+    if index is not None:
+        _index(index, "index")
+        P = index.shape[0]
+    rows = P
+    if out_index is not None:
+        _index(out_index, "out_index")
+        if out is None:
+            raise ValueError("out_index needs out")
+        if out_index.shape[0] != P:
+            raise ValueError(f"out_index must have {P} positions, got {out_index.shape[0]}")
+        if out.ndim == 2:
+            rows = out.shape[0]
+    code = _act(act)
+    rt, ldr = _residual(residual, rows, N)
+    fresh = out is None
+    out, ot, ldo = _result(out, out_dtype, x, rows, N, "residual", residual, x=x, w=w, offsets=offsets, bias=bias,
+                           index=index, out_index=out_index)
+    args = _lib.GROUPED_PACK.pack(ty, x.data_ptr(), ldx, Mx, w.data_ptr(), P, S, K, N, offsets.data_ptr(), _ptr(index),
+                                  _ptr(out_index), _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), ot, ldo, rows, fresh)
+    _on(d, "pmg_grouped_linear", args)
+    return out
+
+
+def combine(y: torch.Tensor, weights: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+            out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A row's experts put together: sum over the slots j of weights[m, j] y[m, j], plus residual[m], in fp32 and rounded once.
+
+    y: (M, k, N) fp32 / fp16 / bf16, N contiguous, k up to 32; weights: (M, k) fp32; residual: (M, N) of any of the three types. A
+    slot of weight 0 is not read: it may hold anything, as pairs without an expert do. `out` may be the residual itself.
+    Forward only."""
+    d = _one_gpu(y, weights, residual, out) if y is not None and weights is not None else -1
+    if d < 0:
+        d = _refuse("y weights", y=y, weights=weights, residual=residual, out=out)
+    ty = _floating(y, "y")
+    if y.ndim != 3 or (y.stride(2) != 1 and y.shape[2] > 1):
+        raise ValueError(f"y must be (rows, slots, N) with contiguous N, got {tuple(y.shape)}, strides {y.stride()}")
+    M, k, N = y.shape
+    if not 1 <= k <= 32:
+        raise ValueError(f"y must have 1 to 32 slots, got {k}")
+    if weights.dtype != torch.float32 or weights.shape != (M, k) or not weights.is_contiguous():
+        raise ValueError(f"weights must be a contiguous float32 ({M}, {k}) tensor")
+    rt, ldr = _residual(residual, M, N)
+    out, ot, ldo = _result(out, out_dtype, y, M, N, "residual", residual, y=y, weights=weights)
+    args = _lib.COMBINE_PACK.pack(ty, y.data_ptr(), y.stride(0), y.stride(1), M, k, N, weights.data_ptr(), _ptr(residual), rt, ldr,
+                                  out.data_ptr(), ot, ldo)
+    _on(d, "pmg_combine", args)
+    return out
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, down: torch.Tensor, up: torch.Tensor, adapter: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, *, offsets: Optional[torch.Tensor] = None,
+                scale: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear with a low-rank adapter per segment: act(x w^T + bias + scale[i] (x down[i]^T) up[i]^T) + residual, i = adapter[s] for
+    the rows of segment s. A batch's frames, each with the adapter of its sensor, share one projection.
+
+    x: (M, K) fp32 / fp16 / bf16 (rows may be strided); w: (N, K), down: (A, r, K), up: (A, N, r) of x's type, r up to 128;
+    adapter: (S,) int32, one outside 0 .. A - 1: none; scale: (A,) fp32; offsets: (S + 1,) int64, rising: segment s holds the rows
+    offsets[s] .. offsets[s + 1] - 1; without, S is M and every row is a segment. Rows of no segment have the projection alone.
+    x down^T is held to fp32's accuracy for the second product; sums in fp32, one rounding, to out_dtype (default: out's,
+    or x's). `out` may be the residual itself. Where offsets fall, what the rows get is not said. Forward only."""
+    d = -1
+    if x is not None and w is not None and down is not None and up is not None and adapter is not None:
+        d = _one_gpu(x, w, down, up, adapter, bias, offsets, scale, residual, out)
+    if d < 0:
+        d = _refuse("x w down up adapter", x=x, w=w, down=down, up=up, adapter=adapter, bias=bias, offsets=offsets,
+                    scale=scale, residual=residual, out=out)
+    ty, ldx = _floating(x, "x"), _rows(x, "x")
+    M, K = x.shape
+    if w.dtype != x.dtype or down.dtype != x.dtype or up.dtype != x.dtype:
+        raise ValueError(f"w, down and up must be {x.dtype}")
+    if w.ndim != 2 or w.shape[1] != K or not w.is_contiguous():
+        raise ValueError(f"w must be a contiguous (N, {K}) matrix, got {tuple(w.shape)}")
+    N = w.shape[0]
+    if down.ndim != 3 or down.shape[2] != K or not down.is_contiguous():
+        raise ValueError(f"down must be a contiguous (A, r, {K}) tensor, got {tuple(down.shape)}")
+    A, r = down.shape[:2]
+    if up.shape != (A, N, r) or not up.is_contiguous():
+        raise ValueError(f"up must be a contiguous ({A}, {N}, {r}) tensor, got {tuple(up.shape)}")
+    if not 1 <= r <= 128:
+        raise ValueError(f"adapters of rank 1 to 128, got {r}")
+    S = M
+    if offsets is not None:
+        _offsets(offsets, "offsets")
+        S = offsets.shape[0] - 1
+    if adapter.dtype != torch.int32 or adapter.shape != (S,) or not adapter.is_contiguous():
+        raise ValueError(f"adapter must be a contiguous int32 ({S},) tensor")
+    if bias is not None:
+        _vector(bias, "bias", N)
+    if scale is not None:
+        _vector(scale, "scale", A)
+    code = _act(act)
+    rt, ldr = _residual(residual, M, N)
+    out, ot, ldo = _result(out, out_dtype, x, M, N, "residual", residual, x=x, w=w, down=down, up=up, adapter=adapter, bias=bias,
+                           offsets=offsets, scale=scale)
+    args = _lib.LORA_PACK.pack(ty, x.data_ptr(), ldx, M, K, N, w.data_ptr(), down.data_ptr(), up.data_ptr(), r, A, _ptr(scale),
+                               adapter.data_ptr(), _ptr(offsets), S, _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), ot, ldo)
+    ws, n = _workspace("pmg_lora_linear_workspace_bytes", x, args)
+    _on(d, "pmg_lora_linear", args, _ptr(ws), n)
     return out
