@@ -39,45 +39,52 @@ __device__ inline float sigmoid_wide(float z) {
     return z < 0.0f ? e * r : r;
 }
 
+// act(y), WIDE: for fp32 outputs.
+template <int ACT, bool WIDE>
+__device__ inline float activated(float y) {
+    if constexpr (ACT == PMG_ACT_RELU) {
+        return y < 0.0f ? 0.0f : y;  // (NaN stays)
+    } else if constexpr (ACT == PMG_ACT_SILU) {
+        return WIDE ? y * sigmoid_wide(y) : silu_fast(y);
+    } else if constexpr (ACT == PMG_ACT_GELU) {
+        return WIDE ? 0.5f * y * (1.0f + erff(y * 0.70710678f)) : gelu_16(y);
+    } else if constexpr (ACT == PMG_ACT_GELU_TANH) {  // (1 + tanh(c u)) / 2 = 1 / (1 + exp(-2 c u)), c = sqrt(2 / pi)
+        constexpr float c2 = 2.0f * 0.7978845608f;
+        const float u = __builtin_fmaf(0.044715f * y * y, y, y);
+        return WIDE ? y * sigmoid_wide(u * c2) : y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * (-c2 * PMG_LOG2E)));
+    } else {
+        return y;
+    }
+}
+
+// f(constant of act): code for each activation of its own, chosen once.
+template <int ACT>
+struct ActOf {
+    static constexpr int value = ACT;
+};
+template <class F>
+__device__ inline void with_act(int act, const F& f) {
+    switch (act) {
+        case PMG_ACT_RELU: f(ActOf<PMG_ACT_RELU>{}); break;
+        case PMG_ACT_SILU: f(ActOf<PMG_ACT_SILU>{}); break;
+        case PMG_ACT_GELU: f(ActOf<PMG_ACT_GELU>{}); break;
+        case PMG_ACT_GELU_TANH: f(ActOf<PMG_ACT_GELU_TANH>{}); break;
+        default: f(ActOf<PMG_ACT_NONE>{}); break;
+    }
+}
+
 // act of 8 values in place; wide: for fp32 outputs.
 __device__ inline void activate8(float (&v)[8], int act, bool wide) {
-    switch (act) {
-        case PMG_ACT_RELU:
+    with_act(act, [&](auto one) {
+        constexpr int ACT = decltype(one)::value;
+        if (wide) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
-            break;
-        case PMG_ACT_SILU:
-            if (wide) {
+            for (int i = 0; i < 8; ++i) v[i] = activated<ACT, true>(v[i]);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * sigmoid_wide(v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = silu_fast(v[i]);
-            }
-            break;
-        case PMG_ACT_GELU:
-            if (wide) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = gelu_16(v[i]);
-            }
-            break;
-        case PMG_ACT_GELU_TANH: {  // (1 + tanh(c u)) / 2 = 1 / (1 + exp(-2 c u)), c = sqrt(2 / pi)
-            constexpr float c2 = 2.0f * 0.7978845608f;
-            const auto u = [](float y) { return __builtin_fmaf(0.044715f * y * y, y, y); };
-            if (wide) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * sigmoid_wide(u(v[i]) * c2);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u(v[i]) * (-c2 * PMG_LOG2E)));
-            }
-            break;
+            for (int i = 0; i < 8; ++i) v[i] = activated<ACT, false>(v[i]);
         }
-        default: break;
-    }
+    });
 }
 
 template <class E>
@@ -146,24 +153,32 @@ __device__ inline void numbers8(const Epilogue& a, const Raw8& r, float (&v)[8])
     }
 }
 
+// n <= 8 values of the residual's row m from column n0 on, as numbers.
+__device__ inline void residual8(const Epilogue& a, int64_t m, int n0, int n, float (&r)[8]) {
+    const int64_t o = m * a.ldr + n0;
+    if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
+    else if (a.res_type == PMG_TYPE_F16) load8((const _Float16*)a.res + o, n, a.vec_res, r);
+    else load8((const __bf16*)a.res + o, n, a.vec_res, r);
+}
+// n <= 8 finished values of row m from column n0 on, rounded and stored.
+__device__ inline void put8(const Epilogue& a, int64_t m, int n0, int n, const float (&v)[8]) {
+    const int64_t o = m * a.ldo + n0;
+    if (a.out_type == PMG_TYPE_F32) store8((float*)a.out + o, n, a.vec_out, v);
+    else if (a.out_type == PMG_TYPE_F16) store8((_Float16*)a.out + o, n, a.vec_out, v);
+    else store8((__bf16*)a.out + o, n, a.vec_out, v);
+}
 // n <= 8 outputs of row m from column n0 on: v holds scaled sums plus bias. `early`: the residual, if it is there already.
 __device__ inline void finish8(const Epilogue& a, int64_t m, int n0, int n, float (&v)[8], const Raw8* early = nullptr) {
     const bool wide = a.out_type == PMG_TYPE_F32;
     activate8(v, a.act, wide);
     if (a.res) {
         float r[8];
-        const int64_t o = m * a.ldr + n0;
         if (early) numbers8(a, *early, r);
-        else if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
-        else if (a.res_type == PMG_TYPE_F16) load8((const _Float16*)a.res + o, n, a.vec_res, r);
-        else load8((const __bf16*)a.res + o, n, a.vec_res, r);
+        else residual8(a, m, n0, n, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] + r[i];
     }
-    const int64_t o = m * a.ldo + n0;
-    if (a.out_type == PMG_TYPE_F32) store8((float*)a.out + o, n, a.vec_out, v);
-    else if (a.out_type == PMG_TYPE_F16) store8((_Float16*)a.out + o, n, a.vec_out, v);
-    else store8((__bf16*)a.out + o, n, a.vec_out, v);
+    put8(a, m, n0, n, v);
 }
 
 // 16 bytes of a row from element k on, element by element: zeros behind K (rows of any alignment).

@@ -2,18 +2,18 @@
 // with low-rank adapters (each segment has an adapter). Segment s of S holds the positions offsets[s] .. offsets[s + 1] - 1.
 #pragma once
 #include "pmg_epilogue.h"
+#include "pmg_pieces.h"
 
 namespace pmg {
 
-struct GroupArgs : Epilogue {
+struct GroupArgs : Epilogue, Pieces {  // (adapters may have no offsets: a row a segment)
     const void* x;            // [x_rows] rows of ldx
     const void* w;            // [N][K], the next segment's w_next elements on
     const float* bias;        // [N] or NULL, the next segment's b_next elements on
-    const int64_t* offsets;   // [S + 1]; adapters may have none: a row a segment
     const int32_t* index;     // row of x of each position, or NULL
     const int32_t* out_index; // row of the result of each position, or NULL
-    int64_t x_rows, out_rows, S, ldx, w_next, b_next;
-    int P, K, N;
+    int64_t x_rows, out_rows, ldx, w_next, b_next;
+    int K, N;
     int fresh;                // rows that no position names are set to 0
     // adapters: scale[i] (x down[i]^T) of each row, as the kernel that uses it reads it, then up [adapters][N][r]
     const void* low;
@@ -27,57 +27,14 @@ struct GroupArgs : Epilogue {
     uint32_t tiles_n, tiles, id0;
 };
 
-// Positions [0, P) fall into S + 2 pieces: those in front of segment 0, the segments, those behind the last. Piece j starts at
-// bound(j). Tiles of BM positions start where a piece starts; piece j's have the numbers bound(j) / BM + j and up, so that a
-// tile's piece is found without a sum over the pieces (a piece may have a number more than it has tiles): P / BM + S + 2 in all.
-__device__ inline int piece_bound(const GroupArgs& a, int64_t j) {
-    if (j <= 0) return 0;
-    if (j > a.S + 1) return a.P;
-    const int64_t o = a.offsets[j - 1];
-    return o < 0 ? 0 : o > a.P ? a.P : (int)o;
-}
-struct Piece {
-    int first, n, s;  // positions first .. first + n - 1 (n < 1: none) of segment s (-1: of none)
-};
-// A wave looks at 64 pieces at a time; all lanes return the same. Where offsets fall, some tile within [0, P).
-template <int BM>
-__device__ inline Piece piece_of(const GroupArgs& a, uint32_t id) {
-    const int lane = threadIdx.x & 63;
-    int64_t lo = 0, n = a.S + 2;
-    while (n > 1) {
-        const int64_t step = (n + 63) >> 6, c = lo + lane * step;
-        const bool in = lane * step < n && (int64_t)((uint32_t)piece_bound(a, c) / BM) + c <= (int64_t)id;
-        const uint64_t not_in = ~__ballot(in);
-        int64_t cnt = not_in ? __builtin_ctzll(not_in) : 64;
-        cnt = cnt < 1 ? 0 : cnt - 1;
-        lo += cnt * step;
-        n = n - cnt * step < step ? n - cnt * step : step;
-    }
-    const int p0 = piece_bound(a, lo), p1 = piece_bound(a, lo + 1);
-    const int64_t first = p0 + ((int64_t)id - ((int64_t)((uint32_t)p0 / BM) + lo)) * BM;
-    Piece p;
-    p.n = first < p0 || first >= p1 ? 0 : p1 - first < BM ? (int)(p1 - first) : BM;
-    p.first = p.n ? (int)first : 0;
-    p.s = lo >= 1 && lo <= a.S ? (int)(lo - 1) : -1;
-    p.first = __builtin_amdgcn_readfirstlane(p.first);
-    p.n = __builtin_amdgcn_readfirstlane(p.n);
-    p.s = __builtin_amdgcn_readfirstlane(p.s);
-    return p;
-}
-inline uint32_t piece_tiles(int64_t P, int64_t S, int BM) { return (uint32_t)(P / BM + S + 2); }
-
-// The row of x that position p reads, or -1 (absent).
-__device__ inline int64_t row_in(const GroupArgs& a, int p) {
-    if (!a.index) return p;
-    const int32_t i = a.index[p];
-    return i >= 0 && i < a.x_rows ? i : -1;
-}
-// Where position p's result goes: a row of the result, -1 (nowhere), or -2 - row: a row that is set to 0.
-__device__ inline int row_out(const GroupArgs& a, int p) {
-    const bool there = row_in(a, p) >= 0;
-    if (!a.out_index) return there ? p : a.fresh ? -2 - p : -1;
-    const int32_t o = a.out_index[p];
-    return there && o >= 0 && o < a.out_rows ? o : -1;
+// The row of x that position p reads (any value where there is none), and whether it is one.
+__device__ inline int row_in(const GroupArgs& a, int p) { return a.index ? a.index[p] : p; }
+__device__ inline bool in_x(const GroupArgs& a, int row) { return row >= 0 && row < a.x_rows; }
+// Where position p's result goes, `from` its row of x: a row of the result, -1 (nowhere), or -2 - row: a row that is set to 0.
+__device__ inline int row_out(const GroupArgs& a, int p, int from) {
+    const int o = a.out_index ? a.out_index[p] : p;
+    if (!a.out_index) return in_x(a, from) ? p : a.fresh ? -2 - p : -1;
+    return in_x(a, from) && o >= 0 && o < a.out_rows ? o : -1;
 }
 __device__ inline int adapter_of(const GroupArgs& a, int s) {
     if (s < 0) return -1;
@@ -87,9 +44,20 @@ __device__ inline int adapter_of(const GroupArgs& a, int s) {
 
 // Bias of columns n .. n + 7 of segment s (0 behind N).
 __device__ inline void bias8(const GroupArgs& a, int s, int n, float (&b)[8]) {
-    const float* p = a.bias ? a.bias + (int64_t)s * a.b_next : nullptr;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = p && n + i < a.N ? p[n + i] : 0.0f;
+    for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+    if (!a.bias) return;
+    const float* p = a.bias + (int64_t)s * a.b_next + n;
+    if (n + 8 <= a.N) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = p[i];
+    } else {
+        for (int i = 0; i < a.N - n; ++i) {
+            const float v = p[i];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) b[q] = q == i ? v : b[q];
+        }
+    }
 }
 
 // n <= 8 zeros in row m of the result from column n0 on.

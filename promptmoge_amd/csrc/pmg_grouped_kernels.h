@@ -36,7 +36,7 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
         pc.n = a.P - pc.first < BM ? a.P - pc.first : BM;
         pc.s = 0;
     } else {
-        pc = piece_of<BM>(a, id);
+        pc = piece_of(a, id, BM);
     }
     if (pc.n < 1) return;
     const int rows_n = a.N - n0 < BN ? a.N - n0 : BN;
@@ -56,9 +56,29 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
     const T* xb = (const T*)a.x + (gather ? 0 : (int64_t)pc.first * a.ldx);
     const T* wb = (const T*)a.w + (int64_t)seg * a.w_next + (int64_t)n0 * a.K;
     const int nk = (a.K + KE - 1) / KE;
-    for (int e = tid; e < BM; e += NT) {
-        to[e] = e >= pc.n ? -1 : KIND == kExperts ? row_out(a, pc.first + e) : pc.first + e;
-        if constexpr (!VEC) from[e] = e >= pc.n ? -1 : gather ? (int)row_in(a, pc.first + e) : e;
+    constexpr int LPR = TN / 8, RPP = 64 / LPR, NP = 32 / RPP;  // lanes a row, rows a pass, passes
+    const int nc = n0 + wn * TN + 8 * (lane % LPR);
+    const int left = a.N - nc < 8 ? a.N - nc : 8;
+    // All that the tile looks up in tables is asked for at once: the rows of the lane's loads, a row's place, the bias.
+    static_assert(BM <= NT, "a row's place a thread");
+    int rows[VEC ? NL : 1];
+    float bs[8];
+    if constexpr (VEC) {
+        const int last = pc.first + pc.n - 1;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int p = pc.first + (i * NW + wave) * RPL + lane / CPR;
+            rows[i] = gather ? a.index[p < last ? p : last] : p - pc.first;
+        }
+    }
+    {
+        const int p = pc.first + (tid < pc.n ? tid : 0), from_p = gather ? a.index[p] : p;
+        const int to_p = KIND == kExperts ? row_out(a, p, from_p) : p;
+        bias8(a, seg, nc, bs);
+        if (tid < BM) {
+            to[tid] = tid < pc.n ? to_p : -1;
+            if constexpr (!VEC) from[tid] = tid >= pc.n || !in_x(a, from_p) ? -1 : gather ? from_p : tid;
+        }
     }
     if constexpr (!VEC) __syncthreads();
 
@@ -72,11 +92,6 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
     int at[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) at[s] = r * KB + 16 * swizzle<CPR>(r, 2 * s + (lane >> 5));
-    constexpr int LPR = TN / 8, RPP = 64 / LPR, NP = 32 / RPP;  // lanes a row, rows a pass, passes
-    const int nc = n0 + wn * TN + 8 * (lane % LPR);
-    const int left = a.N - nc < 8 ? a.N - nc : 8;
-    float bs[8];
-    bias8(a, seg, nc, bs);
 
     chunk fx[2][MT], fw[2][NTL];
     const auto operands = [&](const char* st, int s) {  // step s of the tile at st
@@ -116,11 +131,10 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
             const int rr = isx ? row : row - BM;
             kc[i] = 16 * swizzle<CPR>(rr, lane % CPR);
             if (isx) {
-                int64_t m = rr < pc.n ? rr : -1;
-                if (gather && rr < pc.n) m = row_in(a, pc.first + rr);
-                off[i] = m >= 0 ? (uint32_t)(m * a.ldx * ES) + kc[i] : kBehind;
+                // (gathered: below 2 GiB; else a tile's rows are, of 4 MiB each)
+                off[i] = rr < pc.n && (!gather || in_x(a, rows[i])) ? (uint32_t)rows[i] * ((uint32_t)a.ldx * ES) + kc[i] : kBehind;
             } else {
-                off[i] = rr < rows_n ? (uint32_t)((int64_t)rr * a.K * ES) + kc[i] : kBehind;
+                off[i] = rr < rows_n ? (uint32_t)rr * ((uint32_t)a.K * ES) + kc[i] : kBehind;
             }
         }
         const uint32_t base = lds_address(lds);
@@ -206,9 +220,18 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
     }
     __syncthreads();
 
-    // Sums through LDS: 32 rows of the wave's TN columns at a time, in fp32.
+    // Sums through LDS: 32 rows of the wave's TN columns at a time, in fp32. The passes over them are a loop that loads nothing from
+    // memory, for a load would have the wave wait for the stores in front of it too (loads and stores share one counter);
+    // where a wave has 32 rows, their residuals are numbers in registers before the first store.
     constexpr int LD = TN + 4;
     float* st = (float*)lds + wave * 32 * LD;
+    const auto place = [&](int i, int p) { return left > 0 ? to[wm * TM + 32 * i + p * RPP + lane / LPR] : -1; };
+    const auto sums = [&](int p, float (&v)[8]) {
+        const float* from = st + (p * RPP + lane / LPR) * LD + 8 * (lane % LPR);
+        const v4f u0 = *(const v4f*)from, u1 = *(const v4f*)(from + 4);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (q < 4 ? u0[q & 3] : u1[q & 3]) + bs[q];
+    };
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -220,23 +243,40 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
                 for (int q = 0; q < 4; ++q) v[q] = acc[i][j][4 * e + q];
                 *(v4f*)(st + r * LD + 32 * j + 8 * e + 4 * (lane >> 5)) = v;
             }
+        float res[MT == 1 ? NP : 1][8];
+        if (MT == 1 && a.res) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int m = place(i, p);
+                if (m >= 0) residual8(a, m, nc, left, res[MT == 1 ? p : 0]);
+            }
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int p = 0; p < NP; ++p) {
-            const int row = p * RPP + lane / LPR;
-            const int m = to[wm * TM + 32 * i + row];
-            const v4f u0 = *(const v4f*)(st + row * LD + 8 * (lane % LPR)), u1 = *(const v4f*)(st + row * LD + 8 * (lane % LPR) + 4);
-            if (m == -1 || left <= 0) continue;
-            if (KIND == kExperts && m < 0) {
-                zero8(a, -2 - m, nc, left);
-                continue;
-            }
+        const auto pass = [&](int p, const float* add) {
+            const int m = place(i, p);
             float v[8];
+            sums(p, v);
+            if (m >= 0) {
+                if constexpr (KIND == kRowAdapters) add_low<T>(a, m, nc, left, v);
+                if (add) {
+                    activate8(v, a.act, a.out_type == PMG_TYPE_F32);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = (q < 4 ? u0[q & 3] : u1[q & 3]) + bs[q];
-            if constexpr (KIND == kRowAdapters) add_low<T>(a, m, nc, left, v);
-            finish8(a, m, nc, left, v);
+                    for (int q = 0; q < 8; ++q) v[q] = v[q] + add[q];
+                    put8(a, m, nc, left, v);
+                } else {
+                    finish8(a, m, nc, left, v);
+                }
+            } else if (KIND == kExperts && m < -1) {
+                zero8(a, -2 - m, nc, left);
+            }
+        };
+        if (MT == 1 && a.res) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) pass(p, res[MT == 1 ? p : 0]);
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < NP; ++p) pass(p, nullptr);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -246,11 +286,11 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
 // --------------------------------------------------------------------------------------------------------- few rows
 // 16 positions of a segment (kRowAdapters: 16 rows) by 16 NC columns a block, k shared out over the block's NW waves in steps
 // of 64 bytes, operands straight to registers; the waves' sums are added in wave order through LDS.
-template <class T, int NC, int NW, bool VEC, int KIND>
+template <class T, int NC, int U, int NW, bool VEC, int KIND>
 __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
     typedef typename Mat<T>::chunk chunk;
     typedef typename Mat<T>::acc16 acc16;
-    constexpr int PER = Mat<T>::kPer, U = 4 / NC < 1 ? 1 : 4 / NC;
+    constexpr int PER = Mat<T>::kPer;
     __shared__ float red[NW][16][16 * NC + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t id = a.id0 + blockIdx.x / a.tiles_n;
@@ -261,7 +301,7 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
         pc.n = a.P - pc.first < 16 ? a.P - pc.first : 16;
         pc.s = 0;
     } else {
-        pc = piece_of<16>(a, id);
+        pc = piece_of(a, id, 16);
     }
     if (pc.n < 1) return;
     const int t = threadIdx.x, row = t / (2 * NC), c = n0 + 8 * (t % (2 * NC));  // 8 outputs a thread
@@ -278,9 +318,12 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
         const int n = n0 + 16 * j + r;
         wr[j] = (const T*)a.w + (int64_t)seg * a.w_next + (int64_t)(n < a.N ? n : a.N - 1) * a.K;
     }
-    const int64_t m = KIND == kExperts ? row_in(a, pc.first + (r < pc.n ? r : pc.n - 1)) : pc.first + (r < pc.n ? r : pc.n - 1);
-    const T* xr = (const T*)a.x + (m < 0 ? 0 : m) * a.ldx;  // (an absent position's sums are not used)
-    const int place = !out ? -1 : KIND == kExperts ? row_out(a, pc.first + row) : pc.first + row;
+    const int p_in = pc.first + (r < pc.n ? r : pc.n - 1), p_out = pc.first + (out ? row : 0);
+    const int m = KIND == kExperts ? row_in(a, p_in) : p_in, m_out = KIND == kExperts ? row_in(a, p_out) : p_out;
+    const T* xr = (const T*)a.x + (int64_t)(KIND != kExperts || in_x(a, m) ? m : 0) * a.ldx;  // (an absent position's sums are not used)
+    const int place = !out ? -1 : KIND == kExperts ? row_out(a, p_out, m_out) : p_out;
+    float v[8];
+    bias8(a, seg, c < a.N ? c : 0, v);
     const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
     acc16 acc[NC];
 #pragma unroll
@@ -301,8 +344,9 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
             const int k = (4 * (s0 + u * NW) + g) * PER;
 #pragma unroll
             for (int j = 0; j < NC; ++j) fw[u][j] = get(wr[j], k);
-            fx[u] = get(xr, k);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) fx[u] = get(xr, (4 * (s0 + u * NW) + g) * PER);  // (w's rows are known before x's)
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -318,8 +362,6 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
         zero8(a, -2 - place, c, left);
         return;
     }
-    float v[8];
-    bias8(a, seg, c, v);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
         float s = 0.0f;
@@ -345,24 +387,11 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t id = a.id0 + blockIdx.x;
     Piece pc;
-    if (a.offsets) pc = piece_of<16>(a, id);
-    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id};
+    if (a.offsets) pc = piece_of(a, id, 16);
+    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id, (int)id, (int)id + 1, id};
     if (pc.n < 1) return;
-    const int ad = adapter_of(a, pc.s);
-    const int t = threadIdx.x, row = t >> 4, c = t & 15;
-    if (!PARTS && t < pc.n) a.row_adapter[pc.first + t] = ad;
-    if (ad < 0) return;  // (nothing reads its rows' low products)
     const T* xr = (const T*)a.x + (int64_t)(pc.first + (r < pc.n ? r : pc.n - 1)) * a.ldx;
-    const T* wr[NR];
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        const int n = 16 * j + r;
-        wr[j] = (const T*)a.down + ((int64_t)ad * a.r + (n < a.r ? n : a.r - 1)) * a.K;
-    }
     const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
-    acc16 acc[NR];
-#pragma unroll
-    for (int j = 0; j < NR; ++j) acc[j] = acc16{};
     auto get = [&](const T* p, int k) -> chunk {
         if constexpr (VEC) {
             const chunk v = *(const chunk*)(p + (k < a.K ? k : 0));
@@ -371,14 +400,34 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
             return load_chunk_any<T>(p, k, a.K);
         }
     };
+    chunk fx[U];  // (the first round's rows of x are on their way while the adapter is looked up)
+    const auto rows_of = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) fx[u] = get(xr, (4 * (s0 + u * NW) + g) * PER);
+    };
+    if (wave < nsteps) rows_of(wave);
+    const int ad = adapter_of(a, pc.s);
+    const int t = threadIdx.x, row = t >> 4, c = t & 15;
+    if (!PARTS && t < pc.n) a.row_adapter[pc.first + t] = ad;
+    if (ad < 0) return;  // (nothing reads its rows' low products)
+    const float sc = a.scale ? a.scale[ad] : 1.0f;
+    const T* wr[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int n = 16 * j + r;
+        wr[j] = (const T*)a.down + ((int64_t)ad * a.r + (n < a.r ? n : a.r - 1)) * a.K;
+    }
+    acc16 acc[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) acc[j] = acc16{};
     for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
-        chunk fw[U][NR], fx[U];
+        chunk fw[U][NR];
+        if (s0 != wave) rows_of(s0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (4 * (s0 + u * NW) + g) * PER;
 #pragma unroll
             for (int j = 0; j < NR; ++j) fw[u][j] = get(wr[j], k);
-            fx[u] = get(xr, k);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -391,7 +440,6 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
         for (int e = 0; e < 4; ++e) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
     __syncthreads();
     if (t >= 256) return;
-    const float sc = a.scale ? a.scale[ad] : 1.0f;
     const int m = pc.first + row;
     float v[NR], top = 0.0f;
 #pragma unroll
@@ -455,7 +503,7 @@ static int launch_grouped_tile(GroupArgs& a, hipStream_t s) {
     return PMG_OK;
 }
 
-template <class T, int NC, int NW, bool VEC, int KIND>
+template <class T, int NC, int U, int NW, bool VEC, int KIND>
 static int launch_grouped_rows(GroupArgs& a, hipStream_t s) {
     a.tiles_n = (uint32_t)((a.N + 16 * NC - 1) / (16 * NC));
     const uint32_t ids = KIND == kRowAdapters ? (uint32_t)(((int64_t)a.P + 15) / 16) : piece_tiles(a.P, a.S, 16);
@@ -463,7 +511,7 @@ static int launch_grouped_rows(GroupArgs& a, hipStream_t s) {
     for (uint32_t i = 0; i < ids; i += most) {
         a.id0 = i;
         a.tiles = (ids - i < most ? ids - i : most) * a.tiles_n;
-        hipLaunchKernelGGL((grouped_rows_k<T, NC, NW, VEC, KIND>), dim3(a.tiles), dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL((grouped_rows_k<T, NC, U, NW, VEC, KIND>), dim3(a.tiles), dim3(64 * NW), 0, s, a);
         if (int e = check_launch("grouped_rows_k")) return e;
         if (ids - i <= most) break;
     }
@@ -487,32 +535,44 @@ static int launch_low(GroupArgs& a, hipStream_t s) {
     return PMG_OK;
 }
 
+// 16-bit tiles, by what a CU's share of them costs, fitted to the times of 20 products (within 0.6 % of the best shape's by the mean,
+// 7 % at the most): k in units of 128 bytes, in microseconds. Measured, us, rows gathered, 8 experts (the last row 4):
+//                              64 x 64, 2 places   3 places   64 x 128   128 x 128   128 x 256
+//   300 x 1024 to 1024                9.2             9.3        9.8        12.8        20.5
+//   1000 x 1024 to 1024              12.7            11.3       13.4        14.0        21.9
+//   4800 x 1024 to 1024              26.2            27.8       22.0        21.6        24.6
+//   9600 x 1024 to 4096, gelu       179             186        157         130         123
+//   9600 x 4096 to 1024             129             135        106         106         120
+//   76800 x 128 to 512, gelu         50.5            54.8       42.9        42.3        41.4
+// and 600 x 4096 to 512 by 16 experts 33.9 with two places and 23.3 with three, whose loads are further ahead where a CU has few
+// blocks. A library's product of 9600 x 1024 by one matrix to 4096 without an epilogue takes 97. fp32, whose products are 16 times
+// as long, and rows of any alignment take 64 x 64.
 template <class T, bool VEC, int KIND>
 static int launch_tiles(GroupArgs& a, hipStream_t s) {
     if constexpr (VEC && sizeof(T) < 4) {
         const double k = (double)(((int64_t)a.K * (int)sizeof(T) + 127) / 128);
-        const double half = KIND == kRowAdapters ? 0.0 : 0.5 * (double)a.S;  // segments end inside a tile
-        const auto rounds = [&](int bm, int bn) {
-            const double t = ((double)a.P / bm + half) * ((a.N + bn - 1) / bn) / 256.0;
-            return t < 1.0 ? 1.0 : __builtin_ceil(t);
+        const double ends = KIND == kRowAdapters ? 0.0 : 0.5 * (double)a.S;  // segments end inside a tile
+        const auto rounds = [&](int bm, int bn, double least) {
+            const double q = ((double)a.P / bm + ends) * ((a.N + bn - 1) / bn) / 256.0, r = q < 6.0 ? __builtin_ceil(q) : q + 0.5;
+            return r < least ? least : r;
         };
-        const double r = rounds(128, 128);
-        const double c[4] = {rounds(64, 64) * (0.24 * k + 0.6), rounds(128, 64) * (0.31 * k + 1.5),
-                             r > 2.0 ? r * (0.55 * k + 3.5) : (r < 2.0 ? 1.5 : r) * (0.36 * k + 4.7),
-                             rounds(256, 256) * (2.0 * k + 15.0)};
+        const double c[5] = {3.9 + rounds(64, 64, 2.0) * (0.195 * k + 0.77), 2.9 + rounds(64, 64, 2.0) * (0.185 * k + 1.02),
+                             0.6 + rounds(64, 128, 2.0) * (0.257 * k + 2.06), 3.3 + rounds(128, 128, 1.0) * (0.495 * k + 2.87),
+                             5.1 + rounds(128, 256, 1.0) * (0.888 * k + 4.08)};
         int best = 0;
-        for (int i = 1; i < 4; ++i)
+        for (int i = 1; i < 5; ++i)
             if (c[i] < c[best]) best = i;
-        if (best == 1) return launch_grouped_tile<T, 128, 64, 4, 2, 128, 2, VEC, KIND>(a, s);
-        if (best == 2) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
-        if (best == 3) return launch_grouped_tile<T, 256, 256, 2, 4, 64, 4, VEC, KIND>(a, s);
+        if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 128, 3, VEC, KIND>(a, s);
+        if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
+        if (best == 3) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
+        if (best == 4) return launch_grouped_tile<T, 128, 256, 2, 4, 64, 3, VEC, KIND>(a, s);
     }
     return launch_grouped_tile<T, 64, 64, 2, 2, 128, 2, VEC, KIND>(a, s);
 }
 
 template <class T>
 int launch_experts(GroupArgs& a, bool vec, hipStream_t s) {
-    if ((int64_t)a.P <= 16 * a.S) return vec ? launch_grouped_rows<T, 1, 8, true, kExperts>(a, s) : launch_grouped_rows<T, 1, 4, false, kExperts>(a, s);
+    if ((int64_t)a.P <= 16 * a.S) return vec ? launch_grouped_rows<T, 2, 4, 4, true, kExperts>(a, s) : launch_grouped_rows<T, 1, 4, 4, false, kExperts>(a, s);
     return vec ? launch_tiles<T, true, kExperts>(a, s) : launch_tiles<T, false, kExperts>(a, s);
 }
 
@@ -524,7 +584,7 @@ int launch_lora(GroupArgs& a, bool vec, bool by_segment, hipStream_t s) {
     }
     if (int e = vec ? launch_low<T, true, false>(a, s) : launch_low<T, false, false>(a, s)) return e;
     if (((int64_t)a.P + 15) / 16 * ((a.N + 15) / 16) <= 512)
-        return vec ? launch_grouped_rows<T, 1, 8, true, kRowAdapters>(a, s) : launch_grouped_rows<T, 1, 4, false, kRowAdapters>(a, s);
+        return vec ? launch_grouped_rows<T, 1, 4, 8, true, kRowAdapters>(a, s) : launch_grouped_rows<T, 1, 4, 4, false, kRowAdapters>(a, s);
     return vec ? launch_tiles<T, true, kRowAdapters>(a, s) : launch_tiles<T, false, kRowAdapters>(a, s);
 }
 

@@ -5,107 +5,123 @@
 // accuracy where the mean is 10^4 times the spread (for fp32 inputs E[x^2] - mean^2 in 64 bits loses 2^-53 (mean / spread)^2).
 // The mean is subtracted in two fp32 parts.
 #include "pmg_epilogue.h"
+#include "pmg_pieces.h"
 
 namespace pmg {
 
-struct NormArgs : Epilogue {
+struct NormArgs : Epilogue, Pieces {
     const void* x;
     const float* weight;  // [C] or NULL
     const float* bias;
-    const int64_t* offsets;  // [S + 1], or NULL: one segment of all rows
-    double2* parts;          // [tile][G]: sums of x and x^2
-    int64_t ldx, S;
-    int M, C, G, gw, type;  // gw: channels a group
-    int slab, slabs;        // groups a block takes; blocks over the groups
-    int rows;               // a tile's rows
+    double2* parts;       // [G][ids]: sums of x and x^2 of each tile
+    int64_t ldx, ids;
+    int C, G, gw;         // gw: channels a group
+    int slab, slabs;      // groups a block takes; blocks over the groups
+    int rows;             // a tile's rows
     int vec_x, fresh;
     float eps;
-    uint32_t tiles, id0;
+    uint32_t id0;
 };
 
-// Pieces and the numbers of their tiles: as in the grouped products, those in front of segment 0, the segments, those behind the last.
-__device__ inline int norm_bound(const NormArgs& a, int64_t j) {
-    if (j <= 0) return 0;
-    if (j > a.S + 1) return a.M;
-    if (!a.offsets) return j == 1 ? 0 : a.M;
-    const int64_t o = a.offsets[j - 1];
-    return o < 0 ? 0 : o > a.M ? a.M : (int)o;
-}
-struct NormPiece {
-    int first, n, p0, p1, s;  // a tile's rows first .. first + n - 1 of the piece p0 .. p1; segment s (-1: of none)
-    uint32_t id0;             // number of the piece's first tile
-};
-__device__ inline NormPiece norm_piece(const NormArgs& a, uint32_t id, bool whole) {
-    const int lane = threadIdx.x & 63;
-    int64_t lo = 0;
-    if (whole) {
-        lo = id;
-    } else {
-        int64_t n = a.S + 2;
-        while (n > 1) {
-            const int64_t step = (n + 63) >> 6, c = lo + lane * step;
-            const bool in = lane * step < n && (int64_t)((uint32_t)norm_bound(a, c) / (uint32_t)a.rows) + c <= (int64_t)id;
-            const uint64_t not_in = ~__ballot(in);
-            int64_t cnt = not_in ? __builtin_ctzll(not_in) : 64;
-            cnt = cnt < 1 ? 0 : cnt - 1;
-            lo += cnt * step;
-            n = n - cnt * step < step ? n - cnt * step : step;
-        }
-    }
-    NormPiece p;
-    p.p0 = __builtin_amdgcn_readfirstlane(norm_bound(a, lo));
-    p.p1 = __builtin_amdgcn_readfirstlane(norm_bound(a, lo + 1));
-    p.s = __builtin_amdgcn_readfirstlane(lo >= 1 && lo <= a.S ? (int)(lo - 1) : -1);
-    p.id0 = whole ? id : __builtin_amdgcn_readfirstlane((uint32_t)p.p0 / (uint32_t)a.rows + (uint32_t)lo);
-    const int64_t first = whole ? p.p0 : p.p0 + (int64_t)(id - p.id0) * a.rows;
-    const int64_t end = whole || p.p1 - first < a.rows ? p.p1 : first + a.rows;
-    p.n = first < p.p0 || first >= p.p1 ? 0 : (int)(end - first);
-    p.first = p.n > 0 ? (int)first : 0;
-    return p;
-}
-
-template <class T>
-__device__ inline void get8(const NormArgs& a, int64_t m, int c, int n, float (&v)[8]) {
-    load8((const T*)a.x + m * a.ldx + c, n, a.vec_x, v);
-}
-
-constexpr int kNormThreads = 512;
 
 struct Stat {
     float hi, lo, r;  // mean in two parts, 1 / spread
 };
 
+// 8 values of a row as they lie in memory (16-bit types: the first half), and as numbers.
+template <class T, bool VEC>
+__device__ inline Raw8 norm_get(const NormArgs& a, int64_t m, int c, int n) {
+    const T* p = (const T*)a.x + m * a.ldx + c;
+    Raw8 r{};
+    if (VEC || (a.vec_x && n == 8)) {
+        r.a = *(const uint4*)p;
+        if constexpr (sizeof(T) == 4) r.b = *(const uint4*)(p + 4);
+    } else {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+        __builtin_memcpy(&r, v, sizeof(v));
+    }
+    return r;
+}
+template <class T>
+__device__ inline void norm_numbers(const Raw8& r, float (&v)[8]) {
+    typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int C = 16 / sizeof(T);
+    const vec_t x = __builtin_bit_cast(vec_t, r.a), y = __builtin_bit_cast(vec_t, r.b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)(i < C ? x[i % C] : y[i % C]);
+}
+
 // A block's slab of whole groups (8 channels a thread, `wide` threads a row) of a tile's rows. WHOLE: a tile is a segment, sums
-// and results in one launch; else SUMS writes the tile's sums, and without it the segment's are added up (in the order of its
-// tiles) and applied.
-template <class T, bool WHOLE, bool SUMS>
-__global__ __launch_bounds__(kNormThreads) void norm_k(NormArgs a) {
-    __shared__ double red[kNormThreads * 8];
+// and results in one launch; else SUMS writes the tile's sums, and without it the segment's are added up (in an order that only
+// their number sets) and applied, behind the loads of the block's first rows.
+template <class T, class O, int NT, bool WHOLE, bool SUMS>
+__global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
+    __shared__ double red[SUMS ? NT * 8 : 1];
     __shared__ Stat stats[64];  // (a slab has at most 64 groups)
-    double2 total{0.0, 0.0};
+    // Rows a thread has under way twice. The loops over whole rounds of rows have neither conditional loads nor conditional stores:
+    // loads and stores share one counter, and where the compiler cannot count them it waits for all of them (307,200 rows: 22 us the
+    // second launch).
+    constexpr int U = SUMS && !WHOLE ? 4 : 2;
     const int tid = threadIdx.x;
     const int slab = (int)(blockIdx.x % (uint32_t)a.slabs);
     const uint32_t id = a.id0 + blockIdx.x / (uint32_t)a.slabs;
-    const NormPiece p = norm_piece(a, id, WHOLE);
+    Piece p;
+    if constexpr (WHOLE) {
+        p.p0 = a.bound(id);
+        p.p1 = a.bound((int64_t)id + 1);
+        p.first = p.p0;
+        p.n = p.p1 - p.p0;
+        p.s = id >= 1 && (int64_t)id <= a.S ? (int)(id - 1) : -1;
+    } else {
+        p = piece_of(a, id, a.rows);
+    }
     if (p.n < 1) return;
-    if (p.s < 0 && (SUMS ? !WHOLE || !a.fresh : !a.fresh)) return;
+    if (p.s < 0 && ((SUMS && !WHOLE) || !a.fresh)) return;
     const int g0 = slab * a.slab, ng = a.G - g0 < a.slab ? a.G - g0 : a.slab;
     const int c0 = g0 * a.gw, width = ng * a.gw, wide = (width + 7) / 8;
-    const int tx = tid % wide, ty = tid / wide, deep = kNormThreads / wide;  // (threads behind the last whole row: ty == deep, idle)
+    const int tx = tid % wide, ty = tid / wide, deep = NT / wide;  // (threads behind the last whole row: ty == deep, idle)
     const int c = c0 + 8 * tx, n = c0 + width - c < 8 ? c0 + width - c : 8;
     const bool busy = ty < deep;
     if (p.s < 0) {
         const float z[8] = {};
         for (int r = ty; busy && r < p.n; r += deep) {
             const int64_t o = (int64_t)(p.first + r) * a.ldo + c;
-            if (a.out_type == PMG_TYPE_F32) store8((float*)a.out + o, n, a.vec_out, z);
-            else store8((_Float16*)a.out + o, n, a.vec_out, z);
+            store8((O*)a.out + o, n, a.vec_out, z);
         }
         return;
     }
+    const int full = p.n / deep, rounds = full / U;  // rows that every thread has; rounds of U of them
+    const auto row = [&](int j) { return (int64_t)p.first + ty + (j < full ? j : full - 1) * deep; };
+    Raw8 now[U], next[U];
+    float weight[8], shift[8];
+    if constexpr (!SUMS || WHOLE) {
+        const float* w = a.weight && busy ? a.weight + c : nullptr;
+        const float* b = a.bias && busy ? a.bias + c : nullptr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight[i] = 1.0f, shift[i] = 0.0f;
+        if (w)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) weight[i] = w[i < n ? i : n - 1];
+        if (b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) shift[i] = b[i < n ? i : n - 1];
+    }
+    const bool quick = busy && rounds && a.vec_x && a.vec_out && n == 8;
+    const auto start = [&] {
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = norm_get<T, true>(a, row(u), c, 8);
+    };
+    if (!SUMS && quick) start();
+    // `per` lanes of a wave share a group's sums
+    const int per = ng <= NT / 64 ? 64 : ng <= NT / 32 ? 32 : ng <= NT / 16 ? 16 : 8, g = tid / per, l = tid % per;
+    double2 t{0.0, 0.0};
     if constexpr (SUMS) {
         double s[8] = {}, q[8] = {};
-        const auto add = [&](const float (&v)[8]) {
+        const auto add = [&](const Raw8& raw) {
+            float v[8];
+            norm_numbers<T>(raw, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const double d = (double)v[i];
@@ -113,120 +129,149 @@ __global__ __launch_bounds__(kNormThreads) void norm_k(NormArgs a) {
                 q[i] = __builtin_fma(d, d, q[i]);
             }
         };
-        if (busy) {
-            int r = ty;
-            for (; r + 3 * deep < p.n; r += 4 * deep) {
-                float v[4][8];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) get8<T>(a, p.first + r + u * deep, c, n, v[u]);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) add(v[u]);
-            }
-            for (; r < p.n; r += deep) {
-                float v[8];
-                get8<T>(a, p.first + r, c, n, v);
-                add(v);
-            }
-        }
-        // over the block's rows, then over a group's channels
-        double2 t{0.0, 0.0};
+        int r = ty;
+        if (quick) {
+            start();
 #pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-            if (busy)
+            for (int j = 0; j < rounds; ++j) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) red[(ty * wide + tx) * 8 + i] = k ? q[i] : s[i];
-            __syncthreads();
-            double col[8];
+                for (int u = 0; u < U; ++u) next[u] = norm_get<T, true>(a, row((j + 1) * U + u), c, 8);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = tid + i * kNormThreads;
-                col[i] = 0.0;
-                if (e < 8 * wide)
-                    for (int y = 0; y < deep; ++y) col[i] += red[y * wide * 8 + e];
+                for (int u = 0; u < U; ++u) add(now[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u) now[u] = next[u];
+            }
+            r += rounds * U * deep;
+        }
+        if (busy)
+#pragma unroll 1
+            for (; r < p.n; r += deep) add(norm_get<T, false>(a, p.first + r, c, n));
+        // The threads' sums of each group: where 8 channels lie in one group (or two), a value a thread and group, else one a channel.
+        const int fold = a.gw % 8 == 0 ? 1 : a.gw == 4 ? 2 : 0;
+        if (fold) {
+            double2* f = (double2*)red;
+            const double s0 = (s[0] + s[1]) + (s[2] + s[3]), s1 = (s[4] + s[5]) + (s[6] + s[7]);
+            const double q0 = (q[0] + q[1]) + (q[2] + q[3]), q1 = (q[4] + q[5]) + (q[6] + q[7]);
+            if (fold == 1) {
+                f[tid] = double2{s0 + s1, q0 + q1};
+            } else {
+                f[2 * tid] = double2{s0, q0};
+                f[2 * tid + 1] = double2{s1, q1};
             }
             __syncthreads();
+            const int cw = fold == 1 ? a.gw / 8 : 1, all = deep * cw;  // values a row and group; a group's
+            if (g < ng)
+                for (int e = l; e < all; e += per) {
+                    const int y = e / cw, x = e - y * cw;
+                    const double2 v = fold == 1 ? f[y * wide + g * cw + x] : f[y * 2 * wide + g];
+                    t.x += v.x;
+                    t.y += v.y;
+                }
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+                if (busy)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (tid + i * kNormThreads < 8 * wide) red[tid + i * kNormThreads] = col[i];
-            __syncthreads();
-            if (tid < ng) {
+                    for (int i = 0; i < 8; ++i) red[(ty * wide + tx) * 8 + i] = k ? q[i] : s[i];
+                __syncthreads();
                 double sum = 0.0;
-                for (int e = tid * a.gw; e < (tid + 1) * a.gw; ++e) sum += red[e];
+                if (g < ng)
+                    for (int e = l; e < deep * a.gw; e += per) {
+                        const int y = e / a.gw;
+                        sum += red[y * wide * 8 + g * a.gw + (e - y * a.gw)];
+                    }
                 if (k) t.y = sum;
                 else t.x = sum;
+                __syncthreads();
             }
-            __syncthreads();
         }
-        if constexpr (!WHOLE) {
-            if (tid < ng) a.parts[(int64_t)id * a.G + g0 + tid] = t;
-            return;
-        }
-        total = t;
     } else {
-        // the sums of the segment's tiles, shared out over the threads and added in order
-        const uint32_t tiles = (uint32_t)(p.p1 - p.p0 + a.rows - 1) / (uint32_t)a.rows;
-        const int of = kNormThreads / ng, part = tid / ng, g = tid % ng;
-        double2 t{0.0, 0.0};
-        if (part < of) {
-            for (uint32_t i = part; i < tiles; i += of) {
-                const double2 v = a.parts[(int64_t)(p.id0 + i) * a.G + g0 + g];
-                t.x += v.x;
-                t.y += v.y;
+        const int tiles = (int)((uint32_t)(p.p1 - p.p0 + a.rows - 1) / (uint32_t)a.rows);
+        if (g < ng) {
+            const double2* v = a.parts + (int64_t)(g0 + g) * a.ids + p.id0;
+            for (int i = l; i < tiles; i += 8 * per) {  // (eight on their way at a time)
+                double2 u[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) u[k] = v[i + k * per < tiles ? i + k * per : tiles - 1];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bool in = i + k * per < tiles;
+                    t.x += in ? u[k].x : 0.0;
+                    t.y += in ? u[k].y : 0.0;
+                }
             }
-            red[part * ng + g] = t.x;
-            red[kNormThreads + part * ng + g] = t.y;
+        }
+    }
+    for (int o = 1; o < per; o <<= 1) {
+        t.x += __shfl_xor(t.x, o, 64);
+        t.y += __shfl_xor(t.y, o, 64);
+    }
+    if constexpr (SUMS && !WHOLE) {
+        if (g < ng && l == 0) a.parts[(int64_t)(g0 + g) * a.ids + id] = t;
+        return;
+    } else {
+        if (g < ng && l == 0) {
+            // (quotient and root by one step of Newton each on the unit's values, to 2^-40 and better: a few instructions, where the
+            // library's take a kilobyte of code)
+            const double count = (double)(p.p1 - p.p0) * (double)a.gw;
+            double one = __builtin_amdgcn_rcp(count);
+            one = __builtin_fma(__builtin_fma(-count, one, 1.0), one, one);
+            one = __builtin_fma(__builtin_fma(-count, one, 1.0), one, one);
+            const double mean = t.x * one;
+            double var = t.y * one - mean * mean;
+            var = (var < 0.0 ? 0.0 : var) + (double)a.eps;  // (NaN stays)
+            double r = __builtin_amdgcn_rsq(var);
+            r = r * __builtin_fma(-0.5 * var * r, r, 1.5);
+            Stat st;
+            st.hi = (float)mean;
+            st.lo = (float)(mean - (double)st.hi);
+            st.r = (float)r;
+            stats[g] = st;
         }
         __syncthreads();
-        if (tid < ng)
-            for (int i = 0; i < of; ++i) {
-                total.x += red[i * ng + tid];
-                total.y += red[kNormThreads + i * ng + tid];
+        if (!busy) return;
+        // per channel: x less the mean (two parts), times scale, plus shift
+        float hi[8], lo[8], scale[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Stat st = stats[(c - c0 + (i < n ? i : n - 1)) / a.gw];
+            hi[i] = st.hi;
+            lo[i] = st.lo;
+            scale[i] = st.r * weight[i];
+        }
+        // (a loop for each activation, short: what a block has to fetch of its code for the first time costs it a microsecond a
+        // few KB)
+        with_act(a.act, [&](auto one) {
+            const auto result = [&](const Raw8& raw, float (&v)[8]) {
+                norm_numbers<T>(raw, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<decltype(one)::value, sizeof(O) == 4>(__builtin_fmaf((v[i] - hi[i]) - lo[i], scale[i], shift[i]));
+            };
+            int r = ty;
+            if (quick) {
+                if constexpr (SUMS) start();
+#pragma unroll 1
+                for (int j = 0; j < rounds; ++j) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) next[u] = norm_get<T, true>(a, row((j + 1) * U + u), c, 8);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        float v[8];
+                        result(now[u], v);
+                        store8((O*)a.out + row(j * U + u) * a.ldo + c, 8, true, v);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) now[u] = next[u];
+                }
+                r += rounds * U * deep;
             }
-    }
-    if (tid < ng) {
-        const double count = (double)(p.p1 - p.p0) * (double)a.gw, mean = total.x / count;
-        double var = total.y / count - mean * mean;
-        var = var < 0.0 ? 0.0 : var;  // (NaN stays)
-        Stat t;
-        t.hi = (float)mean;
-        t.lo = (float)(mean - (double)t.hi);
-        t.r = (float)(1.0 / __builtin_sqrt(var + (double)a.eps));
-        stats[tid] = t;
-    }
-    __syncthreads();
-    if (!busy) return;
-    // per channel: x less the mean (two parts), times scale, plus shift
-    float hi[8], lo[8], scale[8], shift[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int ch = c + (i < n ? i : n - 1);
-        const Stat t = stats[(ch - c0) / a.gw];
-        hi[i] = t.hi;
-        lo[i] = t.lo;
-        scale[i] = a.weight ? t.r * a.weight[ch] : t.r;
-        shift[i] = a.bias ? a.bias[ch] : 0.0f;
-    }
-    const auto apply = [&](int64_t m, float (&v)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf((v[i] - hi[i]) - lo[i], scale[i], shift[i]);
-        activate8(v, a.act, a.out_type == PMG_TYPE_F32);
-        const int64_t o = m * a.ldo + c;
-        if (a.out_type == PMG_TYPE_F32) store8((float*)a.out + o, n, a.vec_out, v);
-        else if (a.out_type == PMG_TYPE_F16) store8((_Float16*)a.out + o, n, a.vec_out, v);
-        else store8((__bf16*)a.out + o, n, a.vec_out, v);
-    };
-    int r = ty;
-    for (; r + 3 * deep < p.n; r += 4 * deep) {
-        float v[4][8];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) get8<T>(a, p.first + r + u * deep, c, n, v[u]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) apply(p.first + r + u * deep, v[u]);
-    }
-    for (; r < p.n; r += deep) {
-        float v[8];
-        get8<T>(a, p.first + r, c, n, v);
-        apply(p.first + r, v);
+#pragma unroll 1
+            for (; r < p.n; r += deep) {
+                float v[8];
+                result(norm_get<T, false>(a, p.first + r, c, n), v);
+                store8((O*)a.out + (int64_t)(p.first + r) * a.ldo + c, n, a.vec_out, v);
+            }
+        });
     }
 }
 
@@ -248,28 +293,37 @@ static NormPlan norm_plan(const pmg_group_norm_args& q) {
     p.ids = q.segments + 2;
     const double mean = (double)q.M / (double)(q.segments > 0 ? q.segments : 1);
     if (mean > 512.0) {
-        const int64_t want = (512 + p.slabs - 1) / p.slabs;  // tiles, for about two blocks a CU
-        p.rows = (int)((q.M + want - 1) / want);
+        const int64_t want = 256 / p.slabs - q.segments;  // (a segment ends inside a tile)
+        p.rows = (int)((q.M + (want > 1 ? want : 1) - 1) / (want > 1 ? want : 1));
         if (p.rows < 64) p.rows = 64;
-        p.ids = q.M / p.rows + q.segments + 2;
+        if (p.rows > mean) p.rows = (int)mean;
+        p.ids = piece_tiles(q.M, q.segments, p.rows);
     }
     return p;
 }
 
-template <class T>
-static int launch_norm(NormArgs& a, const NormPlan& pl, hipStream_t s) {
-    const int64_t most = grid_blocks(kNormThreads) / pl.slabs;
-    for (int sums = pl.rows ? 1 : 0; sums >= 0; --sums) {
-        for (int64_t i = 0; i < pl.ids; i += most) {
-            a.id0 = (uint32_t)i;
-            const dim3 grid((uint32_t)((pl.ids - i < most ? pl.ids - i : most) * pl.slabs));
-            if (!pl.rows) hipLaunchKernelGGL((norm_k<T, true, true>), grid, dim3(kNormThreads), 0, s, a);
-            else if (sums) hipLaunchKernelGGL((norm_k<T, false, true>), grid, dim3(kNormThreads), 0, s, a);
-            else hipLaunchKernelGGL((norm_k<T, false, false>), grid, dim3(kNormThreads), 0, s, a);
-            if (int e = check_launch("norm_k")) return e;
-        }
+template <class T, class O, int NT, bool WHOLE, bool SUMS>
+static int launch_norm_k(NormArgs& a, const NormPlan& pl, hipStream_t s) {
+    const int64_t most = grid_blocks(NT) / pl.slabs;
+    for (int64_t i = 0; i < pl.ids; i += most) {
+        a.id0 = (uint32_t)i;
+        const dim3 grid((uint32_t)((pl.ids - i < most ? pl.ids - i : most) * pl.slabs));
+        hipLaunchKernelGGL((norm_k<T, O, NT, WHOLE, SUMS>), grid, dim3(NT), 0, s, a);
+        if (int e = check_launch("norm_k")) return e;
     }
     return PMG_OK;
+}
+template <class T, class O>
+static int launch_norm_to(NormArgs& a, const NormPlan& pl, hipStream_t s) {
+    return pl.rows ? launch_norm_k<T, O, 1024, false, false>(a, pl, s) : launch_norm_k<T, O, 512, true, true>(a, pl, s);
+}
+template <class T>
+static int launch_norm(NormArgs& a, const NormPlan& pl, hipStream_t s) {
+    if (pl.rows)
+        if (int e = launch_norm_k<T, T, 1024, false, true>(a, pl, s)) return e;
+    if (a.out_type == PMG_TYPE_F32) return launch_norm_to<T, float>(a, pl, s);
+    if (a.out_type == PMG_TYPE_F16) return launch_norm_to<T, _Float16>(a, pl, s);
+    return launch_norm_to<T, __bf16>(a, pl, s);
 }
 
 }  // namespace pmg
@@ -309,11 +363,11 @@ extern "C" int pmg_group_norm(const pmg_group_norm_args* p, void* workspace, siz
     NormArgs a{};
     a.x = q.x;
     a.ldx = q.ldx;
-    a.M = (int)q.M;
+    a.P = (int)q.M;
+    a.ids = pl.ids;
     a.C = q.C;
     a.G = q.groups;
     a.gw = q.C / q.groups;
-    a.type = q.type;
     a.weight = q.weight;
     a.bias = q.bias;
     a.offsets = q.offsets;

@@ -1,0 +1,61 @@
+// Segments of positions, found by the blocks themselves (the offsets are on the device).
+#pragma once
+#include "pmg_common.h"
+
+namespace pmg {
+
+// Positions [0, P) fall into S + 2 pieces: those in front of segment 0, the segments, those behind the last. Tiles of `rows`
+// positions start where a piece starts; piece j's have the numbers bound(j) / rows + j and up, so that a tile's piece is found
+// without a sum over the pieces (a piece may have a number more than it has tiles): P / rows + S + 2 in all.
+struct Pieces {
+    const int64_t* offsets;  // [S + 1], or NULL: one segment of all positions (S = 1)
+    int64_t S;
+    int P;
+    __device__ inline int bound(int64_t j) const {
+        if (j <= 0) return 0;
+        if (j > S + 1) return P;
+        if (!offsets) return j == 1 ? 0 : P;
+        const int64_t o = offsets[j - 1];
+        return o < 0 ? 0 : o > P ? P : (int)o;
+    }
+};
+inline uint32_t piece_tiles(int64_t P, int64_t S, int rows) { return (uint32_t)(P / rows + S + 2); }
+
+struct Piece {
+    int first, n;  // positions first .. first + n - 1 (n < 1: none)
+    int s;         // of segment s (-1: of none)
+    int p0, p1;    // which holds p0 .. p1 - 1
+    uint32_t id0;  // and whose tiles have the numbers from id0 on
+};
+// The positions of tile `id`; all lanes of a wave return the same. A wave looks at 64 pieces at a time. Where offsets fall, some tile
+// within [0, P).
+__device__ inline Piece piece_of(const Pieces& a, uint32_t id, int rows) {
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, n = a.S + 2;
+    int here = 0;  // the lane's piece's bound, in the last round
+    int64_t cnt = 0;
+    for (;;) {
+        const int64_t step = (n + 63) >> 6, c = lo + lane * step;
+        here = a.bound(c);
+        const bool in = lane * step < n && (int64_t)((uint32_t)here / (uint32_t)rows) + c <= (int64_t)id;
+        const uint64_t not_in = ~__ballot(in);
+        cnt = not_in ? __builtin_ctzll(not_in) : 64;
+        cnt = cnt < 1 ? 0 : cnt - 1;
+        lo += cnt * step;
+        if (step == 1) break;
+        n = n - cnt * step < step ? n - cnt * step : step;
+    }
+    const int at = __builtin_amdgcn_readfirstlane((int)cnt);
+    Piece p;
+    p.p0 = __builtin_amdgcn_readlane(here, at);
+    p.p1 = __builtin_amdgcn_readfirstlane(at < 63 ? __builtin_amdgcn_readlane(here, (at + 1) & 63) : a.bound(lo + 1));
+    p.s = __builtin_amdgcn_readfirstlane(lo >= 1 && lo <= a.S ? (int)(lo - 1) : -1);
+    p.id0 = __builtin_amdgcn_readfirstlane((uint32_t)p.p0 / (uint32_t)rows + (uint32_t)lo);
+    const int64_t first = p.p0 + (int64_t)(id - p.id0) * rows;
+    const bool there = first >= p.p0 && first < p.p1;
+    p.n = __builtin_amdgcn_readfirstlane(!there ? 0 : p.p1 - first < rows ? (int)(p.p1 - first) : rows);
+    p.first = __builtin_amdgcn_readfirstlane(there ? (int)first : 0);
+    return p;
+}
+
+}  // namespace pmg

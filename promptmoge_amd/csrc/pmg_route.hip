@@ -14,18 +14,12 @@ struct RouteArgs {
     int32_t* rows;     // [M k]
     int32_t* counts;   // [blocks][E + 1]: a block's pairs of each expert (E: of none)
     int64_t ld;
-    int M, E, k, type, sigmoid, normalize;
+    int M, E, k, sigmoid, normalize;
     int lanes, per;    // lanes a row; rows a block
     int blocks;
 };
 
 constexpr int kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
-
-__device__ inline float logit(const RouteArgs& a, int64_t at) {
-    if (a.type == PMG_TYPE_F32) return ((const float*)a.logits)[at];
-    if (a.type == PMG_TYPE_F16) return (float)((const _Float16*)a.logits)[at];
-    return (float)((const __bf16*)a.logits)[at];
-}
 
 // A key that rises with x, 0 for what is not chosen (-infinity, NaN); and x of a key. -0 is 0, as in a comparison.
 __device__ inline uint32_t key_of(float x) {
@@ -34,16 +28,30 @@ __device__ inline uint32_t key_of(float x) {
 }
 __device__ inline float of_key(uint32_t k) { return u2f(k >> 31 ? k & 0x7fffffffu : ~k); }
 
-// The k best of a row on a.lanes lanes of a wave, I experts a lane, in k rounds of a largest (key, lowest index first).
-template <int I>
-__device__ inline void choose(const RouteArgs& a, int64_t m, bool there, int l) {
+// exp(d) for d <= 0, within 2^-21 of its value, its argument in two parts; below 2^-126 it may be 0. NaN stays.
+__device__ inline float exp_below(float d) {
+    const float b = __builtin_fminf(-d, 200.0f), hi = b * -PMG_LOG2E;
+    const float lo = __builtin_fmaf(b, -1.92596299e-8f, __builtin_fmaf(b, -PMG_LOG2E, -hi));
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return d != d ? d : __builtin_fmaf(e, lo * 0.69314718f, e);
+}
+
+// The k best of a row on a.lanes lanes of a wave, I experts a lane, in k rounds of a largest (key, lowest index first). Gives the
+// lane's slot's expert (-1: none).
+template <class T, int I>
+__device__ inline int choose(const RouteArgs& a, int64_t m, bool there, int l) {
     const int L = a.lanes;
+    const bool on = there && (!a.mask || a.mask[m]);
+    const T* row = (const T*)a.logits + m * a.ld;
     uint32_t key[I];
     float top = -__builtin_inff(), sum = 0.0f, x[I];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
         const int e = l + i * L;
-        x[i] = there && e < a.E ? logit(a, m * a.ld + e) : -__builtin_inff();
+        x[i] = there && e < a.E ? (float)row[e] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
         key[i] = key_of(x[i]);
         top = x[i] > top ? x[i] : top;
     }
@@ -52,13 +60,13 @@ __device__ inline void choose(const RouteArgs& a, int64_t m, bool there, int l) 
             const float t = __shfl_xor(top, o, 64);
             top = t > top ? t : top;
         }
-        const float base = top > -__builtin_inff() ? top : 0.0f;
+        top = top > -__builtin_inff() ? top : 0.0f;
 #pragma unroll
-        for (int i = 0; i < I; ++i) sum += expf(x[i] - base);  // (NaN, and infinity less itself: the row's weights are NaN)
+        for (int i = 0; i < I; ++i) sum += exp_below(x[i] - top);  // (NaN, and infinity less itself: the row's weights are NaN)
         for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        top = base;
     }
     float mine = 0.0f, chosen = 0.0f;  // lane j keeps the j-th
+    float base = 0.0f;                 // sigmoids that are only looked at relative to each other: times exp(-base), none is lost
     int expert = -1;
     for (int j = 0; j < a.k; ++j) {
         uint32_t k = key[0];
@@ -78,7 +86,9 @@ __device__ inline void choose(const RouteArgs& a, int64_t m, bool there, int l) 
             }
         }
         const float v = of_key(k);
-        const float w = k == 0 ? 0.0f : a.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / sum;
+        if (j == 0 && a.normalize && k != 0 && v < 0.0f) base = v;
+        const float s = base == 0.0f ? sigmoid_wide(v) : exp_below(v - base) * sigmoid_wide(-v);
+        const float w = k == 0 ? 0.0f : a.sigmoid ? s : exp_below(v - top) * __builtin_amdgcn_rcpf(sum);
         chosen += w;
         if (l == j) {
             mine = w;
@@ -88,48 +98,43 @@ __device__ inline void choose(const RouteArgs& a, int64_t m, bool there, int l) 
         for (int i = 0; i < I; ++i)
             if (l + i * L == e) key[i] = 0;
     }
-    if (a.normalize) mine = chosen == 0.0f ? 0.0f : mine / chosen;
+    if (a.normalize) mine = chosen == 0.0f ? 0.0f : mine * __builtin_amdgcn_rcpf(chosen);
+    expert = on ? expert : -1;
     if (there && l < a.k) {
-        const bool on = !a.mask || a.mask[m];
-        a.weights[m * a.k + l] = on && expert >= 0 ? mine : 0.0f;
-        a.experts[m * a.k + l] = on ? expert : -1;
+        a.weights[m * a.k + l] = expert >= 0 ? mine : 0.0f;
+        a.experts[m * a.k + l] = expert;
     }
+    return expert;
 }
 
-// Choices of a block's rows.
-__device__ inline void choose_rows(const RouteArgs& a, int first, int end) {
+// Choices of a block's rows, counted in `table` [E + 1] (E: no expert), or kept in `kept` as they are written.
+template <class T, int I>
+__device__ inline void choose_rows(const RouteArgs& a, int first, int end, int32_t* table, int16_t* kept) {
     const int per = kRouteThreads / a.lanes, l = (int)threadIdx.x & (a.lanes - 1);
     for (int m0 = first; m0 < end; m0 += per) {  // (every lane takes part: those behind the last row bring nothing)
         const int m = m0 + (int)threadIdx.x / a.lanes;
-        if (a.E <= a.lanes) choose<1>(a, m, m < end, l);
-        else if (a.E <= 4 * a.lanes) choose<4>(a, m, m < end, l);
-        else choose<16>(a, m, m < end, l);
+        const int e = choose<T, I>(a, m, m < end, l);
+        if (m < end && l < a.k) {
+            if (table) atomicAdd(table + (e < 0 ? a.E : e), 1);
+            else kept[(m - first) * a.k + l] = (int16_t)e;
+        }
     }
 }
 
-// The counts of a range of pairs into an LDS table of E + 1 (by experts; none: E), added atomically (whole numbers).
-__device__ inline void count_pairs(const RouteArgs& a, int64_t first, int64_t end, int step, int32_t* table) {
-    for (int64_t i = first; i < end; i += step) {
-        const int e = a.experts[i];
-        atomicAdd(table + (e < 0 ? a.E : e), 1);
-    }
-}
-
+template <class T, int I>
 __global__ __launch_bounds__(kRouteThreads) void route_choose_k(RouteArgs a) {
     extern __shared__ int32_t table[];
     const int first = (int)blockIdx.x * a.per, end = a.M - first < a.per ? a.M : first + a.per;
     for (int e = threadIdx.x; e <= a.E; e += kRouteThreads) table[e] = 0;
-    choose_rows(a, first, end);
-    __threadfence_block();
     __syncthreads();
-    count_pairs(a, (int64_t)first * a.k + threadIdx.x, (int64_t)end * a.k, kRouteThreads, table);
+    choose_rows<T, I>(a, first, end, table, nullptr);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.E; e += kRouteThreads) a.counts[(int64_t)blockIdx.x * (a.E + 1) + e] = table[e];
 }
 
 // The place of each pair: pairs of lower experts, of this expert in earlier blocks, in this block's earlier waves (a wave has a
 // range of its pairs), and in the wave itself, which goes over them 64 at a time. ONE: the choices too, in one block.
-template <bool ONE>
+template <class T, int I, bool ONE>
 __global__ __launch_bounds__(kRouteThreads) void route_order_k(RouteArgs a) {
     constexpr int NW = kRouteWaves;
     extern __shared__ int32_t table[];
@@ -137,25 +142,35 @@ __global__ __launch_bounds__(kRouteThreads) void route_order_k(RouteArgs a) {
     int32_t* base = table;                    // [E1] each expert's first place, then this block's
     int32_t* all = table + E1;                // [E1] pairs of each expert in all
     int32_t* next = table + (2 + wave) * E1;  // [E1] a wave's: its pairs of each expert, then their next place
+    int16_t* kept = (int16_t*)(table + (2 + NW) * E1);  // ONE: the pairs' experts
     const auto of_wave = [&](int w, int e) -> int32_t& { return table[(2 + w) * E1 + e]; };
     const int first = (int)blockIdx.x * a.per, end = a.M - first < a.per ? a.M : first + a.per;
     for (int e = tid; e < (2 + NW) * E1; e += kRouteThreads) table[e] = 0;
-    if constexpr (ONE) {
-        choose_rows(a, first, end);
-        __threadfence_block();
-    }
+    if constexpr (ONE) choose_rows<T, I>(a, first, end, nullptr, kept);
     __syncthreads();
     // this block's pairs, a range a wave
     const int64_t p0 = (int64_t)first * a.k, np = (int64_t)(end - first) * a.k;
     const int64_t share = (np + 64 * NW - 1) / (64 * NW) * 64;
     const int64_t w0 = p0 + (wave * share < np ? wave * share : np), w1 = p0 + ((wave + 1) * share < np ? (wave + 1) * share : np);
-    count_pairs(a, w0 + lane, w1, 64, next);
+    const auto expert = [&](int64_t i) -> int {
+        const int e = ONE ? (int)kept[i - p0] : a.experts[i];
+        return e < 0 ? a.E : e;
+    };
+    for (int64_t i = w0 + lane; i < w1; i += 64) atomicAdd(next + expert(i), 1);
     if constexpr (!ONE) {
-        for (uint32_t i = tid; i < (uint32_t)(a.blocks * E1); i += kRouteThreads) {
-            const int b = (int)(i / (uint32_t)E1), e = (int)(i - (uint32_t)(b * E1)), n = a.counts[i];
-            if (n) {
-                atomicAdd(all + e, n);
-                if (b < (int)blockIdx.x) atomicAdd(base + e, n);
+        const uint32_t all_counts = (uint32_t)(a.blocks * E1);
+        for (uint32_t i0 = tid; i0 < all_counts; i0 += 8 * kRouteThreads) {  // (eight on their way at a time)
+            int32_t n[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) n[u] = a.counts[i0 + u * kRouteThreads < all_counts ? i0 + u * kRouteThreads : i0];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const uint32_t i = i0 + u * kRouteThreads;
+                const int b = (int)(i / (uint32_t)E1), e = (int)(i - (uint32_t)(b * E1));
+                if (n[u] && i < all_counts) {
+                    atomicAdd(all + e, n[u]);
+                    if (b < (int)blockIdx.x) atomicAdd(base + e, n[u]);
+                }
             }
         }
     }
@@ -193,9 +208,8 @@ __global__ __launch_bounds__(kRouteThreads) void route_order_k(RouteArgs a) {
     for (int64_t i0 = w0; i0 < w1; i0 += 64) {
         const int64_t i = i0 + lane;
         const bool there = i < w1;
-        int e = there ? a.experts[i] : -1;
-        const bool none = e < 0;
-        e = none ? a.E : e;
+        const int e = there ? expert(i) : a.E;
+        const bool none = e == a.E;
         uint64_t same = __ballot(there);
         for (int b = 0; b < bits; ++b) {
             const uint64_t set = __ballot((e >> b) & 1);
@@ -278,6 +292,23 @@ int route_args(const pmg_route_args& q) {
     return PMG_OK;
 }
 
+template <class T, int I>
+int launch_route(const RouteArgs& a, int bytes, hipStream_t s) {
+    if (a.blocks <= 1) {
+        hipLaunchKernelGGL((route_order_k<T, I, true>), dim3(1), dim3(kRouteThreads), bytes + 2 * a.M * a.k, s, a);
+        return check_launch("route_order_k");
+    }
+    hipLaunchKernelGGL((route_choose_k<T, I>), dim3(a.blocks), dim3(kRouteThreads), (a.E + 1) * 4, s, a);
+    if (int e = check_launch("route_choose_k")) return e;
+    hipLaunchKernelGGL((route_order_k<float, 1, false>), dim3(a.blocks), dim3(kRouteThreads), bytes, s, a);
+    return check_launch("route_order_k");
+}
+template <class T>
+int launch_route_of(const RouteArgs& a, int bytes, hipStream_t s) {  // experts a lane
+    if (a.E <= a.lanes) return launch_route<T, 1>(a, bytes, s);
+    return a.E <= 4 * a.lanes ? launch_route<T, 4>(a, bytes, s) : launch_route<T, 16>(a, bytes, s);
+}
+
 }  // namespace
 
 extern "C" size_t pmg_route_workspace_bytes(const pmg_route_args* p) {
@@ -308,7 +339,6 @@ extern "C" int pmg_route(const pmg_route_args* p, void* workspace, size_t worksp
     a.M = (int)q.M;
     a.E = q.E;
     a.k = q.k;
-    a.type = q.type;
     a.sigmoid = q.score == PMG_SCORE_SIGMOID;
     a.normalize = q.normalize;
     a.lanes = pl.lanes;
@@ -316,14 +346,9 @@ extern "C" int pmg_route(const pmg_route_args* p, void* workspace, size_t worksp
     a.blocks = pl.blocks;
     const int bytes = (2 + kRouteWaves) * (q.E + 1) * 4;
     hipStream_t s = (hipStream_t)stream;
-    if (pl.blocks <= 1) {
-        hipLaunchKernelGGL((route_order_k<true>), dim3(1), dim3(kRouteThreads), bytes, s, a);
-        return check_launch("route_order_k");
-    }
-    hipLaunchKernelGGL(route_choose_k, dim3(pl.blocks), dim3(kRouteThreads), (q.E + 1) * 4, s, a);
-    if (int e = check_launch("route_choose_k")) return e;
-    hipLaunchKernelGGL((route_order_k<false>), dim3(pl.blocks), dim3(kRouteThreads), bytes, s, a);
-    return check_launch("route_order_k");
+    if (q.type == PMG_TYPE_F32) return launch_route_of<float>(a, bytes, s);
+    if (q.type == PMG_TYPE_F16) return launch_route_of<_Float16>(a, bytes, s);
+    return launch_route_of<__bf16>(a, bytes, s);
 }
 
 extern "C" int pmg_combine(const pmg_combine_args* p, void* stream) {

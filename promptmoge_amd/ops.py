@@ -688,6 +688,9 @@ def _layout(t: torch.Tensor) -> Tuple[int, int, int, int]:
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors share memory. Columns of one buffer (equal widest strides) are told apart; of other tensors
     laced into each other it is taken that they do."""
+    if a.is_contiguous() and b.is_contiguous():  # (most are)
+        a0, b0, na, nb = a.data_ptr(), b.data_ptr(), a.nbytes, b.nbytes
+        return na > 0 and nb > 0 and a0 < b0 + nb and b0 < a0 + na
     if not a.numel() or not b.numel():
         return False
     (a0, a1, pa, wa), (b0, b1, pb, wb) = _layout(a), _layout(b)
@@ -1004,7 +1007,7 @@ def _result(out: Optional[torch.Tensor], out_dtype: Optional[torch.dtype], like:
     """The (rows, N) result, its type and its row stride: a new one, or `out`, which may be `same_as` (named `same`) itself but lie
     on nothing else of the call."""
     if out is None:
-        out = like.new_empty((rows, N), dtype=like.dtype if out_dtype is None else out_dtype)
+        out = like.new_empty((rows, N)) if out_dtype is None else like.new_empty((rows, N), dtype=out_dtype)
         return out, _floating(out, "out"), N
     if out.shape != (rows, N):
         raise ValueError(f"out must be ({rows}, {N}), got {tuple(out.shape)}")
@@ -1049,9 +1052,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     code = _act(act)
     fresh = out is None
     out, ot, ldo = _result(out, out_dtype, x, M, C_, "x", x, weight=weight, bias=bias, offsets=offsets)
-    args = _lib.GROUP_NORM_PACK.pack(ty, x.data_ptr(), ldx, M, C_, groups, _ptr(weight), _ptr(bias), _ptr(offsets),
-                                     1 if offsets is None else offsets.shape[0] - 1, eps, code, out.data_ptr(), ot, ldo, fresh)
-    ws, n = _workspace("pmg_group_norm_workspace_bytes", x, args)
+    S = 1 if offsets is None else offsets.shape[0] - 1
+    args = _lib.GROUP_NORM_PACK.pack(ty, x.data_ptr(), ldx, M, C_, groups, _ptr(weight), _ptr(bias), _ptr(offsets), S, eps, code,
+                                     out.data_ptr(), ot, ldo, fresh)
+    ws, n = (None, 0) if M <= 512 * S else _workspace("pmg_group_norm_workspace_bytes", x, args)  # (short segments need none)
     _on(d, "pmg_group_norm", args, _ptr(ws), n)
     return out
 
@@ -1077,8 +1081,8 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", normalize: bo
         z = combine(y.view(M, k, N), r.weights, residual=x)
 
     logits: (M, E) fp32 / fp16 / bf16 (rows may be strided), E up to 1024, k up to 32; score: "softmax" over the row's
-    logits, or "sigmoid"; normalize: the weights over the sum of the row's (0 where that is 0). An expert whose logit is -inf
-    or NaN is not chosen: the slot holds -1 and weight 0. So do the rows with 0 in mask, (M,) bool / uint8, whose pairs come
+    logits, or "sigmoid"; normalize: the weights over the sum of the row's. An expert whose logit is -inf or NaN is not
+    chosen: the slot holds -1 and weight 0. So do the rows with 0 in mask, (M,) bool / uint8, whose pairs come
     in no segment. Forward only."""
     d = _one_gpu(logits, mask) if logits is not None else -1
     if d < 0:
@@ -1093,12 +1097,15 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", normalize: bo
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (M,) or not mask.is_contiguous()):
         raise ValueError(f"mask must be a contiguous ({M},) bool or uint8 tensor")
     weights = logits.new_empty((M, k), dtype=torch.float32)
-    tables = logits.new_empty((3 * M * k,), dtype=torch.int32)
+    P = M * k
+    tables = logits.new_empty((3 * P,), dtype=torch.int32)
     offsets = logits.new_empty((E + 1,), dtype=torch.int64)
-    experts, pairs, rows = tables[:M * k].view(M, k), tables[M * k:2 * M * k], tables[2 * M * k:]
+    experts = tables.as_strided((M, k), (k, 1))
+    pairs, rows = tables.as_strided((P,), (1,), P), tables.as_strided((P,), (1,), 2 * P)
+    at = tables.data_ptr()
     args = _lib.ROUTE_PACK.pack(ty, logits.data_ptr(), ld, M, E, k, code, bool(normalize), _ptr(mask), weights.data_ptr(),
-                                experts.data_ptr(), offsets.data_ptr(), pairs.data_ptr(), rows.data_ptr())
-    ws, n = _workspace("pmg_route_workspace_bytes", logits, args)
+                                at, offsets.data_ptr(), at + 4 * P, at + 8 * P)
+    ws, n = (None, 0) if M <= 64 else _workspace("pmg_route_workspace_bytes", logits, args)  # (one block needs none)
     _on(d, "pmg_route", args, _ptr(ws), n)
     return Routes(weights, experts, offsets, pairs, rows)
 
@@ -1236,6 +1243,8 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, down: torch.Tensor, up: torch.
                            offsets=offsets, scale=scale)
     args = _lib.LORA_PACK.pack(ty, x.data_ptr(), ldx, M, K, N, w.data_ptr(), down.data_ptr(), up.data_ptr(), r, A, _ptr(scale),
                                adapter.data_ptr(), _ptr(offsets), S, _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), ot, ldo)
-    ws, n = _workspace("pmg_lora_linear_workspace_bytes", x, args)
-    _on(d, "pmg_lora_linear", args, _ptr(ws), n)
+    # (what the entry asks for at the most: r values of 6 bytes and one of 4 a row, on 256 bytes)
+    n = (6 * r + 4) * M + 512
+    ws = x.new_empty((n,), dtype=torch.uint8)
+    _on(d, "pmg_lora_linear", args, ws.data_ptr(), n)
     return out

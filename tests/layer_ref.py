@@ -74,8 +74,13 @@ def route(logits, k, *, score="softmax", normalize=False, mask=None):
         w = torch.exp(v - top) / torch.exp(x - top).sum(-1, keepdim=True)
         rel = 2.0 ** -20 + E * 2.0 ** -23 + 2.0 ** -22 * (v - top).abs().nan_to_num(0, 0, 0)
     else:
+        # (over their sum: of their logarithms, for sigmoids far below the least number are not lost beside each other)
         w = torch.sigmoid(v)
-        rel = 2.0 ** -20 + 2.0 ** -22 * v.abs().nan_to_num(0, 0, 0)
+        if normalize:
+            log = torch.where(ok, torch.nn.functional.logsigmoid(v), torch.full_like(v, float("-inf")))
+            top = log.amax(-1, keepdim=True)
+            w = torch.where(torch.isinf(top), torch.zeros_like(w), torch.exp(log - top))
+        rel = 2.0 ** -20 + 2.0 ** -22 * v.abs().clamp(max=200).nan_to_num(0, 0, 0)
     w = torch.where(ok, w, torch.zeros_like(w))
     if normalize:
         total = w.sum(-1, keepdim=True)

@@ -189,6 +189,9 @@ def test_route_equal_and_absent_logits(gpu, M):
         for score in ("softmax", "sigmoid"):
             check_route(x.to(gpu), 6, score=score, normalize=normalize)
     assert not bool(ops.route(x[1:2].to(gpu), 6, normalize=True).weights.any())
+    low = torch.tensor([[-87.5, -88.0, -90.0, -200.0], [-1000.0, -1001.0, -1000.0, -3e38], [-3e38, -3e38, -3e38, -3e38]]).to(gpu)
+    check_route(low, 2, score="sigmoid", normalize=True)
+    check_route(low, 4, score="sigmoid", normalize=True)
 
 
 def test_route_values_that_are_no_numbers(gpu):

@@ -116,6 +116,22 @@ def test_workspaces_are_asked_for_and_checked(libpmg):
         assert getattr(libpmg, entry + "_workspace_bytes")(None) == 0
 
 
+def test_workspaces_that_the_wrappers_do_not_ask_for(libpmg):
+    """Short segments' norms and one block's routes need none; adapters at most 6 r + 4 bytes a row and 512."""
+    for S in (1, 3, 1000):
+        for M in (1, 512 * S - 1, 512 * S):
+            assert libpmg.pmg_group_norm_workspace_bytes(C.byref(norm_args(M=M, segments=S))) == 0
+    for E in (1, 2, 16, 300, 1024):
+        for k in {1, min(E, 2), min(E, 32)}:
+            for M in (0, 1, 63, 64):
+                assert libpmg.pmg_route_workspace_bytes(C.byref(route_args(M=M, E=E, ld=E, k=k))) == 0
+    for type_ in (0, 1, 2):
+        for M, S in ((1, 1), (7, 7), (5000, 2), (1 << 20, 9)):
+            for r in (1, 8, 20, 128):
+                a = lora_args(type=type_, M=M, segments=S, rank=r)
+                assert 0 < libpmg.pmg_lora_linear_workspace_bytes(C.byref(a)) <= (6 * r + 4) * M + 512
+
+
 def test_workspaces_stay_small(libpmg):
     for M, S in ((1 << 20, 1), ((1 << 31) - 600, 5), (1 << 24, 1 << 12)):
         assert libpmg.pmg_group_norm_workspace_bytes(C.byref(norm_args(M=M, segments=S, C=4096, groups=32, ldx=4096, ldo=4096))) < 1 << 23
