@@ -15,8 +15,7 @@ struct RouteArgs {
     int32_t* counts;   // [blocks][E + 1]: a block's pairs of each expert (E: of none)
     int64_t ld;
     int M, E, k, sigmoid, normalize;
-    int lanes, per;    // lanes a row; rows a block
-    int blocks;
+    int per, blocks;   // rows a block
 };
 
 constexpr int kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
@@ -36,11 +35,27 @@ __device__ inline float exp_below(float d) {
     return d != d ? d : __builtin_fmaf(e, lo * 0.69314718f, e);
 }
 
-// The k best of a row on a.lanes lanes of a wave, I experts a lane, in k rounds of a largest (key, lowest index first). Gives the
+// f(value of another lane) over groups of L lanes, until all of a group have met: within 16 lanes by moves between
+// neighbours (quads, then mirrored, which after a step is as good as swapped), beyond by the exchange through LDS. A register move
+// takes a tenth of that exchange, and a row's k rounds are one behind the other.
+template <int CTRL>
+__device__ inline uint32_t from_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int L, class F>
+__device__ inline void over_lanes(const F& f) {
+    if constexpr (L > 1) f([](uint32_t v) { return from_lane<0xb1>(v); });   // lane ^ 1
+    if constexpr (L > 2) f([](uint32_t v) { return from_lane<0x4e>(v); });   // lane ^ 2
+    if constexpr (L > 4) f([](uint32_t v) { return from_lane<0x141>(v); });  // 7 - lane of eight
+    if constexpr (L > 8) f([](uint32_t v) { return from_lane<0x140>(v); });  // 15 - lane of 16
+    if constexpr (L > 16) f([](uint32_t v) { return (uint32_t)__shfl_xor((int)v, 16, 64); });
+    if constexpr (L > 32) f([](uint32_t v) { return (uint32_t)__shfl_xor((int)v, 32, 64); });
+}
+
+// The k best of a row on L lanes of a wave, I experts a lane, in k rounds of a largest (key, lowest index first). Gives the
 // lane's slot's expert (-1: none).
-template <class T, int I>
+template <class T, int I, int L>
 __device__ inline int choose(const RouteArgs& a, int64_t m, bool there, int l) {
-    const int L = a.lanes;
     const bool on = there && (!a.mask || a.mask[m]);
     const T* row = (const T*)a.logits + m * a.ld;
     uint32_t key[I];
@@ -56,14 +71,14 @@ __device__ inline int choose(const RouteArgs& a, int64_t m, bool there, int l) {
         top = x[i] > top ? x[i] : top;
     }
     if (!a.sigmoid) {
-        for (int o = 1; o < L; o <<= 1) {
-            const float t = __shfl_xor(top, o, 64);
+        over_lanes<L>([&](auto other) {
+            const float t = u2f(other(f2u(top)));
             top = t > top ? t : top;
-        }
+        });
         top = top > -__builtin_inff() ? top : 0.0f;
 #pragma unroll
         for (int i = 0; i < I; ++i) sum += exp_below(x[i] - top);  // (NaN, and infinity less itself: the row's weights are NaN)
-        for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        over_lanes<L>([&](auto other) { sum += u2f(other(f2u(sum))); });
     }
     float mine = 0.0f, chosen = 0.0f;  // lane j keeps the j-th
     float base = 0.0f;                 // sigmoids that are only looked at relative to each other: times exp(-base), none is lost
@@ -77,14 +92,13 @@ __device__ inline int choose(const RouteArgs& a, int64_t m, bool there, int l) {
                 k = key[i];
                 e = l + i * L;
             }
-        for (int o = 1; o < L; o <<= 1) {
-            const uint32_t k2 = __shfl_xor(k, o, 64);
-            const int e2 = __shfl_xor(e, o, 64);
-            if (k2 > k || (k2 == k && e2 < e)) {
-                k = k2;
-                e = e2;
-            }
-        }
+        over_lanes<L>([&](auto other) {
+            const uint32_t k2 = other(k);
+            const int e2 = (int)other((uint32_t)e);
+            const bool better = k2 > k || (k2 == k && e2 < e);
+            k = better ? k2 : k;
+            e = better ? e2 : e;
+        });
         const float v = of_key(k);
         if (j == 0 && a.normalize && k != 0 && v < 0.0f) base = v;
         const float s = base == 0.0f ? sigmoid_wide(v) : exp_below(v - base) * sigmoid_wide(-v);
@@ -108,12 +122,13 @@ __device__ inline int choose(const RouteArgs& a, int64_t m, bool there, int l) {
 }
 
 // Choices of a block's rows, counted in `table` [E + 1] (E: no expert), or kept in `kept` as they are written.
-template <class T, int I>
+template <class T, int I, int L>
 __device__ inline void choose_rows(const RouteArgs& a, int first, int end, int32_t* table, int16_t* kept) {
-    const int per = kRouteThreads / a.lanes, l = (int)threadIdx.x & (a.lanes - 1);
+    constexpr int per = kRouteThreads / L;
+    const int l = (int)threadIdx.x % L;
     for (int m0 = first; m0 < end; m0 += per) {  // (every lane takes part: those behind the last row bring nothing)
-        const int m = m0 + (int)threadIdx.x / a.lanes;
-        const int e = choose<T, I>(a, m, m < end, l);
+        const int m = m0 + (int)threadIdx.x / L;
+        const int e = choose<T, I, L>(a, m, m < end, l);
         if (m < end && l < a.k) {
             if (table) atomicAdd(table + (e < 0 ? a.E : e), 1);
             else kept[(m - first) * a.k + l] = (int16_t)e;
@@ -121,20 +136,20 @@ __device__ inline void choose_rows(const RouteArgs& a, int first, int end, int32
     }
 }
 
-template <class T, int I>
+template <class T, int I, int L>
 __global__ __launch_bounds__(kRouteThreads) void route_choose_k(RouteArgs a) {
     extern __shared__ int32_t table[];
     const int first = (int)blockIdx.x * a.per, end = a.M - first < a.per ? a.M : first + a.per;
     for (int e = threadIdx.x; e <= a.E; e += kRouteThreads) table[e] = 0;
     __syncthreads();
-    choose_rows<T, I>(a, first, end, table, nullptr);
+    choose_rows<T, I, L>(a, first, end, table, nullptr);
     __syncthreads();
     for (int e = threadIdx.x; e <= a.E; e += kRouteThreads) a.counts[(int64_t)blockIdx.x * (a.E + 1) + e] = table[e];
 }
 
 // The place of each pair: pairs of lower experts, of this expert in earlier blocks, in this block's earlier waves (a wave has a
 // range of its pairs), and in the wave itself, which goes over them 64 at a time. ONE: the choices too, in one block.
-template <class T, int I, bool ONE>
+template <class T, int I, int L, bool ONE>
 __global__ __launch_bounds__(kRouteThreads) void route_order_k(RouteArgs a) {
     constexpr int NW = kRouteWaves;
     extern __shared__ int32_t table[];
@@ -146,7 +161,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_order_k(RouteArgs a) {
     const auto of_wave = [&](int w, int e) -> int32_t& { return table[(2 + w) * E1 + e]; };
     const int first = (int)blockIdx.x * a.per, end = a.M - first < a.per ? a.M : first + a.per;
     for (int e = tid; e < (2 + NW) * E1; e += kRouteThreads) table[e] = 0;
-    if constexpr (ONE) choose_rows<T, I>(a, first, end, nullptr, kept);
+    if constexpr (ONE) choose_rows<T, I, L>(a, first, end, nullptr, kept);
     __syncthreads();
     // this block's pairs, a range a wave
     const int64_t p0 = (int64_t)first * a.k, np = (int64_t)(end - first) * a.k;
@@ -268,15 +283,17 @@ namespace {
 struct RoutePlan {
     int lanes, per, blocks;  // lanes a row, rows a block
 };
-// Four experts a lane, as far as k lanes are left and 64 reach. One block where it goes over its rows at most four times; else a
-// block for 256 rows or more, as few as keep the table of their counts, which each block reads whole, within 16,384.
+// Four experts a lane of up to 64, 16 of more (a lane's own are looked through faster than other lanes'), and at least k lanes. One block where it goes over its rows at most four times; else 512
+// blocks or fewer, of as many rows as they take at once or more, whose table of counts, which each block reads whole, stays within
+// 32,768. (307,200 rows to 2 of 8, 256 rows a block: 31 us)
 RoutePlan route_plan(const pmg_route_args& q) {
     RoutePlan p;
-    p.lanes = 1;
-    while (p.lanes < 64 && (p.lanes < q.k || 4 * p.lanes < q.E)) p.lanes *= 2;
-    const int64_t most = 16384 / (q.E + 1);
+    p.lanes = q.E > 64 ? 8 : 1;
+    while (p.lanes < q.k || (q.E > 64 ? 16 : 4) * p.lanes < q.E) p.lanes *= 2;
+    int64_t most = 32768 / (q.E + 1);
+    most = most > 512 ? 512 : most;
     int64_t per = (q.M + most - 1) / most;
-    per = per < 256 ? 256 : per;
+    if (per < kRouteThreads / p.lanes) per = kRouteThreads / p.lanes;
     if (q.M * p.lanes <= 4 * kRouteThreads && q.M * q.k <= 4096) per = q.M > 0 ? q.M : 1;
     p.per = (int)per;
     p.blocks = (int)((q.M + per - 1) / per);
@@ -292,21 +309,35 @@ int route_args(const pmg_route_args& q) {
     return PMG_OK;
 }
 
-template <class T, int I>
+template <class T, int I, int L>
 int launch_route(const RouteArgs& a, int bytes, hipStream_t s) {
     if (a.blocks <= 1) {
-        hipLaunchKernelGGL((route_order_k<T, I, true>), dim3(1), dim3(kRouteThreads), bytes + 2 * a.M * a.k, s, a);
+        hipLaunchKernelGGL((route_order_k<T, I, L, true>), dim3(1), dim3(kRouteThreads), bytes + 2 * a.M * a.k, s, a);
         return check_launch("route_order_k");
     }
-    hipLaunchKernelGGL((route_choose_k<T, I>), dim3(a.blocks), dim3(kRouteThreads), (a.E + 1) * 4, s, a);
+    hipLaunchKernelGGL((route_choose_k<T, I, L>), dim3(a.blocks), dim3(kRouteThreads), (a.E + 1) * 4, s, a);
     if (int e = check_launch("route_choose_k")) return e;
-    hipLaunchKernelGGL((route_order_k<float, 1, false>), dim3(a.blocks), dim3(kRouteThreads), bytes, s, a);
+    hipLaunchKernelGGL((route_order_k<float, 1, 1, false>), dim3(a.blocks), dim3(kRouteThreads), bytes, s, a);
     return check_launch("route_order_k");
 }
 template <class T>
-int launch_route_of(const RouteArgs& a, int bytes, hipStream_t s) {  // experts a lane
-    if (a.E <= a.lanes) return launch_route<T, 1>(a, bytes, s);
-    return a.E <= 4 * a.lanes ? launch_route<T, 4>(a, bytes, s) : launch_route<T, 16>(a, bytes, s);
+int launch_route_of(const RouteArgs& a, int lanes, int bytes, hipStream_t s) {
+    if (a.E <= 64) {
+        switch (lanes) {
+            case 1: return launch_route<T, 4, 1>(a, bytes, s);
+            case 2: return launch_route<T, 4, 2>(a, bytes, s);
+            case 4: return launch_route<T, 4, 4>(a, bytes, s);
+            case 8: return launch_route<T, 4, 8>(a, bytes, s);
+            case 16: return launch_route<T, 4, 16>(a, bytes, s);
+            default: return launch_route<T, 4, 32>(a, bytes, s);
+        }
+    }
+    switch (lanes) {
+        case 8: return launch_route<T, 16, 8>(a, bytes, s);
+        case 16: return launch_route<T, 16, 16>(a, bytes, s);
+        case 32: return launch_route<T, 16, 32>(a, bytes, s);
+        default: return launch_route<T, 16, 64>(a, bytes, s);
+    }
 }
 
 }  // namespace
@@ -341,14 +372,13 @@ extern "C" int pmg_route(const pmg_route_args* p, void* workspace, size_t worksp
     a.k = q.k;
     a.sigmoid = q.score == PMG_SCORE_SIGMOID;
     a.normalize = q.normalize;
-    a.lanes = pl.lanes;
     a.per = pl.per;
     a.blocks = pl.blocks;
     const int bytes = (2 + kRouteWaves) * (q.E + 1) * 4;
     hipStream_t s = (hipStream_t)stream;
-    if (q.type == PMG_TYPE_F32) return launch_route_of<float>(a, bytes, s);
-    if (q.type == PMG_TYPE_F16) return launch_route_of<_Float16>(a, bytes, s);
-    return launch_route_of<__bf16>(a, bytes, s);
+    if (q.type == PMG_TYPE_F32) return launch_route_of<float>(a, pl.lanes, bytes, s);
+    if (q.type == PMG_TYPE_F16) return launch_route_of<_Float16>(a, pl.lanes, bytes, s);
+    return launch_route_of<__bf16>(a, pl.lanes, bytes, s);
 }
 
 extern "C" int pmg_combine(const pmg_combine_args* p, void* stream) {

@@ -1002,13 +1002,18 @@ def _residual(residual: Optional[torch.Tensor], rows: int, N: int) -> Tuple[int,
     return rt, ldr
 
 
-def _result(out: Optional[torch.Tensor], out_dtype: Optional[torch.dtype], like: torch.Tensor, rows: int, N: int, same: str,
-            same_as: Optional[torch.Tensor], **others: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int, int]:
-    """The (rows, N) result, its type and its row stride: a new one, or `out`, which may be `same_as` (named `same`) itself but lie
-    on nothing else of the call."""
-    if out is None:
-        out = like.new_empty((rows, N)) if out_dtype is None else like.new_empty((rows, N), dtype=out_dtype)
-        return out, _floating(out, "out"), N
+def _new(like: torch.Tensor, ty: int, rows: int, N: int, out_dtype: Optional[torch.dtype]) -> Tuple[torch.Tensor, int, int]:
+    """A new (rows, N) result of out_dtype (None: of `like`'s type, whose code is ty), its type and its row stride."""
+    if out_dtype is None or out_dtype == like.dtype:
+        return like.new_empty((rows, N)), ty, N
+    out = like.new_empty((rows, N), dtype=out_dtype)
+    return out, _floating(out, "out"), N
+
+
+def _given(out: torch.Tensor, out_dtype: Optional[torch.dtype], rows: int, N: int, same: str, same_as: Optional[torch.Tensor],
+           **others: Optional[torch.Tensor]) -> Tuple[torch.Tensor, int, int]:
+    """A given (rows, N) result, its type and its row stride. It may be `same_as` (named `same`) itself but lie on nothing else
+    of the call."""
     if out.shape != (rows, N):
         raise ValueError(f"out must be ({rows}, {N}), got {tuple(out.shape)}")
     if out_dtype is not None and out_dtype != out.dtype:
@@ -1051,7 +1056,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         _offsets(offsets, "offsets")
     code = _act(act)
     fresh = out is None
-    out, ot, ldo = _result(out, out_dtype, x, M, C_, "x", x, weight=weight, bias=bias, offsets=offsets)
+    if fresh:
+        out, ot, ldo = _new(x, ty, M, C_, out_dtype)
+    else:
+        out, ot, ldo = _given(out, out_dtype, M, C_, "x", x, weight=weight, bias=bias, offsets=offsets)
     S = 1 if offsets is None else offsets.shape[0] - 1
     args = _lib.GROUP_NORM_PACK.pack(ty, x.data_ptr(), ldx, M, C_, groups, _ptr(weight), _ptr(bias), _ptr(offsets), S, eps, code,
                                      out.data_ptr(), ot, ldo, fresh)
@@ -1097,16 +1105,15 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", normalize: bo
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (M,) or not mask.is_contiguous()):
         raise ValueError(f"mask must be a contiguous ({M},) bool or uint8 tensor")
     weights = logits.new_empty((M, k), dtype=torch.float32)
-    P = M * k
-    tables = logits.new_empty((3 * P,), dtype=torch.int32)
+    P, W = M * k, 0 if M <= 64 else 32_768  # (W: the entry's workspace at the most; one block, of up to 64 rows, needs none)
+    tables = logits.new_empty((3 * P + W,), dtype=torch.int32)
     offsets = logits.new_empty((E + 1,), dtype=torch.int64)
     experts = tables.as_strided((M, k), (k, 1))
     pairs, rows = tables.as_strided((P,), (1,), P), tables.as_strided((P,), (1,), 2 * P)
     at = tables.data_ptr()
     args = _lib.ROUTE_PACK.pack(ty, logits.data_ptr(), ld, M, E, k, code, bool(normalize), _ptr(mask), weights.data_ptr(),
                                 at, offsets.data_ptr(), at + 4 * P, at + 8 * P)
-    ws, n = (None, 0) if M <= 64 else _workspace("pmg_route_workspace_bytes", logits, args)  # (one block needs none)
-    _on(d, "pmg_route", args, _ptr(ws), n)
+    _on(d, "pmg_route", args, at + 12 * P if W else 0, 4 * W)
     return Routes(weights, experts, offsets, pairs, rows)
 
 
@@ -1161,8 +1168,11 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
     code = _act(act)
     rt, ldr = _residual(residual, rows, N)
     fresh = out is None
-    out, ot, ldo = _result(out, out_dtype, x, rows, N, "residual", residual, x=x, w=w, offsets=offsets, bias=bias,
-                           index=index, out_index=out_index)
+    if fresh:
+        out, ot, ldo = _new(x, ty, rows, N, out_dtype)
+    else:
+        out, ot, ldo = _given(out, out_dtype, rows, N, "residual", residual, x=x, w=w, offsets=offsets, bias=bias, index=index,
+                              out_index=out_index)
     args = _lib.GROUPED_PACK.pack(ty, x.data_ptr(), ldx, Mx, w.data_ptr(), P, S, K, N, offsets.data_ptr(), _ptr(index),
                                   _ptr(out_index), _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), ot, ldo, rows, fresh)
     _on(d, "pmg_grouped_linear", args)
@@ -1188,7 +1198,10 @@ def combine(y: torch.Tensor, weights: torch.Tensor, *, residual: Optional[torch.
     if weights.dtype != torch.float32 or weights.shape != (M, k) or not weights.is_contiguous():
         raise ValueError(f"weights must be a contiguous float32 ({M}, {k}) tensor")
     rt, ldr = _residual(residual, M, N)
-    out, ot, ldo = _result(out, out_dtype, y, M, N, "residual", residual, y=y, weights=weights)
+    if out is None:
+        out, ot, ldo = _new(y, ty, M, N, out_dtype)
+    else:
+        out, ot, ldo = _given(out, out_dtype, M, N, "residual", residual, y=y, weights=weights)
     args = _lib.COMBINE_PACK.pack(ty, y.data_ptr(), y.stride(0), y.stride(1), M, k, N, weights.data_ptr(), _ptr(residual), rt, ldr,
                                   out.data_ptr(), ot, ldo)
     _on(d, "pmg_combine", args)
@@ -1213,18 +1226,19 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, down: torch.Tensor, up: torch.
     if d < 0:
         d = _refuse("x w down up adapter", x=x, w=w, down=down, up=up, adapter=adapter, bias=bias, offsets=offsets,
                     scale=scale, residual=residual, out=out)
-    ty, ldx = _floating(x, "x"), _rows(x, "x")
+    ty, ldx, t = _floating(x, "x"), _rows(x, "x"), x.dtype
     M, K = x.shape
-    if w.dtype != x.dtype or down.dtype != x.dtype or up.dtype != x.dtype:
-        raise ValueError(f"w, down and up must be {x.dtype}")
-    if w.ndim != 2 or w.shape[1] != K or not w.is_contiguous():
-        raise ValueError(f"w must be a contiguous (N, {K}) matrix, got {tuple(w.shape)}")
-    N = w.shape[0]
-    if down.ndim != 3 or down.shape[2] != K or not down.is_contiguous():
-        raise ValueError(f"down must be a contiguous (A, r, {K}) tensor, got {tuple(down.shape)}")
-    A, r = down.shape[:2]
-    if up.shape != (A, N, r) or not up.is_contiguous():
-        raise ValueError(f"up must be a contiguous ({A}, {N}, {r}) tensor, got {tuple(up.shape)}")
+    if w.dtype != t or down.dtype != t or up.dtype != t:
+        raise ValueError(f"w, down and up must be {t}")
+    ws_, ds, us = w.shape, down.shape, up.shape
+    if len(ws_) != 2 or ws_[1] != K or not w.is_contiguous():
+        raise ValueError(f"w must be a contiguous (N, {K}) matrix, got {tuple(ws_)}")
+    N = ws_[0]
+    if len(ds) != 3 or ds[2] != K or not down.is_contiguous():
+        raise ValueError(f"down must be a contiguous (A, r, {K}) tensor, got {tuple(ds)}")
+    A, r, _ = ds
+    if us != (A, N, r) or not up.is_contiguous():
+        raise ValueError(f"up must be a contiguous ({A}, {N}, {r}) tensor, got {tuple(us)}")
     if not 1 <= r <= 128:
         raise ValueError(f"adapters of rank 1 to 128, got {r}")
     S = M
@@ -1239,8 +1253,11 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, down: torch.Tensor, up: torch.
         _vector(scale, "scale", A)
     code = _act(act)
     rt, ldr = _residual(residual, M, N)
-    out, ot, ldo = _result(out, out_dtype, x, M, N, "residual", residual, x=x, w=w, down=down, up=up, adapter=adapter, bias=bias,
-                           offsets=offsets, scale=scale)
+    if out is None:
+        out, ot, ldo = _new(x, ty, M, N, out_dtype)
+    else:
+        out, ot, ldo = _given(out, out_dtype, M, N, "residual", residual, x=x, w=w, down=down, up=up, adapter=adapter, bias=bias,
+                              offsets=offsets, scale=scale)
     args = _lib.LORA_PACK.pack(ty, x.data_ptr(), ldx, M, K, N, w.data_ptr(), down.data_ptr(), up.data_ptr(), r, A, _ptr(scale),
                                adapter.data_ptr(), _ptr(offsets), S, _ptr(bias), code, _ptr(residual), rt, ldr, out.data_ptr(), ot, ldo)
     # (what the entry asks for at the most: r values of 6 bytes and one of 4 a row, on 256 bytes)

@@ -117,7 +117,8 @@ def test_workspaces_are_asked_for_and_checked(libpmg):
 
 
 def test_workspaces_that_the_wrappers_do_not_ask_for(libpmg):
-    """Short segments' norms and one block's routes need none; adapters at most 6 r + 4 bytes a row and 512."""
+    """Short segments' norms and one block's routes need none; other routes 32,768 counts at the most; adapters at most 6 r + 4 bytes
+    a row and 512."""
     for S in (1, 3, 1000):
         for M in (1, 512 * S - 1, 512 * S):
             assert libpmg.pmg_group_norm_workspace_bytes(C.byref(norm_args(M=M, segments=S))) == 0
