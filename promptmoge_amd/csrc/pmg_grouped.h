@@ -6,7 +6,7 @@
 
 namespace pmg {
 
-struct GroupArgs : Epilogue, Pieces {  // (adapters may have no offsets: a row a segment)
+struct GroupArgs : Epilogue, Pieces {  // (tag: the segments' adapters, which may have no offsets: a row a segment)
     const void* x;            // [x_rows] rows of ldx
     const void* w;            // [N][K], the next segment's w_next elements on
     const float* bias;        // [N] or NULL, the next segment's b_next elements on
@@ -22,7 +22,6 @@ struct GroupArgs : Epilogue, Pieces {  // (adapters may have no offsets: a row a
     const void* down;         // [adapters][r][K]
     const void* up;
     const float* scale;       // [adapters] or NULL
-    const int32_t* adapter;   // [S]
     int r, adapters, vec_up;
     uint32_t tiles_n, tiles, id0;
 };
@@ -36,11 +35,7 @@ __device__ inline int row_out(const GroupArgs& a, int p, int from) {
     if (!a.out_index) return in_x(a, from) ? p : a.fresh ? -2 - p : -1;
     return in_x(a, from) && o >= 0 && o < a.out_rows ? o : -1;
 }
-__device__ inline int adapter_of(const GroupArgs& a, int s) {
-    if (s < 0) return -1;
-    const int i = a.adapter[s];
-    return i >= 0 && i < a.adapters ? i : -1;
-}
+__device__ inline int adapter_of(const GroupArgs& a, int tag) { return tag >= 0 && tag < a.adapters ? tag : -1; }
 
 // Bias of columns n .. n + 7 of segment s (0 behind N).
 __device__ inline void bias8(const GroupArgs& a, int s, int n, float (&b)[8]) {

@@ -128,7 +128,7 @@ extern "C" int pmg_lora_linear(const pmg_lora_linear_args* p, void* workspace, s
     a.down = q.down;
     a.up = q.up;
     a.scale = q.scale;
-    a.adapter = q.adapter;
+    a.tag = q.adapter;
     a.r = q.rank;
     a.adapters = q.adapters;
     a.vec_up = at(q.up, 16) && q.rank * es % 16 == 0;

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
         return;
     }
     const int seg = KIND == kExperts ? pc.s : 0;
-    const int ad = KIND == kAdapters ? adapter_of(a, pc.s) : -1;
+    const int ad = KIND == kAdapters ? adapter_of(a, pc.tag) : -1;
     const bool gather = KIND == kExperts && a.index;
     const T* xb = (const T*)a.x + (gather ? 0 : (int64_t)pc.first * a.ldx);
     const T* wb = (const T*)a.w + (int64_t)seg * a.w_next + (int64_t)n0 * a.K;
@@ -263,9 +263,9 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
                     activate8(v, a.act, a.out_type == PMG_TYPE_F32);
 #pragma unroll
                     for (int q = 0; q < 8; ++q) v[q] = v[q] + add[q];
-                    put8(a, m, nc, left, v);
+                    put8<true>(a, m, nc, left, v);
                 } else {
-                    finish8(a, m, nc, left, v);
+                    finish8<true>(a, m, nc, left, v);
                 }
             } else if (KIND == kExperts && m < -1) {
                 zero8(a, -2 - m, nc, left);
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
     const uint32_t id = a.id0 + blockIdx.x;
     Piece pc;
     if (a.offsets) pc = piece_of(a, id, 16);
-    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id, (int)id, (int)id + 1, id};
+    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id, (int)id, (int)id + 1, id, (int)id < a.P ? a.tag[id] : -1};
     if (pc.n < 1) return;
     const T* xr = (const T*)a.x + (int64_t)(pc.first + (r < pc.n ? r : pc.n - 1)) * a.ldx;
     const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
         for (int u = 0; u < U; ++u) fx[u] = get(xr, (4 * (s0 + u * NW) + g) * PER);
     };
     if (wave < nsteps) rows_of(wave);
-    const int ad = adapter_of(a, pc.s);
+    const int ad = adapter_of(a, pc.tag);
     const int t = threadIdx.x, row = t >> 4, c = t & 15;
     if (!PARTS && t < pc.n) a.row_adapter[pc.first + t] = ad;
     if (ad < 0) return;  // (nothing reads its rows' low products)

@@ -11,6 +11,7 @@ struct Pieces {
     const int64_t* offsets;  // [S + 1], or NULL: one segment of all positions (S = 1)
     int64_t S;
     int P;
+    const int32_t* tag;      // [S], or NULL: a number of each segment, looked up with its bounds
     __device__ inline int bound(int64_t j) const {
         if (j <= 0) return 0;
         if (j > S + 1) return P;
@@ -26,17 +27,19 @@ struct Piece {
     int s;         // of segment s (-1: of none)
     int p0, p1;    // which holds p0 .. p1 - 1
     uint32_t id0;  // and whose tiles have the numbers from id0 on
+    int tag;       // the segment's (-1: none)
 };
 // The positions of tile `id`; all lanes of a wave return the same. A wave looks at 64 pieces at a time. Where offsets fall, some tile
 // within [0, P).
 __device__ inline Piece piece_of(const Pieces& a, uint32_t id, int rows) {
     const int lane = threadIdx.x & 63;
     int64_t lo = 0, n = a.S + 2;
-    int here = 0;  // the lane's piece's bound, in the last round
+    int here = 0, tag = -1;  // the lane's piece's bound and tag, in the last round
     int64_t cnt = 0;
     for (;;) {
         const int64_t step = (n + 63) >> 6, c = lo + lane * step;
         here = a.bound(c);
+        if (a.tag && c >= 1 && c <= a.S) tag = a.tag[c - 1];
         const bool in = lane * step < n && (int64_t)((uint32_t)here / (uint32_t)rows) + c <= (int64_t)id;
         const uint64_t not_in = ~__ballot(in);
         cnt = not_in ? __builtin_ctzll(not_in) : 64;
@@ -50,6 +53,7 @@ __device__ inline Piece piece_of(const Pieces& a, uint32_t id, int rows) {
     p.p0 = __builtin_amdgcn_readlane(here, at);
     p.p1 = __builtin_amdgcn_readfirstlane(at < 63 ? __builtin_amdgcn_readlane(here, (at + 1) & 63) : a.bound(lo + 1));
     p.s = __builtin_amdgcn_readfirstlane(lo >= 1 && lo <= a.S ? (int)(lo - 1) : -1);
+    p.tag = p.s < 0 ? -1 : __builtin_amdgcn_readlane(tag, at);
     p.id0 = __builtin_amdgcn_readfirstlane((uint32_t)p.p0 / (uint32_t)rows + (uint32_t)lo);
     const int64_t first = p.p0 + (int64_t)(id - p.id0) * rows;
     const bool there = first >= p.p0 && first < p.p1;

@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256) void combine_k(CombineArgs a) {
                 for (int q = 0; q < 8; ++q) v[q] = __builtin_fmaf(w, u[q], v[q]);
             }
         }
-        finish8(a, m, c, n, v);
+        finish8<true>(a, m, c, n, v);
     }
 }
 
