@@ -545,7 +545,8 @@ static int launch_low(GroupArgs& a, hipStream_t s) {
 //   9600 x 4096 to 1024             129             135        106         106         120
 //   76800 x 128 to 512, gelu         50.5            54.8       42.9        42.3        41.4
 // and 600 x 4096 to 512 by 16 experts 33.9 with two places and 23.3 with three, whose loads are further ahead where a CU has few
-// blocks. A library's product of 9600 x 1024 by one matrix to 4096 without an epilogue takes 97. fp32, whose products are 16 times
+// blocks. 192 x 128, a block a CU, where all tiles find a CU of their own: 4800 x 1024 to 1024 by 4 matrices 18.6 (64 x 128: 20.7).
+// A library's product of 9600 x 1024 by one matrix to 4096 without an epilogue takes 97. fp32, whose products are 16 times
 // as long, and rows of any alignment take 64 x 64.
 template <class T, bool VEC, int KIND>
 static int launch_tiles(GroupArgs& a, hipStream_t s) {
@@ -556,16 +557,18 @@ static int launch_tiles(GroupArgs& a, hipStream_t s) {
             const double q = ((double)a.P / bm + ends) * ((a.N + bn - 1) / bn) / 256.0, r = q < 6.0 ? __builtin_ceil(q) : q + 0.5;
             return r < least ? least : r;
         };
-        const double c[5] = {3.9 + rounds(64, 64, 2.0) * (0.195 * k + 0.77), 2.9 + rounds(64, 64, 2.0) * (0.185 * k + 1.02),
+        const bool once = ((double)a.P / 192 + (KIND == kRowAdapters ? 1.0 : (double)a.S)) * ((a.N + 127) / 128) <= 256.0;
+        const double c[6] = {3.9 + rounds(64, 64, 2.0) * (0.195 * k + 0.77), 2.9 + rounds(64, 64, 2.0) * (0.185 * k + 1.02),
                              0.6 + rounds(64, 128, 2.0) * (0.257 * k + 2.06), 3.3 + rounds(128, 128, 1.0) * (0.495 * k + 2.87),
-                             5.1 + rounds(128, 256, 1.0) * (0.888 * k + 4.08)};
+                             5.1 + rounds(128, 256, 1.0) * (0.888 * k + 4.08), once ? 7.0 + 0.72 * k : 1e30};
         int best = 0;
-        for (int i = 1; i < 5; ++i)
+        for (int i = 1; i < 6; ++i)
             if (c[i] < c[best]) best = i;
         if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 128, 3, VEC, KIND>(a, s);
         if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
         if (best == 3) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
         if (best == 4) return launch_grouped_tile<T, 128, 256, 2, 4, 64, 3, VEC, KIND>(a, s);
+        if (best == 5) return launch_grouped_tile<T, 192, 128, 6, 2, 128, 3, VEC, KIND>(a, s);
     }
     return launch_grouped_tile<T, 64, 64, 2, 2, 128, 2, VEC, KIND>(a, s);
 }
