@@ -39,12 +39,17 @@ int products(GroupArgs& a, int type, const void* x, int64_t ldx, int K, int N, i
     return PMG_OK;
 }
 
-// The low products' form. By segment (more k of 16-byte parts in tiles that start where a segment starts) where whole tiles and parts
-// allow it and segments have 64 rows or more by the mean, else row by row in the epilogue.
+// The low products' form: more k of 16-byte parts, in tiles that start where a segment starts, where parts and whole tiles allow it and
+// the rows that tiles of 64 hold (segments fill them by mean / 64) cost less than 80 products a rank and row in the epilogue,
+// which the row form takes as long as. Measured, bf16, row form and segment form, us: 33 segments of 8 rows, K = 1024 to 4096,
+// rank 16: 24 and 38; of 40 rows: 46 and 42; K = 512 to 1024, rank 64: 42 and 17; 130 of 4 rows, 1024 to 1024, rank 16: 17 and 33; 130
+// of 40: 47 and 39.
 bool by_segment(const pmg_lora_linear_args& q) {
     const int es = type_bytes(q.type);
-    return q.offsets && q.segments >= 1 && q.M >= 64 * q.segments && at(q.x, 16) && at(q.w, 16) && at(q.down, 16) && at(q.up, 16) &&
-           q.ldx * es % 16 == 0 && q.K * es % 16 == 0 && q.rank * es % 16 == 0;
+    if (!q.offsets || q.segments < 1 || !(at(q.x, 16) && at(q.w, 16) && at(q.down, 16) && at(q.up, 16))) return false;
+    if (q.ldx * es % 16 != 0 || (int64_t)q.K * es % 16 != 0 || q.rank * es % 16 != 0) return false;
+    const double held = (double)q.segments * 64.0 * __builtin_ceil((double)q.M / 64.0 / (double)q.segments);
+    return held * q.K <= (double)q.M * (q.K + 80.0 * q.rank);
 }
 int parts_of(int type) { return type == PMG_TYPE_F32 ? kParts<float> : type == PMG_TYPE_F16 ? kParts<_Float16> : kParts<__bf16>; }
 size_t low_bytes(const pmg_lora_linear_args& q) {

@@ -374,23 +374,32 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------- the adapters' first half
-// low[m][j] = scale[i] sum_k x[m][k] down[i][j][k], i the adapter of row m's segment, for 16 rows of a segment (a row, where each
-// row is a segment) and all r <= 16 NR of its values: x is read once. For grouped_tile_k's kAdapters (PARTS) as [m][part][r] in T, fp16's
-// multiplied by a power of two that brings the row's largest value to 2^14 .. 2^15 (low_factor: its inverse), which
-// neither overflows nor is lost below 2^-24; else as [m][r] in fp32, with each row's adapter.
+// low[m][j] = scale[i] sum_k x[m][k] down[i][j][k], i the adapter of row m's segment, for 16 rows of a segment and all r <= 16 NR of
+// its values: x is read once. Where each row is a segment: for `rows` (1 or 16) rows, once for each adapter among them.
+// For grouped_tile_k's kAdapters (PARTS) as [m][part][r] in T, fp16's multiplied by a power of two that brings the row's largest
+// value to 2^14 .. 2^15 (low_factor: its inverse), which neither overflows nor is lost below 2^-24; else as [m][r] in fp32, with
+// each row's adapter.
 template <class T, int NR, int NW, bool VEC, bool PARTS>
-__global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
+__global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
     typedef typename Mat<T>::chunk chunk;
     typedef typename Mat<T>::acc16 acc16;
     constexpr int PER = Mat<T>::kPer, U = 4 / NR < 1 ? 1 : 4 / NR;
     __shared__ float red[NW][16][16 * NR + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t id = a.id0 + blockIdx.x;
-    Piece pc;
-    if (a.offsets) pc = piece_of(a, id, 16);
-    else pc = Piece{(int)id, (int)id < a.P ? 1 : 0, (int)id, (int)id, (int)id + 1, id, (int)id < a.P ? a.tag[id] : -1};
-    if (pc.n < 1) return;
-    const T* xr = (const T*)a.x + (int64_t)(pc.first + (r < pc.n ? r : pc.n - 1)) * a.ldx;
+    int first, n, tag = -1;
+    if (a.offsets) {
+        const Piece pc = piece_of(a, id, 16);
+        first = pc.first;
+        n = pc.n;
+        tag = pc.tag;
+    } else {
+        first = (int)id * rows;
+        n = a.P - first < rows ? a.P - first : rows;
+    }
+    if (n < 1) return;
+    const int mine = r < n ? r : n - 1;
+    const T* xr = (const T*)a.x + (int64_t)(first + mine) * a.ldx;
     const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
     auto get = [&](const T* p, int k) -> chunk {
         if constexpr (VEC) {
@@ -406,77 +415,84 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a) {
         for (int u = 0; u < U; ++u) fx[u] = get(xr, (4 * (s0 + u * NW) + g) * PER);
     };
     if (wave < nsteps) rows_of(wave);
-    const int ad = adapter_of(a, pc.tag);
+    const int own = adapter_of(a, a.offsets ? tag : a.tag[first + mine]);  // of the lane's row r
     const int t = threadIdx.x, row = t >> 4, c = t & 15;
-    if (!PARTS && t < pc.n) a.row_adapter[pc.first + t] = ad;
-    if (ad < 0) return;  // (nothing reads its rows' low products)
-    const float sc = a.scale ? a.scale[ad] : 1.0f;
-    const T* wr[NR];
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        const int n = 16 * j + r;
-        wr[j] = (const T*)a.down + ((int64_t)ad * a.r + (n < a.r ? n : a.r - 1)) * a.K;
-    }
-    acc16 acc[NR];
-#pragma unroll
-    for (int j = 0; j < NR; ++j) acc[j] = acc16{};
-    for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
-        chunk fw[U][NR];
-        if (s0 != wave) rows_of(s0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = (4 * (s0 + u * NW) + g) * PER;
-#pragma unroll
-            for (int j = 0; j < NR; ++j) fw[u][j] = get(wr[j], k);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < NR; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NR; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
-    __syncthreads();
-    if (t >= 256) return;
-    const int m = pc.first + row;
-    float v[NR], top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) s = s + red[w][row][16 * j + c];
-        v[j] = 16 * j + c < a.r ? s * sc : 0.0f;
-        top = __builtin_fmaxf(top, __builtin_fabsf(v[j]));
-    }
-    if constexpr (!PARTS) {
-        if (row >= pc.n) return;
-        float* h = (float*)a.low + (int64_t)m * a.r;
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-            if (16 * j + c < a.r) h[16 * j + c] = v[j];
-    } else {
-        float f = 1.0f;
-        if constexpr (__is_same(T, _Float16)) {
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 16));
-            const int e = (int)(f2u(top) >> 23);  // (0: zero or subnormal, 255: infinite)
-            const int up = 127 + 14 + 127 - e;    // exponent field of 2^14 / 2^(e - 127)
-            f = e == 255 || top == 0.0f ? 1.0f : u2f((uint32_t)(up > 247 ? 247 : up) << 23);
-            if (c == 0 && row < pc.n) a.low_factor[m] = 1.0f / f;
-        }
-        if (row >= pc.n) return;
-        T* h = (T*)a.low + (int64_t)m * kParts<T> * a.r;
+    if (!PARTS && t < n) a.row_adapter[first + t] = own;  // (t is r there)
+    uint32_t todo = (uint32_t)(__ballot(own >= 0) & (n < 16 ? (1u << n) - 1u : 0xffffu));  // rows of an adapter (nothing reads the others' low products)
+    bool again = false;
+    while (todo) {
+        const int ad = __builtin_amdgcn_readlane(own, __builtin_ctz(todo));
+        const uint32_t these = (uint32_t)__ballot(own == ad) & todo;
+        todo &= ~these;
+        const float sc = a.scale ? a.scale[ad] : 1.0f;
+        const T* wr[NR];
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
-            float x = v[j] * f;
-            const bool ends = !(__builtin_fabsf(x) < 3.0e38f);  // (infinity less itself would be NaN)
+            const int q = 16 * j + r;
+            wr[j] = (const T*)a.down + ((int64_t)ad * a.r + (q < a.r ? q : a.r - 1)) * a.K;
+        }
+        acc16 acc[NR];
 #pragma unroll
-            for (int p = 0; p < kParts<T>; ++p) {
-                const T y = (T)x;
-                if (16 * j + c < a.r) h[p * a.r + 16 * j + c] = y;
-                x = ends ? 0.0f : x - (float)y;
+        for (int j = 0; j < NR; ++j) acc[j] = acc16{};
+        for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
+            chunk fw[U][NR];
+            if (s0 != wave || again) rows_of(s0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = (4 * (s0 + u * NW) + g) * PER;
+#pragma unroll
+                for (int j = 0; j < NR; ++j) fw[u][j] = get(wr[j], k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < NR; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
+        }
+        if (again) __syncthreads();
+        again = true;
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
+        __syncthreads();
+        if (t >= 256) continue;
+        const int m = first + row;
+        const bool writes = (these >> row) & 1;
+        float v[NR], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) s = s + red[w][row][16 * j + c];
+            v[j] = 16 * j + c < a.r ? s * sc : 0.0f;
+            top = __builtin_fmaxf(top, __builtin_fabsf(v[j]));
+        }
+        if constexpr (!PARTS) {
+            float* h = (float*)a.low + (int64_t)m * a.r;
+#pragma unroll
+            for (int j = 0; j < NR; ++j)
+                if (writes && 16 * j + c < a.r) h[16 * j + c] = v[j];
+        } else {
+            float f = 1.0f;
+            if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 16));
+                const int e = (int)(f2u(top) >> 23);  // (0: zero or subnormal, 255: infinite)
+                const int up = 127 + 14 + 127 - e;    // exponent field of 2^14 / 2^(e - 127)
+                f = e == 255 || top == 0.0f ? 1.0f : u2f((uint32_t)(up > 247 ? 247 : up) << 23);
+                if (writes && c == 0) a.low_factor[m] = 1.0f / f;
+            }
+            T* h = (T*)a.low + (int64_t)m * kParts<T> * a.r;
+#pragma unroll
+            for (int j = 0; j < NR; ++j) {
+                float x = v[j] * f;
+                const bool ends = !(__builtin_fabsf(x) < 3.0e38f);  // (infinity less itself would be NaN)
+#pragma unroll
+                for (int p = 0; p < kParts<T>; ++p) {
+                    const T y = (T)x;
+                    if (writes && 16 * j + c < a.r) h[p * a.r + 16 * j + c] = y;
+                    x = ends ? 0.0f : x - (float)y;
+                }
             }
         }
     }
@@ -518,17 +534,19 @@ static int launch_grouped_rows(GroupArgs& a, hipStream_t s) {
     return PMG_OK;
 }
 
+// Without offsets a block takes a row, or 16 of many rows (which may have one adapter).
 template <class T, bool VEC, bool PARTS>
 static int launch_low(GroupArgs& a, hipStream_t s) {
-    const uint32_t ids = a.offsets ? piece_tiles(a.P, a.S, 16) : (uint32_t)a.P;
+    const int rows = a.P <= 4096 ? 1 : 16;
+    const uint32_t ids = a.offsets ? piece_tiles(a.P, a.S, 16) : (uint32_t)(((int64_t)a.P + rows - 1) / rows);
     const uint32_t most = (uint32_t)grid_blocks(512);
     for (uint32_t i = 0; i < ids; i += most) {
         a.id0 = i;
         const dim3 grid(ids - i < most ? ids - i : most);
-        if (a.r <= 16) hipLaunchKernelGGL((lora_low_k<T, 1, 8, VEC, PARTS>), grid, dim3(512), 0, s, a);
-        else if (a.r <= 32) hipLaunchKernelGGL((lora_low_k<T, 2, 8, VEC, PARTS>), grid, dim3(512), 0, s, a);
-        else if (a.r <= 64) hipLaunchKernelGGL((lora_low_k<T, 4, 4, VEC, PARTS>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((lora_low_k<T, 8, 4, VEC, PARTS>), grid, dim3(256), 0, s, a);
+        if (a.r <= 16) hipLaunchKernelGGL((lora_low_k<T, 1, 8, VEC, PARTS>), grid, dim3(512), 0, s, a, rows);
+        else if (a.r <= 32) hipLaunchKernelGGL((lora_low_k<T, 2, 8, VEC, PARTS>), grid, dim3(512), 0, s, a, rows);
+        else if (a.r <= 64) hipLaunchKernelGGL((lora_low_k<T, 4, 4, VEC, PARTS>), grid, dim3(256), 0, s, a, rows);
+        else hipLaunchKernelGGL((lora_low_k<T, 8, 4, VEC, PARTS>), grid, dim3(256), 0, s, a, rows);
         if (int e = check_launch("lora_low_k")) return e;
         if (ids - i <= most) break;
     }

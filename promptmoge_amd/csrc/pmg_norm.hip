@@ -63,7 +63,7 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
     // Rows a thread has under way twice. The loops over whole rounds of rows have neither conditional loads nor conditional stores:
     // loads and stores share one counter, and where the compiler cannot count them it waits for all of them (307,200 rows: 22 us the
     // second launch).
-    constexpr int U = SUMS && !WHOLE ? 4 : 2;
+    constexpr int U = SUMS && NT > 512 ? 4 : 2;
     const int tid = threadIdx.x;
     const int slab = (int)(blockIdx.x % (uint32_t)a.slabs);
     const uint32_t id = a.id0 + blockIdx.x / (uint32_t)a.slabs;
@@ -115,7 +115,9 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
     };
     if (!SUMS && quick) start();
     // `per` lanes of a wave share a group's sums
-    const int per = ng <= NT / 64 ? 64 : ng <= NT / 32 ? 32 : ng <= NT / 16 ? 16 : 8, g = tid / per, l = tid % per;
+    int per = 64;
+    while (per * ng > NT) per >>= 1;
+    const int g = tid / per, l = tid % per;
     double2 t{0.0, 0.0};
     if constexpr (SUMS) {
         double s[8] = {}, q[8] = {};
@@ -276,9 +278,14 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
 }
 
 struct NormPlan {
-    int slab, slabs, rows;  // rows 0: a tile is a segment
+    int slab, slabs, rows, threads;  // rows 0: a tile is a segment
     int64_t ids;
 };
+// A block a segment and slab where segments have up to 512 rows by the mean (a wave where up to 32, or up to 256 and 1024 such blocks
+// and more: 76,800 segments of one row of 256 fp16 303 us, 1000 of 40 13, 422 of 182 22; with 512 threads 2347, 43, 29), or where that is the shorter of two estimates, in
+// microseconds: a CU goes over 1000 rows of a slab in 11 (fp32 16), against two launches, 14 and the bytes of two reads and a
+// write. Measured, us, in one launch and in two: 33 segments of 700 rows of 256 fp16: 17 and 37; 33 of 2500: 33 and 67; 8 of 1200
+// of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23.
 static NormPlan norm_plan(const pmg_group_norm_args& q) {
     NormPlan p;
     const int gw = q.C / q.groups;
@@ -290,15 +297,32 @@ static NormPlan norm_plan(const pmg_group_norm_args& q) {
     if (p.slab > q.groups) p.slab = q.groups;
     p.slabs = (q.groups + p.slab - 1) / p.slab;
     p.rows = 0;
+    p.threads = 512;
     p.ids = q.segments + 2;
-    const double mean = (double)q.M / (double)(q.segments > 0 ? q.segments : 1);
-    if (mean > 512.0) {
-        const int64_t want = 256 / p.slabs - q.segments;  // (a segment ends inside a tile)
-        p.rows = (int)((q.M + (want > 1 ? want : 1) - 1) / (want > 1 ? want : 1));
-        if (p.rows < 64) p.rows = 64;
-        if (p.rows > mean) p.rows = (int)mean;
-        p.ids = piece_tiles(q.M, q.segments, p.rows);
+    const int64_t S = q.segments > 0 ? q.segments : 1;
+    const double mean = (double)q.M / (double)S;
+    if ((mean <= 32.0 || (mean <= 256.0 && S * p.slabs >= 1024)) && p.slab * gw <= 512) p.threads = 64;
+    if (mean <= 512.0) return p;
+    const int es = q.type == PMG_TYPE_F32 ? 4 : 2, os = q.out_type == PMG_TYPE_F32 ? 4 : 2;
+    const double one = 6.0 + (double)((S * p.slabs + 255) / 256) * mean * (es == 4 ? 0.016 : 0.011);
+    // (one or two rounds of a block a CU, which take 13 each whatever they do, by how much of them the segments' tiles fill; one a
+    // segment may end inside a tile)
+    const double bytes = (double)q.M * q.C * (2 * es + os) / 7.5e6;
+    double two = 1e30;
+    int64_t each = 1;
+    for (int rounds = 1; rounds <= 2; ++rounds) {
+        const int64_t want = 256 * rounds / p.slabs, e = (want - (S + 1) / 2) / S;
+        if (e < 1) continue;
+        const double t = 1.0 + 13.0 * rounds + bytes * want / (double)(S * e);
+        if (t < two) {
+            two = t;
+            each = e;
+        }
     }
+    p.threads = 1024;
+    if (one < two) return p;
+    p.rows = (int)__builtin_ceil(mean / (double)each);
+    p.ids = piece_tiles(q.M, q.segments, p.rows);
     return p;
 }
 
@@ -315,7 +339,9 @@ static int launch_norm_k(NormArgs& a, const NormPlan& pl, hipStream_t s) {
 }
 template <class T, class O>
 static int launch_norm_to(NormArgs& a, const NormPlan& pl, hipStream_t s) {
-    return pl.rows ? launch_norm_k<T, O, 1024, false, false>(a, pl, s) : launch_norm_k<T, O, 512, true, true>(a, pl, s);
+    if (pl.rows) return launch_norm_k<T, O, 1024, false, false>(a, pl, s);
+    if (pl.threads == 64) return launch_norm_k<T, O, 64, true, true>(a, pl, s);
+    return pl.threads == 512 ? launch_norm_k<T, O, 512, true, true>(a, pl, s) : launch_norm_k<T, O, 1024, true, true>(a, pl, s);
 }
 template <class T>
 static int launch_norm(NormArgs& a, const NormPlan& pl, hipStream_t s) {

@@ -60,6 +60,14 @@ def test_norm_large(gpu, dt):
     check_norm(gpu, (9_000, 9_100, 8_800, 9_050), 128, 32, dt, seed=4)
 
 
+@pytest.mark.parametrize("C,groups", [(256, 32), (64, 16), (24, 8), (7, 7), (512, 1), (4096, 2), (320, 5)])
+def test_norm_many_short_segments(gpu, C, groups):
+    g = gen(C)
+    sizes = tuple(torch.randint(0, 9, (3000,), generator=g).tolist())
+    check_norm(gpu, sizes, C, groups, F16, start=2, behind=3)
+    check_norm(gpu, (1,) * 700, C, groups, F32, act="gelu_tanh", out_dtype=BF16)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dt,out", [(F16, F16), (BF16, BF16), (F32, F32), (F32, F16), (F16, F32), (F32, BF16)])
 def test_norm_epilogues(gpu, act, dt, out):
@@ -248,6 +256,19 @@ SIZES = [((1,), 64, 16), ((0, 3, 0, 1), 128, 48), ((5, 1, 9), 72, 40), ((16, 17,
 @pytest.mark.parametrize("sizes,K,N", SIZES)
 def test_grouped_sizes(gpu, dt, sizes, K, N):
     check_grouped(gpu, cuts(gpu, *sizes), sum(sizes), K, N, dt, seed=K + N)
+
+
+def test_many_segments(gpu):
+    """More of them than a wave looks at twice, most of them empty."""
+    g = gen(11)
+    sizes = torch.zeros(9000, dtype=torch.int64)
+    sizes[torch.randint(0, 9000, (60,), generator=g)] = torch.randint(1, 30, (60,), generator=g)
+    check_grouped(gpu, cuts(gpu, *sizes.tolist(), start=3), int(sizes.sum()) + 10, 32, 24, F16)
+    check_lora(gpu, tuple(sizes.tolist()), 32, 24, 8, 5, F16, start=3, behind=7)
+    check_norm(gpu, tuple(sizes.tolist()), 64, 8, F16, start=3, behind=7)
+    sizes[[100, 5000]] = 3000
+    check_lora(gpu, tuple(sizes.tolist()), 32, 24, 8, 5, F16)
+    check_norm(gpu, tuple((sizes * 600).tolist()[4990:5010]) + (1,) * 100, 8, 8, F16)
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -449,6 +470,20 @@ def test_lora_ranks_and_sizes(gpu, dt, r, sizes, K, N):
 @pytest.mark.parametrize("M,K,N,r", [(1, 1024, 64, 8), (33, 1024, 200, 16), (17, 72, 48, 4), (130, 256, 1024, 32), (700, 64, 264, 8), (2500, 40, 130, 16)])
 def test_lora_of_single_rows(gpu, dt, M, K, N, r):
     check_lora(gpu, (1,) * M, K, N, r, 7, dt, rows=True, seed=M)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("r", [8, 24, 64, 100])
+def test_lora_of_many_single_rows(gpu, dt, r):
+    """Blocks of 16 rows that have one adapter, several in runs, or as many as there are."""
+    M, K, N, A = 4500, 64, 40, 19
+    g = gen(r)
+    x, w = randn(g, M, K).to(dt).to(gpu), (randn(g, N, K) / 8).to(dt).to(gpu)
+    down, up = (randn(g, A, r, K) / 8).to(dt).to(gpu), (randn(g, A, N, r) / math.sqrt(r)).to(dt).to(gpu)
+    for run in (1, 5, 16, 700):
+        ids = torch.randint(-2, A + 2, (M // run + 1,), generator=g, dtype=torch.int32).repeat_interleave(run)[:M].contiguous().to(gpu)
+        announce(f"lora_linear {dt} r={r}: runs of {run}")
+        assert_within(ops.lora_linear(x, w, down, up, ids), *ref.lora_linear(x, w, down, up, ids, out_dtype=dt))
 
 
 @pytest.mark.parametrize("dt", TYPES)
