@@ -682,7 +682,7 @@ enum { PMG_SCORE_SOFTMAX = 0, PMG_SCORE_SIGMOID = 1 };
 /* pmg_group_norm -- out[m][c] = act((x[m][c] - mean) rsqrt(var + eps) weight[c] + bias[c]), mean and var (of the values there are,
  *   not less one) over the rows of m's segment and the C / groups channels of c's group; sums in 64 bits, one rounding, to
  *   out_type. Rows of no segment are left as they were, or with zero_rest set to 0. out may be x (same type and stride). C 1 ..
- *   4096, M 0 .. 2^31 - 513, any alignment of whole elements. */
+ *   4096, M 0 .. 2^31 - 2049, any alignment of whole elements. */
 typedef struct {
     int type; /* f32, f16 or bf16 */
     const void* x;
@@ -729,7 +729,8 @@ int pmg_route(const pmg_route_args* args, void* workspace, size_t workspace_byte
 /* pmg_grouped_linear -- position p of segment s reads row i = index[p] of x (or row p) and gives row o = out_index[p] of the result (or
  *   row p): out[o] = act(x[i] w[s]^T + bias[s]) + residual[o], products, sums and rounding as in pmg_linear. Positions of no
  *   segment, and those whose row lies outside x or the result, write nothing; with zero_rest (without out_index) their rows are
- *   set to 0. Two positions with one result row: it gets either's (with residual = out: not said). Limits as in pmg_linear; N to
+ *   set to 0. Two positions with one result row: each of its values is either's (with residual = out:
+ *   not said). Limits as in pmg_linear; N to
  *   2^22, positions, rows of x and of the result 0 .. 2^31 - 513, segments below 2^24. Indexed rows of x that span 2 GiB and more are read
  *   element by element. */
 typedef struct {

@@ -286,8 +286,8 @@ struct NormPlan {
 // A block a segment and slab where segments have up to 512 rows by the mean (a wave where up to 32, or up to 256 and 1024 such blocks
 // and more: 76,800 segments of one row of 256 fp16 303 us, 1000 of 40 13, 422 of 182 22; with 512 threads 2347, 43, 29), or where
 // that is the shorter of two estimates, in microseconds: a CU goes over 1000 rows of a slab in 11 (fp32 16), against two launches, 14
-// and the bytes of two reads and a write. Measured, us, in one launch and in two: 33 segments of 700 rows of 256 fp16: 17 and 37; 33 of 2500: 33 and 67; 8 of 1200
-// of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23.
+// and the bytes of two reads and a write. Measured, us, in one launch and in two: 33 segments of 700 rows of 256 fp16: 17 and 37; 33
+// of 2500: 33 and 67; 8 of 1200 of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23.
 static NormPlan norm_plan(const pmg_group_norm_args& q) {
     NormPlan p;
     const int gw = q.C / q.groups;
@@ -362,7 +362,7 @@ static int norm_args(const pmg_group_norm_args& q) {
     PMG_REQUIRE(q.type >= PMG_TYPE_F32 && q.type <= PMG_TYPE_BF16, "type must be f32, f16 or bf16");
     PMG_REQUIRE(q.out_type >= PMG_TYPE_F32 && q.out_type <= PMG_TYPE_BF16, "out_type must be f32, f16 or bf16");
     PMG_REQUIRE(q.act >= PMG_ACT_NONE && q.act <= PMG_ACT_GELU_TANH, "unknown activation");
-    PMG_REQUIRE(q.M >= 0 && q.M < ((int64_t)1 << 31) - 512, "M out of range");
+    PMG_REQUIRE(q.M >= 0 && q.M < ((int64_t)1 << 31) - 2048, "M out of range");  // (a block counts a round of up to 1024 rows past the last)
     PMG_REQUIRE(q.C >= 1 && q.C <= 4096 && q.groups >= 1 && q.C % q.groups == 0, "C must be 1 .. 4096 and a multiple of groups");
     PMG_REQUIRE(q.ldx >= q.C && q.ldo >= q.C, "row strides must cover the row");
     PMG_REQUIRE(q.segments >= 0 && q.segments < (int64_t)1 << 31, "segments out of range");

@@ -1130,8 +1130,8 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
     fp32, one rounding, to out_dtype (default: out's, or x's).
 
     Positions of no segment and those whose index lies outside the rows give nothing: their rows are 0 in a new result and
-    left as they were in a given `out`, which may be the residual itself. A row named by two positions of out_index gets
-    either's result. Where offsets fall, what the rows get is not said. Forward only."""
+    left as they were in a given `out`, which may be the residual itself. Where two positions of out_index name a row, each of
+    its values is either's. Where offsets fall, what the rows get is not said. Forward only."""
     d = -1
     if x is not None and w is not None and offsets is not None:
         d = _one_gpu(x, w, offsets, bias, index, out_index, residual, out)
