@@ -16,7 +16,7 @@ struct GroupArgs : Epilogue, Pieces {  // (tag: the segments' adapters, which ma
     int K, N;
     int fresh;                // rows that no position names are set to 0
     // adapters: scale[i] (x down[i]^T) of each row, as the kernel that uses it reads it, then up [adapters][N][r]
-    const void* low;
+    const void* low;          // NULL: lora_few_k forms them itself
     float* low_factor;        // fp16 parts: what a row's sums of parts are multiplied by
     int32_t* row_adapter;     // each row's adapter, or -1
     const void* down;         // [adapters][r][K]
@@ -63,12 +63,9 @@ __device__ inline void zero8(const GroupArgs& a, int64_t m, int n0, int n) {
     else store8((_Float16*)a.out + o, n, a.vec_out, v);  // (0 is the same in both 16-bit types)
 }
 
-// v += low[m] up[row m's adapter]^T for columns n0 .. n0 + n - 1, in fp32: r products a value, one behind the other.
+// v += h up[ad]^T for columns n0 .. n0 + n - 1, in fp32: r products a value, one behind the other.
 template <class T>
-__device__ inline void add_low(const GroupArgs& a, int64_t m, int n0, int n, float (&v)[8]) {
-    const int ad = a.row_adapter[m];
-    if ((uint32_t)ad >= (uint32_t)a.adapters) return;  // (none; or where offsets fall and nothing wrote it)
-    const float* h = (const float*)a.low + m * a.r;
+__device__ inline void add_low8(const GroupArgs& a, int ad, const float* h, int n0, int n, float (&v)[8]) {
     const T* u = (const T*)a.up + ((int64_t)ad * a.N + n0) * a.r;
     typedef typename Mat<T>::chunk chunk;
     typedef T vec_t __attribute__((ext_vector_type(Mat<T>::kPer)));
@@ -93,6 +90,13 @@ __device__ inline void add_low(const GroupArgs& a, int64_t m, int n0, int n, flo
                 if (q < n) v[q] = __builtin_fmaf(t, (float)u[q * a.r + j], v[q]);
         }
     }
+}
+// The same of row m's low products and adapter, as lora_low_k wrote them.
+template <class T>
+__device__ inline void add_low(const GroupArgs& a, int64_t m, int n0, int n, float (&v)[8]) {
+    const int ad = a.row_adapter[m];
+    if ((uint32_t)ad >= (uint32_t)a.adapters) return;  // (none; or where offsets fall and nothing wrote it)
+    add_low8<T>(a, ad, (const float*)a.low + m * a.r, n0, n, v);
 }
 
 // Parts that a type's low products are carried in: their sum is fp32's value to 2^-24 of it (fp16: of the row's largest).

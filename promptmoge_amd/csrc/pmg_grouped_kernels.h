@@ -503,6 +503,111 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
     }
 }
 
+// -------------------------------------------------------------------------------------- few rows of an adapter each, in one launch
+// Up to 16 rows by 16 NC columns a block, where every row is a segment and r <= 16: each wave forms its share of k of the low
+// products too, once for each adapter among the rows (a lane keeps what its own row's adapter gave), and the epilogue adds them
+// from LDS.
+template <class T, int NC, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) void lora_few_k(GroupArgs a) {
+    typedef typename Mat<T>::chunk chunk;
+    typedef typename Mat<T>::acc16 acc16;
+    constexpr int PER = Mat<T>::kPer, U = 4, A = 4;
+    __shared__ float red[NW][16][16 * NC + 1], red_low[NW][16][17], low[16][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int first = (int)(blockIdx.x / a.tiles_n) * 16, n0 = (int)(blockIdx.x % a.tiles_n) * 16 * NC;
+    const int n = a.P - first < 16 ? a.P - first : 16, mine = r < n ? r : n - 1;
+    const T* xr = (const T*)a.x + (int64_t)(first + mine) * a.ldx;
+    const T* wr[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        const int c = n0 + 16 * j + r;
+        wr[j] = (const T*)a.w + (int64_t)(c < a.N ? c : a.N - 1) * a.K;
+    }
+    const int own = adapter_of(a, a.tag[first + mine]);  // of the lane's row r
+    const float own_scale = own >= 0 ? (a.scale ? a.scale[own] : 1.0f) : 0.0f;
+    const int t = threadIdx.x, row = t / (2 * NC), c = n0 + 8 * (t % (2 * NC));  // 8 outputs a thread
+    const int left = a.N - c < 8 ? a.N - c : 8;
+    const bool out = t < 32 * NC && row < n && left > 0;
+    float v[8];
+    bias8(a, 0, c < a.N ? c : 0, v);
+    const uint32_t rows = (uint32_t)(__ballot(own >= 0) & (n < 16 ? (1u << n) - 1u : 0xffffu));  // rows of an adapter
+    const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
+    acc16 acc[NC], acc_low = acc16{};
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[j] = acc16{};
+    auto get = [&](const T* p, int k) -> chunk {
+        if constexpr (VEC) {
+            // (a chunk behind K reads the row's first one instead and counts as zeros)
+            const chunk x = *(const chunk*)(p + (k < a.K ? k : 0));
+            return k < a.K ? x : chunk{};
+        } else {
+            return load_chunk_any<T>(p, k, a.K);
+        }
+    };
+    for (int s0 = wave; s0 < nsteps; s0 += NW * U) {
+        chunk fw[U][NC], fx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (4 * (s0 + u * NW) + g) * PER;
+            fx[u] = get(xr, k);
+#pragma unroll
+            for (int j = 0; j < NC; ++j) fw[u][j] = get(wr[j], k);
+        }
+        for (uint32_t todo = rows; todo;) {  // four adapters' loads on their way at a time
+            chunk fd[A][U];
+            int ad[A];
+#pragma unroll
+            for (int i = 0; i < A; ++i) {
+                ad[i] = todo ? __builtin_amdgcn_readlane(own, __builtin_ctz(todo)) : -1;
+                if (ad[i] < 0) continue;
+                todo &= ~(uint32_t)__ballot(own == ad[i]);
+                const T* dr = (const T*)a.down + ((int64_t)ad[i] * a.r + (r < a.r ? r : a.r - 1)) * a.K;
+#pragma unroll
+                for (int u = 0; u < U; ++u) fd[i][u] = get(dr, (4 * (s0 + u * NW) + g) * PER);
+            }
+#pragma unroll
+            for (int i = 0; i < A; ++i) {
+                if (ad[i] < 0) continue;
+                acc16 got = acc_low;
+#pragma unroll
+                for (int u = 0; u < U; ++u) got = Mat<T>::mma16(fd[i][u], fx[u], got);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc_low[e] = own == ad[i] ? got[e] : acc_low[e];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
+        red_low[wave][r][4 * g + e] = acc_low[e];
+    }
+    __syncthreads();
+    if (t < 256) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) s = s + red_low[w][t >> 4][t & 15];
+        const float sc = __shfl(own_scale, t >> 4, 64);  // (lanes 0 .. 15 of every wave hold the rows' scales)
+        low[t >> 4][t & 15] = s * sc;
+    }
+    __syncthreads();
+    if (!out) return;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) s = s + red[w][row][8 * (t % (2 * NC)) + q];
+        v[q] = s + v[q];
+    }
+    const int ad = adapter_of(a, a.tag[first + row]);
+    if (ad >= 0) add_low8<T>(a, ad, low[row], c, left, v);
+    finish8(a, first + row, c, left, v);
+}
+
 // ------------------------------------------------------------------------------------------------------------- launch
 template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC, int KIND>
 static int launch_grouped_tile(GroupArgs& a, hipStream_t s) {
@@ -604,6 +709,14 @@ int launch_experts(GroupArgs& a, bool vec, hipStream_t s) {
 
 template <class T>
 int launch_lora(GroupArgs& a, bool vec, bool by_segment, hipStream_t s) {
+    if (!a.low) {
+        constexpr int NC = 2;
+        a.tiles_n = (uint32_t)((a.N + 16 * NC - 1) / (16 * NC));
+        const dim3 grid((uint32_t)((a.P + 15) / 16) * a.tiles_n);  // (2^17 at the most)
+        if (vec) hipLaunchKernelGGL((lora_few_k<T, NC, 8, true>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((lora_few_k<T, NC, 8, false>), grid, dim3(512), 0, s, a);
+        return check_launch("lora_few_k");
+    }
     if (by_segment) {
         if (int e = launch_low<T, true, true>(a, s)) return e;
         return launch_tiles<T, true, kAdapters>(a, s);

@@ -467,7 +467,9 @@ def test_lora_ranks_and_sizes(gpu, dt, r, sizes, K, N):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("M,K,N,r", [(1, 1024, 64, 8), (33, 1024, 200, 16), (17, 72, 48, 4), (130, 256, 1024, 32), (700, 64, 264, 8), (2500, 40, 130, 16)])
+@pytest.mark.parametrize("M,K,N,r", [(1, 1024, 64, 8), (33, 1024, 200, 16), (17, 72, 48, 4), (130, 256, 1024, 32), (700, 64, 264, 8), (2500, 40, 130, 16),
+                                     (64, 2056, 40, 16), (8, 2056, 40, 8), (8, 64, 1000, 1), (3, 130, 33, 13), (4, 1024, 96, 16), (5, 33, 7, 12),
+                                     (2, 1024, 1000, 16), (9, 64, 40, 7)])
 def test_lora_of_single_rows(gpu, dt, M, K, N, r):
     check_lora(gpu, (1,) * M, K, N, r, 7, dt, rows=True, seed=M)
 

@@ -127,8 +127,10 @@ def test_workspaces_that_the_wrappers_do_not_ask_for(libpmg):
             for M in (0, 1, 63, 64):
                 assert libpmg.pmg_route_workspace_bytes(C.byref(route_args(M=M, E=E, ld=E, k=k))) == 0
     for type_ in (0, 1, 2):
-        for M, S in ((1, 1), (7, 7), (5000, 2), (1 << 20, 9)):
-            for r in (1, 8, 20, 128):
+        for M, S in ((1, 1), (7, 7), (8, 8), (9, 9), (5000, 2), (1 << 20, 9)):
+            for r in (1, 8, 9, 16, 17, 128):
+                few = lora_args(type=type_, M=M, segments=M, rank=r, offsets=None)
+                assert (libpmg.pmg_lora_linear_workspace_bytes(C.byref(few)) == 0) == (M <= 8 and r <= 16 and M * r <= 64)
                 a = lora_args(type=type_, M=M, segments=S, rank=r)
                 assert 0 < libpmg.pmg_lora_linear_workspace_bytes(C.byref(a)) <= (6 * r + 4) * M + 512
 
