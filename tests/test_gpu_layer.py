@@ -258,6 +258,29 @@ def test_grouped_sizes(gpu, dt, sizes, K, N):
     check_grouped(gpu, cuts(gpu, *sizes), sum(sizes), K, N, dt, seed=K + N)
 
 
+@pytest.mark.parametrize("table", [[0, 500, 200, 900], [900, 0, 300, 100], [-5, 700, 2 ** 40, 50], [2 ** 62, -2 ** 62, 0, 1200], [1000, 1000, 0, 0]])
+def test_falling_offsets_stay_inside(gpu, table):
+    """What the rows get is not said, but nothing around them is touched, and segments that do rise have theirs where no other takes
+    their rows."""
+    M, g = 1200, gen(3)
+    off = torch.tensor(table, device=gpu)
+    x = randn(g, M, 64).to(F16).to(gpu)
+    w = randn(g, 3, 64, 64).to(F16).to(gpu)
+    down, up = randn(g, 2, 8, 64).to(F16).to(gpu), randn(g, 2, 64, 8).to(F16).to(gpu)
+    ids = torch.tensor([0, 1, 0], dtype=torch.int32, device=gpu)
+    few = torch.tensor(table, device=gpu).clamp(-1, 40)
+    calls = [lambda o, x, off: ops.group_norm(x, 8, offsets=off, out=o), lambda o, x, off: ops.grouped_linear(x, w, off, out=o),
+             lambda o, x, off: ops.lora_linear(x, w[0], down, up, ids, offsets=off, out=o)]
+    for i, f in enumerate(calls):
+        for rows, offsets in ((M, off), (40, few)):
+            announce(f"falling offsets {table} call {i} rows {rows}")
+            buf = torch.full((rows + 64, 96), 7.0, dtype=F16, device=gpu)
+            f(buf[32:32 + rows, 16:80], x[:rows], offsets)
+            buf[32:32 + rows, 16:80] = 7.0
+            assert bool((buf == 7.0).all())
+            assert f(None, x[:rows], offsets).shape == (rows, 64)
+
+
 def test_many_segments(gpu):
     """More of them than a wave looks at twice, most of them empty."""
     g = gen(11)
