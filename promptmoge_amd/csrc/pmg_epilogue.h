@@ -4,6 +4,7 @@
 
 namespace pmg {
 
+// What the functions below take from a kernel's arguments, which derive from it or have members of these names.
 struct Epilogue {
     const void* res;  // rows of ldr or NULL
     void* out;        // rows of ldo
@@ -75,16 +76,40 @@ __device__ inline void with_act(int act, const F& f) {
 
 // act of 8 values in place; wide: for fp32 outputs.
 __device__ inline void activate8(float (&v)[8], int act, bool wide) {
-    with_act(act, [&](auto one) {
-        constexpr int ACT = decltype(one)::value;
-        if (wide) {
+    switch (act) {
+        case PMG_ACT_RELU:
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = activated<ACT, true>(v[i]);
-        } else {
+            for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_RELU, false>(v[i]);
+            break;
+        case PMG_ACT_SILU:
+            if (wide) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = activated<ACT, false>(v[i]);
-        }
-    });
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_SILU, true>(v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_SILU, false>(v[i]);
+            }
+            break;
+        case PMG_ACT_GELU:
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_GELU, true>(v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_GELU, false>(v[i]);
+            }
+            break;
+        case PMG_ACT_GELU_TANH:
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_GELU_TANH, true>(v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = activated<PMG_ACT_GELU_TANH, false>(v[i]);
+            }
+            break;
+        default: break;
+    }
 }
 
 template <class E>
@@ -129,7 +154,8 @@ __device__ inline void store8(E* p, int n, bool vec, const float (&v)[8]) {
 struct Raw8 {
     uint4 a, b;
 };
-__device__ inline Raw8 raw8(const Epilogue& a, int64_t m, int n0) {
+template <class A>
+__device__ inline Raw8 raw8(const A& a, int64_t m, int n0) {
     Raw8 r{};
     const int64_t o = m * a.ldr + n0;
     if (a.res_type == PMG_TYPE_F32) {
@@ -140,7 +166,8 @@ __device__ inline Raw8 raw8(const Epilogue& a, int64_t m, int n0) {
     }
     return r;
 }
-__device__ inline void numbers8(const Epilogue& a, const Raw8& r, float (&v)[8]) {
+template <class A>
+__device__ inline void numbers8(const A& a, const Raw8& r, float (&v)[8]) {
     if (a.res_type == PMG_TYPE_F32) {
         const v4f x = __builtin_bit_cast(v4f, r.a), y = __builtin_bit_cast(v4f, r.b);
 #pragma unroll
@@ -157,33 +184,40 @@ __device__ inline void numbers8(const Epilogue& a, const Raw8& r, float (&v)[8])
 }
 
 // n <= 8 values of the residual's row m from column n0 on, as numbers.
-__device__ inline void residual8(const Epilogue& a, int64_t m, int n0, int n, float (&r)[8]) {
+template <class A>
+__device__ inline void residual8(const A& a, int64_t m, int n0, int n, float (&r)[8]) {
     const int64_t o = m * a.ldr + n0;
     if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
     else if (a.res_type == PMG_TYPE_F16) load8((const _Float16*)a.res + o, n, a.vec_res, r);
     else load8((const __bf16*)a.res + o, n, a.vec_res, r);
 }
 // n <= 8 finished values of row m from column n0 on, rounded and stored.
-template <bool PAST = false>
-__device__ inline void put8(const Epilogue& a, int64_t m, int n0, int n, const float (&v)[8]) {
+template <bool PAST = false, class A>
+__device__ inline void put8(const A& a, int64_t m, int n0, int n, const float (&v)[8]) {
     const int64_t o = m * a.ldo + n0;
     if (a.out_type == PMG_TYPE_F32) store8<PAST>((float*)a.out + o, n, a.vec_out, v);
     else if (a.out_type == PMG_TYPE_F16) store8<PAST>((_Float16*)a.out + o, n, a.vec_out, v);
     else store8<PAST>((__bf16*)a.out + o, n, a.vec_out, v);
 }
 // n <= 8 outputs of row m from column n0 on: v holds scaled sums plus bias. `early`: the residual, if it is there already.
-template <bool PAST = false>
-__device__ inline void finish8(const Epilogue& a, int64_t m, int n0, int n, float (&v)[8], const Raw8* early = nullptr) {
+template <bool PAST = false, class A>
+__device__ inline void finish8(const A& a, int64_t m, int n0, int n, float (&v)[8], const Raw8* early = nullptr) {
     const bool wide = a.out_type == PMG_TYPE_F32;
     activate8(v, a.act, wide);
     if (a.res) {
         float r[8];
+        const int64_t o = m * a.ldr + n0;
         if (early) numbers8(a, *early, r);
-        else residual8(a, m, n0, n, r);
+        else if (a.res_type == PMG_TYPE_F32) load8((const float*)a.res + o, n, a.vec_res, r);
+        else if (a.res_type == PMG_TYPE_F16) load8((const _Float16*)a.res + o, n, a.vec_res, r);
+        else load8((const __bf16*)a.res + o, n, a.vec_res, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] + r[i];
     }
-    put8<PAST>(a, m, n0, n, v);
+    const int64_t o = m * a.ldo + n0;
+    if (a.out_type == PMG_TYPE_F32) store8<PAST>((float*)a.out + o, n, a.vec_out, v);
+    else if (a.out_type == PMG_TYPE_F16) store8<PAST>((_Float16*)a.out + o, n, a.vec_out, v);
+    else store8<PAST>((__bf16*)a.out + o, n, a.vec_out, v);
 }
 
 // 16 bytes of a row from element k on, element by element: zeros behind K (rows of any alignment).

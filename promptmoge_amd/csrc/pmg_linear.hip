@@ -14,14 +14,18 @@
 
 namespace pmg {
 
-struct LinearArgs : Epilogue {
+struct LinearArgs {
     const void* x;
     const void* w;
     const float* bias;     // [N] or NULL
     const float* w_scale;  // int8: [N] or NULL (ones)
-    int64_t M, ldx;
+    const void* res;       // [M][N] or NULL
+    void* out;
+    int64_t M, ldx, ldr, ldo;
     int K, N, ldw;
+    int act, res_type, out_type;
     float a_scale;
+    int vec_res, vec_out;  // rows of res / out take 16-byte accesses
     uint32_t tiles_n, tiles;
 };
 
