@@ -32,17 +32,25 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
     __shared__ int from[VEC ? 1 : BM];       // and in x
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const uint32_t tile = xcd_tile(blockIdx.x, a.tiles);
-    const int n0 = (int)(tile % a.tiles_n) * BN;
-    const uint32_t id = a.id0 + tile / a.tiles_n;
+    uint32_t tile;
     Piece pc;
     if constexpr (KIND == kRowAdapters) {
-        pc.first = (int)(id * BM);
+        tile = xcd_tile(blockIdx.x, a.tiles);
+        pc.first = (int)((a.id0 + tile / a.tiles_n) * BM);
         pc.n = a.P - pc.first < BM ? a.P - pc.first : BM;
         pc.s = 0;
+    } else if (a.S <= kCounted) {
+        const PieceCount c = count_pieces(a, BM, KIND == kAdapters || a.fresh);
+        const uint32_t rest = c.total > a.id0 ? c.total - a.id0 : 0u, most = a.tiles / a.tiles_n;
+        const uint32_t tiles = (rest < most ? rest : most) * a.tiles_n;
+        if (blockIdx.x >= tiles) return;
+        tile = xcd_tile(blockIdx.x, tiles);
+        pc = piece_at(a, c, a.id0 + tile / a.tiles_n, BM);
     } else {
-        pc = piece_of(a, id, BM);
+        tile = xcd_tile(blockIdx.x, a.tiles);
+        pc = piece_of(a, a.id0 + tile / a.tiles_n, BM);
     }
+    const int n0 = (int)(tile % a.tiles_n) * BN;
     if (pc.n < 1) return;
     const int rows_n = a.N - n0 < BN ? a.N - n0 : BN;
     if (KIND == kExperts && pc.s < 0) {  // positions of no segment

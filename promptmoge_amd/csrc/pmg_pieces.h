@@ -62,4 +62,42 @@ __device__ inline Piece piece_of(const Pieces& a, uint32_t id, int rows) {
     return p;
 }
 
+// Up to kCounted segments, a lane a piece: their tiles numbered without gaps, so that the blocks that have one come first and lie
+// evenly on the chip. ends: the pieces in front of the segments and behind them have tiles too. Where offsets fall, a tile within
+// [0, P) or none.
+constexpr int64_t kCounted = 62;
+struct PieceCount {
+    int here, next;       // the lane's piece: its bounds,
+    uint32_t upto, tiles; // the tiles up to its end and its own
+    uint32_t total;
+    int tag;
+};
+__device__ inline PieceCount count_pieces(const Pieces& a, int rows, bool ends) {
+    const int lane = threadIdx.x & 63;
+    PieceCount c;
+    c.here = a.bound(lane);
+    c.tag = a.tag && lane >= 1 && lane <= a.S ? a.tag[lane - 1] : -1;
+    c.next = a.bound(lane + 1);
+    if (c.next < c.here) c.next = c.here;
+    c.tiles = !ends && (lane == 0 || lane == a.S + 1) ? 0u : ((uint32_t)(c.next - c.here) + (uint32_t)rows - 1u) / (uint32_t)rows;
+    c.upto = wave_incl_scan_u32(c.tiles);
+    c.total = __builtin_amdgcn_readlane(c.upto, 63);
+    return c;
+}
+__device__ inline Piece piece_at(const Pieces& a, const PieceCount& c, uint32_t id, int rows) {
+    const uint64_t from = __ballot(c.upto > id);
+    const int at = from ? __builtin_ctzll(from) : 63;
+    Piece p;
+    p.p0 = __builtin_amdgcn_readlane(c.here, at);
+    p.p1 = __builtin_amdgcn_readlane(c.next, at);
+    p.s = at >= 1 && at <= a.S ? at - 1 : -1;
+    p.tag = __builtin_amdgcn_readlane(c.tag, at);
+    p.id0 = __builtin_amdgcn_readlane(c.upto - c.tiles, at);
+    const int64_t first = p.p0 + (int64_t)(id - p.id0) * rows;
+    const bool there = first < p.p1;
+    p.n = !there ? 0 : p.p1 - first < rows ? (int)(p.p1 - first) : rows;
+    p.first = there ? (int)first : 0;
+    return p;
+}
+
 }  // namespace pmg
