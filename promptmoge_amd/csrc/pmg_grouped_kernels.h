@@ -1,7 +1,7 @@
 // Kernels of the grouped products; both have w's rows as the matrix instruction's row operand, so that a lane holds four
 // neighbouring columns of one row of the result.
 //
-// Measured (MI355X), and what bounds it: 9600 gathered rows of 1024 bf16, 8 experts, to 4096, gelu: 114 to 125 us, 640 to 710
+// Measured (MI355X), and what bounds it: 9600 gathered rows of 1024 bf16, 8 experts, to 4096, gelu: 110 to 117 us, 690 to 730
 // TFLOP/s (the matrix units at what the chip's power leaves of their rate, a third round of tiles half full, the epilogue under them);
 // 131k rows of 256 fp16, 16 experts, to 128, scattered: 25 to 27 us, 4 TB/s; 8 rows, 8 experts, 1024 to 4096 bf16: 12 us, 44 MB of
 // weights; 4800 rows of 1024 fp16 to 1024 with adapters of rank 16 and a residual: 30 us, 6 of them the first half.
@@ -39,13 +39,17 @@ __global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 
         pc.first = (int)((a.id0 + tile / a.tiles_n) * BM);
         pc.n = a.P - pc.first < BM ? a.P - pc.first : BM;
         pc.s = 0;
-    } else if (a.S <= kCounted) {
-        const PieceCount c = count_pieces(a, BM, KIND == kAdapters || a.fresh);
-        const uint32_t rest = c.total > a.id0 ? c.total - a.id0 : 0u, most = a.tiles / a.tiles_n;
-        const uint32_t tiles = (rest < most ? rest : most) * a.tiles_n;
-        if (blockIdx.x >= tiles) return;
-        tile = xcd_tile(blockIdx.x, tiles);
-        pc = piece_at(a, c, a.id0 + tile / a.tiles_n, BM);
+    } else if (a.S <= 254) {
+        const auto counted = [&](const auto& c) {
+            const uint32_t rest = c.total > a.id0 ? c.total - a.id0 : 0u, most = a.tiles / a.tiles_n;
+            const uint32_t tiles = (rest < most ? rest : most) * a.tiles_n;
+            if (blockIdx.x >= tiles) return false;
+            tile = xcd_tile(blockIdx.x, tiles);
+            pc = c.at(a, a.id0 + tile / a.tiles_n, BM);
+            return true;
+        };
+        const bool ends = KIND == kAdapters || a.fresh;
+        if (!(a.S <= 62 ? counted(PieceCount<1>(a, BM, ends)) : counted(PieceCount<4>(a, BM, ends)))) return;
     } else {
         tile = xcd_tile(blockIdx.x, a.tiles);
         pc = piece_of(a, a.id0 + tile / a.tiles_n, BM);
@@ -671,40 +675,64 @@ static int launch_low(GroupArgs& a, hipStream_t s) {
     return PMG_OK;
 }
 
-// 16-bit tiles, by what a CU's share of them costs, fitted to the times of 20 products (within 0.6 % of the best shape's by the mean,
-// 7 % at the most): k in units of 128 bytes, in microseconds. Measured, us, rows gathered, 8 experts (the last row 4):
-//                              64 x 64, 2 places   3 places   64 x 128   128 x 128   128 x 256
-//   300 x 1024 to 1024                9.2             9.3        9.8        12.8        20.5
-//   1000 x 1024 to 1024              12.7            11.3       13.4        14.0        21.9
-//   4800 x 1024 to 1024              26.2            27.8       22.0        21.6        24.6
-//   9600 x 1024 to 4096, gelu       179             186        157         130         123
-//   9600 x 4096 to 1024             129             135        106         106         120
-//   76800 x 128 to 512, gelu         50.5            54.8       42.9        42.3        41.4
-// and 600 x 4096 to 512 by 16 experts 33.9 with two places and 23.3 with three, whose loads are further ahead where a CU has few
-// blocks. 192 x 128, a block a CU, where all tiles find a CU of their own: 4800 x 1024 to 1024 by 4 matrices 18.6 (64 x 128: 20.7).
-// A library's product of 9600 x 1024 by one matrix to 4096 without an epilogue takes 97. fp32, whose products are 16 times
-// as long, and rows of any alignment take 64 x 64.
+// Tiles by what a CU's share of them costs, in microseconds, k in units of 128 bytes, fitted to the times of 400 (16 bits) and 250
+// (fp32) products of random sizes: 2 % and 0.6 % above the best shape's by the mean, a third and 7 % at the most (uneven segments may
+// end in one tile more than the chip holds at a time). Measured, us, rows gathered, 8 segments or as many as said:
+//   bf16                       64 x 64, 2 places   3 places   64 x 128   128 x 128   128 x 256   192 x 128
+//   300 x 1024 to 1024                9.6             9.9       10.7        13.6        21.4        16.6
+//   1000 x 1024 to 1024              13.0            12.0       13.8        14.3        22.0        17.5
+//   4800 x 1024 to 1024, by 4        26.2            23.9       22.3        21.5        25.2        20.2
+//   9600 x 1024 to 4096, gelu       185             187        163         122         117         147
+//   9600 x 4096 to 1024             135             140        111         110         125         109
+//   76800 x 128 to 512, by 4, gelu   55.4            54.9       45.9        45.1        40.9        60.6
+//   600 x 4096 to 512, by 16         34.2            24.2       39.2        43.2        63.9        47.5
+//   fp32                       64 x 64, 2 places   3 of 64 bytes   64 x 128
+//   600 x 512 to 512                 15.6            16.8           22.7
+//   2048 x 2048 to 512, by 1         48.3            52.8           73.3
+//   9600 x 256 to 1024               61.8            58.2           55.5
+//   76800 x 64 to 128, by 4          24.7            22.4           23.4
+// A library's product of 9600 x 1024 bf16 by one matrix to 4096 without an epilogue takes 97, of 2048 x 2048 fp32 to 512 35. Rows of
+// any alignment take 64 x 64.
 template <class T, bool VEC, int KIND>
 static int launch_tiles(GroupArgs& a, hipStream_t s) {
-    if constexpr (VEC && sizeof(T) < 4) {
+    if constexpr (VEC) {
         const double k = (double)(((int64_t)a.K * (int)sizeof(T) + 127) / 128);
-        const double ends = KIND == kRowAdapters ? 0.0 : 0.5 * (double)a.S;  // segments end inside a tile
+        const double ends = KIND == kRowAdapters ? 0.0 : (double)(a.S - 1);  // as many segments may end inside a tile
         const auto rounds = [&](int bm, int bn, double least) {
-            const double q = ((double)a.P / bm + ends) * ((a.N + bn - 1) / bn) / 256.0, r = q < 6.0 ? __builtin_ceil(q) : q + 0.5;
-            return r < least ? least : r;
+            // fp32: the mean if none do, half, and all; else if a quarter and if three do. Fewer than `whole` are counted whole.
+            constexpr int n = sizeof(T) == 4 ? 3 : 2;
+            constexpr double whole = sizeof(T) == 4 ? 2.0 : 6.0;
+            double sum = 0.0;
+            for (int i = 0; i < n; ++i) {
+                const double some = sizeof(T) == 4 ? 0.5 * i : 0.25 + 0.5 * i;
+                const double q = (__builtin_ceil((double)a.P / bm) + some * ends) * ((a.N + bn - 1) / bn) / 256.0;
+                sum += q < whole ? __builtin_ceil(q) : q + 0.5;
+            }
+            return sum < n * least ? least : sum / n;
         };
-        const bool once = ((double)a.P / 192 + (KIND == kRowAdapters ? 1.0 : (double)a.S)) * ((a.N + 127) / 128) <= 256.0;
-        const double c[6] = {3.9 + rounds(64, 64, 2.0) * (0.195 * k + 0.77), 2.9 + rounds(64, 64, 2.0) * (0.185 * k + 1.02),
-                             0.6 + rounds(64, 128, 2.0) * (0.257 * k + 2.06), 3.3 + rounds(128, 128, 1.0) * (0.495 * k + 2.87),
-                             5.1 + rounds(128, 256, 1.0) * (0.888 * k + 4.08), once ? 7.0 + 0.72 * k : 1e30};
-        int best = 0;
-        for (int i = 1; i < 6; ++i)
-            if (c[i] < c[best]) best = i;
-        if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 128, 3, VEC, KIND>(a, s);
-        if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
-        if (best == 3) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
-        if (best == 4) return launch_grouped_tile<T, 128, 256, 2, 4, 64, 3, VEC, KIND>(a, s);
-        if (best == 5) return launch_grouped_tile<T, 192, 128, 6, 2, 128, 3, VEC, KIND>(a, s);
+        const auto cheapest = [](const auto& c) {
+            int best = 0;
+            for (int i = 1; i < (int)(sizeof(c) / sizeof(c[0])); ++i)
+                if (c[i] < c[best]) best = i;
+            return best;
+        };
+        if constexpr (sizeof(T) == 4) {
+            const double c[3] = {5.5 + 0.129 * k + rounds(64, 64, 1.0) * (0.489 * k + 1.5), 5.4 + 0.263 * k + rounds(64, 64, 1.0) * (0.477 * k + 0.8),
+                                 5.2 + 0.097 * k + rounds(64, 128, 1.0) * (k + 1.7)};
+            const int best = cheapest(c);
+            if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 64, 3, VEC, KIND>(a, s);
+            if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
+        } else {
+            const double c[6] = {1.7 + rounds(64, 64, 2.0) * (0.21 * k + 1.19), 3.2 + rounds(64, 64, 2.0) * (0.17 * k + 1.02),
+                                 1.1 + rounds(64, 128, 2.0) * (0.331 * k + 1.72), 4.3 + rounds(128, 128, 1.0) * (0.545 * k + 1.95),
+                                 6.1 + rounds(128, 256, 1.0) * (0.868 * k + 3.2), 1.5 + rounds(192, 128, 1.0) * (0.78 * k + 6.1)};
+            const int best = cheapest(c);
+            if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 128, 3, VEC, KIND>(a, s);
+            if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
+            if (best == 3) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
+            if (best == 4) return launch_grouped_tile<T, 128, 256, 2, 4, 64, 3, VEC, KIND>(a, s);
+            if (best == 5) return launch_grouped_tile<T, 192, 128, 6, 2, 128, 3, VEC, KIND>(a, s);
+        }
     }
     return launch_grouped_tile<T, 64, 64, 2, 2, 128, 2, VEC, KIND>(a, s);
 }

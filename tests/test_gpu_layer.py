@@ -397,6 +397,33 @@ def test_grouped_large(gpu, dt, sizes, K, N):
         at += n
 
 
+@pytest.mark.parametrize("dt,sizes,K,N", [(F16, (23, 17), 64, 40), (F16, (41, 19), 1032, 40), (F16, (7001, 4999), 64, 136), (BF16, (300, 2200), 64, 3000),
+                                          (BF16, (2101, 2099), 128, 3000), (F16, (3001, 1199), 520, 1000), (F32, (1, 39), 264, 40), (F32, (5000, 1003), 520, 136),
+                                          (F32, (20, 30), 64, 40), (F32, (3001, 2999), 64, 264)])
+def test_grouped_tile_shapes(gpu, dt, sizes, K, N):
+    check_grouped(gpu, cuts(gpu, *sizes, start=3), sum(sizes) + 70, K, N, dt, residual=F32)
+
+
+@pytest.mark.parametrize("S", [61, 62, 63, 126, 253, 254, 255])
+def test_numbers_of_segments(gpu, S):
+    """Around those up to which a block counts the tiles itself: empty segments, rows in front and behind."""
+    g = gen(S)
+    sizes = torch.randint(0, 70, (S,), generator=g)
+    sizes[torch.randint(0, S, (S // 4,), generator=g)] = 0
+    sizes[0], sizes[-1] = 33, 129
+    for start, behind in ((0, 0), (70, 300)):
+        M = start + int(sizes.sum()) + behind
+        for dt in (F16, F32):
+            check_grouped(gpu, cuts(gpu, *sizes.tolist(), start=start), M, 64, 72, dt)
+        check_lora(gpu, tuple(sizes.tolist()), 128, 72, 8, 5, F16, start=start, behind=behind)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_mostly_positions_of_no_segment(gpu, dt):
+    check_grouped(gpu, cuts(gpu, 40, 0, 90, start=9000), 20_000, 64, 72, dt)
+    check_lora(gpu, (40, 0, 90), 64, 72, 8, 2, dt, start=9000, behind=9000)
+
+
 def test_grouped_offsets_beyond_32_bits(gpu):
     """Rows in order behind 4 GiB, and indexed ones (which are read element by element there)."""
     M, K = 2_200_000, 1024
