@@ -1,7 +1,7 @@
 // Kernels of the grouped products; both have w's rows as the matrix instruction's row operand, so that a lane holds four
 // neighbouring columns of one row of the result.
 //
-// Measured (MI355X), and what bounds it: 9600 gathered rows of 1024 bf16, 8 experts, to 4096, gelu: 110 to 117 us, 690 to 730
+// Measured (MI355X), and what bounds it: 9600 gathered rows of 1024 bf16, 8 experts, to 4096, gelu: 110 to 120 us, 670 to 730
 // TFLOP/s (the matrix units at what the chip's power leaves of their rate, a third round of tiles half full, the epilogue under them);
 // 131k rows of 256 fp16, 16 experts, to 128, scattered: 25 to 27 us, 4 TB/s; 8 rows, 8 experts, 1024 to 4096 bf16: 12 us, 44 MB of
 // weights; 4800 rows of 1024 fp16 to 1024 with adapters of rank 16 and a residual: 30 us, 6 of them the first half.
