@@ -682,7 +682,10 @@ enum { PMG_SCORE_SOFTMAX = 0, PMG_SCORE_SIGMOID = 1 };
 /* pmg_group_norm -- out[m][c] = act((x[m][c] - mean) rsqrt(var + eps) weight[c] + bias[c]), mean and var (of the values there are,
  *   not less one) over the rows of m's segment and the C / groups channels of c's group; sums in 64 bits, one rounding, to
  *   out_type. Rows of no segment are left as they were, or with zero_rest set to 0. out may be x (same type and stride). C 1 ..
- *   4096, M 0 .. 2^31 - 2049, any alignment of whole elements. */
+ *   4096, M 0 .. 2^31 - 2049, any alignment of whole elements. The form is chosen by M / segments, for the offsets are on the device:
+ *   up to 512, each segment is one block's (a wave's where they are short) per 64 channels, so that one far longer than
+ *   the others is right but slow: 9 us for 1000 of its rows (a wave: 50), where alone it is spread over the chip. Give such
+ *   frames a call of their own. */
 typedef struct {
     int type; /* f32, f16 or bf16 */
     const void* x;

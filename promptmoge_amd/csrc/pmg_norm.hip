@@ -304,7 +304,9 @@ struct NormPlan {
 // and more: 76,800 segments of one row of 256 fp16 303 us, 1000 of 40 13, 422 of 182 22; with 512 threads 2347, 43, 29), or where
 // that is the shorter of two estimates, in microseconds: a CU goes over 1000 rows of a slab in 11 (fp32 16), against two launches, 14
 // and the bytes of two reads and a write. Measured, us, in one launch and in two: 33 segments of 700 rows of 256 fp16: 17 and 37; 33
-// of 2500: 33 and 67; 8 of 1200 of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23.
+// of 2500: 33 and 67; 8 of 1200 of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23. What this costs
+// where lengths differ: one segment of 300,000 rows of 64 fp16 among 600 of one row takes 2.7 ms (alone 31 us), one of 100,000 among
+// 20,000, which a wave goes over, 5.0 ms.
 static NormPlan norm_plan(const pmg_group_norm_args& q) {
     NormPlan p;
     const int gw = q.C / q.groups;

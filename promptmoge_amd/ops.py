@@ -1040,7 +1040,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     segment s holds the rows offsets[s] .. offsets[s + 1] - 1 (a batch's frames); without, all rows are one segment. act:
     as for linear. Sums in 64 bits, one rounding, to out_dtype (default: out's, or x's). Rows of no segment are 0 in a new
     result and left as they were in a given `out`, which may be x itself. Where offsets fall, what the rows get is
-    not said. Forward only."""
+    not said. The form goes by M / S: a segment far longer than the others, where M / S is at most 512, is right but slow (one
+    block goes over it, 9 to 50 us for 1000 rows). Forward only."""
     d = _one_gpu(x, weight, bias, offsets, out) if x is not None else -1
     if d < 0:
         d = _refuse("x", x=x, weight=weight, bias=bias, offsets=offsets, out=out)

@@ -53,3 +53,11 @@ def test_norm_rows_of_no_segment_are_everybodys(gpu, S, n, rows, C):
     announce(f"group_norm {S} segments of {n} in {rows} rows, timed")
     few, full = microseconds(lambda: ops.group_norm(x, 16, offsets=some)), microseconds(lambda: ops.group_norm(x, 16, offsets=all_))
     assert few < 3 * full, f"{few:.0f} us, {full:.0f} with all rows in segments"
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("short,n,long_,C,groups", [(300, 1, 60_000, 64, 16), (3000, 1, 20_000, 64, 16), (200, 3, 30_001, 40, 5), (40, 300, 9001, 256, 32), (1200, 2, 9000, 130, 13)])
+def test_norm_one_long_segment_among_short_ones(gpu, dt, short, n, long_, C, groups):
+    """In the form of one launch, which goes by the mean length: first, last and in the middle, by a block and by a wave."""
+    for at in (0, short // 2, short):
+        check_norm(gpu, (n,) * at + (long_,) + (n,) * (short - at), C, groups, dt, act="silu", mean=3.0, seed=at)
