@@ -806,6 +806,13 @@ typedef struct {
 size_t pmg_lora_linear_workspace_bytes(const pmg_lora_linear_args* args);
 int pmg_lora_linear(const pmg_lora_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Test hooks: which kernel takes a call, chosen from its sizes and alignment alone (nothing is launched, no buffer is read). form: int
+ * [5]: what the rows have (0: a matrix a segment, 1: tiles of one adapter, 2: an adapter a row, 3: up to eight rows in one launch), a
+ * block's rows and columns, its tiles of k in LDS at a time (0: operands straight to registers), and whether rows are read 16
+ * bytes at a time. */
+int pmg_debug_grouped_form(const pmg_grouped_linear_args* args, int* form);
+int pmg_debug_lora_form(const pmg_lora_linear_args* args, int* form);
+
 #ifdef __cplusplus
 }
 #endif

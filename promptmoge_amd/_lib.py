@@ -249,6 +249,8 @@ SIGNATURES = {
     "pmg_combine": (i32, [vp, vp]),  # CombineArgs
     "pmg_lora_linear_workspace_bytes": (sz, [vp]),  # LoraLinearArgs
     "pmg_lora_linear": (i32, [vp, vp, sz, vp]),
+    "pmg_debug_grouped_form": (i32, [vp, C.POINTER(i32)]),
+    "pmg_debug_lora_form": (i32, [vp, C.POINTER(i32)]),
 }
 
 _lib: C.CDLL | None = None

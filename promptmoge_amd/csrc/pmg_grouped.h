@@ -103,7 +103,61 @@ __device__ inline void add_low(const GroupArgs& a, int64_t m, int n0, int n, flo
 template <class T>
 constexpr int kParts = sizeof(T) == 4 ? 1 : __is_same(T, __bf16) ? 3 : 2;
 
-enum { kExperts = 0, kAdapters = 1, kRowAdapters = 2 };
+enum { kExperts = 0, kAdapters = 1, kRowAdapters = 2, kFewRows = 3 };
+
+// ------------------------------------------------------------------------------------------------- which kernel takes a call
+// Tiles by what a CU's share of them costs, in microseconds, k in units of 128 bytes, fitted to the times of 400 (16 bits) and 250
+// (fp32) products of random sizes: 2 % and 0.6 % above the best shape's by the mean, a third and 7 % at the most (uneven segments may
+// end in one tile more than the chip holds at a time). Measured, us, rows gathered, 8 segments or as many as said:
+//   bf16                       64 x 64, 2 places   3 places   64 x 128   128 x 128   128 x 256   192 x 128
+//   300 x 1024 to 1024                9.6             9.9       10.7        13.6        21.4        16.6
+//   1000 x 1024 to 1024              13.0            12.0       13.8        14.3        22.0        17.5
+//   4800 x 1024 to 1024, by 4        26.2            23.9       22.3        21.5        25.2        20.2
+//   9600 x 1024 to 4096, gelu       185             187        163         122         117         147
+//   9600 x 4096 to 1024             135             140        111         110         125         109
+//   76800 x 128 to 512, by 4, gelu   55.4            54.9       45.9        45.1        40.9        60.6
+//   600 x 4096 to 512, by 16         34.2            24.2       39.2        43.2        63.9        47.5
+//   fp32                       64 x 64, 2 places   3 of 64 bytes   64 x 128
+//   600 x 512 to 512                 15.6            16.8           22.7
+//   2048 x 2048 to 512, by 1         48.3            52.8           73.3
+//   9600 x 256 to 1024               61.8            58.2           55.5
+//   76800 x 64 to 128, by 4          24.7            22.4           23.4
+// A library's product of 9600 x 1024 bf16 by one matrix to 4096 without an epilogue takes 97, of 2048 x 2048 fp32 to 512 35. Rows of
+// any alignment take 64 x 64.
+inline int tile_shape(bool fp32, bool vec, int kind, int64_t P, int64_t S, int K, int N) {
+    if (!vec) return 0;
+    const double k = (double)(((int64_t)K * (fp32 ? 4 : 2) + 127) / 128);
+    const double ends = kind == kRowAdapters ? 0.0 : (double)(S - 1);  // as many segments may end inside a tile
+    const auto rounds = [&](int bm, int bn, double least) {
+        // fp32: the mean if none do, half, and all; else if a quarter and if three do. Fewer than `whole` are counted whole.
+        const int n = fp32 ? 3 : 2;
+        const double whole = fp32 ? 2.0 : 6.0;
+        double sum = 0.0;
+        for (int i = 0; i < n; ++i) {
+            const double some = fp32 ? 0.5 * i : 0.25 + 0.5 * i;
+            const double q = (__builtin_ceil((double)P / bm) + some * ends) * ((N + bn - 1) / bn) / 256.0;
+            sum += q < whole ? __builtin_ceil(q) : q + 0.5;
+        }
+        return sum < n * least ? least : sum / n;
+    };
+    const double f[3] = {5.5 + 0.129 * k + rounds(64, 64, 1.0) * (0.489 * k + 1.5), 5.4 + 0.263 * k + rounds(64, 64, 1.0) * (0.477 * k + 0.8),
+                         5.2 + 0.097 * k + rounds(64, 128, 1.0) * (k + 1.7)};
+    const double h[6] = {1.7 + rounds(64, 64, 2.0) * (0.21 * k + 1.19), 3.2 + rounds(64, 64, 2.0) * (0.17 * k + 1.02),
+                         1.1 + rounds(64, 128, 2.0) * (0.331 * k + 1.72), 4.3 + rounds(128, 128, 1.0) * (0.545 * k + 1.95),
+                         6.1 + rounds(128, 256, 1.0) * (0.868 * k + 3.2), 1.5 + rounds(192, 128, 1.0) * (0.78 * k + 6.1)};
+    const double* c = fp32 ? f : h;
+    int best = 0;
+    for (int i = 1; i < (fp32 ? 3 : 6); ++i)
+        if (c[i] < c[best]) best = i;
+    return best;
+}
+// Rows, columns and LDS places of each.
+constexpr int kShapes32[6][3] = {{64, 64, 2}, {64, 64, 3}, {64, 128, 2}};
+constexpr int kShapes16[6][3] = {{64, 64, 2}, {64, 64, 3}, {64, 128, 2}, {128, 128, 2}, {128, 256, 3}, {192, 128, 3}};
+
+// Experts: 16 positions a block (grouped_rows_k) where segments have no more by the mean. Row adapters: where that is 512 blocks or fewer.
+inline bool few_a_segment(int64_t P, int64_t S) { return P <= 16 * S; }
+inline bool few_outputs(int64_t P, int N) { return (P + 15) / 16 * ((N + 15) / 16) <= 512; }
 
 template <class T>
 int launch_experts(GroupArgs& a, bool vec, hipStream_t s);

@@ -68,12 +68,8 @@ int lora_args(const pmg_lora_linear_args& q, GroupArgs& a) {
     return PMG_OK;
 }
 
-}  // namespace
-
-extern "C" int pmg_grouped_linear(const pmg_grouped_linear_args* p, void* stream) {
-    PMG_REQUIRE(p, "null args");
-    const pmg_grouped_linear_args& q = *p;
-    GroupArgs a{};
+// Checks the call and fills in `a` (P stays 0 where there is nothing to do); vec: rows are read 16 bytes at a time.
+int grouped_args(const pmg_grouped_linear_args& q, GroupArgs& a, bool& vec) {
     if (int e = products(a, q.type, q.x, q.ldx, q.K, q.N, q.act, q.residual, q.residual_type, q.ldr, q.out, q.out_type, q.ldo)) return e;
     const int64_t big = ((int64_t)1 << 31) - 512;
     PMG_REQUIRE(q.positions >= 0 && q.positions < big && q.x_rows >= 0 && q.x_rows < big && q.out_rows >= 0 && q.out_rows < big, "positions or rows out of range");
@@ -97,8 +93,57 @@ extern "C" int pmg_grouped_linear(const pmg_grouped_linear_args* p, void* stream
     a.b_next = q.N;
     a.P = (int)q.positions;
     a.fresh = q.zero_rest;
-    const bool vec = at(q.x, 16) && at(q.w, 16) && q.ldx * es % 16 == 0 && (int64_t)q.K * es % 16 == 0 &&
-                     (!q.index || ((q.x_rows - 1) * q.ldx + q.K) * es < 0x7ffffff0);
+    vec = at(q.x, 16) && at(q.w, 16) && q.ldx * es % 16 == 0 && (int64_t)q.K * es % 16 == 0 &&
+          (!q.index || ((q.x_rows - 1) * q.ldx + q.K) * es < 0x7ffffff0);
+    return PMG_OK;
+}
+bool lora_vec(const pmg_lora_linear_args& q) {
+    const int es = type_bytes(q.type);
+    return at(q.x, 16) && at(q.w, 16) && at(q.down, 16) && q.ldx * es % 16 == 0 && (int64_t)q.K * es % 16 == 0;
+}
+
+int set_form(int* form, int kind, int rows, int cols, int places, bool vec) {
+    const int f[5] = {kind, rows, cols, places, vec};
+    for (int i = 0; i < 5; ++i) form[i] = f[i];
+    return PMG_OK;
+}
+int set_tile(int* form, int type, int kind, bool vec, int64_t P, int64_t S, int K, int N) {
+    const bool fp32 = type == PMG_TYPE_F32;
+    const int i = tile_shape(fp32, vec, kind, P, S, K, N);
+    const int* p = fp32 ? kShapes32[i] : kShapes16[i];
+    return set_form(form, kind, p[0], p[1], vec ? p[2] : 1, vec);
+}
+
+}  // namespace
+
+extern "C" int pmg_debug_grouped_form(const pmg_grouped_linear_args* p, int* form) {
+    PMG_REQUIRE(p && form, "null args");
+    GroupArgs a{};
+    bool vec = false;
+    if (int e = grouped_args(*p, a, vec)) return e;
+    if (few_a_segment(a.P, a.S)) return set_form(form, kExperts, 16, vec ? 32 : 16, 0, vec);
+    return set_tile(form, p->type, kExperts, vec, a.P, a.S, a.K, a.N);
+}
+
+extern "C" int pmg_debug_lora_form(const pmg_lora_linear_args* p, int* form) {
+    PMG_REQUIRE(p && form, "null args");
+    const pmg_lora_linear_args& q = *p;
+    GroupArgs a{};
+    if (int e = lora_args(q, a)) return e;
+    const bool vec = lora_vec(q);
+    if (few_rows(q)) return set_form(form, kFewRows, 8, 32, 0, vec);
+    if (by_segment(q)) return set_tile(form, q.type, kAdapters, true, q.M, q.segments, q.K, q.N);
+    if (few_outputs(q.M, q.N)) return set_form(form, kRowAdapters, 16, 16, 0, vec);
+    return set_tile(form, q.type, kRowAdapters, vec, q.M, q.segments, q.K, q.N);
+}
+
+extern "C" int pmg_grouped_linear(const pmg_grouped_linear_args* p, void* stream) {
+    PMG_REQUIRE(p, "null args");
+    const pmg_grouped_linear_args& q = *p;
+    GroupArgs a{};
+    bool vec = false;
+    if (int e = grouped_args(q, a, vec)) return e;
+    if (a.P == 0) return PMG_OK;
     hipStream_t s = (hipStream_t)stream;
     if (q.type == PMG_TYPE_F32) return launch_experts<float>(a, vec, s);
     if (q.type == PMG_TYPE_F16) return launch_experts<_Float16>(a, vec, s);
@@ -143,7 +188,7 @@ extern "C" int pmg_lora_linear(const pmg_lora_linear_args* p, void* workspace, s
     a.r = q.rank;
     a.adapters = q.adapters;
     a.vec_up = at(q.up, 16) && q.rank * es % 16 == 0;
-    const bool vec = at(q.x, 16) && at(q.w, 16) && at(q.down, 16) && q.ldx * es % 16 == 0 && (int64_t)q.K * es % 16 == 0;
+    const bool vec = lora_vec(q);
     const bool seg = by_segment(q);
     hipStream_t s = (hipStream_t)stream;
     if (q.type == PMG_TYPE_F32) return launch_lora<float>(a, vec, seg, s);

@@ -675,71 +675,33 @@ static int launch_low(GroupArgs& a, hipStream_t s) {
     return PMG_OK;
 }
 
-// Tiles by what a CU's share of them costs, in microseconds, k in units of 128 bytes, fitted to the times of 400 (16 bits) and 250
-// (fp32) products of random sizes: 2 % and 0.6 % above the best shape's by the mean, a third and 7 % at the most (uneven segments may
-// end in one tile more than the chip holds at a time). Measured, us, rows gathered, 8 segments or as many as said:
-//   bf16                       64 x 64, 2 places   3 places   64 x 128   128 x 128   128 x 256   192 x 128
-//   300 x 1024 to 1024                9.6             9.9       10.7        13.6        21.4        16.6
-//   1000 x 1024 to 1024              13.0            12.0       13.8        14.3        22.0        17.5
-//   4800 x 1024 to 1024, by 4        26.2            23.9       22.3        21.5        25.2        20.2
-//   9600 x 1024 to 4096, gelu       185             187        163         122         117         147
-//   9600 x 4096 to 1024             135             140        111         110         125         109
-//   76800 x 128 to 512, by 4, gelu   55.4            54.9       45.9        45.1        40.9        60.6
-//   600 x 4096 to 512, by 16         34.2            24.2       39.2        43.2        63.9        47.5
-//   fp32                       64 x 64, 2 places   3 of 64 bytes   64 x 128
-//   600 x 512 to 512                 15.6            16.8           22.7
-//   2048 x 2048 to 512, by 1         48.3            52.8           73.3
-//   9600 x 256 to 1024               61.8            58.2           55.5
-//   76800 x 64 to 128, by 4          24.7            22.4           23.4
-// A library's product of 9600 x 1024 bf16 by one matrix to 4096 without an epilogue takes 97, of 2048 x 2048 fp32 to 512 35. Rows of
-// any alignment take 64 x 64.
+// Shape I of tile_shape's, by WM x WN waves, tiles of KB bytes of k.
+template <class T, int I, int WM, int WN, int KB, bool VEC, int KIND>
+static int launch_shape(GroupArgs& a, hipStream_t s) {
+    constexpr const int* p = sizeof(T) == 4 ? kShapes32[I] : kShapes16[I];
+    return launch_grouped_tile<T, p[0], p[1], WM, WN, KB, p[2], VEC, KIND>(a, s);
+}
 template <class T, bool VEC, int KIND>
 static int launch_tiles(GroupArgs& a, hipStream_t s) {
     if constexpr (VEC) {
-        const double k = (double)(((int64_t)a.K * (int)sizeof(T) + 127) / 128);
-        const double ends = KIND == kRowAdapters ? 0.0 : (double)(a.S - 1);  // as many segments may end inside a tile
-        const auto rounds = [&](int bm, int bn, double least) {
-            // fp32: the mean if none do, half, and all; else if a quarter and if three do. Fewer than `whole` are counted whole.
-            constexpr int n = sizeof(T) == 4 ? 3 : 2;
-            constexpr double whole = sizeof(T) == 4 ? 2.0 : 6.0;
-            double sum = 0.0;
-            for (int i = 0; i < n; ++i) {
-                const double some = sizeof(T) == 4 ? 0.5 * i : 0.25 + 0.5 * i;
-                const double q = (__builtin_ceil((double)a.P / bm) + some * ends) * ((a.N + bn - 1) / bn) / 256.0;
-                sum += q < whole ? __builtin_ceil(q) : q + 0.5;
-            }
-            return sum < n * least ? least : sum / n;
-        };
-        const auto cheapest = [](const auto& c) {
-            int best = 0;
-            for (int i = 1; i < (int)(sizeof(c) / sizeof(c[0])); ++i)
-                if (c[i] < c[best]) best = i;
-            return best;
-        };
+        const int shape = tile_shape(sizeof(T) == 4, true, KIND, a.P, a.S, a.K, a.N);
         if constexpr (sizeof(T) == 4) {
-            const double c[3] = {5.5 + 0.129 * k + rounds(64, 64, 1.0) * (0.489 * k + 1.5), 5.4 + 0.263 * k + rounds(64, 64, 1.0) * (0.477 * k + 0.8),
-                                 5.2 + 0.097 * k + rounds(64, 128, 1.0) * (k + 1.7)};
-            const int best = cheapest(c);
-            if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 64, 3, VEC, KIND>(a, s);
-            if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
+            if (shape == 1) return launch_shape<T, 1, 2, 2, 64, VEC, KIND>(a, s);
+            if (shape == 2) return launch_shape<T, 2, 2, 4, 128, VEC, KIND>(a, s);
         } else {
-            const double c[6] = {1.7 + rounds(64, 64, 2.0) * (0.21 * k + 1.19), 3.2 + rounds(64, 64, 2.0) * (0.17 * k + 1.02),
-                                 1.1 + rounds(64, 128, 2.0) * (0.331 * k + 1.72), 4.3 + rounds(128, 128, 1.0) * (0.545 * k + 1.95),
-                                 6.1 + rounds(128, 256, 1.0) * (0.868 * k + 3.2), 1.5 + rounds(192, 128, 1.0) * (0.78 * k + 6.1)};
-            const int best = cheapest(c);
-            if (best == 1) return launch_grouped_tile<T, 64, 64, 2, 2, 128, 3, VEC, KIND>(a, s);
-            if (best == 2) return launch_grouped_tile<T, 64, 128, 2, 4, 128, 2, VEC, KIND>(a, s);
-            if (best == 3) return launch_grouped_tile<T, 128, 128, 4, 2, 128, 2, VEC, KIND>(a, s);
-            if (best == 4) return launch_grouped_tile<T, 128, 256, 2, 4, 64, 3, VEC, KIND>(a, s);
-            if (best == 5) return launch_grouped_tile<T, 192, 128, 6, 2, 128, 3, VEC, KIND>(a, s);
+            if (shape == 1) return launch_shape<T, 1, 2, 2, 128, VEC, KIND>(a, s);
+            if (shape == 2) return launch_shape<T, 2, 2, 4, 128, VEC, KIND>(a, s);
+            if (shape == 3) return launch_shape<T, 3, 4, 2, 128, VEC, KIND>(a, s);
+            if (shape == 4) return launch_shape<T, 4, 2, 4, 64, VEC, KIND>(a, s);
+            if (shape == 5) return launch_shape<T, 5, 6, 2, 128, VEC, KIND>(a, s);
         }
     }
-    return launch_grouped_tile<T, 64, 64, 2, 2, 128, 2, VEC, KIND>(a, s);
+    return launch_shape<T, 0, 2, 2, 128, VEC, KIND>(a, s);
 }
 
 template <class T>
 int launch_experts(GroupArgs& a, bool vec, hipStream_t s) {
-    if ((int64_t)a.P <= 16 * a.S) return vec ? launch_grouped_rows<T, 2, 4, 4, true, kExperts>(a, s) : launch_grouped_rows<T, 1, 4, 4, false, kExperts>(a, s);
+    if (few_a_segment(a.P, a.S)) return vec ? launch_grouped_rows<T, 2, 4, 4, true, kExperts>(a, s) : launch_grouped_rows<T, 1, 4, 4, false, kExperts>(a, s);
     return vec ? launch_tiles<T, true, kExperts>(a, s) : launch_tiles<T, false, kExperts>(a, s);
 }
 
@@ -758,7 +720,7 @@ int launch_lora(GroupArgs& a, bool vec, bool by_segment, hipStream_t s) {
         return launch_tiles<T, true, kAdapters>(a, s);
     }
     if (int e = vec ? launch_low<T, true, false>(a, s) : launch_low<T, false, false>(a, s)) return e;
-    if (((int64_t)a.P + 15) / 16 * ((a.N + 15) / 16) <= 512)
+    if (few_outputs(a.P, a.N))
         return vec ? launch_grouped_rows<T, 1, 4, 8, true, kRowAdapters>(a, s) : launch_grouped_rows<T, 1, 4, 4, false, kRowAdapters>(a, s);
     return vec ? launch_tiles<T, true, kRowAdapters>(a, s) : launch_tiles<T, false, kRowAdapters>(a, s);
 }

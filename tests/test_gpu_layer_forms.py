@@ -1,0 +1,71 @@
+"""Every kernel of grouped_linear and lora_linear at sizes that take it (layer_forms), against 64 bits on a sample of rows: those around
+the segments' borders, and every so many."""
+import math
+
+import pytest
+import torch
+
+import layer_ref as ref
+from conftest import announce
+from dense_ref import assert_within
+from layer_forms import OF_16_BITS, OF_32_BITS, form_of
+from promptmoge_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+CASES = [(F16, i) for i in range(len(OF_16_BITS))] + [(BF16, i) for i in range(len(OF_16_BITS))] + [(F32, i) for i in range(len(OF_32_BITS))]
+EPILOGUES = [("none", None, None), ("gelu", F32, F32), ("silu", None, "own"), ("gelu_tanh", F32, None), ("relu", None, F32)]  # act, out, residual
+
+
+def table(gpu, g, M, S):
+    """Offsets of S segments of different lengths, one of them empty, with rows in front and behind."""
+    cut = torch.sort(torch.randint(1, M - 2, (S + 1,), generator=g)).values
+    cut[0], cut[-1] = min(3, M // 8), M - min(5, M // 8)
+    cut = torch.cummax(cut.clamp(max=int(cut[-1])), 0).values
+    if S > 2:
+        cut[2] = cut[1]
+    return cut.to(torch.int64).to(gpu)
+
+
+@pytest.mark.parametrize("dt,i", CASES)
+def test_every_kernel(gpu, dt, i):
+    bits = 32 if dt == F32 else 16
+    (M, K, N, rank, S), form = (OF_32_BITS if bits == 32 else OF_16_BITS)[i]
+    assert form_of(_lib.lib(), bits, M, K, N, rank, S) == form
+    act, out, res = EPILOGUES[i % len(EPILOGUES)]
+    out, res = out or dt, dt if res == "own" else res
+    g, d = torch.Generator().manual_seed(i), torch.Generator(device=gpu).manual_seed(i)
+    t = lambda *shape, by=1.0: (torch.randn(shape, device=gpu, generator=d) / by).to(dt)  # noqa: E731
+    announce(f"{('grouped', 'lora')[rank > 0]} {dt} M={M} K={K} N={N} rank={rank} S={S} form={form} {act} {out} {res}")
+    x = t(M, K)
+    r = torch.randn((M, N), device=gpu, generator=d).to(res) if res else None
+    off = None if S is None else table(gpu, g, M, S)
+    ends = torch.tensor([0, M]) if off is None else off.cpu()
+    around = torch.cat([torch.arange(int(e) - 66, int(e) + 66) for e in ends[:6]] + [torch.arange(M - 140, M), torch.arange(0, M, 101)])
+    rows = around[(around >= 0) & (around < M)].unique()
+    segment = torch.full((M,), -1)
+    if off is None:
+        segment = torch.arange(M)
+    else:
+        for s in range(S):
+            segment[int(ends[s]):int(ends[s + 1])] = s
+    of, rows = segment[rows], rows.to(gpu)
+    some = r[rows] if r is not None else None
+    if not rank:
+        w, b = t(S, N, K, by=math.sqrt(K)), torch.randn((S, N), device=gpu, generator=d)
+        got = ops.grouped_linear(x, w, off, b, act=act, residual=r, out_dtype=out)
+        assert not bool(got[(segment < 0).to(gpu)].any())
+        for s in range(S):
+            m = of == s
+            if bool(m.any()):
+                mine = m.to(gpu)
+                assert_within(got[rows[mine]], *ref.linear(x[rows[mine]], w[s], b[s], act=act, residual=None if some is None else some[mine], out_dtype=out), f"segment {s}")
+        return
+    A = 5
+    w, b, sc = t(N, K, by=math.sqrt(K)), torch.randn((N,), device=gpu, generator=d), 0.25 + torch.rand((A,), device=gpu, generator=d)
+    down, up = t(A, rank, K, by=math.sqrt(K)), t(A, N, rank, by=math.sqrt(rank))
+    ids = torch.randint(-1, A, (M if S is None else S,), generator=g, dtype=torch.int32)
+    got = ops.lora_linear(x, w, down, up, ids.to(gpu), b, offsets=off, scale=sc, act=act, residual=r, out_dtype=out)
+    one = torch.where(of < 0, torch.tensor(-1, dtype=torch.int32), ids[of.clamp(min=0)])
+    assert_within(got[rows], *ref.lora_linear(x[rows], w, down, up, one, b, scale=sc, act=act, residual=some, out_dtype=out))
