@@ -8,8 +8,9 @@ import torch
 import layer_ref as ref
 from conftest import announce
 from dense_ref import assert_within
-from layer_forms import OF_16_BITS, OF_32_BITS, form_of
+from layer_forms import OF_16_BITS, OF_32_BITS, SEGMENTS, form_of
 from promptmoge_amd import _lib, ops
+from test_layer_forms import PARTS, low_case
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,18 @@ def test_every_kernel(gpu, dt, i):
     got = ops.lora_linear(x, w, down, up, ids.to(gpu), b, offsets=off, scale=sc, act=act, residual=r, out_dtype=out)
     one = torch.where(of < 0, torch.tensor(-1, dtype=torch.int32), ids[of.clamp(min=0)])
     assert_within(got[rows], *ref.lora_linear(x[rows], w, down, up, one, b, scale=sc, act=act, residual=some, out_dtype=out))
+
+
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("M,N,rank,S", [(300, 40, 16, 2), (700, 300, 8, 3), (2500, 2350, 24, 3), (300, 33, 5, 2), (50, 40, 16, None), (7, 40, 8, None), (4300, 40, 16, None)])
+def test_low_products_are_carried_to_24_bits(gpu, dt, M, N, rank, S):
+    """Low products that are whole numbers of up to 23 bits, exact in fp32, beside a projection of 0: each result is one of them times a
+    power of two, so that nothing hides what their parts leave out (that fewer parts exceed the bound: test_layer_forms)."""
+    K = 128
+    (x, down, up, sc, ids, off), _, want, tol = low_case(M, K, N, rank, S, dt)
+    form = form_of(_lib.lib(), 32 if dt == F32 else 16, M, K, N, rank, S)
+    assert (form[0] == SEGMENTS) == (S is not None and rank % 8 == 0)
+    announce(f"lora parts {dt} M={M} N={N} rank={rank} S={S} form={form} parts={PARTS[dt]}")
+    got = ops.lora_linear(x.to(gpu), torch.zeros((N, K), dtype=dt, device=gpu), down.to(gpu), up.to(gpu), ids.to(gpu), offsets=None if off is None else off.to(gpu),
+                          scale=sc.to(gpu), out_dtype=F32)
+    assert_within(got, want, tol)

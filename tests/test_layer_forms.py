@@ -4,6 +4,7 @@ import re
 from pathlib import Path
 
 import pytest
+import torch
 
 from layer_forms import EXPERTS, FEW, ROWS, SEGMENTS, cases, form_of
 from promptmoge_amd import _lib
@@ -43,3 +44,46 @@ def test_forms_of_refused_and_empty_calls(libpmg):
     refused(libpmg, libpmg.pmg_debug_lora_form(C.byref(lora_args(rank=0)), form), "rank")
     assert libpmg.pmg_debug_grouped_form(C.byref(grouped_args(positions=0)), form) == _lib.PMG_OK
     assert libpmg.pmg_debug_lora_form(C.byref(lora_args(M=0)), form) == _lib.PMG_OK
+
+
+PARTS = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}  # that a type's low products are carried in
+
+
+def low_case(M, K, N, rank, S, dt):
+    """(x, down, up, scale, adapters, offsets) of a call whose low products are whole numbers below 2^23 (255^2 K), the sums of which no
+    order rounds in fp32, times a power of two; each column of `up` has one power of two, so that a result is one of them. Then
+    (them, a column's, times what), the result, and its bound: 2^-24 of it for what the parts leave out, 2^-23 for each of their up to three sums."""
+    g = torch.Generator().manual_seed(M + rank)
+    whole = lambda *shape: torch.randint(0, 256, shape, generator=g).to(dt)  # noqa: E731
+    A = 3
+    x, down = whole(M, K), whole(A, rank, K)
+    up = torch.zeros((A, N, rank))
+    column = torch.arange(N) % rank
+    up[:, torch.arange(N), column] = 2.0 ** torch.randint(-6, 5, (A, N), generator=g)
+    sc = torch.tensor([1.0, 2.0 ** -9, -4.0])
+    ids = torch.randint(0, A, (M if S is None else S,), generator=g, dtype=torch.int32)
+    off = None if S is None else (torch.arange(S + 1) * M // S).to(torch.int64)
+    of = ids.long() if S is None else ids.long().repeat_interleave(off[1:] - off[:-1])
+    low = torch.einsum("mk,mrk->mr", x.double(), down.double()[of]) * sc.double()[of][:, None]
+    by = up.sum(-1).double()[of]
+    want = low[:, column] * by
+    return (x, down, up.to(dt), sc, ids, off), (low, column, by), want, (2.0 ** -24 + 3 * 2.0 ** -23) * want.abs()
+
+
+def in_parts(low, dt, n):
+    """Values carried as the sum of n of dt; fp16: scaled by a power of two that brings the row's largest to 2^14 .. 2^15."""
+    by = 2.0 ** (14 - torch.floor(torch.log2(low.abs().amax(-1, keepdim=True)))) if dt == torch.float16 else torch.ones(1, dtype=torch.float64)
+    rest, total = (low * by).float(), torch.zeros_like(low)
+    for _ in range(n):
+        part = rest.to(dt)
+        total, rest = total + part.double(), rest - part.float()
+    return total / by
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,N,rank,S", [(300, 40, 16, 2), (700, 300, 8, 3)])
+def test_fewer_parts_would_be_seen(dt, M, N, rank, S):
+    """The bound that the GPU's low products are held to is exceeded in most places by one part less, and kept by all of them."""
+    _, (low, column, by), want, tol = low_case(M, 128, N, rank, S, dt)
+    far = lambda n: ((in_parts(low, dt, n)[:, column] * by - want).abs() > tol).double().mean()  # noqa: E731
+    assert float(far(PARTS[dt])) == 0.0 and float(far(PARTS[dt] - 1)) > 0.5
