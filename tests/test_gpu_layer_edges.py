@@ -5,7 +5,7 @@ import torch
 import layer_ref as ref
 from conftest import announce
 from dense_ref import assert_within
-from promptmoge_amd import ops
+from promptmoge_amd import _lib, ops
 from test_gpu_layer import check_norm, cuts, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,60 @@ def test_norm_one_long_segment_among_short_ones(gpu, dt, short, n, long_, C, gro
     """In the form of one launch, which goes by the mean length: first, last and in the middle, by a block and by a wave."""
     for at in (0, short // 2, short):
         check_norm(gpu, (n,) * at + (long_,) + (n,) * (short - at), C, groups, dt, act="silu", mean=3.0, seed=at)
+
+
+# ------------------------------------------------------------------------------------------------------ falling offsets
+def falling(S, M, seed):
+    """A table that rises and falls, with bounds far outside the rows."""
+    o = torch.randint(0, M + 1, (S + 1,), generator=gen(seed), dtype=torch.int64)
+    o[seed % (S + 1)], o[(seed + 2) % (S + 1)] = 2 ** 62, -2 ** 62
+    return o
+
+
+def framed(gpu, M, C_, dt=F16):
+    """(a buffer of sevens, the M rows inside it that a call writes)."""
+    buf = torch.full((M + 64, C_ + 32), 7.0, dtype=dt, device=gpu)
+    return buf, buf[32:32 + M, 16:16 + C_]
+
+
+def untouched(buf, inside):
+    inside.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("S,M", [(2, 30_000), (4, 60_001), (3, 8000)])
+def test_falling_offsets_of_two_launches_stay_inside(gpu, S, M, seed):
+    """The norm whose workspace is addressed from the bounds: what the rows get is not said, but nothing else is written, here nor
+    in memory behind the workspace."""
+    x, off = randn(gen(seed), M, 64).to(F16).to(gpu), falling(S, M, seed).to(gpu)
+    for out in (None, framed(gpu, M, 64)):
+        to = torch.full((M, 64), 7.0, dtype=F16, device=gpu) if out is None else out[1]
+        args = _lib.GROUP_NORM_PACK.pack(_lib.TYPE_F16, x.data_ptr(), 64, M, 64, 16, 0, 0, off.data_ptr(), S, 1e-5, 0, to.data_ptr(), _lib.TYPE_F16, to.stride(0), out is None)
+        need = _lib.lib().pmg_group_norm_workspace_bytes(args)
+        assert need > 0
+        ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device=gpu)
+        announce(f"group_norm falling S={S} M={M} seed={seed}")
+        assert _lib.lib().pmg_group_norm(args, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+        assert bool((ws[need:] == 77).all())
+        if out is not None:
+            untouched(*out)
+
+
+@pytest.mark.parametrize("seed", range(3))
+@pytest.mark.parametrize("S", [40, 63, 130, 254, 255, 300])
+def test_falling_offsets_of_many_segments_stay_inside(gpu, S, seed):
+    """By one and by four segments a lane, and by the search of more."""
+    M, g = 9000, gen(seed)
+    off, x = falling(S, M, seed).to(gpu), randn(g, M, 64).to(F16).to(gpu)
+    w, down, up = randn(g, S, 64, 64).to(F16).to(gpu), randn(g, 2, 8, 64).to(F16).to(gpu), randn(g, 2, 64, 8).to(F16).to(gpu)
+    ids = torch.randint(-1, 2, (S,), generator=g, dtype=torch.int32).to(gpu)
+    index = torch.randint(0, M, (M,), generator=g, dtype=torch.int32).to(gpu)
+    calls = [lambda o: ops.group_norm(x, 8, offsets=off, out=o), lambda o: ops.grouped_linear(x, w, off, out=o), lambda o: ops.grouped_linear(x, w, off, index=index, out=o),
+             lambda o: ops.lora_linear(x, w[0], down, up, ids, offsets=off, out=o)]
+    for i, f in enumerate(calls):
+        announce(f"falling offsets S={S} seed={seed} call {i}")
+        buf, inside = framed(gpu, M, 64)
+        f(inside)
+        untouched(buf, inside)
+        assert f(None).shape == (M, 64)
