@@ -157,6 +157,7 @@ constexpr int kShapes16[6][3] = {{64, 64, 2}, {64, 64, 3}, {64, 128, 2}, {128, 1
 
 // Experts: 16 positions a block (grouped_rows_k) where segments have no more by the mean. Row adapters: where that is 512 blocks or fewer.
 inline bool few_a_segment(int64_t P, int64_t S) { return P <= 16 * S; }
+constexpr int kFew = 8;  // rows that lora_few_k takes at the most
 inline bool few_outputs(int64_t P, int N) { return (P + 15) / 16 * ((N + 15) / 16) <= 512; }
 
 template <class T>

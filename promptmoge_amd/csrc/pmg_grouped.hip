@@ -53,7 +53,7 @@ bool by_segment(const pmg_lora_linear_args& q) {
 }
 // Up to eight rows of an adapter each are done in one launch, without a workspace, where their ranks add up to 64 at most: one row of
 // 1024 bf16 to 1024, rank 8, 7.2 us for 8.6 in two, 8 rows 10.9 for 9.1, but 8.2 and 12 for 12.8 a call from Python; 33 rows 13.5 for 9.6.
-bool few_rows(const pmg_lora_linear_args& q) { return !q.offsets && q.M <= 8 && q.rank <= 16 && q.M * q.rank <= 64; }
+bool few_rows(const pmg_lora_linear_args& q) { return !q.offsets && q.M <= kFew && q.rank <= 16 && q.M * q.rank <= 64; }
 int parts_of(int type) { return type == PMG_TYPE_F32 ? kParts<float> : type == PMG_TYPE_F16 ? kParts<_Float16> : kParts<__bf16>; }
 size_t low_bytes(const pmg_lora_linear_args& q) {
     return up256((size_t)q.M * (size_t)q.rank * (by_segment(q) ? (size_t)(parts_of(q.type) * type_bytes(q.type)) : sizeof(float)));
@@ -131,7 +131,7 @@ extern "C" int pmg_debug_lora_form(const pmg_lora_linear_args* p, int* form) {
     GroupArgs a{};
     if (int e = lora_args(q, a)) return e;
     const bool vec = lora_vec(q);
-    if (few_rows(q)) return set_form(form, kFewRows, 8, 32, 0, vec);
+    if (few_rows(q)) return set_form(form, kFewRows, kFew, 32, 0, vec);
     if (by_segment(q)) return set_tile(form, q.type, kAdapters, true, q.M, q.segments, q.K, q.N);
     if (few_outputs(q.M, q.N)) return set_form(form, kRowAdapters, 16, 16, 0, vec);
     return set_tile(form, q.type, kRowAdapters, vec, q.M, q.segments, q.K, q.N);

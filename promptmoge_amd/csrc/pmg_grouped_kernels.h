@@ -19,7 +19,7 @@ constexpr uint32_t kBehind = 0x7ffffff0u;  // an offset behind every buffer's en
 // kAdapters: the low products come in front, as more k: rows of x's parts against `up` as often, their sums multiplied
 // by the row's factor before the k of x and w.
 template <class T, int BM, int BN, int WM, int WN, int KB, int NS, bool VEC, int KIND>
-__global__ __launch_bounds__(64 * WM * WN, (BM / WM) * (BN / WN) >= 128 * 128 ? 1 : 2) void grouped_tile_k(GroupArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_tile_k(GroupArgs a) {
     static_assert(KIND != kAdapters || VEC, "parts are read 16 bytes at a time");
     constexpr int NW = WM * WN, NT = 64 * NW, KE = KB / (int)sizeof(T), PER = Mat<T>::kPer, ES = (int)sizeof(T);
     constexpr int CPR = KB / 16, RPL = 64 / CPR, STEPS = CPR / 2;  // chunks a row, rows a load, steps a tile
@@ -516,33 +516,32 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
 }
 
 // -------------------------------------------------------------------------------------- few rows of an adapter each, in one launch
-// Up to 16 rows by 16 NC columns a block, where every row is a segment and r <= 16: each wave forms its share of k of the low
-// products too, once for each adapter among the rows (a lane keeps what its own row's adapter gave), and the epilogue adds them
-// from LDS.
+// All rows, kFew at the most, by 16 NC columns a block, where every row is a segment and r <= 16: each wave forms its share of k of
+// the low products too, once for each adapter among the rows (a lane keeps what its own row's adapter gave), and the epilogue adds
+// them from LDS. What the matrix instruction has of rows behind the last is not kept.
 template <class T, int NC, int NW, bool VEC>
 __global__ __launch_bounds__(64 * NW) void lora_few_k(GroupArgs a) {
     typedef typename Mat<T>::chunk chunk;
     typedef typename Mat<T>::acc16 acc16;
-    constexpr int PER = Mat<T>::kPer, U = 4, A = 4;
-    __shared__ float red[NW][16][16 * NC + 1], red_low[NW][16][17], low[16][16];
+    constexpr int PER = Mat<T>::kPer, U = 4, A = 4, R = kFew;
+    __shared__ float red[NW][R][16 * NC + 1], red_low[NW][R][17], low[R][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int first = (int)(blockIdx.x / a.tiles_n) * 16, n0 = (int)(blockIdx.x % a.tiles_n) * 16 * NC;
-    const int n = a.P - first < 16 ? a.P - first : 16, mine = r < n ? r : n - 1;
-    const T* xr = (const T*)a.x + (int64_t)(first + mine) * a.ldx;
+    const int n0 = (int)blockIdx.x * 16 * NC, n = a.P, mine = r < n ? r : n - 1;
+    const T* xr = (const T*)a.x + (int64_t)mine * a.ldx;
     const T* wr[NC];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
         const int c = n0 + 16 * j + r;
         wr[j] = (const T*)a.w + (int64_t)(c < a.N ? c : a.N - 1) * a.K;
     }
-    const int own = adapter_of(a, a.tag[first + mine]);  // of the lane's row r
+    const int own = adapter_of(a, a.tag[mine]);  // of the lane's row r
     const float own_scale = own >= 0 ? (a.scale ? a.scale[own] : 1.0f) : 0.0f;
     const int t = threadIdx.x, row = t / (2 * NC), c = n0 + 8 * (t % (2 * NC));  // 8 outputs a thread
     const int left = a.N - c < 8 ? a.N - c : 8;
-    const bool out = t < 32 * NC && row < n && left > 0;
+    const bool out = row < n && left > 0;
     float v[8];
     bias8(a, 0, c < a.N ? c : 0, v);
-    const uint32_t rows = (uint32_t)(__ballot(own >= 0) & (n < 16 ? (1u << n) - 1u : 0xffffu));  // rows of an adapter
+    const uint32_t rows = (uint32_t)(__ballot(own >= 0) & ((1u << n) - 1u));  // rows of an adapter
     const int nsteps = (a.K + 4 * PER - 1) / (4 * PER);
     acc16 acc[NC], acc_low = acc16{};
 #pragma unroll
@@ -592,18 +591,20 @@ __global__ __launch_bounds__(64 * NW) void lora_few_k(GroupArgs a) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) acc[j] = Mat<T>::mma16(fw[u][j], fx[u], acc[j]);
     }
+    if (r < R) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
-        red_low[wave][r][4 * g + e] = acc_low[e];
+            for (int j = 0; j < NC; ++j) red[wave][r][16 * j + 4 * g + e] = acc[j][e];
+            red_low[wave][r][4 * g + e] = acc_low[e];
+        }
     }
     __syncthreads();
-    if (t < 256) {
+    if (t < 16 * R) {
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) s = s + red_low[w][t >> 4][t & 15];
-        const float sc = __shfl(own_scale, t >> 4, 64);  // (lanes 0 .. 15 of every wave hold the rows' scales)
+        const float sc = __shfl(own_scale, t >> 4, 64);  // (lanes 0 .. R - 1 of every wave hold the rows' scales)
         low[t >> 4][t & 15] = s * sc;
     }
     __syncthreads();
@@ -615,9 +616,9 @@ __global__ __launch_bounds__(64 * NW) void lora_few_k(GroupArgs a) {
         for (int w = 0; w < NW; ++w) s = s + red[w][row][8 * (t % (2 * NC)) + q];
         v[q] = s + v[q];
     }
-    const int ad = adapter_of(a, a.tag[first + row]);
+    const int ad = adapter_of(a, a.tag[row]);
     if (ad >= 0) add_low8<T>(a, ad, low[row], c, left, v);
-    finish8(a, first + row, c, left, v);
+    finish8(a, row, c, left, v);
 }
 
 // ------------------------------------------------------------------------------------------------------------- launch
@@ -709,8 +710,7 @@ template <class T>
 int launch_lora(GroupArgs& a, bool vec, bool by_segment, hipStream_t s) {
     if (!a.low) {
         constexpr int NC = 2;
-        a.tiles_n = (uint32_t)((a.N + 16 * NC - 1) / (16 * NC));
-        const dim3 grid((uint32_t)((a.P + 15) / 16) * a.tiles_n);  // (2^17 at the most)
+        const dim3 grid((uint32_t)((a.N + 16 * NC - 1) / (16 * NC)));  // (2^17 at the most)
         if (vec) hipLaunchKernelGGL((lora_few_k<T, NC, 8, true>), grid, dim3(512), 0, s, a);
         else hipLaunchKernelGGL((lora_few_k<T, NC, 8, false>), grid, dim3(512), 0, s, a);
         return check_launch("lora_few_k");
