@@ -118,3 +118,11 @@ def test_falling_offsets_of_many_segments_stay_inside(gpu, S, seed):
         f(inside)
         untouched(buf, inside)
         assert f(None).shape == (M, 64)
+
+
+# --------------------------------------------------------------------------------------------------------------- route
+@pytest.mark.parametrize("M,E,k", [(1, 16, 2), (64, 1024, 32), (65, 16, 2), (100, 8, 2), (300, 64, 4), (5000, 16, 2), (5000, 1024, 1)])
+def test_route_keeps_little_beside_its_tables(gpu, M, E, k):
+    r = ops.route(randn(gen(1), M, E).to(gpu), k)
+    kept = sum({t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in r}.values())
+    assert kept <= sum(t.nbytes for t in r) + 4 * min((M + 15) // 16 * (E + 1), 32_768)

@@ -1,4 +1,4 @@
-"""Which kernel takes a call of grouped_linear and lora_linear, asked of the library without a GPU."""
+"""Which kernel takes a call of grouped_linear and lora_linear, and what route asks for, asked of the library without a GPU."""
 import ctypes as C
 import re
 from pathlib import Path
@@ -8,7 +8,7 @@ import torch
 
 from layer_forms import EXPERTS, FEW, ROWS, SEGMENTS, cases, form_of
 from promptmoge_amd import _lib
-from test_layer_abi import grouped_args, lora_args, refused
+from test_layer_abi import grouped_args, lora_args, refused, route_args
 
 CSRC = Path(__file__).resolve().parents[1] / "promptmoge_amd" / "csrc"
 
@@ -87,3 +87,12 @@ def test_fewer_parts_would_be_seen(dt, M, N, rank, S):
     _, (low, column, by), want, tol = low_case(M, 128, N, rank, S, dt)
     far = lambda n: ((in_parts(low, dt, n)[:, column] * by - want).abs() > tol).double().mean()  # noqa: E731
     assert float(far(PARTS[dt])) == 0.0 and float(far(PARTS[dt] - 1)) > 0.5
+
+
+def test_routes_need_a_count_of_each_expert_for_16_rows_at_the_most(libpmg):
+    """What the wrapper gives them beside its tables."""
+    for E in (1, 2, 3, 8, 16, 63, 64, 65, 100, 128, 129, 256, 300, 512, 513, 1000, 1024):
+        for k in {1, min(E, 2), min(E, 5), min(E, 9), min(E, 17), min(E, 32)}:
+            for M in (*range(65, 400), 500, 1000, 1023, 1025, 4095, 4097, 8191, 8193, 20_000, 76_800, 1_000_000):
+                need = libpmg.pmg_route_workspace_bytes(C.byref(route_args(M=M, E=E, ld=E, k=k)))
+                assert need <= 4 * min((M + 15) // 16 * (E + 1), 32_768), (M, E, k)
