@@ -708,7 +708,8 @@ int pmg_group_norm(const pmg_group_norm_args* args, void* workspace, size_t work
 
 /* pmg_route -- each row's k experts of largest logit (equal ones: the lowest index first; -inf and NaN are not chosen), and the pairs
  *   m k + slot in the order of their experts, equal ones in their own order.
- *   weights [M][k]: the chosen experts' softmax over the row's E logits, or sigmoid; normalize: over the sum of the row's.
+ *   weights [M][k]: the chosen experts' softmax over the row's E logits, or sigmoid; normalize: over the sum of the row's. A softmax
+ *   over a NaN or +inf is NaN, as its sum is: so are the weights of such a row's chosen experts.
  *   experts [M][k]: -1 (weight 0) for a slot without an expert, and in rows with mask[m] = 0. offsets [E + 1]: where
  *   each expert's pairs start; pairs [M k] and rows [M k] (pair / k): -1 from offsets[E] on.
  *   fp32 arithmetic on the logits of any type. E 1 .. 1024, k 1 .. 32 and at most E, M k below 2^31 - 512. */

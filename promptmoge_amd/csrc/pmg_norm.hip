@@ -232,8 +232,8 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
         return;
     } else {
         if (g < ng && l == 0) {
-            // (quotient and root by one step of Newton each on the unit's values, to 2^-40 and better: a few instructions, where the
-            // library's take a kilobyte of code)
+            // (the quotient by two steps of Newton, the root by one, on the unit's values, to 2^-40 and better: a few instructions,
+            // where the library's take a kilobyte of code)
             const double count = (double)(p.p1 - p.p0) * (double)a.gw;
             double one = __builtin_amdgcn_rcp(count);
             one = __builtin_fma(__builtin_fma(-count, one, 1.0), one, one);
@@ -301,7 +301,7 @@ struct NormPlan {
     int64_t ids;
 };
 // A block a segment and slab where segments have up to 512 rows by the mean (a wave where up to 32, or up to 256 and 1024 such blocks
-// and more: 76,800 segments of one row of 256 fp16 303 us, 1000 of 40 13, 422 of 182 22; with 512 threads 2347, 43, 29), or where
+// and more: 76,800 segments of one row of 256 fp16 303 to 358 us, 1000 of 40 13, 422 of 182 22; with 512 threads 2347, 43, 29), or where
 // that is the shorter of two estimates, in microseconds: a CU goes over 1000 rows of a slab in 11 (fp32 16), against two launches, 14
 // and the bytes of two reads and a write. Measured, us, in one launch and in two: 33 segments of 700 rows of 256 fp16: 17 and 37; 33
 // of 2500: 33 and 67; 8 of 1200 of 1024: 22 and 26; 16 of 4800 of 128: 50 and 25; 4 of 2745 of 512 fp32: 47 and 23. What this costs

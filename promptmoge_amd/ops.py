@@ -1091,8 +1091,8 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", normalize: bo
 
     logits: (M, E) fp32 / fp16 / bf16 (rows may be strided), E up to 1024, k up to 32; score: "softmax" over the row's
     logits, or "sigmoid"; normalize: the weights over the sum of the row's. An expert whose logit is -inf or NaN is not
-    chosen: the slot holds -1 and weight 0. So do the rows with 0 in mask, (M,) bool / uint8, whose pairs come
-    in no segment. Forward only."""
+    chosen: the slot holds -1 and weight 0 (the others' softmax over a row with a NaN or +inf is NaN, as its sum is). So do
+    the rows with 0 in mask, (M,) bool / uint8, whose pairs come in no segment. Forward only."""
     d = _one_gpu(logits, mask) if logits is not None else -1
     if d < 0:
         d = _refuse("logits", logits=logits, mask=mask)
