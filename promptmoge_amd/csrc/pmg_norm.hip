@@ -3,7 +3,7 @@
 //
 // Sums of x and x^2 are held in 64 bits: their products are exact and nothing overflows, and mean and var come out to fp32's
 // accuracy where the mean is 10^4 times the spread (for fp32 inputs E[x^2] - mean^2 in 64 bits loses 2^-53 (mean / spread)^2).
-// The mean is subtracted in two fp32 parts.
+// The mean is subtracted in two fp32 parts; spreads near the ends of fp32's range are brought inside by a power of two.
 //
 // Measured (MI355X), and what bounds it: 307,200 rows of 64 fp16 with silu 31 us (11 the sums, 19 the results; two reads and a write
 // are 23 at a copy's rate, the rest is a block's start: its segment, the segment's sums, a barrier); 4 x 2745 rows of 512 fp32 to bf16
@@ -30,8 +30,14 @@ struct NormArgs : Epilogue, Pieces {
 constexpr int kRest = 2048;  // blocks that rows of no segment are shared out over
 
 struct Stat {
-    float hi, lo, r;  // mean in two parts, 1 / spread
+    float hi, lo, r;  // mean in two parts, 1 / spread; r < 0: -1 / spread, all of the values times a power of two (times())
 };
+// What a group's values are taken times before its mean is subtracted: 1, but where the spread is at an end of fp32's range.
+__device__ inline float times(const Stat& st) { return st.r < 0.0f ? st.r > -1.0f ? 0x1p-64f : 0x1p64f : 1.0f; }
+
+// Types whose values have fp32's range.
+template <class T>
+constexpr bool kWide = !__is_same(T, _Float16);
 
 // 8 values of a row as they lie in memory (16-bit types: the first half), and as numbers.
 template <class T, bool VEC>
@@ -247,29 +253,49 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
             st.hi = (float)mean;
             st.lo = (float)(mean - (double)st.hi);
             st.r = (float)r;
+            if (kWide<T> && !(st.r > 0x1p-100f && st.r < 0x1p100f)) {
+                // Differences from the mean could overflow, or 1 / spread could (eps 0). (A mean above 1 has no differences that small.)
+                const bool large = st.r < 1.0f, small = st.r > 1.0f && mean < 1.0 && mean > -1.0;
+                if (large || small) {
+                    const double by = large ? 0x1p-64 : 0x1p64;
+                    st.hi = (float)(mean * by);
+                    st.lo = (float)(mean * by - (double)st.hi);
+                    st.r = -(float)(r * (large ? 0x1p64 : 0x1p-64));
+                }
+            }
             stats[g] = st;
         }
         __syncthreads();
         if (!busy) return;
         // per channel: x less the mean (two parts), times scale, plus shift
         float hi[8], lo[8], scale[8];
+        bool far = false;  // some are taken times a power of two first
+        const auto stat = [&](int i) { return stats[(c - c0 + (i < n ? i : n - 1)) / a.gw]; };
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const Stat st = stats[(c - c0 + (i < n ? i : n - 1)) / a.gw];
+            const Stat st = stat(i);
             hi[i] = st.hi;
             lo[i] = st.lo;
-            scale[i] = st.r * weight[i];
+            scale[i] = (kWide<T> ? __builtin_fabsf(st.r) : st.r) * weight[i];
+            if (kWide<T>) far = far || st.r < 0.0f;
         }
         // (a loop for each activation, short: what a block has to fetch of its code for the first time costs it a microsecond a
         // few KB)
         with_act(a.act, [&](auto one) {
-            const auto result = [&](const Raw8& raw, float (&v)[8]) {
+            const auto result = [&](const Raw8& raw, float (&v)[8], bool scaled) {
                 norm_numbers<T>(raw, v);
+                if (scaled)
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        const float by = times(stat(i));
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = q == i ? v[q] * by : v[q];
+                    }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = activated<decltype(one)::value, sizeof(O) == 4>(__builtin_fmaf((v[i] - hi[i]) - lo[i], scale[i], shift[i]));
             };
             int r = ty;
-            if (quick) {
+            if (quick && !(kWide<T> && far)) {
                 if constexpr (SUMS) start();
 #pragma unroll 1
                 for (int j = 0; j < rounds; ++j) {
@@ -278,7 +304,7 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         float v[8];
-                        result(now[u], v);
+                        result(now[u], v, false);
                         store8((O*)a.out + row(j * U + u) * a.ldo + c, 8, true, v);
                     }
 #pragma unroll
@@ -289,7 +315,7 @@ __global__ __launch_bounds__(NT) void norm_k(NormArgs a) {
 #pragma unroll 1
             for (; r < p.n; r += deep) {
                 float v[8];
-                result(norm_get<T, false>(a, p.first + r, c, n), v);
+                result(norm_get<T, false>(a, p.first + r, c, n), v, kWide<T> && far);
                 store8((O*)a.out + (int64_t)(p.first + r) * a.ldo + c, n, a.vec_out, v);
             }
         });

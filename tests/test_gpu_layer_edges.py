@@ -63,6 +63,21 @@ def test_norm_one_long_segment_among_short_ones(gpu, dt, short, n, long_, C, gro
         check_norm(gpu, (n,) * at + (long_,) + (n,) * (short - at), C, groups, dt, act="silu", mean=3.0, seed=at)
 
 
+@pytest.mark.parametrize("dt,out", [(F32, F32), (BF16, BF16), (F32, BF16), (BF16, F16)])
+@pytest.mark.parametrize("sizes", [(30,), (300, 20), (1,) * 70 + (40,), (2000,), (9000, 7000)])
+def test_norm_spreads_at_the_ends_of_the_range(gpu, dt, out, sizes):
+    """Values up to the type's largest, of either sign, whose differences overflow fp32, and down to its least without eps, whose
+    spread's reciprocal does; groups in the middle of the range beside them."""
+    M, C, G, g = sum(sizes), 64, 8, gen(len(sizes))
+    largest = torch.finfo(dt).max
+    big = torch.where(torch.rand(M, C, generator=g) < 0.3, -largest, largest) * (1 - torch.rand(M, C, generator=g) / 64)
+    for by, eps in (({0: big, 3: big}, 1e-5), ({1: randn(g, M, C) * 1e-38, 7: randn(g, M, C) * 1e-36}, 0.0), ({2: big, 5: randn(g, M, C) * 1e-37}, 0.0)):
+        x = randn(g, M, C)
+        for group, v in by.items():
+            x[:, 8 * group:8 * group + 8] = v[:, 8 * group:8 * group + 8]
+        check_norm(gpu, sizes, C, G, dt, out_dtype=out, act="silu", x=x.to(dt).to(gpu), eps=eps)
+
+
 # ------------------------------------------------------------------------------------------------------ falling offsets
 def falling(S, M, seed):
     """A table that rises and falls, with bounds far outside the rows."""
