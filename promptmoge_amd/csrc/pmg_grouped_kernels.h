@@ -394,7 +394,7 @@ __global__ __launch_bounds__(64 * NW) void grouped_rows_k(GroupArgs a) {
 // low[m][j] = scale[i] sum_k x[m][k] down[i][j][k], i the adapter of row m's segment, for 16 rows of a segment and all r <= 16 NR of
 // its values: x is read once. Where each row is a segment: for `rows` (1 or 16) rows, once for each adapter among them.
 // For grouped_tile_k's kAdapters (PARTS) as [m][part][r] in T, fp16's multiplied by a power of two that brings the row's largest
-// value to 2^14 .. 2^15 (low_factor: its inverse), which neither overflows nor is lost below 2^-24; else as [m][r] in fp32, with
+// finite value to 2^14 .. 2^15 (low_factor: its inverse), which neither overflows nor is lost below 2^-24; else as [m][r] in fp32, with
 // each row's adapter.
 template <class T, int NR, int NW, bool VEC, bool PARTS>
 __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
 #pragma unroll
             for (int w = 0; w < NW; ++w) s = s + red[w][row][16 * j + c];
             v[j] = 16 * j + c < a.r ? s * sc : 0.0f;
-            top = __builtin_fmaxf(top, __builtin_fabsf(v[j]));
+            top = __builtin_fabsf(v[j]) < __builtin_inff() ? __builtin_fmaxf(top, __builtin_fabsf(v[j])) : top;
         }
         if constexpr (!PARTS) {
             float* h = (float*)a.low + (int64_t)m * a.r;
@@ -494,9 +494,9 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
             if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
                 for (int o = 1; o < 16; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 16));
-                const int e = (int)(f2u(top) >> 23);  // (0: zero or subnormal, 255: infinite)
+                const int e = (int)(f2u(top) >> 23);  // (0: zero or subnormal)
                 const int up = 127 + 14 + 127 - e;    // exponent field of 2^14 / 2^(e - 127)
-                f = e == 255 || top == 0.0f ? 1.0f : u2f((uint32_t)(up > 247 ? 247 : up) << 23);
+                f = top == 0.0f ? 1.0f : u2f((uint32_t)(up > 247 ? 247 : up) << 23);
                 if (writes && c == 0) a.low_factor[m] = 1.0f / f;
             }
             T* h = (T*)a.low + (int64_t)m * kParts<T> * a.r;

@@ -85,3 +85,21 @@ def test_low_products_are_carried_to_24_bits(gpu, dt, M, N, rank, S):
     got = ops.lora_linear(x.to(gpu), torch.zeros((N, K), dtype=dt, device=gpu), down.to(gpu), up.to(gpu), ids.to(gpu), offsets=None if off is None else off.to(gpu),
                           scale=sc.to(gpu), out_dtype=F32)
     assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("S", [3, None])
+def test_an_infinite_low_product_leaves_the_others_finite(gpu, dt, S):
+    """An adapter with an infinity: its rows' results are infinite, of the sign that `up` gives that one, for the others (above fp16's
+    largest) stay finite beside it."""
+    M, K, N, rank, g = 200, 64, 24, 8, torch.Generator().manual_seed(1)
+    x, down = torch.randint(1, 9, (M, K), generator=g) * 128.0, torch.randint(1, 9, (2, rank, K), generator=g) * 128.0
+    up = torch.where(torch.rand(2, N, rank, generator=g) < 0.5, -2.0, 2.0)
+    down[1, 0, 5] = float("inf")
+    x, down, up, w = x.to(dt), down.to(dt), up.to(dt), torch.zeros((N, K), dtype=dt)
+    off, ids = (None, torch.arange(M, dtype=torch.int32) // 70 % 2) if S is None else (torch.tensor([0, 70, 140, M]), torch.tensor([0, 1, 0], dtype=torch.int32))
+    announce(f"lora infinite low product {dt} S={S}")
+    got = ops.lora_linear(x.to(gpu), w.to(gpu), down.to(gpu), up.to(gpu), ids.to(gpu), offsets=None if off is None else off.to(gpu), out_dtype=F32)
+    want, tol = ref.lora_linear(x, w, down, up, ids, offsets=off, out_dtype=F32)
+    assert int(torch.isinf(want).sum()) == 70 * N and not bool(torch.isnan(want).any())
+    assert_within(got, want, tol)
