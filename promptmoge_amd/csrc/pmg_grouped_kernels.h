@@ -503,10 +503,14 @@ __global__ __launch_bounds__(64 * NW) void lora_low_k(GroupArgs a, int rows) {
 #pragma unroll
             for (int j = 0; j < NR; ++j) {
                 float x = v[j] * f;
-                const bool ends = !(__builtin_fabsf(x) < 3.0e38f);  // (infinity less itself would be NaN)
+                const bool ends = !(__builtin_fabsf(x) < __builtin_inff());  // (infinity less itself would be NaN)
 #pragma unroll
                 for (int p = 0; p < kParts<T>; ++p) {
-                    const T y = (T)x;
+                    T y = (T)x;
+                    if constexpr (__is_same(T, __bf16)) {  // (the largest that is finite: what is above it rounds to infinity)
+                        constexpr float most = 0x1.fep127f;
+                        y = ends ? y : (T)__builtin_fminf(__builtin_fmaxf(x, -most), most);
+                    }
                     if (writes && 16 * j + c < a.r) h[p * a.r + 16 * j + c] = y;
                     x = ends ? 0.0f : x - (float)y;
                 }

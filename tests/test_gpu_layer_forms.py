@@ -103,3 +103,25 @@ def test_an_infinite_low_product_leaves_the_others_finite(gpu, dt, S):
     want, tol = ref.lora_linear(x, w, down, up, ids, offsets=off, out_dtype=F32)
     assert int(torch.isinf(want).sum()) == 70 * N and not bool(torch.isnan(want).any())
     assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("S", [3, None])
+def test_low_products_near_the_largest_float(gpu, dt, S):
+    """Up to fp32's largest, above bf16's: sums of two exact products, 2^127 (1 + k / 128) + 2^119 l / 16 with k < 128 and l < 16, by up of
+    2^-20, so that a result is one of them (bounds: those of the 24-bit test)."""
+    M, K, N, rank, g = 200, 64, 24, 8, torch.Generator().manual_seed(2)
+    x, down = torch.zeros(M, K), torch.zeros(1, rank, K)
+    x[:, 0], x[:, 1] = 2.0 ** 60 * (1 + torch.randint(0, 128, (M,), generator=g) / 128), 2.0 ** 60 * torch.randint(0, 16, (M,), generator=g) / 16
+    x[::5, 0], x[::5, 1] = 2.0 ** 60 * (1 + 127 / 128), 2.0 ** 60 * 15 / 16
+    down[:, :, 0], down[:, :, 1] = 2.0 ** 67, 2.0 ** 59
+    up = torch.zeros(1, N, rank)
+    up[:, torch.arange(N), torch.arange(N) % rank] = 2.0 ** -20
+    low = x.double() @ down[0].double().t()
+    assert float(low.max()) <= torch.finfo(F32).max and float(low.max()) > torch.finfo(BF16).max
+    want = low[:, torch.arange(N) % rank] * 2.0 ** -20
+    x, down, up, w = x.to(dt), down.to(dt), up.to(dt), torch.zeros((N, K), dtype=dt)
+    off, ids = (None, torch.zeros(M, dtype=torch.int32)) if S is None else (torch.tensor([0, 70, 140, M]), torch.zeros(3, dtype=torch.int32))
+    announce(f"lora large low products {dt} S={S}")
+    got = ops.lora_linear(x.to(gpu), w.to(gpu), down.to(gpu), up.to(gpu), ids.to(gpu), offsets=None if off is None else off.to(gpu), out_dtype=F32)
+    assert_within(got, want, (2.0 ** -24 + 3 * 2.0 ** -23) * want.abs())
