@@ -7,7 +7,7 @@
 //
 // Measured (MI355X), and what bounds it: 307,200 rows of 64 fp16 with silu 31 us (11 the sums, 19 the results; two reads and a write
 // are 23 at a copy's rate, the rest is a block's start: its segment, the segment's sums, a barrier); 4 x 2745 rows of 512 fp32 to bf16
-// with gelu 21 us (8 and 13); 8 segments of one row of 256: 4.3 us, three latencies.
+// with gelu 21 us (8 and 13); 8 segments of one row of 256: 4.4 us, three latencies.
 #include "pmg_epilogue.h"
 #include "pmg_pieces.h"
 
